@@ -510,6 +510,102 @@ RELM_MP_API int relm_mp_lgan_pool_reduce_backward(relm_mp_dtype dtype, const rel
                                                   void* grad_slot_messages, void* workspace,
                                                   size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Decoder operators: what a decoder that reads the object embeddings needs.
+ * No counterpart in the reference library. Value arrays may be strided
+ * (strides in elements; the last dimension is dense); work is enqueued on
+ * `stream`, no call waits for the device or allocates device memory.
+ * dtype: RELM_MP_FLOAT32, RELM_MP_BFLOAT16 or RELM_MP_FLOAT16.
+ * ------------------------------------------------------------------------- */
+
+/* add_rms_norm: h = x + residual (h = x without residual: residual and h NULL),
+ * y = h * inv * weight, inv = 1 / sqrt(mean(h^2) + eps) of the unrounded sum.
+ * y and h are dense [rows, width]; inv_rms (float[rows]) may be NULL. */
+RELM_MP_API int relm_mp_add_rms_norm(relm_mp_dtype dtype, const void* x, int64_t x_stride, const void* residual,
+                                     int64_t residual_stride, const void* weight, int64_t rows, int64_t width,
+                                     float eps, void* y, void* h, float* inv_rms, void* stream);
+/* The same with y in e4m3 (8 bits): scale[row] = max|y| / 448 (1 for a row of
+ * zeros), q = y / scale rounded to nearest even. */
+RELM_MP_API int relm_mp_add_rms_norm_e4m3(relm_mp_dtype dtype, const void* x, int64_t x_stride,
+                                          const void* residual, int64_t residual_stride, const void* weight,
+                                          int64_t rows, int64_t width, float eps, unsigned char* q, float* scale,
+                                          void* h, void* stream);
+/* Gradient of both addends (they share it) and of the weight: with n = h * inv,
+ * dx = inv * (w * dy - n * mean(w * dy * n)) + dh, dweight = sum over rows of
+ * dy * n (summed in a fixed order). dy, dh or dweight may be NULL. */
+RELM_MP_API size_t relm_mp_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+RELM_MP_API int relm_mp_add_rms_norm_backward(relm_mp_dtype dtype, const void* dy, int64_t dy_stride,
+                                              const void* dh, int64_t dh_stride, const void* h, int64_t h_stride,
+                                              const float* inv_rms, const void* weight, int64_t rows, int64_t width,
+                                              void* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                                              void* stream);
+
+/* Cross attention: queries of sequence b attend to the states (keys, values)
+ * of sequence b; the two lengths are independent and either may be 0.
+ *   o_i = sum_j p_ij v_j, p_i = softmax over the kept keys j of scale * q_i.k_j
+ * A row without a kept key gives o = 0, lse = -inf and no gradient. Query head
+ * i reads key/value head i / (heads / kv_heads).
+ *
+ * Packed sequences: row r of q / k / v holds all sequences one after another
+ * and a plan (below) gives their lengths; dense batches (plan NULL): q is
+ * [seqs, max_q, heads, dim], k and v [seqs, max_kv, kv_heads, dim] with any
+ * strides. Outputs are dense: o / dq [rows, heads, dim], dk / dv [rows,
+ * kv_heads, dim], lse float[heads, q rows]. */
+typedef struct relm_mp_attn_plan {
+   int64_t seqs;
+   int64_t q_rows, kv_rows; /* totals */
+   int64_t max_q, max_kv;
+   int64_t q_tiles, q_pairs, kv_tiles, kv_blocks; /* work items: 128 query rows, 256 query rows, 128 keys, 64 keys */
+   const void* device;      /* relm_mp_attn_plan_bytes(seqs, ...) bytes on the device */
+} relm_mp_attn_plan;
+
+/* Host side of a plan: counts (device left NULL); the bytes of its device
+ * part; and that part written into host memory, for the caller to copy. */
+RELM_MP_API int relm_mp_attn_plan_init(const int64_t* q_lengths, const int64_t* kv_lengths, int64_t seqs,
+                                       relm_mp_attn_plan* plan);
+RELM_MP_API size_t relm_mp_attn_plan_bytes(const relm_mp_attn_plan* plan);
+RELM_MP_API int relm_mp_attn_plan_fill(const int64_t* q_lengths, const int64_t* kv_lengths,
+                                       const relm_mp_attn_plan* plan, void* host_mem, size_t host_bytes);
+
+typedef struct relm_mp_attn {
+   relm_mp_dtype dtype;
+   int32_t heads, kv_heads, dim; /* dim in [1, 256] */
+   float scale;                  /* finite, > 0 */
+   int64_t seqs, q_rows, kv_rows, max_q, max_kv;
+   const relm_mp_attn_plan* plan; /* NULL: dense batch */
+   const void *q, *k, *v;
+   int64_t q_stride[3], k_stride[3], v_stride[3]; /* sequence (dense batches), row, head */
+   const unsigned char* key_mask; /* NULL, or one byte per key row (kv_rows of them): 0 = masked */
+} relm_mp_attn;
+
+RELM_MP_API size_t relm_mp_cross_attention_workspace_bytes(const relm_mp_attn* attn);
+/* lse and o_rest may be NULL; the backward wants both. o_rest, of o's type and
+ * shape (2-byte types only), is what rounding took from o: the backward's
+ * do . o needs it, or the rounding of o would enter every score's gradient. */
+RELM_MP_API int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void* o_rest, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+RELM_MP_API size_t relm_mp_cross_attention_backward_workspace_bytes(const relm_mp_attn* attn);
+/* o, o_rest, grad_o: dense [q rows, heads, dim]; o, lse and o_rest (NULL for
+ * float32) of the forward. */
+RELM_MP_API int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_o, const void* o,
+                                                 const void* o_rest, const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                                                 size_t workspace_bytes, void* stream);
+
+/* Products with 4-bit weights: y[r, n] = x_scale[r] * sum_k x[r, k] * w[n, k],
+ * w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group].
+ * relm_mp_int4_pack lays the weights out once: codes [n, k / 2] bytes (the even
+ * k in the low half), scales fp16 [n, k / group], zeros uint8 [n, k / group]
+ * or NULL (8 everywhere); k a multiple of group, group 32, 64 or 128. x is
+ * [rows, k] of `dtype`, or, with x_e4m3, of e4m3 values with x_scale
+ * (float[rows]); y is dense [rows, n] of `dtype`. */
+RELM_MP_API size_t relm_mp_int4_packed_bytes(int64_t n, int64_t k, int64_t group, int has_zeros);
+RELM_MP_API int relm_mp_int4_pack(const unsigned char* codes, const void* scales, const unsigned char* zeros,
+                                  int64_t n, int64_t k, int64_t group, void* packed, size_t packed_bytes,
+                                  void* stream);
+RELM_MP_API int relm_mp_int4_matvec(relm_mp_dtype dtype, int x_e4m3, const void* x, int64_t x_stride,
+                                    const float* x_scale, int64_t rows, const void* packed, int64_t n, int64_t k,
+                                    int64_t group, int has_zeros, void* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

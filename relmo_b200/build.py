@@ -42,9 +42,13 @@ CUDA_SOURCES = [
     "relm_mp_seg_f16.cu",
     "relm_mp_noalloc.cu",
     "relm_mp_lgan.cu",
+    "relm_mp_norm.cu",
+    "relm_mp_int4.cu",
+    "relm_mp_attn.cu",
+    "relm_mp_attn_simt.cu",
 ]
-TORCH_SOURCES = ["relm_mp_torch.cpp", "relm_mp_cpu.cpp"]
-HEADERS = ["relm_mp_internal.cuh", "relm_mp_segment.cuh", "relm_mp_seg_impl.cuh"]
+TORCH_SOURCES = ["relm_mp_torch.cpp", "relm_mp_cpu.cpp", "relm_mp_decoder.cpp"]
+HEADERS = ["relm_mp_internal.cuh", "relm_mp_segment.cuh", "relm_mp_seg_impl.cuh", "relm_mp_attn.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -129,16 +133,27 @@ def build_torch(force: bool = False) -> Path:
     link = [f"-L{p}" for p in libdirs] + [f"-Wl,-rpath,{p}" for p in libdirs]
     link += ["-lc10", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-ltorch_cuda"]
     link += [f"-L{PKG}", "-l:librelm_mp_b200.so", "-Wl,-rpath,$ORIGIN"]
-    tmp = str(TORCH_LIB) + f".tmp{os.getpid()}"
-    cmd = [
-        "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+    flags = [
+        "-O2", "-std=c++17", "-fPIC",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         f'-DRELM_MP_BUILD_TORCH_VERSION="{version}"',
         f'-DRELM_MP_BUILD_CUDA_TAG="{cuda_tag}"',
         f'-DRELM_MP_ABI_TARGET="{major}.{minor}"',
-        *includes, *map(str, sources), "-o", tmp, *link,
+        *includes,
     ]
-    _run(cmd)
+    BUILD.mkdir(parents=True, exist_ok=True)
+    objs, jobs = [], []
+    shared = [CSRC / "relm_mp_torch.h", INCLUDE / "relm_mp.h", Path(__file__)]
+    with cf.ThreadPoolExecutor(max_workers=len(sources)) as pool:
+        for src in sources:
+            obj = BUILD / f"torch_{src.stem}.o"
+            objs.append(obj)
+            if force or not _newer(obj, [src] + shared):
+                jobs.append(pool.submit(_run, ["g++", *flags, "-c", str(src), "-o", str(obj)]))
+        for j in jobs:
+            j.result()
+    tmp = str(TORCH_LIB) + f".tmp{os.getpid()}"
+    _run(["g++", "-shared", *map(str, objs), "-o", tmp, *link])
     os.replace(tmp, TORCH_LIB)
     return TORCH_LIB
 

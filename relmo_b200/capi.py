@@ -27,6 +27,7 @@ STATUS_NAMES = {
 
 # Every symbol the header declares, with (restype, argtypes).
 _P = ctypes.c_void_p
+_F32 = ctypes.c_float
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 _INT = ctypes.c_int
@@ -71,6 +72,25 @@ class LganGraph(ctypes.Structure):
 
 
 _GRAPHP = ctypes.POINTER(LganGraph)
+
+
+class AttnPlan(ctypes.Structure):
+    """relm_mp_attn_plan: sizes and device memory of a cross attention plan."""
+
+    _fields_ = [(n, ctypes.c_int64) for n in ("seqs", "q_rows", "kv_rows", "max_q", "max_kv", "q_tiles", "q_pairs",
+                                              "kv_tiles", "kv_blocks")] + [("device", ctypes.c_void_p)]
+
+
+class Attn(ctypes.Structure):
+    """relm_mp_attn: one cross attention call's inputs."""
+
+    _fields_ = [("dtype", ctypes.c_int), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("dim", ctypes.c_int32), ("scale", ctypes.c_float),
+                *[(n, ctypes.c_int64) for n in ("seqs", "q_rows", "kv_rows", "max_q", "max_kv")],
+                ("plan", ctypes.POINTER(AttnPlan)),
+                *[(n, ctypes.c_void_p) for n in ("q", "k", "v")],
+                *[(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")],
+                ("key_mask", ctypes.c_void_p)]
 
 
 class LseForm(ctypes.Structure):
@@ -157,6 +177,21 @@ SIGNATURES: dict[str, tuple] = {
         _INT,
         [_INT, _GRAPHP, _P, _P, _P, _I64, _I64, _P, _P, _INT, _P, _P, _SZ, _P],
     ),
+    "relm_mp_add_rms_norm": (_INT, [_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _P, _P, _P, _P]),
+    "relm_mp_add_rms_norm_e4m3": (_INT, [_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _P, _P, _P, _P]),
+    "relm_mp_add_rms_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
+    "relm_mp_add_rms_norm_backward": (
+        _INT, [_INT, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
+    "relm_mp_attn_plan_init": (_INT, [_P, _P, _I64, _P]),
+    "relm_mp_attn_plan_bytes": (_SZ, [_P]),
+    "relm_mp_attn_plan_fill": (_INT, [_P, _P, _P, _P, _SZ]),
+    "relm_mp_cross_attention_workspace_bytes": (_SZ, [_P]),
+    "relm_mp_cross_attention": (_INT, [_P, _P, _P, _P, _P, _SZ, _P]),
+    "relm_mp_cross_attention_backward_workspace_bytes": (_SZ, [_P]),
+    "relm_mp_cross_attention_backward": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "relm_mp_int4_packed_bytes": (_SZ, [_I64, _I64, _I64, _INT]),
+    "relm_mp_int4_pack": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P]),
+    "relm_mp_int4_matvec": (_INT, [_INT, _INT, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _INT, _P, _P]),
 }
 
 _LIB: ctypes.CDLL | None = None

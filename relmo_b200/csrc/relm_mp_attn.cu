@@ -1,0 +1,262 @@
+// Cross attention of packed or dense sequences of queries to sequences of
+// states: argument checks, plans, and the choice of kernel.
+//
+// A plan is the host's knowledge of the lengths laid out for the device: row
+// offsets of both sides and the tiles that exist, ordered so that the tiles
+// with the longest loop start first (query tiles by the length of their keys
+// and the other way round).
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <numeric>
+#include <vector>
+
+#include "relm_mp_attn.cuh"
+
+using namespace relm_mp;
+using namespace relm_mp::attn;
+
+namespace {
+
+constexpr int kMaxDim = 256;
+
+struct PlanLayout {
+   size_t q_off, kv_off, kv_blocks, q_tiles, q_pairs, kv_tiles, bytes;
+};
+
+PlanLayout plan_layout(const relm_mp_attn_plan& p)
+{
+   PlanLayout l;
+   size_t at = 0;
+   auto take = [&](int64_t count) {
+      const size_t here = at;
+      at += align_up((size_t)count * 8, 16);
+      return here;
+   };
+   l.q_off = take(p.seqs + 1);
+   l.kv_off = take(p.seqs + 1);
+   l.kv_blocks = take(p.seqs + 1);
+   l.q_tiles = take(p.q_tiles);
+   l.q_pairs = take(p.q_pairs);
+   l.kv_tiles = take(p.kv_tiles);
+   l.bytes = align_up(at);
+   return l;
+}
+
+int check_attn(const relm_mp_attn* a, const char* op)
+{
+   const std::string name(op);
+   if(!a) return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": attn must not be NULL.");
+   if(a->dtype != RELM_MP_FLOAT32 && a->dtype != RELM_MP_BFLOAT16 && a->dtype != RELM_MP_FLOAT16)
+      return fail(RELM_MP_ERR_UNSUPPORTED, name + ": unsupported dtype (float32, bfloat16, float16).");
+   if(a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads || a->heads > 65535)
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": heads must be a positive multiple of kv_heads, at most 65535.");
+   if(a->dim < 1 || a->dim > kMaxDim) return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": dim must be in [1, 256].");
+   if(!(a->scale > 0.f) || !std::isfinite(a->scale))
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": scale must be positive and finite.");
+   if(a->seqs < 0 || a->q_rows < 0 || a->kv_rows < 0 || a->max_q < 0 || a->max_kv < 0)
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": sizes must be >= 0.");
+   if(a->plan) {
+      const relm_mp_attn_plan& p = *a->plan;
+      if(p.seqs != a->seqs || p.q_rows != a->q_rows || p.kv_rows != a->kv_rows || p.max_q != a->max_q ||
+         p.max_kv != a->max_kv)
+         return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": the plan's sizes are not those of the tensors.");
+      if(p.seqs > 0 && !p.device) return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": the plan has no device memory.");
+   } else if(a->q_rows != a->seqs * a->max_q || a->kv_rows != a->seqs * a->max_kv) {
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": row counts of a dense batch must be seqs * length.");
+   }
+   if(a->max_q >= (1ll << 31) - 256 || a->max_kv >= (1ll << 31) - 256 || a->seqs >= (1ll << 31))
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": lengths must be below 2^31 - 256.");
+   if((a->q_rows && !a->q) || (a->kv_rows && (!a->k || !a->v)))
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, name + ": pointers must not be NULL.");
+   return RELM_MP_OK;
+}
+
+Args make_args(const relm_mp_attn& in)
+{
+   Args a{};
+   a.q = in.q, a.k = in.k, a.v = in.v;
+   for(int i = 0; i < 3; ++i) {
+      a.qs[i] = in.q_stride[i];
+      a.ks[i] = in.k_stride[i];
+      a.vs[i] = in.v_stride[i];
+   }
+   if(in.plan) {
+      const PlanLayout l = plan_layout(*in.plan);
+      const char* d = static_cast< const char* >(in.plan->device);
+      a.q_off = reinterpret_cast< const int64_t* >(d + l.q_off);
+      a.kv_off = reinterpret_cast< const int64_t* >(d + l.kv_off);
+      a.kv_blocks = reinterpret_cast< const int64_t* >(d + l.kv_blocks);
+      a.q_tiles = reinterpret_cast< const Item* >(d + l.q_tiles);
+      a.q_pairs = reinterpret_cast< const Item* >(d + l.q_pairs);
+      a.kv_tiles = reinterpret_cast< const Item* >(d + l.kv_tiles);
+      a.qs[0] = a.ks[0] = a.vs[0] = 0;
+   }
+   a.mask = in.key_mask;
+   a.seqs = in.seqs, a.q_rows = in.q_rows, a.kv_rows = in.kv_rows, a.max_q = in.max_q, a.max_kv = in.max_kv;
+   a.heads = in.heads, a.kv_heads = in.kv_heads, a.dim = in.dim, a.scale = in.scale;
+   return a;
+}
+
+struct Counts {
+   int64_t q_tiles, q_pairs, kv_tiles, kv_blocks;
+};
+
+Counts counts(const relm_mp_attn& in)
+{
+   if(in.plan) return {in.plan->q_tiles, in.plan->q_pairs, in.plan->kv_tiles, in.plan->kv_blocks};
+   return {in.seqs * ceil_div(in.max_q, kTileRows), in.seqs * ceil_div(in.max_q, 2 * kTileRows),
+           in.seqs * ceil_div(in.max_kv, kTileRows), in.seqs * ceil_div(in.max_kv, kBlockKeys)};
+}
+
+// delta[head, row] = sum over dim of go * (o + o_rest), in float32; 8 lanes per row and head.
+template < typename T, int VEC >
+__global__ void __launch_bounds__(256) k_attn_delta(const T* __restrict__ go, const T* __restrict__ o,
+                                                    const T* __restrict__ rest, int64_t rows, int heads, int dim,
+                                                    float* __restrict__ delta)
+{
+   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;
+   const int lane = threadIdx.x & 7;
+   float s = 0.f;
+   if(i < rows * heads) {
+      for(int d = lane * VEC; d < dim; d += 8 * VEC) {
+         struct alignas(sizeof(T) * VEC) V {
+            T v[VEC];
+         };
+         const V x = *reinterpret_cast< const V* >(go + i * dim + d), y = *reinterpret_cast< const V* >(o + i * dim + d);
+#pragma unroll
+         for(int e = 0; e < VEC; ++e) s = fmaf(to_f32(x.v[e]), to_f32(y.v[e]), s);
+         if(rest) {
+            const V z = *reinterpret_cast< const V* >(rest + i * dim + d);
+#pragma unroll
+            for(int e = 0; e < VEC; ++e) s = fmaf(to_f32(x.v[e]), to_f32(z.v[e]), s);
+         }
+      }
+   }
+#pragma unroll
+   for(int m = 4; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+   if(lane == 0 && i < rows * heads) delta[(i % heads) * rows + i / heads] = s;
+}
+
+template < typename T >
+int launch_delta(const void* go, const void* o, const void* rest, int64_t rows, int heads, int dim, float* delta, cudaStream_t st)
+{
+   constexpr int FULL = 16 / sizeof(T);
+   const unsigned grid = (unsigned)ceil_div(rows * heads, 32);
+   const T *g = static_cast< const T* >(go), *y = static_cast< const T* >(o), *z = static_cast< const T* >(rest);
+   const bool vec = dim % FULL == 0 && ((reinterpret_cast< uintptr_t >(go) | reinterpret_cast< uintptr_t >(o) |
+                                         reinterpret_cast< uintptr_t >(rest)) & 15) == 0;
+   if(vec) k_attn_delta< T, FULL ><<< grid, 256, 0, st >>>(g, y, z, rows, heads, dim, delta);
+   else k_attn_delta< T, 1 ><<< grid, 256, 0, st >>>(g, y, z, rows, heads, dim, delta);
+   return check_launch("k_attn_delta");
+}
+
+}  // namespace
+
+int relm_mp_attn_plan_init(const int64_t* q_lengths, const int64_t* kv_lengths, int64_t seqs, relm_mp_attn_plan* plan)
+{
+   if(!plan || seqs < 0 || (seqs && (!q_lengths || !kv_lengths)))
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, "attn_plan: pointers must not be NULL and seqs must be >= 0.");
+   relm_mp_attn_plan p{};
+   p.seqs = seqs;
+   for(int64_t b = 0; b < seqs; ++b) {
+      const int64_t q = q_lengths[b], k = kv_lengths[b];
+      if(q < 0 || k < 0 || q >= (1ll << 31) - 256 || k >= (1ll << 31) - 256)
+         return fail(RELM_MP_ERR_INVALID_ARGUMENT, "attn_plan: lengths must be in [0, 2^31 - 256).");
+      p.q_rows += q, p.kv_rows += k;
+      p.max_q = std::max(p.max_q, q), p.max_kv = std::max(p.max_kv, k);
+      p.q_tiles += ceil_div(q, kTileRows), p.q_pairs += ceil_div(q, 2 * kTileRows);
+      p.kv_tiles += ceil_div(k, kTileRows), p.kv_blocks += ceil_div(k, kBlockKeys);
+   }
+   *plan = p;
+   return RELM_MP_OK;
+}
+
+size_t relm_mp_attn_plan_bytes(const relm_mp_attn_plan* plan) { return plan ? plan_layout(*plan).bytes : 0; }
+
+int relm_mp_attn_plan_fill(const int64_t* q_lengths, const int64_t* kv_lengths, const relm_mp_attn_plan* plan,
+                           void* host_mem, size_t host_bytes)
+{
+   relm_mp_attn_plan p{};
+   if(!plan) return fail(RELM_MP_ERR_INVALID_ARGUMENT, "attn_plan: plan must not be NULL.");
+   const int rc = relm_mp_attn_plan_init(q_lengths, kv_lengths, plan->seqs, &p);
+   if(rc) return rc;
+   if(p.q_tiles != plan->q_tiles || p.q_pairs != plan->q_pairs || p.kv_tiles != plan->kv_tiles)
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, "attn_plan: the lengths are not those of the plan.");
+   const PlanLayout l = plan_layout(p);
+   if(!host_mem || host_bytes < l.bytes) return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "attn_plan: buffer too small.");
+   char* d = static_cast< char* >(host_mem);
+   std::memset(d, 0, l.bytes);
+   int64_t *q_off = reinterpret_cast< int64_t* >(d + l.q_off), *kv_off = reinterpret_cast< int64_t* >(d + l.kv_off);
+   int64_t* blocks = reinterpret_cast< int64_t* >(d + l.kv_blocks);
+   for(int64_t b = 0; b < p.seqs; ++b) {
+      q_off[b + 1] = q_off[b] + q_lengths[b];
+      kv_off[b + 1] = kv_off[b] + kv_lengths[b];
+      blocks[b + 1] = blocks[b] + ceil_div(kv_lengths[b], kBlockKeys);
+   }
+   std::vector< int32_t > order(p.seqs);
+   auto list = [&](size_t at, const int64_t* own, const int64_t* other, int rows) {
+      std::iota(order.begin(), order.end(), 0);
+      std::stable_sort(order.begin(), order.end(), [&](int32_t x, int32_t y) { return other[x] > other[y]; });
+      Item* out = reinterpret_cast< Item* >(d + at);
+      for(const int32_t b : order)
+         for(int64_t t = 0; t < ceil_div(own[b], rows); ++t) *out++ = Item{b, (int32_t)t};
+   };
+   list(l.q_tiles, q_lengths, kv_lengths, kTileRows);
+   list(l.q_pairs, q_lengths, kv_lengths, 2 * kTileRows);
+   list(l.kv_tiles, kv_lengths, q_lengths, kTileRows);
+   return RELM_MP_OK;
+}
+
+size_t relm_mp_cross_attention_workspace_bytes(const relm_mp_attn* attn)
+{
+   if(check_attn(attn, "cross_attention")) return 0;
+   return 0;
+}
+
+int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void* o_rest, void* workspace,
+                            size_t workspace_bytes, void* stream)
+{
+   int rc;
+   if((rc = check_attn(attn, "cross_attention"))) return rc;
+   if(attn->q_rows == 0) return RELM_MP_OK;
+   if(!o) return fail(RELM_MP_ERR_INVALID_ARGUMENT, "cross_attention: o must not be NULL.");
+   if(workspace_bytes < relm_mp_cross_attention_workspace_bytes(attn))
+      return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "cross_attention: workspace too small.");
+   (void)workspace;
+   Args a = make_args(*attn);
+   a.o = o, a.lse = lse, a.o_rest = attn->dtype == RELM_MP_FLOAT32 ? nullptr : o_rest;
+   return simt_forward(attn->dtype, a, counts(*attn).q_tiles, static_cast< cudaStream_t >(stream));
+}
+
+size_t relm_mp_cross_attention_backward_workspace_bytes(const relm_mp_attn* attn)
+{
+   if(check_attn(attn, "cross_attention_backward")) return 0;
+   return align_up((size_t)attn->heads * attn->q_rows * sizeof(float));
+}
+
+int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_o, const void* o, const void* o_rest,
+                                     const float* lse, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                     void* stream)
+{
+   int rc;
+   if((rc = check_attn(attn, "cross_attention_backward"))) return rc;
+   if((attn->q_rows && (!grad_o || !o || !lse || !dq)) || (attn->kv_rows && (!dk || !dv)))
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, "cross_attention_backward: pointers must not be NULL.");
+   if(attn->q_rows && (!workspace || workspace_bytes < relm_mp_cross_attention_backward_workspace_bytes(attn)))
+      return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "cross_attention_backward: workspace too small.");
+   cudaStream_t st = static_cast< cudaStream_t >(stream);
+   Args a = make_args(*attn);
+   float* delta = static_cast< float* >(workspace);
+   a.go = grad_o, a.lse_in = lse, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
+   if(attn->q_rows) {
+      switch(attn->dtype) {
+         case RELM_MP_FLOAT32: rc = launch_delta< float >(grad_o, o, o_rest, attn->q_rows, a.heads, a.dim, delta, st); break;
+         case RELM_MP_BFLOAT16: rc = launch_delta< __nv_bfloat16 >(grad_o, o, o_rest, attn->q_rows, a.heads, a.dim, delta, st); break;
+         default: rc = launch_delta< __half >(grad_o, o, o_rest, attn->q_rows, a.heads, a.dim, delta, st);
+      }
+      if(rc) return rc;
+   }
+   const Counts c = counts(*attn);
+   return simt_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);
+}

@@ -1,0 +1,101 @@
+// Shared declarations of the cross attention sources.
+#pragma once
+
+#include "relm_mp_internal.cuh"
+
+namespace relm_mp {
+namespace attn {
+
+// Work item of a plan: tile `tile` of sequence `seq`.
+struct Item {
+   int32_t seq, tile;
+};
+
+// What every kernel gets. Strides are in elements: {sequence, row, head}; the
+// sequence stride is 0 for packed rows.
+struct Args {
+   const void *q, *k, *v;
+   int64_t qs[3], ks[3], vs[3];
+   const int64_t *q_off, *kv_off; // packed: [seqs + 1]; NULL for a dense batch
+   const Item *q_tiles, *q_pairs, *kv_tiles;
+   const int64_t* kv_blocks; // packed: prefix of 64-key blocks, [seqs + 1]
+   const unsigned char* mask;
+   int64_t seqs, q_rows, kv_rows, max_q, max_kv;
+   int heads, kv_heads, dim;
+   float scale;
+   void *o, *o_rest; // o_rest may be NULL
+   float* lse;       // may be NULL
+   // backward
+   const void *go;
+   const float *lse_in, *delta;
+   void *dq, *dk, *dv;
+};
+
+// First row, length and base offset (elements) of one side of a sequence.
+struct Seq {
+   int64_t first; // row among all rows of that side
+   int64_t base;  // element offset of its first row
+   int len;
+};
+
+__device__ __forceinline__ Seq locate(const int64_t* off, int64_t uniform, const int64_t* stride, int seq)
+{
+   Seq s;
+   if(off) {
+      s.first = off[seq];
+      s.len = (int)(off[seq + 1] - s.first);
+      s.base = s.first * stride[1];
+   } else {
+      s.first = (int64_t)seq * uniform;
+      s.len = (int)uniform;
+      s.base = (int64_t)seq * stride[0];
+   }
+   return s;
+}
+
+// Item `i` of a tiled side.
+__device__ __forceinline__ Item item(const Item* list, int64_t uniform, int tile_rows, int64_t i)
+{
+   if(list) return list[i];
+   const int64_t per = (uniform + tile_rows - 1) / tile_rows;
+   return Item{(int32_t)(i / per), (int32_t)(i % per)};
+}
+
+constexpr int kTileRows = 128; // query rows or keys of a plan's tile
+constexpr int kBlockKeys = 64; // keys of a block of the split form
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template < typename T >
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32< float >(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32< __nv_bfloat16 >(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32< __half >(__half v) { return __half2float(v); }
+template < typename T >
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32< float >(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32< __nv_bfloat16 >(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32< __half >(float v) { return __float2half_rn(v); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+   float y;
+   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+   return y;
+}
+
+// Kernels on the CUDA cores, for every type, dim and stride (relm_mp_attn_simt.cu).
+int simt_forward(relm_mp_dtype dtype, const Args& a, int64_t items, cudaStream_t st);
+int simt_backward(relm_mp_dtype dtype, const Args& a, int64_t q_items, int64_t kv_items, cudaStream_t st);
+
+}  // namespace attn
+}  // namespace relm_mp

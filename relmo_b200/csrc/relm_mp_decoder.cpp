@@ -1,0 +1,481 @@
+// torch.ops.relm_mp_b200 registration of the decoder operators: add + RMS
+// norm, cross attention, products with 4-bit weights. CUDA kernels through
+// librelm_mp_b200.so (include/relm_mp.h), Meta kernels for shapes, and autograd
+// for the two that train. CPU tensors use the Python formulas of
+// relmo_b200/ops/decoder.py.
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "relm_mp.h"
+
+namespace relm_b200 {
+
+using at::Tensor;
+using OptTensor = std::optional< Tensor >;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+relm_mp_dtype dtype_of(at::ScalarType t, const char* op)
+{
+   switch(t) {
+      case at::kFloat: return RELM_MP_FLOAT32;
+      case at::kBFloat16: return RELM_MP_BFLOAT16;
+      case at::kHalf: return RELM_MP_FLOAT16;
+      default: break;
+   }
+   TORCH_CHECK(false, op, ": unsupported dtype ", t, " (float32, bfloat16, float16).");
+   return RELM_MP_FLOAT32;
+}
+
+void check_rc(int rc, const char* op) { TORCH_CHECK(rc == RELM_MP_OK, relm_mp_last_error(), " (", op, ")"); }
+
+void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+Tensor bytes_like(size_t n, const Tensor& like)
+{
+   return at::empty({(int64_t)std::max< size_t >(n, 1)}, like.options().dtype(at::kByte));
+}
+
+void same_device(const Tensor& a, const Tensor& b, const char* op, const char* name)
+{
+   TORCH_CHECK(a.device() == b.device(), op, ": ", name, " must be on ", a.device(), ", got ", b.device(), ".");
+}
+
+bool wants_grad(std::initializer_list< const Tensor* > ts)
+{
+   if(!at::GradMode::is_enabled()) return false;
+   for(const Tensor* t : ts)
+      if(t->defined() && t->requires_grad()) return true;
+   return false;
+}
+
+const Tensor& or_none(const OptTensor& t)
+{
+   static const Tensor none;
+   return t.has_value() ? *t : none;
+}
+
+// ---- add + RMS norm ----------------------------------------------------------------
+
+// [rows, width] with dense rows: a view where the strides allow it.
+Tensor rows_of(const Tensor& t)
+{
+   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+   if(r.stride(1) != 1 && r.size(1) > 1) r = r.contiguous();
+   return r;
+}
+
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+void check_norm(const Tensor& x, const Tensor& weight, const Tensor& residual, const char* op)
+{
+   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, op, ": x must be [..., width] with width >= 1.");
+   TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(-1), op, ": weight must be [", x.size(-1), "], got ",
+               weight.sizes(), ".");
+   TORCH_CHECK(weight.scalar_type() == x.scalar_type(), op, ": weight must share x's dtype.");
+   same_device(x, weight, op, "weight");
+   if(residual.defined()) {
+      TORCH_CHECK(residual.sizes() == x.sizes(), op, ": residual must have x's shape ", x.sizes(), ", got ",
+                  residual.sizes(), ".");
+      TORCH_CHECK(residual.scalar_type() == x.scalar_type(), op, ": residual must share x's dtype.");
+      same_device(x, residual, op, "residual");
+   }
+   dtype_of(x.scalar_type(), op);
+}
+
+// (y, h, inv): h is empty without a residual, inv unless it is asked for.
+std::tuple< Tensor, Tensor, Tensor > norm_forward(const Tensor& x, const Tensor& weight, const Tensor& residual,
+                                                  double eps, bool keep_inv)
+{
+   const char* op = "add_rms_norm";
+   check_norm(x, weight, residual, op);
+   c10::cuda::CUDAGuard guard(x.device());
+   const Tensor x2 = rows_of(x), w = weight.contiguous();
+   const Tensor r2 = residual.defined() ? rows_of(residual) : Tensor();
+   const int64_t rows = x2.size(0), width = x2.size(1);
+   Tensor y = at::empty(x.sizes(), x.options());
+   Tensor h = residual.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+   Tensor inv = at::empty({keep_inv ? rows : 0}, x.options().dtype(at::kFloat));
+   check_rc(relm_mp_add_rms_norm(dtype_of(x.scalar_type(), op), x2.data_ptr(), row_stride(x2),
+                                 r2.defined() ? r2.data_ptr() : nullptr, r2.defined() ? row_stride(r2) : 0, w.data_ptr(),
+                                 rows, width, (float)eps, y.data_ptr(), residual.defined() ? h.data_ptr() : nullptr,
+                                 keep_inv ? inv.data_ptr< float >() : nullptr, stream_of(x)),
+            op);
+   return {y, h, inv};
+}
+
+// (dx, dweight): dweight is empty unless it is asked for.
+std::tuple< Tensor, Tensor > norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& inv,
+                                           const Tensor& weight, bool need_weight)
+{
+   const char* op = "add_rms_norm_backward";
+   c10::cuda::CUDAGuard guard(h.device());
+   const Tensor h2 = rows_of(h), w = weight.contiguous();
+   const Tensor g = dy.defined() ? rows_of(dy) : Tensor(), gh = dh.defined() ? rows_of(dh) : Tensor();
+   const int64_t rows = h2.size(0), width = h2.size(1);
+   Tensor dx = at::empty(h.sizes(), h.options());
+   Tensor dw = at::empty({need_weight ? width : 0}, h.options());
+   const size_t bytes = need_weight ? relm_mp_add_rms_norm_backward_workspace_bytes(rows, width) : 0;
+   const Tensor ws = bytes_like(bytes, h);
+   check_rc(relm_mp_add_rms_norm_backward(dtype_of(h.scalar_type(), op), g.defined() ? g.data_ptr() : nullptr,
+                                          g.defined() ? row_stride(g) : 0, gh.defined() ? gh.data_ptr() : nullptr,
+                                          gh.defined() ? row_stride(gh) : 0, h2.data_ptr(), row_stride(h2),
+                                          inv.data_ptr< float >(), w.data_ptr(), rows, width, dx.data_ptr(),
+                                          need_weight ? dw.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(h)),
+            op);
+   return {dx, dw};
+}
+
+struct AddRmsNorm : torch::autograd::Function< AddRmsNorm > {
+   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                                const OptTensor& residual_in, double eps)
+   {
+      const Tensor& residual = or_none(residual_in);
+      auto [y, h, inv] = norm_forward(x, weight, residual, eps, true);
+      ctx->saved_data["residual"] = residual.defined();
+      ctx->save_for_backward({residual.defined() ? h : x, inv, weight});
+      ctx->set_materialize_grads(false);
+      if(!residual.defined()) ctx->mark_non_differentiable({h});
+      return {y, h};
+   }
+   static variable_list backward(AutogradContext* ctx, variable_list grads)
+   {
+      const auto saved = ctx->get_saved_variables();
+      const bool residual = ctx->saved_data["residual"].toBool();
+      const Tensor& dh = residual ? grads[1] : Tensor();
+      if(!grads[0].defined() && !dh.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dx, dw] = norm_backward(grads[0], dh, saved[0], saved[1], saved[2], ctx->needs_input_grad(1));
+      return {dx, ctx->needs_input_grad(1) ? dw : Tensor(), residual ? dx : Tensor(), Tensor()};
+   }
+};
+
+std::tuple< Tensor, Tensor > add_rms_norm_cuda(const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                                               double eps)
+{
+   auto [y, h, inv] = norm_forward(x, weight, or_none(residual), eps, false);
+   return {y, h};
+}
+
+std::tuple< Tensor, Tensor > add_rms_norm_autograd(const Tensor& x, const Tensor& weight, const OptTensor& residual,
+                                                   double eps)
+{
+   const Tensor& r = or_none(residual);
+   if(wants_grad({&x, &weight, &r})) {
+      const auto out = AddRmsNorm::apply(x, weight, residual, eps);
+      return {out[0], out[1]};
+   }
+   at::AutoDispatchBelowADInplaceOrView below;
+   return add_rms_norm_cuda(x, weight, residual, eps);
+}
+
+std::tuple< Tensor, Tensor > add_rms_norm_meta(const Tensor& x, const Tensor&, const OptTensor& residual, double)
+{
+   return {at::empty(x.sizes(), x.options()),
+           residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options())};
+}
+
+std::tuple< Tensor, Tensor, Tensor > add_rms_norm_e4m3_cuda(const Tensor& x, const Tensor& weight,
+                                                            const OptTensor& residual, double eps)
+{
+   const char* op = "add_rms_norm_e4m3";
+   const Tensor& r = or_none(residual);
+   check_norm(x, weight, r, op);
+   c10::cuda::CUDAGuard guard(x.device());
+   const Tensor x2 = rows_of(x), w = weight.contiguous(), r2 = r.defined() ? rows_of(r) : Tensor();
+   const int64_t rows = x2.size(0), width = x2.size(1);
+   Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+   Tensor h = r.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+   Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+   check_rc(relm_mp_add_rms_norm_e4m3(dtype_of(x.scalar_type(), op), x2.data_ptr(), row_stride(x2),
+                                      r2.defined() ? r2.data_ptr() : nullptr, r2.defined() ? row_stride(r2) : 0,
+                                      w.data_ptr(), rows, width, (float)eps, static_cast< unsigned char* >(q.data_ptr()),
+                                      scale.data_ptr< float >(), r.defined() ? h.data_ptr() : nullptr, stream_of(x)),
+            op);
+   return {q, scale, h};
+}
+
+std::tuple< Tensor, Tensor, Tensor > add_rms_norm_e4m3_meta(const Tensor& x, const Tensor&, const OptTensor& residual,
+                                                            double)
+{
+   return {at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn)),
+           at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat)),
+           residual.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options())};
+}
+
+// ---- cross attention ---------------------------------------------------------------
+
+constexpr size_t kMeta = 9;
+
+relm_mp_attn_plan plan_of(at::IntArrayRef m, const Tensor& memory)
+{
+   TORCH_CHECK(m.size() == kMeta, "cross_attention: a plan has ", kMeta, " sizes.");
+   relm_mp_attn_plan p{m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], m[8], nullptr};
+   TORCH_CHECK(memory.defined() && memory.is_cuda() && memory.scalar_type() == at::kByte && memory.is_contiguous() &&
+                  (size_t)memory.numel() == std::max< size_t >(relm_mp_attn_plan_bytes(&p), 1),
+               "cross_attention: the plan's memory does not belong to its sizes.");
+   p.device = memory.data_ptr();
+   return p;
+}
+
+std::tuple< Tensor, std::vector< int64_t > > attention_plan(at::IntArrayRef q_lengths, at::IntArrayRef kv_lengths,
+                                                           at::Device device)
+{
+   const char* op = "attention_plan";
+   TORCH_CHECK(q_lengths.size() == kv_lengths.size(), op, ": q_lengths and kv_lengths must have one length each per "
+               "sequence, got ", q_lengths.size(), " and ", kv_lengths.size(), ".");
+   TORCH_CHECK(device.is_cuda(), op, ": plans are for CUDA devices, got ", device, ".");
+   relm_mp_attn_plan p;
+   check_rc(relm_mp_attn_plan_init(q_lengths.data(), kv_lengths.data(), (int64_t)q_lengths.size(), &p), op);
+   const size_t bytes = relm_mp_attn_plan_bytes(&p);
+   Tensor host = at::empty({(int64_t)std::max< size_t >(bytes, 1)}, at::TensorOptions().dtype(at::kByte));
+   check_rc(relm_mp_attn_plan_fill(q_lengths.data(), kv_lengths.data(), &p, host.data_ptr(), bytes), op);
+   return {host.to(device), {p.seqs, p.q_rows, p.kv_rows, p.max_q, p.max_kv, p.q_tiles, p.q_pairs, p.kv_tiles, p.kv_blocks}};
+}
+
+// Checked call arguments; tensors whose last dimension is not dense are copied.
+struct Attn {
+   relm_mp_attn a{};
+   relm_mp_attn_plan plan{};
+   Tensor q, k, v, mask;
+
+   Attn(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& memory, at::IntArrayRef meta,
+        double scale, const Tensor& mask_in, const char* op)
+   {
+      const bool packed = memory.defined();
+      const int64_t rank = packed ? 3 : 4;
+      TORCH_CHECK(q_in.dim() == rank && k_in.dim() == rank && v_in.dim() == rank, op, ": q, k and v must be ",
+                  packed ? "[rows, heads, dim] with a plan" : "[batch, length, heads, dim] without a plan", ".");
+      TORCH_CHECK(k_in.sizes() == v_in.sizes(), op, ": k and v must have the same shape, got ", k_in.sizes(), " and ",
+                  v_in.sizes(), ".");
+      TORCH_CHECK(q_in.size(-1) == k_in.size(-1), op, ": q and k must have the same dim.");
+      TORCH_CHECK(k_in.scalar_type() == q_in.scalar_type() && v_in.scalar_type() == q_in.scalar_type(), op,
+                  ": q, k and v must share dtype.");
+      same_device(q_in, k_in, op, "k");
+      same_device(q_in, v_in, op, "v");
+      if(!packed) TORCH_CHECK(q_in.size(0) == k_in.size(0), op, ": q and k must have the same batch.");
+      auto dense = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
+      q = dense(q_in), k = dense(k_in), v = dense(v_in);
+      a.dtype = dtype_of(q.scalar_type(), op);
+      a.heads = (int32_t)q.size(-2), a.kv_heads = (int32_t)k.size(-2), a.dim = (int32_t)q.size(-1);
+      a.scale = (float)scale;
+      if(packed) {
+         same_device(q_in, memory, op, "plan");
+         plan = plan_of(meta, memory);
+         a.plan = &plan;
+         a.seqs = plan.seqs, a.max_q = plan.max_q, a.max_kv = plan.max_kv;
+         a.q_rows = q.size(0), a.kv_rows = k.size(0);
+         TORCH_CHECK(a.q_rows == plan.q_rows && a.kv_rows == plan.kv_rows, op, ": the plan is for ", plan.q_rows,
+                     " query and ", plan.kv_rows, " key rows, got ", a.q_rows, " and ", a.kv_rows, ".");
+      } else {
+         a.seqs = q.size(0), a.max_q = q.size(1), a.max_kv = k.size(1);
+         a.q_rows = a.seqs * a.max_q, a.kv_rows = a.seqs * a.max_kv;
+      }
+      const Tensor* ts[3] = {&q, &k, &v};
+      int64_t* strides[3] = {a.q_stride, a.k_stride, a.v_stride};
+      for(int i = 0; i < 3; ++i) {
+         strides[i][0] = packed ? 0 : ts[i]->stride(0);
+         strides[i][1] = ts[i]->stride(-3);
+         strides[i][2] = ts[i]->stride(-2);
+      }
+      a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
+      if(mask_in.defined()) {
+         TORCH_CHECK(mask_in.scalar_type() == at::kBool, op, ": key_mask must be bool.");
+         same_device(q_in, mask_in, op, "key_mask");
+         TORCH_CHECK(packed ? mask_in.dim() == 1 && mask_in.size(0) == a.kv_rows
+                            : mask_in.dim() == 2 && mask_in.size(0) == a.seqs && mask_in.size(1) == a.max_kv,
+                     op, ": key_mask must have one value per key row, got ", mask_in.sizes(), ".");
+         mask = mask_in.contiguous();
+         a.key_mask = static_cast< const unsigned char* >(mask.data_ptr());
+      }
+   }
+   Attn(const Attn&) = delete;
+};
+
+// (o, lse, o_rest): the last two only for a backward, o_rest only for 2-byte types.
+std::tuple< Tensor, Tensor, Tensor > attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& memory,
+                                               at::IntArrayRef meta, double scale, const Tensor& mask, bool train)
+{
+   const char* op = "cross_attention";
+   c10::cuda::CUDAGuard guard(q.device());
+   const Attn in(q, k, v, memory, meta, scale, mask, op);
+   Tensor o = at::empty(q.sizes(), q.options());
+   Tensor lse, rest;
+   if(train) lse = at::empty({in.a.heads, in.a.q_rows}, q.options().dtype(at::kFloat));
+   if(train && in.a.dtype != RELM_MP_FLOAT32) rest = at::empty(q.sizes(), q.options());
+   const size_t bytes = relm_mp_cross_attention_workspace_bytes(&in.a);
+   const Tensor ws = bytes ? bytes_like(bytes, q) : Tensor();
+   check_rc(relm_mp_cross_attention(&in.a, o.data_ptr(), train ? lse.data_ptr< float >() : nullptr,
+                                    rest.defined() ? rest.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+            op);
+   return {o, lse, rest};
+}
+
+struct CrossAttention : torch::autograd::Function< CrossAttention > {
+   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& plan,
+                         at::IntArrayRef meta, double scale, const OptTensor& key_mask)
+   {
+      const Tensor &memory = or_none(plan), &mask = or_none(key_mask);
+      auto [o, lse, rest] = attention_forward(q, k, v, memory, meta, scale, mask, true);
+      ctx->save_for_backward({q, k, v, o, lse, memory, mask, rest});
+      ctx->saved_data["meta"] = meta.vec();
+      ctx->saved_data["scale"] = scale;
+      return o;
+   }
+   static variable_list backward(AutogradContext* ctx, variable_list grads)
+   {
+      const char* op = "cross_attention_backward";
+      const auto s = ctx->get_saved_variables();
+      const auto meta = ctx->saved_data["meta"].toIntVector();
+      at::AutoDispatchBelowADInplaceOrView below;
+      c10::cuda::CUDAGuard guard(s[0].device());
+      const Attn in(s[0], s[1], s[2], s[5], meta, ctx->saved_data["scale"].toDouble(), s[6], op);
+      const Tensor go = grads[0].contiguous(), o = s[3].contiguous();
+      Tensor dq = at::empty(s[0].sizes(), s[0].options()), dk = at::empty(s[1].sizes(), s[1].options());
+      Tensor dv = at::empty(s[2].sizes(), s[2].options());
+      const size_t bytes = relm_mp_cross_attention_backward_workspace_bytes(&in.a);
+      const Tensor ws = bytes_like(bytes, o);
+      check_rc(relm_mp_cross_attention_backward(&in.a, go.data_ptr(), o.data_ptr(),
+                                                s[7].defined() ? s[7].data_ptr() : nullptr, s[4].data_ptr< float >(),
+                                                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), bytes, stream_of(o)),
+               op);
+      return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+   }
+};
+
+Tensor cross_attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& plan, at::IntArrayRef meta,
+                            double scale, const OptTensor& key_mask)
+{
+   return std::get< 0 >(attention_forward(q, k, v, or_none(plan), meta, scale, or_none(key_mask), false));
+}
+
+Tensor cross_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& plan,
+                                at::IntArrayRef meta, double scale, const OptTensor& key_mask)
+{
+   if(wants_grad({&q, &k, &v})) return CrossAttention::apply(q, k, v, plan, meta, scale, key_mask);
+   at::AutoDispatchBelowADInplaceOrView below;
+   return cross_attention_cuda(q, k, v, plan, meta, scale, key_mask);
+}
+
+Tensor cross_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const OptTensor&, at::IntArrayRef, double,
+                            const OptTensor&)
+{
+   return at::empty(q.sizes(), q.options());
+}
+
+// ---- products with 4-bit weights ---------------------------------------------------
+
+Tensor int4_pack_cuda(const Tensor& codes, const Tensor& scales, const OptTensor& zeros_in)
+{
+   const char* op = "int4_pack";
+   const Tensor& zeros = or_none(zeros_in);
+   TORCH_CHECK(codes.dim() == 2 && codes.scalar_type() == at::kByte, op, ": codes must be uint8 [n, k / 2].");
+   TORCH_CHECK(scales.dim() == 2 && scales.scalar_type() == at::kHalf && scales.size(0) == codes.size(0), op,
+               ": scales must be float16 [n, k / group].");
+   same_device(codes, scales, op, "scales");
+   const int64_t n = codes.size(0), k = codes.size(1) * 2, groups = scales.size(1);
+   TORCH_CHECK(groups > 0 && k % groups == 0, op, ": k = ", k, " is not a multiple of the ", groups, " groups.");
+   if(zeros.defined()) {
+      TORCH_CHECK(zeros.scalar_type() == at::kByte && zeros.sizes() == scales.sizes(), op,
+                  ": zeros must be uint8 [n, k / group].");
+      same_device(codes, zeros, op, "zeros");
+   }
+   c10::cuda::CUDAGuard guard(codes.device());
+   const Tensor c = codes.contiguous(), s = scales.contiguous(), z = zeros.defined() ? zeros.contiguous() : Tensor();
+   const size_t bytes = relm_mp_int4_packed_bytes(n, k, k / groups, z.defined());
+   TORCH_CHECK(bytes > 0, relm_mp_last_error(), " (", op, ")");
+   Tensor packed = bytes_like(bytes, codes);
+   check_rc(relm_mp_int4_pack(c.data_ptr< uint8_t >(), s.data_ptr(), z.defined() ? z.data_ptr< uint8_t >() : nullptr, n, k,
+                              k / groups, packed.data_ptr(), bytes, stream_of(codes)),
+            op);
+   return packed;
+}
+
+Tensor int4_matvec_cuda(const Tensor& x, const Tensor& packed, int64_t n, int64_t k, int64_t group, bool has_zeros,
+                        const OptTensor& x_scale, at::ScalarType out_dtype)
+{
+   const char* op = "int4_matvec";
+   const bool e4m3 = x.scalar_type() == at::kFloat8_e4m3fn;
+   TORCH_CHECK(x.dim() >= 1 && x.size(-1) == k, op, ": x must be [..., ", k, "], got ", x.sizes(), ".");
+   TORCH_CHECK(e4m3 || x.scalar_type() == out_dtype, op, ": the output has x's dtype unless x is float8_e4m3fn.");
+   const relm_mp_dtype dt = dtype_of(out_dtype, op);
+   same_device(x, packed, op, "weight");
+   const size_t bytes = relm_mp_int4_packed_bytes(n, k, group, has_zeros);
+   TORCH_CHECK(bytes > 0 && packed.scalar_type() == at::kByte && packed.is_contiguous() && (size_t)packed.numel() == bytes,
+               op, ": the packed weight does not belong to its sizes.");
+   c10::cuda::CUDAGuard guard(x.device());
+   const Tensor x2 = rows_of(x);
+   Tensor scale;
+   if(x_scale.has_value()) {
+      TORCH_CHECK(x_scale->scalar_type() == at::kFloat && x_scale->sizes() == x.sizes().slice(0, x.dim() - 1), op,
+                  ": x_scale must be float32 with one value per row of x.");
+      same_device(x, *x_scale, op, "x_scale");
+      scale = x_scale->contiguous();
+   }
+   std::vector< int64_t > shape = x.sizes().vec();
+   shape.back() = n;
+   Tensor y = at::empty(shape, x.options().dtype(out_dtype));
+   check_rc(relm_mp_int4_matvec(dt, e4m3, x2.data_ptr(), row_stride(x2), scale.defined() ? scale.data_ptr< float >() : nullptr,
+                                x2.size(0), packed.data_ptr(), n, k, group, has_zeros, y.data_ptr(), stream_of(x)),
+            op);
+   return y;
+}
+
+Tensor int4_matvec_meta(const Tensor& x, const Tensor&, int64_t n, int64_t, int64_t, bool, const OptTensor&,
+                        at::ScalarType out_dtype)
+{
+   std::vector< int64_t > shape = x.sizes().vec();
+   shape.back() = n;
+   return at::empty(shape, x.options().dtype(out_dtype));
+}
+
+}  // namespace
+}  // namespace relm_b200
+
+TORCH_LIBRARY_FRAGMENT(relm_mp_b200, m)
+{
+   m.def("add_rms_norm(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor)");
+   m.def("add_rms_norm_e4m3(Tensor x, Tensor weight, Tensor? residual, float eps) -> (Tensor, Tensor, Tensor)");
+   m.def("attention_plan(int[] q_lengths, int[] kv_lengths, Device device) -> (Tensor, int[])", relm_b200::attention_plan);
+   m.def(
+      "cross_attention(Tensor q, Tensor k, Tensor v, Tensor? plan, int[] plan_sizes, float scale, Tensor? key_mask) -> "
+      "Tensor"
+   );
+   m.def("int4_pack(Tensor codes, Tensor scales, Tensor? zeros) -> Tensor");
+   m.def(
+      "int4_matvec(Tensor x, Tensor packed, int n, int k, int group, bool has_zeros, Tensor? x_scale, ScalarType "
+      "out_dtype) -> Tensor"
+   );
+}
+
+TORCH_LIBRARY_IMPL(relm_mp_b200, CUDA, m)
+{
+   m.impl("add_rms_norm", relm_b200::add_rms_norm_cuda);
+   m.impl("add_rms_norm_e4m3", relm_b200::add_rms_norm_e4m3_cuda);
+   m.impl("cross_attention", relm_b200::cross_attention_cuda);
+   m.impl("int4_pack", relm_b200::int4_pack_cuda);
+   m.impl("int4_matvec", relm_b200::int4_matvec_cuda);
+}
+
+TORCH_LIBRARY_IMPL(relm_mp_b200, AutogradCUDA, m)
+{
+   m.impl("add_rms_norm", relm_b200::add_rms_norm_autograd);
+   m.impl("cross_attention", relm_b200::cross_attention_autograd);
+}
+
+TORCH_LIBRARY_IMPL(relm_mp_b200, Meta, m)
+{
+   m.impl("add_rms_norm", relm_b200::add_rms_norm_meta);
+   m.impl("add_rms_norm_e4m3", relm_b200::add_rms_norm_e4m3_meta);
+   m.impl("cross_attention", relm_b200::cross_attention_meta);
+   m.impl("int4_matvec", relm_b200::int4_matvec_meta);
+}

@@ -1,0 +1,585 @@
+// Root-mean-square norm with the residual's addition, forward (output in the
+// input's type or in e4m3 with a scale per row) and backward.
+//
+//   h = x + r, inv = 1 / sqrt(mean(h^2) + eps), n = h inv, y = w n
+//   dx = dr = inv (w dy - n mean(w dy n)) + dh,  dw = sum over rows of dy n
+//
+// All of it is bound by memory: a row is read once into registers (a group of
+// TPR threads, each NV chunks of VEC elements), reduced by shuffles (and a few
+// words of shared memory when the group is wider than a warp) and written once.
+// Sums and the norm are float32. The norm uses the unrounded float32 sum
+// x + r; h is rounded to the storage type only as it is written, so the
+// backward's n comes from the rounded h and the saved float32 inv.
+#include <cuda_fp8.h>
+
+#include "relm_mp_internal.cuh"
+
+using namespace relm_mp;
+
+namespace {
+
+constexpr float kE4m3Max = 448.f;
+constexpr int kSms = 148;
+
+template < typename T >
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32< float >(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32< __nv_bfloat16 >(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f32< __half >(__half v) { return __half2float(v); }
+template < typename T >
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32< float >(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32< __nv_bfloat16 >(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32< __half >(float v) { return __float2half_rn(v); }
+
+template < typename T, int VEC >
+struct alignas(sizeof(T) * VEC) Pack {
+   T v[VEC];
+};
+
+// Values read once: no line of L1 is kept for them.
+template < typename T, int VEC >
+__device__ __forceinline__ void load_once(const T* p, float* out)
+{
+   Pack< T, VEC > a;
+   if constexpr(sizeof(a) == 16) {
+      const int4 r = __ldcs(reinterpret_cast< const int4* >(p));
+      a = *reinterpret_cast< const Pack< T, VEC >* >(&r);
+   } else {
+      a = *reinterpret_cast< const Pack< T, VEC >* >(p);
+   }
+#pragma unroll
+   for(int i = 0; i < VEC; ++i) out[i] = to_f32(a.v[i]);
+}
+
+template < typename T, int VEC >
+__device__ __forceinline__ void load_kept(const T* p, float* out)
+{
+   const Pack< T, VEC > a = *reinterpret_cast< const Pack< T, VEC >* >(p);
+#pragma unroll
+   for(int i = 0; i < VEC; ++i) out[i] = to_f32(a.v[i]);
+}
+
+template < typename T, int VEC >
+__device__ __forceinline__ void store_vec(T* p, const float* in)
+{
+   Pack< T, VEC > a;
+#pragma unroll
+   for(int i = 0; i < VEC; ++i) a.v[i] = from_f32< T >(in[i]);
+   *reinterpret_cast< Pack< T, VEC >* >(p) = a;
+}
+
+template < int VEC >
+__device__ __forceinline__ void store_e4m3(unsigned char* p, const float* in)
+{
+   if constexpr(VEC == 1) {
+      *p = __nv_cvt_float_to_fp8(in[0], __NV_SATFINITE, __NV_E4M3);
+   } else {
+      Pack< unsigned short, VEC / 2 > a;
+#pragma unroll
+      for(int i = 0; i < VEC / 2; ++i)
+         a.v[i] = __nv_cvt_float2_to_fp8x2(make_float2(in[2 * i], in[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+      *reinterpret_cast< Pack< unsigned short, VEC / 2 >* >(p) = a;
+   }
+}
+
+struct Sum {
+   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+// Unlike fmaxf, keeps a NaN of either side.
+struct MaxNan {
+   __device__ __forceinline__ float operator()(float a, float b) const { return (a > b || a != a) ? a : b; }
+};
+
+// Reduction over the TPR threads of a row; every thread gets the result. Each
+// call of one row has its own `slot` of shared memory, and the slots alternate
+// between rows, so one barrier per call is enough.
+template < int TPR, typename Op >
+__device__ __forceinline__ float reduce_row(float v, float* slot, Op op)
+{
+   constexpr int W = TPR < 32 ? TPR : 32;
+#pragma unroll
+   for(int o = W / 2; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+   if constexpr(TPR > 32) {
+      constexpr int WARPS = TPR / 32;
+      if((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = slot[0];
+#pragma unroll
+      for(int w = 1; w < WARPS; ++w) v = op(v, slot[w]);
+   }
+   return v;
+}
+
+struct FwdArgs {
+   const void *x, *residual, *weight;
+   int64_t x_stride, r_stride, rows;
+   int width;
+   float eps;
+   void *y, *h;
+   float *inv, *scale;
+};
+
+// Threads of a block, and rows that it works on at once.
+template < int TPR >
+constexpr int kBlock = TPR > 32 ? TPR : 256;
+template < int TPR >
+constexpr int kBlockRows = TPR > 32 ? 1 : 256 / TPR;
+
+template < typename T, int VEC, int TPR, int NV, bool E4M3 >
+__global__ void __launch_bounds__(kBlock< TPR >) k_add_rms_norm(FwdArgs a)
+{
+   __shared__ float red[2][2][32];
+   constexpr int ROWS = kBlockRows< TPR >;
+   const int lane = TPR > 32 ? threadIdx.x : threadIdx.x % TPR;
+   const int sub = TPR > 32 ? 0 : threadIdx.x / TPR;
+   const float inv_width = 1.f / (float)a.width;
+   int phase = 0;
+   for(int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.rows; row0 += (int64_t)gridDim.x * ROWS, phase ^= 1) {
+      const int64_t row = row0 + sub;
+      const bool live = row < a.rows;
+      const T* x = static_cast< const T* >(a.x) + row * a.x_stride;
+      const T* r = static_cast< const T* >(a.residual) + row * a.r_stride;
+      float v[NV * VEC];
+      float ss = 0.f;
+#pragma unroll
+      for(int c = 0; c < NV; ++c) {
+         const int col = (c * TPR + lane) * VEC;
+         if(live && col < a.width) {
+            load_once< T, VEC >(x + col, v + c * VEC);
+            if(a.residual) {
+               float t[VEC];
+               load_once< T, VEC >(r + col, t);
+#pragma unroll
+               for(int i = 0; i < VEC; ++i) v[c * VEC + i] += t[i];
+            }
+         } else {
+#pragma unroll
+            for(int i = 0; i < VEC; ++i) v[c * VEC + i] = 0.f;
+         }
+      }
+#pragma unroll
+      for(int i = 0; i < NV * VEC; ++i) ss += v[i] * v[i];
+      ss = reduce_row< TPR >(ss, red[phase][0], Sum());
+      const float inv = rsqrtf(ss * inv_width + a.eps);
+      if(live && a.inv && lane == 0) a.inv[row] = inv;
+      float top = 0.f;
+#pragma unroll
+      for(int c = 0; c < NV; ++c) {
+         const int col = (c * TPR + lane) * VEC;
+         if(!live || col >= a.width) continue;
+         if(a.h) store_vec< T, VEC >(static_cast< T* >(a.h) + row * a.width + col, v + c * VEC);
+         float w[VEC];
+         load_kept< T, VEC >(static_cast< const T* >(a.weight) + col, w);
+#pragma unroll
+         for(int i = 0; i < VEC; ++i) v[c * VEC + i] = v[c * VEC + i] * inv * w[i];
+         if constexpr(!E4M3) {
+            store_vec< T, VEC >(static_cast< T* >(a.y) + row * a.width + col, v + c * VEC);
+         } else {
+#pragma unroll
+            for(int i = 0; i < VEC; ++i) top = MaxNan()(top, fabsf(v[c * VEC + i]));
+         }
+      }
+      if constexpr(E4M3) {
+         top = reduce_row< TPR >(top, red[phase][1], MaxNan());
+         const float scale = top == 0.f ? 1.f : top / kE4m3Max;
+         if(live && lane == 0) a.scale[row] = scale;
+#pragma unroll
+         for(int c = 0; c < NV; ++c) {
+            const int col = (c * TPR + lane) * VEC;
+            if(!live || col >= a.width) continue;
+#pragma unroll
+            for(int i = 0; i < VEC; ++i) v[c * VEC + i] = __fdiv_rn(v[c * VEC + i], scale);
+            store_e4m3< VEC >(static_cast< unsigned char* >(a.y) + row * a.width + col, v + c * VEC);
+         }
+      }
+   }
+}
+
+// Rows too wide for the registers of one block: a block per row, the row read
+// again (from L2) for each pass.
+template < typename T, bool E4M3 >
+__global__ void __launch_bounds__(1024) k_add_rms_norm_long(FwdArgs a)
+{
+   __shared__ float red[2][2][32];
+   int phase = 0;
+   for(int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, phase ^= 1) {
+      const T* x = static_cast< const T* >(a.x) + row * a.x_stride;
+      const T* r = static_cast< const T* >(a.residual) + row * a.r_stride;
+      const T* w = static_cast< const T* >(a.weight);
+      auto sum = [&](int c) { return to_f32(x[c]) + (a.residual ? to_f32(r[c]) : 0.f); };
+      float ss = 0.f;
+      for(int c = threadIdx.x; c < a.width; c += 1024) {
+         const float v = sum(c);
+         ss += v * v;
+      }
+      ss = reduce_row< 1024 >(ss, red[phase][0], Sum());
+      const float inv = rsqrtf(ss / (float)a.width + a.eps);
+      if(a.inv && threadIdx.x == 0) a.inv[row] = inv;
+      float scale = 1.f;
+      if constexpr(E4M3) {
+         float top = 0.f;
+         for(int c = threadIdx.x; c < a.width; c += 1024) top = MaxNan()(top, fabsf(sum(c) * inv * to_f32(w[c])));
+         top = reduce_row< 1024 >(top, red[phase][1], MaxNan());
+         scale = top == 0.f ? 1.f : top / kE4m3Max;
+         if(threadIdx.x == 0) a.scale[row] = scale;
+      }
+      for(int c = threadIdx.x; c < a.width; c += 1024) {
+         const float v = sum(c), y = v * inv * to_f32(w[c]);
+         if(a.h) static_cast< T* >(a.h)[row * a.width + c] = from_f32< T >(v);
+         if constexpr(E4M3)
+            static_cast< unsigned char* >(a.y)[row * a.width + c] =
+               __nv_cvt_float_to_fp8(__fdiv_rn(y, scale), __NV_SATFINITE, __NV_E4M3);
+         else
+            static_cast< T* >(a.y)[row * a.width + c] = from_f32< T >(y);
+      }
+   }
+}
+
+struct BwdArgs {
+   const void *dy, *dh, *h, *weight;
+   int64_t dy_stride, dh_stride, h_stride, rows;
+   const float* inv;
+   int width;
+   void* dx;
+   float* partial; // [gridDim.x, width], or NULL
+};
+
+// One row per group as in the forward; the weight's gradient is summed in
+// registers over the rows of a group, then over the groups of the block, and
+// written as one partial row per block (summed by k_sum_partials).
+template < typename T, int VEC, int TPR, int NV >
+__global__ void __launch_bounds__(kBlock< TPR >) k_add_rms_norm_bwd(BwdArgs a)
+{
+   __shared__ float red[2][32];
+   constexpr int ROWS = kBlockRows< TPR >;
+   const int lane = TPR > 32 ? threadIdx.x : threadIdx.x % TPR;
+   const int sub = TPR > 32 ? 0 : threadIdx.x / TPR;
+   const float inv_width = 1.f / (float)a.width;
+   float dw[NV * VEC];
+#pragma unroll
+   for(int i = 0; i < NV * VEC; ++i) dw[i] = 0.f;
+   int phase = 0;
+   for(int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < a.rows; row0 += (int64_t)gridDim.x * ROWS, phase ^= 1) {
+      const int64_t row = row0 + sub;
+      const bool live = row < a.rows;
+      const float inv = live ? a.inv[row] : 0.f;
+      float n[NV * VEC], g[NV * VEC];
+      float dot = 0.f;
+#pragma unroll
+      for(int c = 0; c < NV; ++c) {
+         const int col = (c * TPR + lane) * VEC;
+         if(live && col < a.width) {
+            load_once< T, VEC >(static_cast< const T* >(a.h) + row * a.h_stride + col, n + c * VEC);
+            if(a.dy) {
+               load_once< T, VEC >(static_cast< const T* >(a.dy) + row * a.dy_stride + col, g + c * VEC);
+            } else {
+#pragma unroll
+               for(int i = 0; i < VEC; ++i) g[c * VEC + i] = 0.f;
+            }
+         } else {
+#pragma unroll
+            for(int i = 0; i < VEC; ++i) n[c * VEC + i] = g[c * VEC + i] = 0.f;
+         }
+      }
+#pragma unroll
+      for(int c = 0; c < NV; ++c) {
+         const int col = (c * TPR + lane) * VEC;
+         float w[VEC];
+         if(col < a.width) {
+            load_kept< T, VEC >(static_cast< const T* >(a.weight) + col, w);
+         } else {
+#pragma unroll
+            for(int i = 0; i < VEC; ++i) w[i] = 0.f;
+         }
+#pragma unroll
+         for(int i = 0; i < VEC; ++i) {
+            const int k = c * VEC + i;
+            n[k] *= inv;
+            dw[k] += g[k] * n[k];
+            g[k] *= w[i];
+            dot += g[k] * n[k];
+         }
+      }
+      dot = reduce_row< TPR >(dot, red[phase], Sum()) * inv_width;
+#pragma unroll
+      for(int c = 0; c < NV; ++c) {
+         const int col = (c * TPR + lane) * VEC;
+         if(!live || col >= a.width) continue;
+         float o[VEC];
+         if(a.dh) {
+            load_once< T, VEC >(static_cast< const T* >(a.dh) + row * a.dh_stride + col, o);
+         } else {
+#pragma unroll
+            for(int i = 0; i < VEC; ++i) o[i] = 0.f;
+         }
+#pragma unroll
+         for(int i = 0; i < VEC; ++i) o[i] += inv * (g[c * VEC + i] - n[c * VEC + i] * dot);
+         store_vec< T, VEC >(static_cast< T* >(a.dx) + row * a.width + col, o);
+      }
+   }
+   if(!a.partial) return;
+   float* out = a.partial + (int64_t)blockIdx.x * a.width;
+   if constexpr(TPR > 32) {
+#pragma unroll
+      for(int c = 0; c < NV; ++c) {
+         const int col = (c * TPR + lane) * VEC;
+         if(col < a.width) store_vec< float, VEC <= 4 ? VEC : 4 >(out + col, dw + c * VEC);
+         if constexpr(VEC > 4)
+            if(col < a.width) store_vec< float, 4 >(out + col + 4, dw + c * VEC + 4);
+      }
+   } else {
+      __shared__ float part[256 * NV * VEC];
+      const int padded = TPR * NV * VEC;
+#pragma unroll
+      for(int c = 0; c < NV; ++c)
+#pragma unroll
+         for(int i = 0; i < VEC; ++i) part[sub * padded + (c * TPR + lane) * VEC + i] = dw[c * VEC + i];
+      __syncthreads();
+      for(int col = threadIdx.x; col < a.width; col += 256) {
+         float s = 0.f;
+         for(int g = 0; g < ROWS; ++g) s += part[g * padded + col];
+         out[col] = s;
+      }
+   }
+}
+
+template < typename T >
+__global__ void __launch_bounds__(1024) k_add_rms_norm_bwd_long(BwdArgs a)
+{
+   __shared__ float red[2][32];
+   int phase = 0;
+   const T* w = static_cast< const T* >(a.weight);
+   float* out = a.partial ? a.partial + (int64_t)blockIdx.x * a.width : nullptr;
+   if(out)
+      for(int c = threadIdx.x; c < a.width; c += 1024) out[c] = 0.f;
+   for(int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, phase ^= 1) {
+      const T* h = static_cast< const T* >(a.h) + row * a.h_stride;
+      const T* dy = static_cast< const T* >(a.dy) + row * a.dy_stride;
+      const T* dh = static_cast< const T* >(a.dh) + row * a.dh_stride;
+      const float inv = a.inv[row];
+      float dot = 0.f;
+      for(int c = threadIdx.x; c < a.width; c += 1024) {
+         const float n = to_f32(h[c]) * inv, g = a.dy ? to_f32(dy[c]) : 0.f;
+         if(out) out[c] += g * n;
+         dot += g * to_f32(w[c]) * n;
+      }
+      dot = reduce_row< 1024 >(dot, red[phase], Sum()) / (float)a.width;
+      for(int c = threadIdx.x; c < a.width; c += 1024) {
+         const float n = to_f32(h[c]) * inv, g = a.dy ? to_f32(dy[c]) * to_f32(w[c]) : 0.f;
+         static_cast< T* >(a.dx)[row * a.width + c] = from_f32< T >(inv * (g - n * dot) + (a.dh ? to_f32(dh[c]) : 0.f));
+      }
+   }
+}
+
+// dweight[c] = sum over the blocks' partial rows, in a fixed order: 32 columns
+// by 32 row lanes per block, then a tree over the lanes.
+template < typename T >
+__global__ void __launch_bounds__(1024) k_sum_partials(const float* __restrict__ partial, int count, int width,
+                                                       T* __restrict__ out)
+{
+   __shared__ float s[32][33];
+   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+   const int col = blockIdx.x * 32 + x;
+   float v = 0.f;
+   if(col < width)
+      for(int r = y; r < count; r += 32) v += partial[(int64_t)r * width + col];
+   s[y][x] = v;
+   __syncthreads();
+   v = s[x][y];
+#pragma unroll
+   for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+   if(x == 0 && blockIdx.x * 32 + y < width) out[blockIdx.x * 32 + y] = from_f32< T >(v);
+}
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast< uintptr_t >(p) & (a - 1)) == 0; }
+
+int64_t grid_cap(int threads) { return (int64_t)kSms * (2048 / threads) * 4; }
+
+// Threads and chunks of a row from its number of chunks. Call as
+// f(integral_constant TPR, integral_constant NV); false if no group is wide enough.
+template < int VEC, typename F >
+bool with_shape(int64_t chunks, F&& f)
+{
+   using std::integral_constant;
+#define RELM_SHAPE(t, n)                                                       \
+   if(chunks <= (int64_t)t * n) {                                              \
+      f(integral_constant< int, t >(), integral_constant< int, n >());         \
+      return true;                                                             \
+   }
+   RELM_SHAPE(8, 1)
+   RELM_SHAPE(16, 1)
+   RELM_SHAPE(32, 1)
+   RELM_SHAPE(32, 2)
+   RELM_SHAPE(32, 4)
+   RELM_SHAPE(128, 2)
+   RELM_SHAPE(256, 2)
+   RELM_SHAPE(256, 4)
+   RELM_SHAPE(512, 4)
+   if constexpr(VEC <= 4) RELM_SHAPE(1024, 4)
+   if constexpr(VEC <= 2) RELM_SHAPE(1024, 8)
+#undef RELM_SHAPE
+   return false;
+}
+
+template < typename T, int VEC, bool E4M3 >
+int launch_forward(const FwdArgs& a, cudaStream_t st)
+{
+   const int64_t chunks = (a.width + VEC - 1) / VEC;
+   const bool done = with_shape< VEC >(chunks, [&](auto tpr, auto nv) {
+      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+      const int64_t blocks = (a.rows + kBlockRows< TPR > - 1) / kBlockRows< TPR >;
+      const int64_t cap = grid_cap(kBlock< TPR >);
+      k_add_rms_norm< T, VEC, TPR, NV, E4M3 >
+         <<< (unsigned)(blocks < cap ? blocks : cap), kBlock< TPR >, 0, st >>>(a);
+   });
+   if(!done) k_add_rms_norm_long< T, E4M3 ><<< (unsigned)(a.rows < 592 ? a.rows : 592), 1024, 0, st >>>(a);
+   return check_launch("k_add_rms_norm");
+}
+
+// Chunks of 16 bytes where every row starts on a 16-byte boundary, else of 4
+// bytes (2-byte types), else single elements.
+template < typename T, bool E4M3 >
+int forward_by_alignment(const FwdArgs& a, cudaStream_t st)
+{
+   auto fits = [&](int vec) {
+      const size_t b = vec * sizeof(T);
+      return a.width % vec == 0 && a.x_stride % vec == 0 && (!a.residual || a.r_stride % vec == 0) &&
+             aligned(a.x, b) && aligned(a.residual, b) && aligned(a.weight, b) && aligned(a.h, b) &&
+             aligned(a.y, E4M3 ? vec : b);
+   };
+   constexpr int FULL = 16 / sizeof(T);
+   if(fits(FULL)) return launch_forward< T, FULL, E4M3 >(a, st);
+   if constexpr(sizeof(T) == 2)
+      if(fits(2)) return launch_forward< T, 2, E4M3 >(a, st);
+   return launch_forward< T, 1, E4M3 >(a, st);
+}
+
+int check_norm(relm_mp_dtype dtype, int64_t rows, int64_t width, const char* op)
+{
+   if(dtype != RELM_MP_FLOAT32 && dtype != RELM_MP_BFLOAT16 && dtype != RELM_MP_FLOAT16)
+      return fail(RELM_MP_ERR_UNSUPPORTED, std::string(op) + ": unsupported dtype (float32, bfloat16, float16).");
+   if(rows < 0) return fail(RELM_MP_ERR_INVALID_ARGUMENT, std::string(op) + ": rows must be >= 0.");
+   if(width < 1 || width > (1 << 24))
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, std::string(op) + ": width must be in [1, 2^24].");
+   return RELM_MP_OK;
+}
+
+template < bool E4M3 >
+int forward_by_type(relm_mp_dtype dtype, const FwdArgs& a, cudaStream_t st)
+{
+   switch(dtype) {
+      case RELM_MP_FLOAT32: return forward_by_alignment< float, E4M3 >(a, st);
+      case RELM_MP_BFLOAT16: return forward_by_alignment< __nv_bfloat16, E4M3 >(a, st);
+      default: return forward_by_alignment< __half, E4M3 >(a, st);
+   }
+}
+
+// Blocks of the backward: enough for the device to be full (each block keeps
+// its own partial row of the weight's gradient, so no more than that).
+template < int TPR >
+int64_t backward_blocks(int64_t rows)
+{
+   const int64_t blocks = (rows + kBlockRows< TPR > - 1) / kBlockRows< TPR >;
+   const int64_t cap = (int64_t)kSms * (kBlock< TPR > >= 1024 ? 1 : kBlock< TPR > == 512 ? 2 : 4);
+   return blocks < cap ? blocks : cap;
+}
+constexpr int64_t kMaxPartials = kSms * 4;
+
+template < typename T, int VEC >
+int64_t launch_backward(const BwdArgs& a, cudaStream_t st)
+{
+   const int64_t chunks = (a.width + VEC - 1) / VEC;
+   int64_t grid = 0;
+   const bool done = with_shape< VEC >(chunks, [&](auto tpr, auto nv) {
+      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+      grid = backward_blocks< TPR >(a.rows);
+      k_add_rms_norm_bwd< T, VEC, TPR, NV ><<< (unsigned)grid, kBlock< TPR >, 0, st >>>(a);
+   });
+   if(!done) {
+      grid = a.rows < kSms ? a.rows : kSms;
+      k_add_rms_norm_bwd_long< T ><<< (unsigned)grid, 1024, 0, st >>>(a);
+   }
+   return grid;
+}
+
+template < typename T >
+int backward(const BwdArgs& a, void* dweight, cudaStream_t st)
+{
+   auto fits = [&](int vec) {
+      const size_t b = vec * sizeof(T);
+      return a.width % vec == 0 && a.h_stride % vec == 0 && (!a.dy || a.dy_stride % vec == 0) &&
+             (!a.dh || a.dh_stride % vec == 0) && aligned(a.dy, b) && aligned(a.dh, b) && aligned(a.h, b) &&
+             aligned(a.weight, b) && aligned(a.dx, b);
+   };
+   constexpr int FULL = 16 / sizeof(T);
+   int64_t grid;
+   if(fits(FULL)) grid = launch_backward< T, FULL >(a, st);
+   else if(sizeof(T) == 2 && fits(2)) grid = launch_backward< T, 2 >(a, st);
+   else grid = launch_backward< T, 1 >(a, st);
+   int rc = check_launch("k_add_rms_norm_bwd");
+   if(rc || !dweight) return rc;
+   k_sum_partials< T ><<< (a.width + 31) / 32, 1024, 0, st >>>(a.partial, (int)grid, a.width, static_cast< T* >(dweight));
+   return check_launch("k_sum_partials");
+}
+
+}  // namespace
+
+int relm_mp_add_rms_norm(relm_mp_dtype dtype, const void* x, int64_t x_stride, const void* residual,
+                         int64_t residual_stride, const void* weight, int64_t rows, int64_t width, float eps, void* y,
+                         void* h, float* inv_rms, void* stream)
+{
+   int rc;
+   if((rc = check_norm(dtype, rows, width, "add_rms_norm"))) return rc;
+   if(rows == 0) return RELM_MP_OK;
+   if(!x || !weight || !y) return fail(RELM_MP_ERR_INVALID_ARGUMENT, "add_rms_norm: pointers must not be NULL.");
+   const FwdArgs a{x, residual, weight, x_stride, residual_stride, rows, (int)width, eps, y, h, inv_rms, nullptr};
+   return forward_by_type< false >(dtype, a, static_cast< cudaStream_t >(stream));
+}
+
+int relm_mp_add_rms_norm_e4m3(relm_mp_dtype dtype, const void* x, int64_t x_stride, const void* residual,
+                              int64_t residual_stride, const void* weight, int64_t rows, int64_t width, float eps,
+                              unsigned char* q, float* scale, void* h, void* stream)
+{
+   int rc;
+   if((rc = check_norm(dtype, rows, width, "add_rms_norm_e4m3"))) return rc;
+   if(rows == 0) return RELM_MP_OK;
+   if(!x || !weight || !q || !scale)
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, "add_rms_norm_e4m3: pointers must not be NULL.");
+   const FwdArgs a{x, residual, weight, x_stride, residual_stride, rows, (int)width, eps, q, h, nullptr, scale};
+   return forward_by_type< true >(dtype, a, static_cast< cudaStream_t >(stream));
+}
+
+size_t relm_mp_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width)
+{
+   if(rows < 0 || width < 1) return 0;
+   return align_up((size_t)(rows < kMaxPartials ? rows : kMaxPartials) * (size_t)width * sizeof(float));
+}
+
+int relm_mp_add_rms_norm_backward(relm_mp_dtype dtype, const void* dy, int64_t dy_stride, const void* dh,
+                                  int64_t dh_stride, const void* h, int64_t h_stride, const float* inv_rms,
+                                  const void* weight, int64_t rows, int64_t width, void* dx, void* dweight,
+                                  void* workspace, size_t workspace_bytes, void* stream)
+{
+   int rc;
+   if((rc = check_norm(dtype, rows, width, "add_rms_norm_backward"))) return rc;
+   cudaStream_t st = static_cast< cudaStream_t >(stream);
+   if(rows == 0) return dweight ? check_cuda(cudaMemsetAsync(dweight, 0, width * dtype_size(dtype), st), "memset") : RELM_MP_OK;
+   if(!h || !inv_rms || !weight || !dx)
+      return fail(RELM_MP_ERR_INVALID_ARGUMENT, "add_rms_norm_backward: pointers must not be NULL.");
+   if(dweight && (!workspace || workspace_bytes < relm_mp_add_rms_norm_backward_workspace_bytes(rows, width)))
+      return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "add_rms_norm_backward: workspace too small.");
+   const BwdArgs a{dy, dh, h, weight, dy_stride, dh_stride, h_stride, rows, inv_rms, (int)width, dx,
+                   dweight ? static_cast< float* >(workspace) : nullptr};
+   switch(dtype) {
+      case RELM_MP_FLOAT32: return backward< float >(a, dweight, st);
+      case RELM_MP_BFLOAT16: return backward< __nv_bfloat16 >(a, dweight, st);
+      default: return backward< __half >(a, dweight, st);
+   }
+}

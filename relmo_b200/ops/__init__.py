@@ -1,5 +1,5 @@
 """Operator wrappers (mirrors ``relmo.ops``)."""
 
-from . import mp
+from . import decoder, mp
 
-__all__ = ["mp"]
+__all__ = ["decoder", "mp"]

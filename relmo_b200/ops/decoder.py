@@ -1,0 +1,302 @@
+"""Decoder operators over a relational model's object embeddings.
+
+What a decoder that reads the embeddings of a batch of states needs beside the
+fan-out / fan-in ops (none of these is in relmo):
+
+- :func:`add_rms_norm`, :func:`add_rms_norm_e4m3` - root-mean-square norm with
+  the residual's addition; trained, or served with an 8-bit output and a scale
+  per row.
+- :func:`cross_attention` with :func:`attention_plan` - queries of each state
+  (candidate actions, tokens) attend to that state's objects. Both sides are
+  ragged and packed the way a batch's objects are; trained, and served for one
+  or a few queries per state.
+- :class:`Int4Weight`, :func:`quantize_int4`, :func:`int4_matvec` - products of
+  a few rows with 4-bit weights and group scales, for the served projections;
+  they take :func:`add_rms_norm_e4m3`'s rows as they are.
+
+CUDA tensors (float32, bfloat16, float16) always run the B200 kernels
+(``torch.ops.relm_mp_b200``): as in ``relmo_b200.ops.mp`` there is no GPU
+fallback, and a missing or disabled library raises. CPU tensors run the formulas
+below, in float32 or wider.
+"""
+
+from __future__ import annotations
+
+import math
+import os
+from dataclasses import dataclass, field
+
+from .mp_dispatch import CUSTOM, route
+from .mp_runtime import _OFF_WORDS, require_torch, torch
+
+E4M3_MAX = 448.0
+
+_loaded = False
+
+
+def _on_cuda(op_name: str, tensor) -> bool:
+    """Whether ``tensor``'s call runs the kernels; raises where it should but cannot."""
+
+    global _loaded
+    if not tensor.is_cuda:
+        return False
+    if not _loaded or os.environ.get("RELM_MP_ENABLE", "1").strip().lower() in _OFF_WORDS:
+        _loaded = route(op_name, tensor) == CUSTOM
+    return True
+
+
+# ---- add + RMS norm ----------------------------------------------------------------
+
+
+def _wide(x):
+    return x if x.dtype == torch.float64 else x.float()
+
+
+def _norm_parts(x, weight, residual, eps, op_name):
+    if weight.dim() != 1 or x.dim() < 1 or weight.size(0) != x.size(-1):
+        raise RuntimeError(f"{op_name}: weight must be [{x.size(-1) if x.dim() else 0}], got {tuple(weight.shape)}.")
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError(f"{op_name}: residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}.")
+    h = _wide(x) if residual is None else _wide(x) + _wide(residual)
+    y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + eps) * _wide(weight)
+    return y, h
+
+
+def add_rms_norm(x, weight, residual=None, *, eps: float = 1e-6):
+    """``h = x + residual``, ``y = h / sqrt(mean(h^2) + eps) * weight`` over the
+    last dimension. Returns ``(y, h)``; ``h`` is ``x`` itself without a residual.
+
+    Sums, the norm and both gradients are float32 (the norm is that of the sum
+    before it is rounded to ``x``'s dtype). Differentiable in x, weight and
+    residual; weight and residual share x's dtype."""
+
+    require_torch("add_rms_norm")
+    if _on_cuda("add_rms_norm", x):
+        y, h = torch.ops.relm_mp_b200.add_rms_norm(x, weight, residual, eps)
+        return y, (x if residual is None else h)
+    y, h = _norm_parts(x, weight, residual, eps, "add_rms_norm")
+    return y.to(x.dtype), (x if residual is None else h.to(x.dtype))
+
+
+def add_rms_norm_e4m3(x, weight, residual=None, *, eps: float = 1e-6):
+    """:func:`add_rms_norm` with ``y`` in 8 bits: ``(q, scale, h)`` with ``q``
+    float8_e4m3fn, ``scale`` float32 of one value per row (``max|y| / 448``, 1 for
+    a row of zeros), ``y = q * scale``. For inference: no gradient."""
+
+    require_torch("add_rms_norm_e4m3")
+    if _on_cuda("add_rms_norm_e4m3", x):
+        with torch.no_grad():
+            q, scale, h = torch.ops.relm_mp_b200.add_rms_norm_e4m3(x, weight, residual, eps)
+        return q, scale, (x if residual is None else h)
+    with torch.no_grad():
+        y, h = _norm_parts(x, weight, residual, eps, "add_rms_norm_e4m3")
+        y = y.float()
+        scale = y.abs().amax(-1) / E4M3_MAX
+        scale = torch.where(scale == 0, torch.ones_like(scale), scale)
+        q = (y / scale.unsqueeze(-1)).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    return q, scale, (x if residual is None else h.to(x.dtype))
+
+
+# ---- cross attention ---------------------------------------------------------------
+
+
+@dataclass(frozen=True)
+class AttentionPlan:
+    """The lengths of a batch of packed sequences, laid out for the device by
+    :func:`attention_plan`. Like a routing it is made once per batch and serves
+    every layer, forward and backward."""
+
+    q_lengths: tuple[int, ...] = field(repr=False)
+    kv_lengths: tuple[int, ...] = field(repr=False)
+    memory: object = field(repr=False)  # device memory, None on the CPU
+    sizes: list[int] = field(default_factory=list)
+
+
+def attention_plan(q_lengths, kv_lengths, device="cuda") -> AttentionPlan:
+    """Plan of ``len(q_lengths)`` sequences: sequence ``b`` owns the next
+    ``q_lengths[b]`` rows of q and the next ``kv_lengths[b]`` rows of k and v.
+    Either may be 0. Lengths are host values (sequences of ints, or integer
+    tensors, which are read back)."""
+
+    require_torch("attention_plan")
+    ql, kl = (x.tolist() if hasattr(x, "tolist") else [int(v) for v in x] for x in (q_lengths, kv_lengths))
+    if len(ql) != len(kl):
+        raise RuntimeError(
+            f"attention_plan: q_lengths and kv_lengths must have one length each per sequence, got {len(ql)} and {len(kl)}."
+        )
+    device = torch.device(device)
+    if device.type != "cuda":
+        if any(n < 0 for n in ql + kl):
+            raise RuntimeError("attention_plan: lengths must be >= 0.")
+        return AttentionPlan(tuple(ql), tuple(kl), None)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    route("attention_plan", torch.empty(0, device=device))
+    memory, sizes = torch.ops.relm_mp_b200.attention_plan(ql, kl, device)
+    return AttentionPlan(tuple(ql), tuple(kl), memory, sizes)
+
+
+def cross_attention(q, k, v, plan: AttentionPlan | None = None, *, scale: float | None = None, key_mask=None):
+    """Softmax attention of queries to the states of their own sequence.
+
+    With a plan, q is ``[query rows, heads, dim]`` and k, v are ``[key rows,
+    kv_heads, dim]``, sequences one after another; without one they are dense
+    batches ``[batch, length, heads, dim]`` (the two lengths are independent).
+    ``heads`` is a multiple of ``kv_heads`` and query head i reads key/value head
+    ``i // (heads // kv_heads)``. dim is at most 256; ``scale`` (> 0) defaults to
+    ``dim ** -0.5``. ``key_mask`` is bool with one value per key row (``[key
+    rows]`` or ``[batch, key length]``), True where the key takes part; what
+    masked rows hold is never used.
+
+    Rows may be strided (the last dimension is copied if it is not dense). A
+    query without a key to attend to (none, or all masked) gives 0 and has no
+    gradient. Returns q's shape and dtype; differentiable in q, k and v, with
+    the same bits on every run."""
+
+    require_torch("cross_attention")
+    if scale is None:
+        scale = q.size(-1) ** -0.5
+    if _on_cuda("cross_attention", q):
+        if plan is None:
+            return torch.ops.relm_mp_b200.cross_attention(q, k, v, None, [], scale, key_mask)
+        if plan.memory is None:
+            raise RuntimeError("cross_attention: the plan was made for the CPU.")
+        return torch.ops.relm_mp_b200.cross_attention(q, k, v, plan.memory, plan.sizes, scale, key_mask)
+    return _cross_attention_formula(q, k, v, plan, scale, key_mask)
+
+
+def _attend(q, k, v, scale, keep):
+    """One sequence: q [t, heads, dim], k and v [s, kv_heads, dim], keep [s] or None."""
+
+    if keep is not None:
+        k, v = k[keep], v[keep]
+    if k.size(0) == 0:
+        return q * 0
+    group = q.size(1) // k.size(1)
+    k, v = k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)
+    p = torch.softmax(torch.einsum("thd,shd->hts", q, k) * scale, -1)
+    return torch.einsum("hts,shd->thd", p, v)
+
+
+def _cross_attention_formula(q, k, v, plan, scale, key_mask):
+    rank = 4 if plan is None else 3
+    if q.dim() != rank or k.dim() != rank or k.shape != v.shape or q.size(-1) != k.size(-1):
+        raise RuntimeError("cross_attention: q, k and v must be [rows, heads, dim] with a plan, [batch, length, heads, "
+                           "dim] without one; k and v alike.")
+    if q.size(-2) % k.size(-2):
+        raise RuntimeError("cross_attention: heads must be a positive multiple of kv_heads, at most 65535.")
+    if not (scale > 0 and math.isfinite(scale)):
+        raise RuntimeError("cross_attention: scale must be positive and finite.")
+    if key_mask is not None and (key_mask.dtype != torch.bool or key_mask.shape != k.shape[: rank - 2]):
+        raise RuntimeError("cross_attention: key_mask must be bool with one value per key row.")
+    wide = (_wide(q), _wide(k), _wide(v))
+    if plan is None:
+        parts = [(wide[0][b], wide[1][b], wide[2][b], None if key_mask is None else key_mask[b]) for b in range(q.size(0))]
+        out = torch.stack([_attend(*p[:3], scale, p[3]) for p in parts]) if parts else wide[0]
+        return out.to(q.dtype)
+    if q.size(0) != sum(plan.q_lengths) or k.size(0) != sum(plan.kv_lengths):
+        raise RuntimeError(f"cross_attention: the plan is for {sum(plan.q_lengths)} query and {sum(plan.kv_lengths)} key "
+                           f"rows, got {q.size(0)} and {k.size(0)}.")
+    qs, ks, vs = wide[0].split(plan.q_lengths), wide[1].split(plan.kv_lengths), wide[2].split(plan.kv_lengths)
+    ms = [None] * len(qs) if key_mask is None else key_mask.split(plan.kv_lengths)
+    out = torch.cat([_attend(a, b, c, scale, m) for a, b, c, m in zip(qs, ks, vs, ms)]) if qs else wide[0]
+    return out.to(q.dtype)
+
+
+# ---- products with 4-bit weights ---------------------------------------------------
+
+
+class Int4Weight:
+    """A weight ``[n, k]`` in 4 bits: ``w = (code - zero) * scale`` with a scale
+    (and zero point) per ``group`` consecutive columns of a row.
+
+    ``codes`` is uint8 ``[n, k / 2]`` (the even column in the low half of a
+    byte), ``scales`` float16 ``[n, k / group]``, ``zeros`` uint8 ``[n, k /
+    group]`` or None (8 everywhere); group is 32, 64 or 128. On a CUDA device the
+    codes are laid out for the kernel once, here."""
+
+    def __init__(self, codes, scales, zeros=None):
+        require_torch("Int4Weight")
+        if codes.dim() != 2 or codes.dtype != torch.uint8:
+            raise RuntimeError("int4_pack: codes must be uint8 [n, k / 2].")
+        self.n, self.k = int(codes.size(0)), 2 * int(codes.size(1))
+        if scales.dim() != 2 or scales.dtype != torch.float16 or scales.size(0) != self.n:
+            raise RuntimeError("int4_pack: scales must be float16 [n, k / group].")
+        groups = max(int(scales.size(1)), 1)
+        self.group = self.k // groups
+        if self.group not in (32, 64, 128) or self.k != self.group * groups:
+            raise RuntimeError(f"int4_pack: group must be 32, 64 or 128, got k = {self.k} in {scales.size(1)} groups.")
+        if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+            raise RuntimeError("int4_pack: zeros must be uint8 [n, k / group].")
+        self.has_zeros = zeros is not None
+        self.packed = self._plain = None
+        if _on_cuda("int4_pack", codes):
+            self.packed = torch.ops.relm_mp_b200.int4_pack(codes, scales, zeros)
+        else:
+            self._plain = (codes, scales, zeros)
+
+    def dequantized(self):
+        """The float32 weight of a handle on the CPU."""
+
+        if self._plain is None:
+            raise RuntimeError("Int4Weight: only handles on the CPU keep their codes.")
+        codes, scales, zeros = self._plain
+        c = torch.stack((codes & 15, codes >> 4), dim=-1).view(self.n, -1, self.group).float()
+        c = c - (8.0 if zeros is None else zeros.float().unsqueeze(-1))
+        return (c * scales.float().unsqueeze(-1)).view(self.n, self.k)
+
+
+def quantize_int4(weight, group: int = 128, *, symmetric: bool = True) -> Int4Weight:
+    """Round ``weight`` ``[n, k]`` to 4 bits, nearest code: symmetric groups use
+    codes -7 .. 7 of ``max|w| / 7``, asymmetric ones the 16 codes of the group's
+    range (which always includes 0) with a zero point."""
+
+    require_torch("quantize_int4")
+    if weight.dim() != 2 or group not in (32, 64, 128) or weight.size(1) % group:
+        raise RuntimeError("quantize_int4: weight must be [n, k] with k a multiple of group (32, 64 or 128).")
+    w = weight.detach().float().view(weight.size(0), -1, group)
+    if symmetric:
+        scale = (w.abs().amax(-1) / 7).half()
+        zeros = None
+        zero = 8.0
+    else:
+        lo, hi = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
+        scale = ((hi - lo) / 15).half()
+    s = scale.float()
+    s = torch.where(s == 0, torch.ones_like(s), s).unsqueeze(-1)
+    if not symmetric:
+        zeros = (-lo.unsqueeze(-1) / s).round().clamp(0, 15)
+        zero, zeros = zeros, zeros.squeeze(-1).to(torch.uint8)
+    codes = ((w / s).round() + zero).clamp(0, 15).to(torch.uint8).view(weight.size(0), -1)
+    return Int4Weight((codes[:, 0::2] | codes[:, 1::2] << 4).contiguous(), scale, zeros)
+
+
+def int4_matvec(x, weight: Int4Weight, *, x_scale=None, out_dtype=None):
+    """``x @ w.T`` for a few rows ``[..., k]`` and a 4-bit weight: ``[..., n]``.
+
+    ``x`` is float32, bfloat16 or float16 (the output has its dtype), or
+    float8_e4m3fn with ``x_scale`` float32 of one value per row, as
+    :func:`add_rms_norm_e4m3` gives them (the output has ``out_dtype``, default
+    bfloat16). x enters the products exactly and sums are float32. For inference:
+    no gradient."""
+
+    require_torch("int4_matvec")
+    low = x.dtype == torch.float8_e4m3fn
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if low else x.dtype
+    if _on_cuda("int4_matvec", x):
+        if weight.packed is None:
+            raise RuntimeError("int4_matvec: the weight is on the CPU.")
+        with torch.no_grad():
+            return torch.ops.relm_mp_b200.int4_matvec(
+                x, weight.packed, weight.n, weight.k, weight.group, weight.has_zeros, x_scale, out_dtype
+            )
+    if x.size(-1) != weight.k:
+        raise RuntimeError(f"int4_matvec: x must be [..., {weight.k}], got {tuple(x.shape)}.")
+    if not low and out_dtype != x.dtype:
+        raise RuntimeError("int4_matvec: the output has x's dtype unless x is float8_e4m3fn.")
+    with torch.no_grad():
+        y = x.float() @ weight.dequantized().t()
+        if x_scale is not None:
+            y = y * x_scale.unsqueeze(-1)
+        return y.to(out_dtype)

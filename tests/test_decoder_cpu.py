@@ -1,0 +1,106 @@
+"""Decoder operators without a GPU: the CPU formulas, plans, Meta shapes, the C ABI's refusals."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from relmo_b200 import capi
+from relmo_b200.ops import decoder, mp
+from tests import _decoder_ref as ref
+
+
+def rnd(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_formula(residual):
+    x, w, r = rnd(5, 33, seed=1), rnd(33, seed=2), rnd(5, 33, seed=3) if residual else None
+    y, h = decoder.add_rms_norm(x, w, r, eps=1e-5)
+    ye, he = ref.norm(x.double(), w.double(), None if r is None else r.double(), 1e-5)
+    ref.close(y, ye)
+    ref.close(h, he)
+    q, scale, h8 = decoder.add_rms_norm_e4m3(x, w, r, eps=1e-5)
+    assert q.dtype == torch.float8_e4m3fn and torch.equal(h8, h)
+    assert bool(((q.float() * scale[:, None] - ye).abs() <= ye.abs() * 2**-4 + scale[:, None] * 2**-9).all())
+
+
+def test_attention_formula_with_gradients():
+    ql, kl = [3, 0, 2, 4], [5, 2, 0, 7]
+    q, k, v = (rnd(n, h, 8, seed=i).requires_grad_() for i, (n, h) in enumerate([(9, 4), (14, 2), (14, 2)]))
+    mask = torch.ones(14, dtype=torch.bool)
+    mask[::3] = False
+    o = decoder.cross_attention(q, k, v, decoder.attention_plan(ql, kl, "cpu"), key_mask=mask)
+    wide = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    want = ref.attention(*wide, ql, kl, 8**-0.5, mask)
+    ref.close(o.detach(), want.detach())
+    assert bool((o[3:5] == 0).all())
+    do = rnd(9, 4, 8, seed=9)
+    for g, e in zip(torch.autograd.grad(o, (q, k, v), do), torch.autograd.grad(want, wide, do.double())):
+        ref.close(g, e)
+    dense = decoder.cross_attention(q[None, :3], k[None, :5], v[None, :5], key_mask=mask[None, :5])
+    ref.close(dense[0].detach(), want[:3].detach())
+    with pytest.raises(RuntimeError, match="the plan is for"):
+        decoder.cross_attention(q[1:], k, v, decoder.attention_plan(ql, kl, "cpu"))
+
+
+def test_int4_formula_and_quantization():
+    w = rnd(10, 128, seed=1)
+    for sym in (True, False):
+        q = decoder.quantize_int4(w, 32, symmetric=sym)
+        assert (q.n, q.k, q.group, q.has_zeros) == (10, 128, 32, not sym)
+        ref.close(q.dequantized(), ref.dequantize(*q._plain, 32), torch.float32)
+        x = rnd(3, 128, seed=2)
+        ref.close(decoder.int4_matvec(x, q), x.double() @ q.dequantized().double().t())
+    with pytest.raises(RuntimeError, match="multiple of group"):
+        decoder.quantize_int4(w, 48)
+
+
+def test_meta_shapes():
+    assert mp.available()
+    ops = torch.ops.relm_mp_b200
+    x, w = torch.empty(4, 6, 32, device="meta"), torch.empty(32, device="meta")
+    assert [t.shape for t in ops.add_rms_norm(x, w, x, 1e-6)] == [x.shape, x.shape]
+    q, s, _ = ops.add_rms_norm_e4m3(x, w, None, 1e-6)
+    assert q.shape == x.shape and q.dtype == torch.float8_e4m3fn and s.shape == (4, 6)
+    t = torch.empty(2, 5, 4, 16, device="meta")
+    assert ops.cross_attention(t, t[:, :, :2], t[:, :, :2], None, [], 0.25, None).shape == t.shape
+    assert ops.int4_matvec(x, w, 100, 32, 32, False, None, torch.float32).shape == (4, 6, 100)
+
+
+def test_plan_on_the_host():
+    lib = capi.lib()
+    arr = lambda *v: (ctypes.c_int64 * len(v))(*v)  # noqa: E731
+    ql, kl, plan = arr(130, 0, 300), arr(5, 200, 64), capi.AttnPlan()
+    assert lib.relm_mp_attn_plan_init(ql, kl, 3, ctypes.byref(plan)) == 0
+    assert (plan.q_rows, plan.kv_rows, plan.max_q, plan.max_kv) == (430, 269, 300, 200)
+    assert (plan.q_tiles, plan.q_pairs, plan.kv_tiles, plan.kv_blocks) == (5, 3, 4, 6)
+    n = lib.relm_mp_attn_plan_bytes(ctypes.byref(plan))
+    buf = (ctypes.c_int32 * (n // 4))()
+    assert lib.relm_mp_attn_plan_fill(ql, kl, ctypes.byref(plan), buf, n) == 0
+    wide = ctypes.cast(buf, ctypes.POINTER(ctypes.c_int64))
+    assert [wide[i] for i in range(4)] == [0, 130, 130, 430]
+    assert lib.relm_mp_attn_plan_fill(ql, kl, ctypes.byref(plan), buf, n - 256) == 3
+    assert lib.relm_mp_attn_plan_fill(arr(1, 0, 300), kl, ctypes.byref(plan), buf, n) == 1
+    assert lib.relm_mp_attn_plan_init(arr(-1), arr(1), 1, ctypes.byref(plan)) == 1
+
+
+def test_c_abi_refusals():
+    lib = capi.lib()
+    attn = capi.Attn(dtype=capi.FLOAT32, heads=4, kv_heads=3, dim=16, scale=0.25)
+    for change, text in [(dict(), "multiple of kv_heads"), (dict(kv_heads=2, dim=300), "dim must be"),
+                         (dict(kv_heads=2, scale=0.0), "scale must be"), (dict(kv_heads=2, dtype=1), "unsupported dtype"),
+                         (dict(kv_heads=2, seqs=2, max_q=3, q_rows=5), "seqs * length"),
+                         (dict(kv_heads=2, seqs=1, max_q=3, q_rows=3), "must not be NULL")]:
+        a = capi.Attn.from_buffer_copy(attn)
+        for name, value in change.items():
+            setattr(a, name, value)
+        assert lib.relm_mp_cross_attention(ctypes.byref(a), None, None, None, None, 0, None) != 0
+        assert text in lib.relm_mp_last_error().decode()
+    assert lib.relm_mp_int4_packed_bytes(16, 100, 32, 0) == 0 and lib.relm_mp_int4_packed_bytes(16, 128, 48, 0) == 0
+    assert lib.relm_mp_int4_packed_bytes(16, 128, 32, 1) > lib.relm_mp_int4_packed_bytes(16, 128, 32, 0) > 16 * 64
+    assert lib.relm_mp_add_rms_norm(capi.FLOAT32, None, 8, None, 0, None, 2, 8, 1e-6, None, None, None, None) == 1
+    assert lib.relm_mp_add_rms_norm(1, None, 8, None, 0, None, 2, 8, 1e-6, None, None, None, None) == 4

@@ -1,0 +1,479 @@
+"""Decoder operators on the GPU against plain 64-bit forms: sizes and masks where they can go wrong,
+strides, streams, refusals, gradients against the formula's and against differences."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from relmo_b200.ops import decoder
+from tests import _decoder_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF16, F16, F32]
+
+
+def rnd(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+# ---- add + RMS norm ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (1, 4096), (5, 32), (64, 64), (33, 128), (129, 250), (17, 1001),
+                                        (700, 96), (9, 2048), (4, 5120), (3, 8192), (2, 8191), (2, 16384), (2, 20001),
+                                        (1300, 16), (0, 64)])
+@pytest.mark.parametrize("residual", [True, False])
+def test_norm_forward_and_backward(dtype, rows, width, residual):
+    x, w = rnd((rows, width), dtype, 1), (1 + rnd((width,), F32, 2, 0.2)).to(dtype)
+    r = rnd((rows, width), dtype, 3, 2.0) if residual else None
+    dy, dh = rnd((rows, width), dtype, 4), rnd((rows, width), dtype, 5)
+    leaves = [t.requires_grad_() for t in (x, w, r) if t is not None]
+    y, h = decoder.add_rms_norm(x, w, r, eps=1e-5)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    ye, he = ref.norm(wide[0], wide[1], wide[2] if residual else None, 1e-5)
+    ref.close(y.detach(), ye.detach(), what="y")
+    ref.close(h.detach(), he.detach(), what="h")
+    if rows == 0:
+        torch.autograd.grad((y, h), leaves, (dy, dh), allow_unused=True)
+        return
+    got = torch.autograd.grad((y, h), leaves, (dy, dh))
+    want = torch.autograd.grad((ye, he), wide, (dy.double(), dh.double()))
+    for g, e, name in zip(got, want, ("dx", "dweight", "dresidual")):
+        ref.close(g, e, what=name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(1, 1), (3, 7), (1, 4096), (64, 64), (33, 128), (129, 250), (17, 1001), (9, 8192),
+                                        (2, 20001)])
+def test_norm_e4m3(dtype, rows, width):
+    x, w, r = rnd((rows, width), dtype, 1), (1 + rnd((width,), F32, 2, 0.2)).to(dtype), rnd((rows, width), dtype, 3)
+    q, scale, h = decoder.add_rms_norm_e4m3(x, w, r, eps=1e-5)
+    ye, he = ref.norm(x.double(), w.double(), r.double(), 1e-5)
+    assert q.dtype == torch.float8_e4m3fn and scale.shape == (rows,) and scale.dtype == F32
+    ref.close(h, he, what="h")
+    ref.close(scale, ye.abs().amax(1) / 448, what="scale")
+    # half a step of a 3-bit mantissa, and of the smallest normal's steps, plus float32 error
+    err = (q.double() * scale.double()[:, None] - ye).abs()
+    step = torch.maximum(ye.abs() * 2.0**-4, scale.double()[:, None] * 2.0**-10)
+    assert bool((err <= step * (1 + 1e-4) + 1e-12).all())
+
+
+def test_norm_rows_of_zeros_infinity_and_nan():
+    x = torch.zeros(4, 64, device="cuda")
+    x[1, 3], x[2, 5] = math.inf, math.nan
+    x[3] = 1e-30
+    w = torch.ones(64, device="cuda")
+    y, h = decoder.add_rms_norm(x, w, torch.zeros_like(x))
+    assert bool((y[0] == 0).all()) and math.isnan(y[1, 3].item()) and bool((y[1, :3] == 0).all())
+    assert bool(torch.isnan(y[2]).all()) and torch.equal(h[1], x[1])
+    q, scale, _ = decoder.add_rms_norm_e4m3(x, w)
+    assert scale[0].item() == 1 and bool((q[0].float() == 0).all()) and math.isnan(scale[2].item())
+
+
+def test_norm_strided_views_unaligned_and_3d():
+    base = rnd((40, 3, 80), BF16, 1)
+    w = torch.ones(64, device="cuda", dtype=BF16)
+    for x, r in [(base[:, 1, 8:72], base[:, 2, :64]), (base[:, 1, 3:67], base[:, 0, 1:65]), (base[::2, 0, 16:], base[1::2, 0, 16:]),
+                 (base[:, :, :64], base[:, :, 16:]), (base.transpose(0, 2)[:64].transpose(0, 2), base[:, :, 8:72])]:
+        y, h = decoder.add_rms_norm(x, w, r)
+        ye, he = ref.norm(x.double(), w.double(), r.double(), 1e-6)
+        ref.close(y, ye)
+        ref.close(h, he)
+    x = rnd((6, 64), F32, 2)
+    x1 = x.t().contiguous().t()  # columns first
+    ref.close(decoder.add_rms_norm(x1, torch.ones(64, device="cuda"))[0], ref.norm(x.double(), 1.0, None, 1e-6)[0])
+
+
+def test_norm_only_one_output_used_and_broadcast_residual():
+    x, r, w = (t.requires_grad_() for t in (rnd((37, 100), F32, 1), rnd((1, 100), F32, 2), rnd((100,), F32, 3)))
+    dy = rnd((37, 100), F32, 4)
+    xe, re, we = (t.detach().double().requires_grad_() for t in (x, r, w))
+    for which in (0, 1):
+        out = decoder.add_rms_norm(x, w, r.expand(37, 100))[which]
+        want = ref.norm(xe, we, re.expand(37, 100), 1e-6)[which]
+        got = torch.autograd.grad(out, (x, r, w), dy, allow_unused=True)
+        exp = torch.autograd.grad(want, (xe, re, we), dy.double(), allow_unused=True)
+        for g, e in zip(got, exp):
+            if e is None:
+                assert g is None or bool((g == 0).all())
+            else:
+                ref.close(g, e)
+
+
+def test_norm_gradient_against_differences():
+    x, r, w, dy, dh = (rnd(s, F32, i) for i, s in enumerate([(5, 33), (5, 33), (33,), (5, 33), (5, 33)]))
+    leaves = [t.clone().requires_grad_() for t in (x, w, r)]
+    y, h = decoder.add_rms_norm(*leaves)
+    grads = torch.autograd.grad((y, h), leaves, (dy, dh))
+    step = 1e-5
+
+    def loss(a, b, c):
+        y, h = ref.norm(a, b, c, 1e-6)
+        return (y * dy.double()).sum() + (h * dh.double()).sum()
+
+    point = [t.double() for t in (x, w, r)]
+    for i in range(3):
+        d = rnd(point[i].shape, F32, 20 + i).double()
+        up, down = ([p + s * step * d if j == i else p for j, p in enumerate(point)] for s in (1, -1))
+        diff = (loss(*up) - loss(*down)) / (2 * step)
+        # differences of a smooth function: error step^2 times its third derivative, far below float32's
+        assert abs((grads[i].double() * d).sum() - diff) <= 1e-4 * d.norm() * grads[i].double().norm()
+
+
+def test_norm_refusals():
+    x, w = rnd((4, 8), F32, 1), rnd((8,), F32, 2)
+    with pytest.raises(RuntimeError, match="weight must be"):
+        decoder.add_rms_norm(x, w[:4])
+    with pytest.raises(RuntimeError, match="share x's dtype"):
+        decoder.add_rms_norm(x, w.half())
+    with pytest.raises(RuntimeError, match="x's shape"):
+        decoder.add_rms_norm(x, w, x[:2])
+    with pytest.raises(RuntimeError, match="must be on"):
+        decoder.add_rms_norm(x, w.cpu())
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        decoder.add_rms_norm(x.double(), w.double())
+    with pytest.raises(RuntimeError, match="width >= 1"):
+        decoder.add_rms_norm(x[:, :0], w[:0])
+
+
+# ---- cross attention ---------------------------------------------------------------
+
+
+LENGTHS = [
+    ([1], [1]),
+    ([5], [3]),
+    ([3, 0, 7, 2], [4, 5, 0, 1]),
+    ([127, 128, 129, 1, 64], [63, 64, 65, 128, 129]),
+    ([257, 30], [300, 511]),
+    ([1, 1, 1, 1, 1], [700, 0, 1, 64, 129]),
+    ([4, 3, 4], [1000, 65, 2]),
+    ([40], [4097]),
+    ([600], [33]),
+]
+HEADS = [(1, 1, 64), (4, 4, 32), (8, 2, 128), (4, 1, 64), (3, 3, 20), (2, 1, 80), (6, 2, 16), (1, 1, 192), (2, 2, 256),
+         (2, 1, 7), (5, 5, 96)]
+
+
+def make(dtype, ql, kl, heads, kv_heads, dim, seed=0):
+    q = rnd((sum(ql), heads, dim), dtype, seed + 1)
+    k, v = rnd((sum(kl), kv_heads, dim), dtype, seed + 2), rnd((sum(kl), kv_heads, dim), dtype, seed + 3)
+    return q, k, v, rnd((sum(ql), heads, dim), dtype, seed + 4)
+
+
+def check(q, k, v, do, ql, kl, mask=None, scale=None, backward=True):
+    plan = decoder.attention_plan(ql, kl)
+    s = scale or q.size(-1) ** -0.5
+    clean_k, clean_v = k, v
+    if mask is not None:  # what masked rows hold plays no part
+        clean_k, clean_v = (torch.where(mask[:, None, None], t, torch.zeros_like(t)) for t in (k, v))
+    with torch.no_grad():
+        served = decoder.cross_attention(q, k, v, plan, scale=scale, key_mask=mask)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+    wide = [t.detach().double().requires_grad_() for t in (q, clean_k, clean_v)]
+    want = ref.attention(*wide, ql, kl, s, mask)
+    ref.close(served, want.detach(), what="o without gradients")
+    if not backward:
+        return
+    o = decoder.cross_attention(*leaves, plan, scale=scale, key_mask=mask)
+    ref.close(o.detach(), want.detach(), what="o")
+    got = torch.autograd.grad(o, leaves, do)
+    if not want.requires_grad or want.numel() == 0 or sum(kl) == 0:
+        return
+    exp = torch.autograd.grad(want, wide, do.double(), allow_unused=True)
+    for g, e, name in zip(got, exp, ("dq", "dk", "dv")):
+        e = torch.zeros_like(g, dtype=torch.float64) if e is None else e
+        # one key: its weight is 1 and score gradients are differences of equal numbers; compare on the inputs' scale
+        if name != "dv" and e.norm() <= 1e-2 * math.sqrt(max(e.numel(), 1)):
+            assert (g.double() - e).norm() <= 3 * ref.U[g.dtype] * 4 * math.sqrt(max(e.numel(), 1) * q.size(-1)), name
+            continue
+        ref.close(g, e, what=name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("ql,kl", LENGTHS)
+def test_attention_lengths(dtype, heads, kv_heads, dim, ql, kl):
+    check(*make(dtype, ql, kl, heads, kv_heads, dim), ql, kl)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 4, 32), (8, 2, 128), (2, 1, 64), (2, 2, 20)])
+@pytest.mark.parametrize("filler", [0.0, math.inf, math.nan, -65504.0])
+def test_attention_masks_hide_what_masked_rows_hold(dtype, heads, kv_heads, dim, filler):
+    ql, kl = [70, 3, 1, 130, 9], [200, 64, 150, 131, 5]
+    q, k, v, do = make(dtype, ql, kl, heads, kv_heads, dim)
+    mask = torch.rand(sum(kl), generator=torch.Generator().manual_seed(3)).cuda() < 0.7
+    mask[200:264] = False            # a sequence without any key left
+    mask[264:264 + 130] = False      # whole tiles masked, the last keys kept
+    mask[-1] = False
+    k[~mask], v[~mask] = filler, filler
+    check(q, k, v, do, ql, kl, mask)
+    plan = decoder.attention_plan(ql, kl)
+    o = decoder.cross_attention(q, k, v, plan, key_mask=mask)
+    assert bool((o[70:73] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("t,s", [(1, 300), (150, 200), (2, 64), (300, 1)])
+def test_attention_neighbours_infinite(dtype, t, s):
+    """A sequence next to one that holds infinities and NaN is not touched by them."""
+
+    ql, kl = [t, 5, t], [s, 7, s]
+    q, k, v, do = make(dtype, ql, kl, 2, 1, 64)
+    alone = decoder.cross_attention(q[:t], k[:s], v[:s], decoder.attention_plan([t], [s]))
+    bad = slice(t, t + 5), slice(s, s + 7)
+    q[bad[0]], k[bad[1]], v[bad[1]], do[bad[0]] = math.nan, math.inf, math.nan, math.nan
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o = decoder.cross_attention(*leaves, decoder.attention_plan(ql, kl))
+    assert bool(torch.isfinite(o[:t]).all()) and bool(torch.isfinite(o[t + 5:]).all())
+    ref.close(o[:t].detach(), alone.double())
+    for g, n, rows in zip(torch.autograd.grad(o, leaves, do), ("dq", "dk", "dv"), ((t, 5), (s, 7), (s, 7))):
+        assert bool(torch.isfinite(g[:rows[0]]).all()) and bool(torch.isfinite(g[rows[0] + rows[1]:]).all()), n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_large_scores(dtype):
+    """Scores of a few hundred: one key takes all, earlier maxima are replaced."""
+
+    ql, kl = [130, 2], [400, 300]
+    q, k, v, do = make(dtype, ql, kl, 2, 2, 64)
+    q = (q * 4).detach()
+    k = k * torch.linspace(0.1, 6, k.size(0), device="cuda")[:, None, None].to(dtype)
+    plan = decoder.attention_plan(ql, kl)
+    o = decoder.cross_attention(q, k, v, plan)
+    want = ref.attention(q.double(), k.double(), v.double(), ql, kl, 0.125)
+    # float32 scores of up to 400 have errors of 400 * 2^-24 * a few: below 1e-4 in the weights
+    assert (o.double() - want).norm() <= (3 * ref.U[dtype] + 2e-4) * want.norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,s,heads,kv_heads,dim", [(3, 1, 77, 4, 2, 32), (2, 140, 65, 4, 4, 64), (2, 5, 260, 8, 1, 128), (1, 0, 4, 1, 1, 8),
+                                                      (2, 3, 0, 2, 2, 16), (0, 3, 3, 2, 2, 16)])
+def test_attention_dense_batches_and_strides(dtype, b, t, s, heads, kv_heads, dim):
+    q = rnd((b, heads, t, dim + 24), dtype, 1)[..., 8:dim + 8].transpose(1, 2)
+    kv = rnd((b, s, 2, kv_heads, dim), dtype, 2)
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    mask = torch.ones(b, s, dtype=torch.bool, device="cuda")
+    mask[:, ::5] = False
+    do = rnd((b, t, heads, dim), dtype, 3)
+    for m in (None, mask):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        o = decoder.cross_attention(*leaves, key_mask=m)
+        assert o.shape == q.shape
+        got = torch.autograd.grad(o, leaves, do)
+        if o.numel() == 0:
+            continue
+        flat = [x.detach().reshape(-1, x.size(2), dim).double().requires_grad_() for x in (q, k, v)]
+        want = ref.attention(*flat, [t] * b, [s] * b, dim**-0.5, None if m is None else m.reshape(-1))
+        ref.close(o.detach().reshape(-1, heads, dim), want.detach(), dtype)
+        if s:
+            exp = torch.autograd.grad(want, flat, do.reshape(-1, heads, dim).double())
+            for g, e in zip(got, exp):
+                ref.close(g.reshape(e.shape), e, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_packed_strides_broadcast_heads_and_unaligned(dtype):
+    ql, kl = [33, 140], [70, 129]
+    dim = 64
+    qkv = rnd((sum(ql), 6, dim + 8), dtype, 1)
+    kk = rnd((sum(kl), 1, dim), dtype, 2)
+    v = rnd((sum(kl) * dim * 4 + 3,), dtype, 3)[3:].view(sum(kl), 4, dim)  # not on a 16-byte boundary
+    q = qkv[:, 1:5, :dim]
+    k = kk.expand(-1, 4, -1)  # stride 0 over heads
+    qe, ke, ve = (x.detach().double().requires_grad_() for x in (q, kk, v))
+    leaves = [x.requires_grad_() for x in (q.detach(), kk, v)]
+    plan = decoder.attention_plan(ql, kl)
+    o = decoder.cross_attention(leaves[0], leaves[1].expand(-1, 4, -1), leaves[2], plan)
+    want = ref.attention(qe, ke.expand(-1, 4, -1), ve, ql, kl, 0.125)
+    ref.close(o.detach(), want.detach())
+    do = rnd((sum(ql), 4, dim), dtype, 4)
+    for g, e in zip(torch.autograd.grad(o, leaves, do), torch.autograd.grad(want, (qe, ke, ve), do.double())):
+        ref.close(g, e)
+    odd = q.transpose(1, 2).contiguous().transpose(1, 2)  # last dimension not dense
+    ref.close(decoder.cross_attention(odd, k, v, plan).detach(), want.detach())
+
+
+def test_attention_same_bits_other_stream_and_plan_reuse():
+    ql, kl = [200, 31, 1], [333, 64, 500]
+    for dtype in (BF16, F32):
+        q, k, v, do = make(dtype, ql, kl, 4, 2, 64)
+        plan = decoder.attention_plan(ql, kl)
+        runs = []
+        side = torch.cuda.Stream()
+        for i in range(4):
+            with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+                side.wait_stream(torch.cuda.default_stream())
+                leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+                o = decoder.cross_attention(*leaves, plan)
+                runs.append([o.detach(), *torch.autograd.grad(o, leaves, do)])
+            torch.cuda.synchronize()
+        for r in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+def test_attention_gradient_against_differences():
+    ql, kl = [5, 3], [7, 4]
+    q, k, v, do = make(F32, ql, kl, 4, 2, 16)
+    plan = decoder.attention_plan(ql, kl)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(decoder.cross_attention(*leaves, plan), leaves, do)
+    point, step = [x.double() for x in (q, k, v)], 1e-5
+    for i in range(3):
+        d = rnd(point[i].shape, F32, 30 + i).double()
+        up, down = ([p + s * step * d if j == i else p for j, p in enumerate(point)] for s in (1, -1))
+        diff = sum(s * (ref.attention(*p, ql, kl, 0.25) * do.double()).sum() for s, p in ((1, up), (-1, down))) / (2 * step)
+        assert abs((grads[i].double() * d).sum() - diff) <= 1e-4 * d.norm() * grads[i].double().norm()
+
+
+def test_attention_rows_past_32_bits():
+    """Element offsets beyond 2^31 in a long cache."""
+
+    rows, heads, dim = 2**31 // (8 * 128) + 300, 8, 128
+    kv = torch.zeros(rows, heads, dim, dtype=BF16, device="cuda")
+    tail = 200
+    k, v = rnd((tail, heads, dim), BF16, 1), rnd((tail, heads, dim), BF16, 2)
+    kv[-tail:] = k
+    vv = torch.zeros_like(kv)
+    vv[-tail:] = v
+    q = rnd((2, 16, dim), BF16, 3)
+    plan = decoder.attention_plan([0, 2], [rows - tail, tail])
+    o = decoder.cross_attention(q, kv, vv, plan)
+    ref.close(o, ref.attention(q.double(), k.double(), v.double(), [2], [tail], dim**-0.5))
+    q2 = rnd((150, 16, dim), BF16, 4)
+    o = decoder.cross_attention(q2, kv, vv, decoder.attention_plan([0, 150], [rows - tail, tail]))
+    ref.close(o, ref.attention(q2.double(), k.double(), v.double(), [150], [tail], dim**-0.5))
+
+
+def test_attention_refusals():
+    ql, kl = [3], [4]
+    q, k, v, _ = make(F32, ql, kl, 4, 2, 16)
+    plan = decoder.attention_plan(ql, kl)
+    call = decoder.cross_attention
+    with pytest.raises(RuntimeError, match="lengths must be in"):
+        decoder.attention_plan([-1], [2])
+    with pytest.raises(RuntimeError, match="one length each"):
+        decoder.attention_plan([1, 2], [2])
+    with pytest.raises(RuntimeError, match="without a plan"):
+        call(q, k, v)
+    with pytest.raises(RuntimeError, match="with a plan"):
+        call(q[None], k[None], v[None], plan)
+    with pytest.raises(RuntimeError, match="the plan is for"):
+        call(q[:2], k, v, plan)
+    with pytest.raises(RuntimeError, match="same shape"):
+        call(q, k, v[:, :1], plan)
+    with pytest.raises(RuntimeError, match="share dtype"):
+        call(q, k.half(), v.half(), plan)
+    with pytest.raises(RuntimeError, match="multiple of kv_heads"):
+        call(q[:, :3], k, v, plan)
+    with pytest.raises(RuntimeError, match="scale must be"):
+        call(q, k, v, plan, scale=-1.0)
+    with pytest.raises(RuntimeError, match="scale must be"):
+        call(q, k, v, plan, scale=math.nan)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        call(q.double(), k.double(), v.double(), plan)
+    with pytest.raises(RuntimeError, match="key_mask must"):
+        call(q, k, v, plan, key_mask=torch.ones(3, dtype=torch.bool, device="cuda"))
+    with pytest.raises(RuntimeError, match="key_mask must be bool"):
+        call(q, k, v, plan, key_mask=torch.ones(4, device="cuda"))
+    with pytest.raises(RuntimeError, match="must be on"):
+        call(q, k.cpu(), v.cpu(), plan)
+    with pytest.raises(RuntimeError, match="dim must be"):
+        call(*(rnd((n, 1, 300), F32, 1) for n in (3, 4, 4)), plan)
+    with pytest.raises(RuntimeError, match="made for the CPU"):
+        call(q, k, v, decoder.attention_plan(ql, kl, "cpu"))
+    with pytest.raises(RuntimeError, match="does not belong to its sizes"):
+        call(q, k, v, decoder.AttentionPlan((3,), (4,), plan.memory, [*plan.sizes[:5], 9, 9, 9, 9]))
+
+
+# ---- products with 4-bit weights ---------------------------------------------------
+
+
+def make_int4(n, k, group, zeros, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 256, (n, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = ((torch.rand((n, k // group), generator=g, device="cuda") + 0.5) / math.sqrt(k)).half()
+    z = torch.randint(0, 16, (n, k // group), generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    return codes, scales, z
+
+
+@pytest.mark.parametrize("dtype", [*TYPES, torch.float8_e4m3fn])
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (16, 64, 64), (17, 96, 32), (100, 128, 128), (300, 1056, 32), (64, 4096, 128),
+                                       (1000, 704, 64), (33, 16384, 128)])
+@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 16, 17, 40])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_int4_matvec(dtype, n, k, group, rows, zeros):
+    codes, scales, z = make_int4(n, k, group, zeros)
+    w = ref.dequantize(codes, scales, z, group)
+    weight = decoder.Int4Weight(codes, scales, z)
+    x = rnd((rows, k), F32, 5)
+    if dtype is torch.float8_e4m3fn:
+        xs = torch.rand(rows, device="cuda") + 0.5
+        x8 = (x * 20).to(dtype)
+        for out in TYPES:
+            y = decoder.int4_matvec(x8, weight, x_scale=xs, out_dtype=out)
+            ref.close(y, (x8.double() * xs.double()[:, None]) @ w.t(), out)
+        return
+    x = x.to(dtype)
+    y = decoder.int4_matvec(x, weight)
+    assert y.dtype == dtype
+    ref.close(y, x.double() @ w.t())
+
+
+def test_int4_views_shapes_and_special_values():
+    codes, scales, z = make_int4(70, 256, 64, True)
+    w, weight = ref.dequantize(codes, scales, z, 64), decoder.Int4Weight(codes, scales, z)
+    base = rnd((4, 3, 300), F32, 1)
+    for x in (base[:, 1, 5:261], base[:, :, 40:296], base[0, 0, 1:257], base.bfloat16()[:, 2, 3:259], base.half()[..., 7:263],
+              base[:0, 0, :256]):
+        y = decoder.int4_matvec(x, weight)
+        assert y.shape == (*x.shape[:-1], 70)
+        ref.close(y, x.double() @ w.t())
+    x = torch.zeros(3, 256, device="cuda")
+    x[0, 7], x[1, 9], x[2, 0] = math.inf, math.nan, 1e-39
+    y = decoder.int4_matvec(x, weight)
+    assert bool((torch.isinf(y[0]) | torch.isnan(y[0])).all()) and bool(torch.isnan(y[1]).all()) and bool(torch.isfinite(y[2]).all())
+
+
+def test_int4_quantize_and_refusals():
+    w = rnd((48, 256), F32, 1)
+    for sym in (True, False):
+        q = decoder.quantize_int4(w, 64, symmetric=sym)
+        y = decoder.int4_matvec(torch.eye(256, device="cuda"), q).t()
+        span = w.view(48, -1, 64)
+        step = span.abs().amax(-1) / 7 if sym else (span.amax(-1).clamp_min(0) - span.amin(-1).clamp_max(0)) / 15
+        # half a step; a rounded zero point moves the range by half a step more
+        assert bool(((y - w).view(48, -1, 64).abs() <= step.unsqueeze(-1) * (0.52 if sym else 1.02)).all())
+    codes, scales, z = make_int4(16, 128, 64, True)
+    weight = decoder.Int4Weight(codes, scales, z)
+    with pytest.raises(RuntimeError, match="x must be"):
+        decoder.int4_matvec(w, weight)
+    with pytest.raises(RuntimeError, match="output has x's dtype"):
+        decoder.int4_matvec(w[:, :128], weight, out_dtype=BF16)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        decoder.int4_matvec(w[:, :128].double(), weight)
+    with pytest.raises(RuntimeError, match="x_scale must be"):
+        decoder.int4_matvec(w[:, :128], weight, x_scale=torch.ones(3, device="cuda"))
+    with pytest.raises(RuntimeError, match="must be on"):
+        torch.ops.relm_mp_b200.int4_matvec(w[:, :128], weight.packed.cpu(), 16, 128, 64, True, None, F32)
+    with pytest.raises(RuntimeError, match="does not belong"):
+        torch.ops.relm_mp_b200.int4_matvec(w, weight.packed, 16, 256, 64, True, None, F32)
+    with pytest.raises(RuntimeError, match="group must be"):
+        decoder.Int4Weight(codes, scales[:, :1].repeat(1, 8))
+    with pytest.raises(RuntimeError, match="scales must be"):
+        decoder.Int4Weight(codes, scales.float())
+    with pytest.raises(RuntimeError, match="zeros must be"):
+        decoder.Int4Weight(codes, scales, z[:, :1])
+
+
+def test_disabled_library_raises(monkeypatch):
+    monkeypatch.setenv("RELM_MP_ENABLE", "0")
+    with pytest.raises(RuntimeError, match="no GPU fallback"):
+        decoder.add_rms_norm(torch.ones(2, 8, device="cuda"), torch.ones(8, device="cuda"))
