@@ -46,6 +46,7 @@ CUDA_SOURCES = [
     "relm_mp_int4.cu",
     "relm_mp_attn.cu",
     "relm_mp_attn_simt.cu",
+    "relm_mp_attn_split.cu",
 ]
 TORCH_SOURCES = ["relm_mp_torch.cpp", "relm_mp_cpu.cpp", "relm_mp_decoder.cpp"]
 HEADERS = ["relm_mp_internal.cuh", "relm_mp_segment.cuh", "relm_mp_seg_impl.cuh", "relm_mp_attn.cuh"]

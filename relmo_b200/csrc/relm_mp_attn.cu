@@ -109,6 +109,22 @@ Counts counts(const relm_mp_attn& in)
            in.seqs * ceil_div(in.max_kv, kTileRows), in.seqs * ceil_div(in.max_kv, kBlockKeys)};
 }
 
+// 16-byte copies of k and v rows: every row of every head starts on a 16-byte boundary.
+bool aligned_rows(const relm_mp_attn& in)
+{
+   if(in.dtype == RELM_MP_FLOAT32 || in.dim % 8) return false;
+   auto ok = [&](const void* p, const int64_t* s) {
+      return (reinterpret_cast< uintptr_t >(p) & 15) == 0 && (in.plan || s[0] % 8 == 0) && s[1] % 8 == 0 && s[2] % 8 == 0;
+   };
+   return ok(in.k, in.k_stride) && ok(in.v, in.v_stride) && ok(in.q, in.q_stride);
+}
+
+// The form split over the keys takes up to 16 rows (tokens x heads of a group).
+bool use_split(const relm_mp_attn& in)
+{
+   return aligned_rows(in) && in.max_q * (in.heads / in.kv_heads) <= 16;
+}
+
 // delta[head, row] = sum over dim of go * (o + o_rest), in float32; 8 lanes per row and head.
 template < typename T, int VEC >
 __global__ void __launch_bounds__(256) k_attn_delta(const T* __restrict__ go, const T* __restrict__ o,
@@ -210,8 +226,8 @@ int relm_mp_attn_plan_fill(const int64_t* q_lengths, const int64_t* kv_lengths, 
 
 size_t relm_mp_cross_attention_workspace_bytes(const relm_mp_attn* attn)
 {
-   if(check_attn(attn, "cross_attention")) return 0;
-   return 0;
+   if(check_attn(attn, "cross_attention") || attn->q_rows == 0) return 0;
+   return use_split(*attn) ? split_plan(make_args(*attn), counts(*attn).kv_blocks).bytes : 0;
 }
 
 int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void* o_rest, void* workspace,
@@ -223,10 +239,12 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
    if(!o) return fail(RELM_MP_ERR_INVALID_ARGUMENT, "cross_attention: o must not be NULL.");
    if(workspace_bytes < relm_mp_cross_attention_workspace_bytes(attn))
       return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "cross_attention: workspace too small.");
-   (void)workspace;
    Args a = make_args(*attn);
    a.o = o, a.lse = lse, a.o_rest = attn->dtype == RELM_MP_FLOAT32 ? nullptr : o_rest;
-   return simt_forward(attn->dtype, a, counts(*attn).q_tiles, static_cast< cudaStream_t >(stream));
+   const Counts c = counts(*attn);
+   cudaStream_t st = static_cast< cudaStream_t >(stream);
+   if(use_split(*attn)) return split_forward(attn->dtype, a, c.kv_blocks, workspace, st);
+   return simt_forward(attn->dtype, a, c.q_tiles, st);
 }
 
 size_t relm_mp_cross_attention_backward_workspace_bytes(const relm_mp_attn* attn)

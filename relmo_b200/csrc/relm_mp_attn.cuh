@@ -1,6 +1,8 @@
 // Shared declarations of the cross attention sources.
 #pragma once
 
+#include <algorithm>
+
 #include "relm_mp_internal.cuh"
 
 namespace relm_mp {
@@ -96,6 +98,14 @@ __device__ __forceinline__ float exp2_fast(float x)
 // Kernels on the CUDA cores, for every type, dim and stride (relm_mp_attn_simt.cu).
 int simt_forward(relm_mp_dtype dtype, const Args& a, int64_t items, cudaStream_t st);
 int simt_backward(relm_mp_dtype dtype, const Args& a, int64_t q_items, int64_t kv_items, cudaStream_t st);
+
+// Few query rows per sequence, 2-byte types, work split over the keys (relm_mp_attn_split.cu).
+struct SplitPlan {
+   int parts, row_groups;
+   size_t part_o, part_ml, bytes; // workspace
+};
+SplitPlan split_plan(const Args& a, int64_t blocks);
+int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* workspace, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace relm_mp

@@ -1,0 +1,407 @@
+// Cross attention of few query rows per sequence (a served token, a readout
+// query): bound by reading k and v once, so the work is split over the keys.
+//
+// All sequences' keys form one line of 64-key blocks, cut into equal parts: one
+// part per block of threads (and key/value head), whatever the lengths. A part
+// may end inside a sequence; then its running maximum, sum and unnormalised
+// output go to the workspace and k_attn_join combines the parts of a sequence
+// in key order:
+//   m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m) / l
+// Parts and sequences are both in order, so (part + sequence) numbers every
+// (part, sequence) overlap uniquely.
+//
+// The group's query heads and tokens are the 16 rows of the matrix instruction
+// (m16n8k16). Each warp is its own pipeline: it takes 16 keys at a time, three
+// steps ahead by asynchronous copies into its own shared memory, and keeps its
+// own maximum, sum and output; the four warps of a block are joined once at the
+// end of a segment. No block-wide barrier is in the loop.
+#include <math_constants.h>
+
+#include "relm_mp_attn.cuh"
+
+namespace relm_mp {
+namespace attn {
+namespace {
+
+constexpr int kWarps = 4, kChunk = 16, kRows = 16, kStages = 3;
+constexpr int kThreads4 = kWarps * 32;
+
+struct SplitArgs {
+   Args a;
+   int64_t blocks; // 64-key blocks of all sequences
+   int parts;
+   float* part_o; // [parts + seqs][kv_heads][row groups * 16][DP]
+   float2* part_ml;
+   int row_groups;
+};
+
+__device__ __forceinline__ int64_t block_of(const Args& a, int64_t seq)
+{
+   return a.kv_blocks ? a.kv_blocks[seq] : seq * ((a.max_kv + kBlockKeys - 1) / kBlockKeys);
+}
+
+__device__ __forceinline__ int64_t part_start(int64_t blocks, int parts, int p) { return blocks * p / parts; }
+// The part that holds block x: the largest p with part_start(p) <= x.
+__device__ __forceinline__ int part_of(int64_t blocks, int parts, int64_t x) { return (int)(((x + 1) * parts - 1) / blocks); }
+
+template < typename T >
+struct Mma;
+template <>
+struct Mma< __nv_bfloat16 > {
+   static __device__ __forceinline__ void run(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
+   {
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+   }
+   static __device__ __forceinline__ uint32_t pack(float lo, float hi)
+   {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+      return *reinterpret_cast< const uint32_t* >(&v);
+   }
+};
+template <>
+struct Mma< __half > {
+   static __device__ __forceinline__ void run(float* c, const uint32_t* a, uint32_t b0, uint32_t b1)
+   {
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+   }
+   static __device__ __forceinline__ uint32_t pack(float lo, float hi)
+   {
+      const __half2 v = __floats2half2_rn(lo, hi);
+      return *reinterpret_cast< const uint32_t* >(&v);
+   }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr)
+{
+   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t* r, uint32_t addr)
+{
+   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                : "r"(addr));
+}
+// 16 bytes, or zeros when !in (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in)
+{
+   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+
+// Byte offset of 16-byte chunk c of row r: chunks of 8 consecutive rows lie in different banks.
+template < int DP >
+__device__ __forceinline__ uint32_t swizzled(int r, int c)
+{
+   constexpr int CH = DP / 8;
+   return (uint32_t)(r * DP * 2 + ((c ^ (CH >= 8 ? r & 7 : (r >> 1) & 3)) * 16));
+}
+
+template < typename T, int DP >
+__global__ void __launch_bounds__(kThreads4) k_attn_split(SplitArgs s)
+{
+   const Args& a = s.a;
+   constexpr int KS = DP / 16, CH = DP / 8;
+   constexpr uint32_t TILE = kChunk * DP * 2, STAGE = 2 * TILE;
+   extern __shared__ __align__(128) unsigned char smem[];
+   __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, row0 = blockIdx.z * kRows;
+   unsigned char* const mine = smem + warp * (kStages * STAGE);
+   const uint32_t base = (uint32_t)__cvta_generic_to_shared(mine);
+   const int64_t first = part_start(s.blocks, s.parts, blockIdx.x), last = part_start(s.blocks, s.parts, blockIdx.x + 1);
+   const float sc = a.scale * kLog2e;
+
+   // First sequence of this part: those that end at or before `first` are done (an empty one at `first` is ours).
+   int64_t seq = 0;
+   for(int64_t b0 = 0; b0 < a.seqs; b0 += kThreads4) {
+      const int64_t b = b0 + threadIdx.x;
+      const int n = __syncthreads_count(b < a.seqs && block_of(a, b) < first && block_of(a, b + 1) <= first);
+      seq += n;
+      if(n < kThreads4) break;
+   }
+
+   for(; seq < a.seqs; ++seq) {
+      const int64_t blk0 = block_of(a, seq), blk1 = block_of(a, seq + 1);
+      const bool final_part = blockIdx.x == s.parts - 1;
+      if(blk0 >= last && !final_part) break;
+      const Seq qs = locate(a.q_off, a.max_q, a.qs, (int)seq);
+      const int rows = qs.len * group;
+      if(row0 >= rows) continue;
+      const Seq ks = locate(a.kv_off, a.max_kv, a.ks, (int)seq), vs = locate(a.kv_off, a.max_kv, a.vs, (int)seq);
+      const int64_t lo = blk0 > first ? blk0 : first, hi = blk1 < last ? blk1 : last;
+      const bool whole = lo == blk0 && hi == blk1;
+      const int key_lo = (int)(lo - blk0) * kBlockKeys;
+      const int key_hi = whole || hi == blk1 ? ks.len : (int)(hi - blk0) * kBlockKeys;
+      const T* kp = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
+      const T* vp = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
+      const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+
+      // Row r of the group: token r / group, query head r % group.
+      uint32_t qf[KS][4];
+#pragma unroll
+      for(int half = 0; half < 2; ++half) {
+         const int r = row0 + g + 8 * half;
+         const T* q = static_cast< const T* >(a.q) + qs.base + (int64_t)(r / group) * a.qs[1] + (kv_head * group + r % group) * a.qs[2];
+#pragma unroll
+         for(int kk = 0; kk < KS; ++kk)
+#pragma unroll
+            for(int c = 0; c < 2; ++c) {
+               const int d = kk * 16 + c * 8 + 2 * t4;
+               qf[kk][half + 2 * c] = r < rows && d < a.dim ? *reinterpret_cast< const uint32_t* >(q + d) : 0u;
+            }
+      }
+      float o[DP / 8][4], m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+#pragma unroll
+      for(int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+      const int steps = key_hi > key_lo + warp * kChunk ? (key_hi - key_lo - warp * kChunk + kChunk * kWarps - 1) / (kChunk * kWarps) : 0;
+      unsigned kept[kStages]; // bit per key of a stage's chunk
+      auto issue = [&](int step, int stage) {
+         const int key0 = key_lo + (step * kWarps + warp) * kChunk;
+         const bool any = step < steps;
+         if(any) {
+            const uint32_t sk = base + stage * STAGE, sv = sk + TILE;
+#pragma unroll
+            for(int i = 0; i < CH * kChunk / 32; ++i) {
+               const int c = (i * 32 + lane) % CH, r = (i * 32 + lane) / CH;
+               const bool in = key0 + r < key_hi && c * 8 < a.dim;
+               const int64_t key = in ? key0 + r : 0;
+               copy16(sk + swizzled< DP >(r, c), in ? kp + key * a.ks[1] + c * 8 : kp, in);
+               copy16(sv + swizzled< DP >(r, c), in ? vp + key * a.vs[1] + c * 8 : vp, in);
+            }
+         }
+         asm volatile("cp.async.commit_group;" ::: "memory");
+         kept[stage] = any && lane < kChunk && key0 + lane < key_hi && (!keep || keep[key0 + lane]) ? 1u : 0u;
+      };
+#pragma unroll
+      for(int i = 0; i < kStages - 1; ++i) issue(i, i);
+      for(int step0 = 0; step0 < steps; step0 += kStages) {
+#pragma unroll
+         for(int stage = 0; stage < kStages; ++stage) {
+            const int step = step0 + stage;
+            if(step >= steps) break;
+            issue(step + kStages - 1, (stage + kStages - 1) % kStages);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+            __syncwarp();
+            const unsigned in = __ballot_sync(0xffffffffu, kept[stage]) & 0xffffu;
+            const uint32_t sk = base + stage * STAGE, sv = sk + TILE;
+            if(in != 0xffffu && keep) { // masked rows may hold anything: their weight is 0, so must they be
+               for(int i = lane; i < kChunk * CH; i += 32)
+                  if(!(in >> (i / CH) & 1)) *reinterpret_cast< uint4* >(mine + stage * STAGE + TILE + swizzled< DP >(i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
+               __syncwarp();
+            }
+            float c[2][4];
+#pragma unroll
+            for(int n = 0; n < 2; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+#pragma unroll
+            for(int kk = 0; kk < KS; ++kk) {
+               uint32_t b[4];
+               ldmatrix4(b, sk + swizzled< DP >((lane >> 4) * 8 + (lane & 7), kk * 2 + ((lane >> 3) & 1)));
+               Mma< T >::run(c[0], qf[kk], b[0], b[1]);
+               Mma< T >::run(c[1], qf[kk], b[2], b[3]);
+            }
+#pragma unroll
+            for(int n = 0; n < 2; ++n)
+#pragma unroll
+               for(int e = 0; e < 4; ++e)
+                  c[n][e] = in >> (n * 8 + 2 * t4 + (e & 1)) & 1 ? c[n][e] * sc : -CUDART_INF_F;
+#pragma unroll
+            for(int h = 0; h < 2; ++h) {
+               float top = fmaxf(fmaxf(c[0][2 * h], c[0][2 * h + 1]), fmaxf(c[1][2 * h], c[1][2 * h + 1]));
+               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+               if(top > m[h]) {
+                  const float f = exp2_fast(m[h] - top);
+                  m[h] = top;
+                  l[h] *= f;
+#pragma unroll
+                  for(int i = 0; i < DP / 8; ++i) o[i][2 * h] *= f, o[i][2 * h + 1] *= f;
+               }
+               // No kept key so far: every score is -inf and every weight 0, whatever the reference.
+               const float ref = m[h] == -CUDART_INF_F ? 0.f : m[h];
+#pragma unroll
+               for(int n = 0; n < 2; ++n)
+#pragma unroll
+                  for(int e = 0; e < 2; ++e) {
+                     c[n][2 * h + e] = exp2_fast(c[n][2 * h + e] - ref);
+                     l[h] += c[n][2 * h + e];
+                  }
+            }
+            // The weights enter the second product in the inputs' type, their sum l stays float32.
+            const uint32_t p[4] = {Mma< T >::pack(c[0][0], c[0][1]), Mma< T >::pack(c[0][2], c[0][3]),
+                                   Mma< T >::pack(c[1][0], c[1][1]), Mma< T >::pack(c[1][2], c[1][3])};
+#pragma unroll
+            for(int dd = 0; dd < DP / 16; ++dd) {
+               uint32_t b[4];
+               ldmatrix4_trans(b, sv + swizzled< DP >(((lane >> 3) & 1) * 8 + (lane & 7), dd * 2 + (lane >> 4)));
+               Mma< T >::run(o[2 * dd], p, b[0], b[1]);
+               Mma< T >::run(o[2 * dd + 1], p, b[2], b[3]);
+            }
+            __syncwarp(); // the stage is free for the next copies
+         }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+      for(int h = 0; h < 2; ++h) {
+         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      }
+      // Join the warps: each leaves its output in its own buffer.
+      __syncwarp();
+      float* out = reinterpret_cast< float* >(mine);
+#pragma unroll
+      for(int i = 0; i < DP / 8; ++i) {
+         *reinterpret_cast< float2* >(out + g * DP + i * 8 + 2 * t4) = make_float2(o[i][0], o[i][1]);
+         *reinterpret_cast< float2* >(out + (g + 8) * DP + i * 8 + 2 * t4) = make_float2(o[i][2], o[i][3]);
+      }
+      if(t4 == 0) {
+         sm_m[warp][g] = m[0], sm_m[warp][g + 8] = m[1];
+         sm_l[warp][g] = l[0], sm_l[warp][g + 8] = l[1];
+      }
+      __syncthreads();
+      const int64_t slot = ((int64_t)blockIdx.x + seq) * a.kv_heads + kv_head;
+      for(int i = threadIdx.x; i < kRows * DP; i += kThreads4) {
+         const int r = i / DP, d = i % DP;
+         if(row0 + r >= rows) break;
+         float M = -CUDART_INF_F;
+#pragma unroll
+         for(int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+         const float ref = M == -CUDART_INF_F ? 0.f : M;
+         float L = 0.f, v = 0.f;
+#pragma unroll
+         for(int w = 0; w < kWarps; ++w) {
+            const float f = exp2_fast(sm_m[w][r] - ref);
+            L += sm_l[w][r] * f;
+            v += reinterpret_cast< const float* >(smem + w * (kStages * STAGE))[i] * f;
+         }
+         if(whole) {
+            const int tok = (row0 + r) / group, head = kv_head * group + (row0 + r) % group;
+            if(d < a.dim) {
+               const int64_t at = ((qs.first + tok) * a.heads + head) * a.dim + d;
+               const float x = L == 0.f ? 0.f : v / L;
+               const T y = from_f32< T >(x);
+               static_cast< T* >(a.o)[at] = y;
+               if(a.o_rest) static_cast< T* >(a.o_rest)[at] = from_f32< T >(x - to_f32(y));
+            }
+            if(d == 0 && a.lse)
+               a.lse[(int64_t)head * a.q_rows + qs.first + tok] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
+         } else {
+            const int64_t at = slot * s.row_groups * kRows + row0 + r;
+            s.part_o[at * DP + d] = v;
+            if(d == 0) s.part_ml[at] = make_float2(M, L);
+         }
+      }
+      __syncthreads();
+   }
+}
+
+// Rows of sequences that more than one part worked on: a warp per row.
+template < typename T, int DP >
+__global__ void __launch_bounds__(128) k_attn_join(SplitArgs s)
+{
+   const Args& a = s.a;
+   const int64_t seq = blockIdx.x;
+   const int64_t blk0 = block_of(a, seq), blk1 = block_of(a, seq + 1);
+   if(blk0 == blk1) return;
+   const int p0 = part_of(s.blocks, s.parts, blk0), p1 = part_of(s.blocks, s.parts, blk1 - 1);
+   if(p0 == p1) return;
+   const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, (int)seq);
+   const int per_head = s.row_groups * kRows;
+   for(int i = blockIdx.y * 4 + (threadIdx.x >> 5); i < qs.len * a.heads; i += gridDim.y * 4) {
+      const int kv_head = i / (qs.len * group), r = i % (qs.len * group);
+      auto row = [&](int p) { return ((p + seq) * a.kv_heads + kv_head) * per_head + r; };
+      float M = -CUDART_INF_F;
+      for(int p = p0 + lane; p <= p1; p += 32) M = fmaxf(M, s.part_ml[row(p)].x);
+#pragma unroll
+      for(int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float ref = M == -CUDART_INF_F ? 0.f : M;
+      float L = 0.f, v[DP / 32];
+#pragma unroll
+      for(int d = 0; d < DP / 32; ++d) v[d] = 0.f;
+#pragma unroll 4
+      for(int p = p0; p <= p1; ++p) {
+         const float2 ml = s.part_ml[row(p)];
+         const float f = exp2_fast(ml.x - ref);
+         L += ml.y * f;
+#pragma unroll
+         for(int d = 0; d < DP / 32; ++d) v[d] += s.part_o[row(p) * DP + d * 32 + lane] * f;
+      }
+      const int tok = r / group, head = kv_head * group + r % group;
+#pragma unroll
+      for(int d = 0; d < DP / 32; ++d) {
+         const int c = d * 32 + lane;
+         if(c >= a.dim) continue;
+         const int64_t at = ((qs.first + tok) * a.heads + head) * a.dim + c;
+         const float x = L == 0.f ? 0.f : v[d] / L;
+         const T y = from_f32< T >(x);
+         static_cast< T* >(a.o)[at] = y;
+         if(a.o_rest) static_cast< T* >(a.o_rest)[at] = from_f32< T >(x - to_f32(y));
+      }
+      if(lane == 0 && a.lse) a.lse[(int64_t)head * a.q_rows + qs.first + tok] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
+   }
+}
+
+int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template < typename T, int DP >
+int launch(const SplitArgs& s, cudaStream_t st)
+{
+   constexpr size_t bytes = (size_t)kWarps * kStages * 2 * kChunk * DP * 2;
+   int rc = check_cuda(cudaFuncSetAttribute(k_attn_split< T, DP >, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
+                       "k_attn_split");
+   if(rc) return rc;
+   k_attn_split< T, DP ><<< dim3(s.parts, s.a.kv_heads, s.row_groups), kThreads4, bytes, st >>>(s);
+   if((rc = check_launch("k_attn_split")) || s.parts == 1) return rc;
+   const int64_t rows = s.a.max_q * s.a.heads;
+   const int64_t y = ceil_div(rows, 4);
+   k_attn_join< T, DP ><<< dim3((unsigned)s.a.seqs, (unsigned)(y < 64 ? y : 64)), 128, 0, st >>>(s);
+   return check_launch("k_attn_join");
+}
+
+template < typename T >
+int launch_dim(const SplitArgs& s, cudaStream_t st)
+{
+   switch(padded_dim(s.a.dim)) {
+      case 32: return launch< T, 32 >(s, st);
+      case 64: return launch< T, 64 >(s, st);
+      case 128: return launch< T, 128 >(s, st);
+      default: return launch< T, 256 >(s, st);
+   }
+}
+
+}  // namespace
+
+// Parts: one wave of resident blocks (shared memory allows about 200 KB per SM),
+// but at least 4 key blocks each, so that a part has work for every warp's pipeline.
+SplitPlan split_plan(const Args& a, int64_t blocks)
+{
+   const int dp = padded_dim(a.dim);
+   SplitPlan p;
+   p.row_groups = (int)ceil_div(a.max_q * (a.heads / a.kv_heads), kRows);
+   const int64_t resident = std::max< int64_t >(1, std::min< int64_t >(8, 200 * 1024 / (kWarps * kStages * 2 * kChunk * dp * 2)));
+   const int64_t slots = 148 * resident / (a.kv_heads * p.row_groups);
+   p.parts = (int)std::max< int64_t >(1, std::min(slots, ceil_div(blocks, 4)));
+   const size_t rows = p.parts == 1 ? 0 : (size_t)(p.parts + a.seqs) * a.kv_heads * p.row_groups * kRows;
+   p.part_o = 0;
+   p.part_ml = align_up(rows * dp * 4);
+   p.bytes = p.part_ml + align_up(rows * 8);
+   return p;
+}
+
+int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* workspace, cudaStream_t st)
+{
+   const SplitPlan p = split_plan(a, blocks);
+   char* w = static_cast< char* >(workspace);
+   const SplitArgs s{a, blocks, p.parts, reinterpret_cast< float* >(w + p.part_o), reinterpret_cast< float2* >(w + p.part_ml),
+                     p.row_groups};
+   return dtype == RELM_MP_BFLOAT16 ? launch_dim< __nv_bfloat16 >(s, st) : launch_dim< __half >(s, st);
+}
+
+}  // namespace attn
+}  // namespace relm_mp
