@@ -591,6 +591,11 @@ RELM_MP_API int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const
                                                  const void* o_rest, const float* lse, void* dq, void* dk, void* dv, void* workspace,
                                                  size_t workspace_bytes, void* stream);
 
+/* Every wait inside the attention kernels has a limit of 2 s. A kernel that
+ * reaches it writes NaN and sets a flag of its device, which this reads and
+ * clears (it waits for the device). */
+RELM_MP_API int relm_mp_attn_gave_up(int* flag);
+
 /* Products with 4-bit weights: y[r, n] = x_scale[r] * sum_k x[r, k] * w[n, k],
  * w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group].
  * relm_mp_int4_pack lays the weights out once: codes [n, k / 2] bytes (the even

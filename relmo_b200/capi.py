@@ -189,6 +189,7 @@ SIGNATURES: dict[str, tuple] = {
     "relm_mp_cross_attention": (_INT, [_P, _P, _P, _P, _P, _SZ, _P]),
     "relm_mp_cross_attention_backward_workspace_bytes": (_SZ, [_P]),
     "relm_mp_cross_attention_backward": (_INT, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "relm_mp_attn_gave_up": (_INT, [_P]),
     "relm_mp_int4_packed_bytes": (_SZ, [_I64, _I64, _I64, _INT]),
     "relm_mp_int4_pack": (_INT, [_P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P]),
     "relm_mp_int4_matvec": (_INT, [_INT, _INT, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _INT, _P, _P]),

@@ -11,7 +11,9 @@
 #include <numeric>
 #include <vector>
 
-#include "relm_mp_attn.cuh"
+#include <atomic>
+
+#include "relm_mp_attn_tc.cuh"
 
 using namespace relm_mp;
 using namespace relm_mp::attn;
@@ -119,6 +121,18 @@ bool aligned_rows(const relm_mp_attn& in)
    return ok(in.k, in.k_stride) && ok(in.v, in.v_stride) && ok(in.q, in.q_stride);
 }
 
+// Tensor maps hold these strides and coordinates.
+bool use_tc(const relm_mp_attn& in)
+{
+   if(!aligned_rows(in) || in.dim > 128) return false;
+   auto ok = [&](const int64_t* s, int64_t rows, int64_t max_rows, int heads) {
+      auto fits = [](int64_t v, int64_t extent) { return extent <= 1 || (v > 0 && v < (1ll << 38)); };
+      return rows < (1ll << 31) - 512 && fits(s[1], max_rows) && fits(s[2], heads) && (in.plan || fits(s[0], in.seqs));
+   };
+   return ok(in.q_stride, in.q_rows, in.max_q, in.heads) && ok(in.k_stride, in.kv_rows, in.max_kv, in.kv_heads) &&
+          ok(in.v_stride, in.kv_rows, in.max_kv, in.kv_heads);
+}
+
 // The form split over the keys takes up to 16 rows (tokens x heads of a group).
 bool use_split(const relm_mp_attn& in)
 {
@@ -167,7 +181,79 @@ int launch_delta(const void* go, const void* o, const void* rest, int64_t rows, 
    return check_launch("k_attn_delta");
 }
 
+// Kernels whose waits on copies or products gave up (they never should) set this.
+__device__ int g_gave_up;
+constexpr int kMaxDevices = 64;
+std::atomic< int* > g_gave_up_ptr[kMaxDevices];
+
+// Address of the flag on the current device, looked up once per device.
+int gave_up_address(int** out)
+{
+   int dev = -1;
+   int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+   if(rc) return rc;
+   if(dev < 0 || dev >= kMaxDevices) return fail(RELM_MP_ERR_UNSUPPORTED, "device index out of range.");
+   int* p = g_gave_up_ptr[dev].load(std::memory_order_acquire);
+   if(!p) {
+      void* v = nullptr;
+      if((rc = check_cuda(cudaGetSymbolAddress(&v, g_gave_up), "cudaGetSymbolAddress"))) return rc;
+      p = static_cast< int* >(v);
+      g_gave_up_ptr[dev].store(p, std::memory_order_release);
+   }
+   *out = p;
+   return RELM_MP_OK;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled()
+{
+   static const EncodeTiled fn = [] {
+      void* p = nullptr;
+      cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+      const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found);
+      return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast< EncodeTiled >(p) : nullptr;
+   }();
+   return fn;
+}
+
 }  // namespace
+
+namespace relm_mp {
+namespace attn {
+
+int tc_map(CUtensorMap* map, relm_mp_dtype dtype, const void* base, const int64_t* strides, int dim, int heads, int64_t rows,
+           int64_t seqs)
+{
+   const EncodeTiled fn = encode_tiled();
+   if(!fn) return fail(RELM_MP_ERR_UNSUPPORTED, "cross_attention: the driver has no tensor maps.");
+   const cuuint64_t size[4] = {(cuuint64_t)dim, (cuuint64_t)std::max< int64_t >(rows, 1), (cuuint64_t)heads,
+                               (cuuint64_t)std::max< int64_t >(seqs, 1)};
+   // The stride of an extent of 1 is never used, but has to be one.
+   auto bytes = [&](int64_t v, cuuint64_t extent) { return (cuuint64_t)(extent > 1 ? v * 2 : align_up((size_t)dim * 2, 16)); };
+   const cuuint64_t stride[3] = {bytes(strides[1], size[1]), bytes(strides[2], size[2]), bytes(strides[0], size[3])};
+   const cuuint32_t box[4] = {64, (cuuint32_t)kTileRows, 1, 1}, one[4] = {1, 1, 1, 1};
+   const CUresult e = fn(map, dtype == RELM_MP_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast< void* >(base), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+   if(e != CUDA_SUCCESS)
+      return fail(RELM_MP_ERR_CUDA, "cuTensorMapEncodeTiled: error " + std::to_string((int)e) + ".");
+   return RELM_MP_OK;
+}
+
+}  // namespace attn
+}  // namespace relm_mp
+
+int relm_mp_attn_gave_up(int* flag)
+{
+   if(!flag) return fail(RELM_MP_ERR_INVALID_ARGUMENT, "attn_gave_up: flag must not be NULL.");
+   const int rc = check_cuda(cudaMemcpyFromSymbol(flag, g_gave_up, sizeof(int)), "cudaMemcpyFromSymbol");
+   if(rc || !*flag) return rc;
+   const int zero = 0;
+   return check_cuda(cudaMemcpyToSymbol(g_gave_up, &zero, sizeof(int)), "cudaMemcpyToSymbol");
+}
 
 int relm_mp_attn_plan_init(const int64_t* q_lengths, const int64_t* kv_lengths, int64_t seqs, relm_mp_attn_plan* plan)
 {
@@ -244,6 +330,10 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
    const Counts c = counts(*attn);
    cudaStream_t st = static_cast< cudaStream_t >(stream);
    if(use_split(*attn)) return split_forward(attn->dtype, a, c.kv_blocks, workspace, st);
+   if(use_tc(*attn)) {
+      if((rc = gave_up_address(&a.gave_up))) return rc;
+      return tc_forward(attn->dtype, a, c.q_tiles, c.q_pairs, st);
+   }
    return simt_forward(attn->dtype, a, c.q_tiles, st);
 }
 

@@ -31,6 +31,7 @@ struct Args {
    const void *go;
    const float *lse_in, *delta;
    void *dq, *dk, *dv;
+   int* gave_up; // set by a kernel that gave up waiting
 };
 
 // First row, length and base offset (elements) of one side of a sequence.
@@ -106,6 +107,10 @@ struct SplitPlan {
 };
 SplitPlan split_plan(const Args& a, int64_t blocks);
 int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* workspace, cudaStream_t st);
+
+// Tensor cores: 2-byte types, dim a multiple of 8 up to 128, rows on 16-byte
+// boundaries (relm_mp_attn_tc.cu).
+int tc_forward(relm_mp_dtype dtype, const Args& a, int64_t tiles, int64_t pairs, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace relm_mp

@@ -1,0 +1,174 @@
+// Thin wrappers of the sm_100a instructions that the tensor-core kernels use:
+// mbarriers, tensor-map copies, tensor memory and tcgen05 products.
+#pragma once
+
+#include <cuda.h>
+
+#include "relm_mp_internal.cuh"
+
+namespace relm_mp {
+namespace tc {
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- mbarriers ----------------------------------------------------------------------
+
+__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count)
+{
+   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes)
+{
+   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* b)
+{
+   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity)
+{
+   uint32_t ok;
+   asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                : "=r"(ok)
+                : "r"(smem_addr(b)), "r"(parity)
+                : "memory");
+   return ok != 0;
+}
+__device__ __forceinline__ uint64_t now_ns()
+{
+   uint64_t t;
+   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+   return t;
+}
+
+// Every wait ends: after 2 s it gives up, and the block leaves its loops.
+constexpr uint64_t kWaitNs = 2000000000ull;
+static __device__ __noinline__ bool mbar_wait_slow(uint64_t* b, uint32_t parity)
+{
+   const uint64_t start = now_ns();
+   for(;;) {
+      for(int i = 0; i < 64; ++i)
+         if(mbar_try(b, parity)) return true;
+      if(now_ns() - start > kWaitNs) return false;
+   }
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity)
+{
+   return mbar_try(b, parity) || mbar_wait_slow(b, parity);
+}
+
+// ---- tensor-map copies ----------------------------------------------------------------
+
+// Box at (column, row, head, sequence) of a [seqs, heads, rows, columns] view.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int head, int seq)
+{
+   asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_addr(bar)), "r"(col), "r"(row), "r"(head), "r"(seq)
+      : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map)
+{
+   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// Shared memory written by threads becomes visible to the tensor cores' and copies' reads.
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- tensor memory --------------------------------------------------------------------
+
+// One warp allocates and frees; `columns` is a power of two of at least 32.
+__device__ __forceinline__ void tmem_alloc(uint32_t* where, uint32_t columns)
+{
+   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(columns) : "memory");
+   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns)
+{
+   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Loaded registers may be used from here on: keeps the compiler from moving uses above wait_ld().
+template < int N >
+__device__ __forceinline__ void loaded(uint32_t* v)
+{
+#pragma unroll
+   for(int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
+}
+
+#define RELM_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+#define RELM_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+
+// 32 (or 16) columns of this thread's lane. The lane part of `addr` is the warp's first lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t* v, uint32_t addr)
+{
+   asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : RELM_R8(v, 0), RELM_R8(v, 8), RELM_R8(v, 16), RELM_R8(v, 24)
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t* v, uint32_t addr)
+{
+   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                : RELM_R8(v, 0), RELM_R8(v, 8)
+                : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v)
+{
+   asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      RELM_I8(v, 0), RELM_I8(v, 8), RELM_I8(v, 16), RELM_I8(v, 24)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v)
+{
+   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+                RELM_I8(v, 0), RELM_I8(v, 8)
+                : "memory");
+}
+
+// ---- products -------------------------------------------------------------------------
+
+// Shared-memory operand of 128-byte swizzled panels (64 two-byte columns by rows):
+//  - contraction along the columns: 8-row groups are 1024 bytes apart (`stride`), `lead` unused;
+//  - contraction along the rows: 8-row groups 1024 bytes apart (`stride`), panels `lead` apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead, uint32_t stride)
+{
+   return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// Instruction word: float32 accumulator, both inputs f16 (bf16 if `bf16`), M x N,
+// the right operand's contraction along its rows if `b_rows`.
+__host__ __device__ constexpr uint32_t instruction(bool bf16, int m, int n, bool b_rows)
+{
+   return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_rows ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
+// d (+)= a b^T, both operands in shared memory. One thread issues.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
+{
+   asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+                : "memory");
+}
+// The left operand in tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate)
+{
+   asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+                "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+                : "memory");
+}
+// The barrier completes when all products that this thread has issued are done.
+__device__ __forceinline__ void mma_commit(uint64_t* bar)
+{
+   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+}  // namespace tc
+}  // namespace relm_mp
