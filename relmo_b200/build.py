@@ -48,6 +48,7 @@ CUDA_SOURCES = [
     "relm_mp_attn_simt.cu",
     "relm_mp_attn_split.cu",
     "relm_mp_attn_tc.cu",
+    "relm_mp_attn_tc_bwd.cu",
 ]
 TORCH_SOURCES = ["relm_mp_torch.cpp", "relm_mp_cpu.cpp", "relm_mp_decoder.cpp"]
 HEADERS = ["relm_mp_internal.cuh", "relm_mp_segment.cuh", "relm_mp_seg_impl.cuh", "relm_mp_attn.cuh", "relm_mp_attn_tc.cuh", "relm_mp_tc.cuh"]

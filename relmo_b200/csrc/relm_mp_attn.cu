@@ -114,6 +114,7 @@ Counts counts(const relm_mp_attn& in)
 // 16-byte copies of k and v rows: every row of every head starts on a 16-byte boundary.
 bool aligned_rows(const relm_mp_attn& in)
 {
+   if(!in.q || !in.k || !in.v) return false;
    if(in.dtype == RELM_MP_FLOAT32 || in.dim % 8) return false;
    auto ok = [&](const void* p, const int64_t* s) {
       return (reinterpret_cast< uintptr_t >(p) & 15) == 0 && (in.plan || s[0] % 8 == 0) && s[1] % 8 == 0 && s[2] % 8 == 0;
@@ -133,11 +134,11 @@ bool use_tc(const relm_mp_attn& in)
           ok(in.v_stride, in.kv_rows, in.max_kv, in.kv_heads);
 }
 
-// The form split over the keys takes up to 16 rows (tokens x heads of a group).
-bool use_split(const relm_mp_attn& in)
-{
-   return aligned_rows(in) && in.max_q * (in.heads / in.kv_heads) <= 16;
-}
+// Few query rows (tokens x heads of a group) per sequence: a tile of 128 would be mostly empty.
+bool few_rows(const relm_mp_attn& in) { return in.max_q * (in.heads / in.kv_heads) <= 16; }
+
+// The form split over the keys.
+bool use_split(const relm_mp_attn& in) { return aligned_rows(in) && few_rows(in); }
 
 // delta[head, row] = sum over dim of go * (o + o_rest), in float32; 8 lanes per row and head.
 template < typename T, int VEC >
@@ -225,7 +226,7 @@ namespace relm_mp {
 namespace attn {
 
 int tc_map(CUtensorMap* map, relm_mp_dtype dtype, const void* base, const int64_t* strides, int dim, int heads, int64_t rows,
-           int64_t seqs)
+           int64_t seqs, int box_rows)
 {
    const EncodeTiled fn = encode_tiled();
    if(!fn) return fail(RELM_MP_ERR_UNSUPPORTED, "cross_attention: the driver has no tensor maps.");
@@ -234,7 +235,7 @@ int tc_map(CUtensorMap* map, relm_mp_dtype dtype, const void* base, const int64_
    // The stride of an extent of 1 is never used, but has to be one.
    auto bytes = [&](int64_t v, cuuint64_t extent) { return (cuuint64_t)(extent > 1 ? v * 2 : align_up((size_t)dim * 2, 16)); };
    const cuuint64_t stride[3] = {bytes(strides[1], size[1]), bytes(strides[2], size[2]), bytes(strides[0], size[3])};
-   const cuuint32_t box[4] = {64, (cuuint32_t)kTileRows, 1, 1}, one[4] = {1, 1, 1, 1};
+   const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
    const CUresult e = fn(map, dtype == RELM_MP_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                          const_cast< void* >(base), size, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -330,7 +331,7 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
    const Counts c = counts(*attn);
    cudaStream_t st = static_cast< cudaStream_t >(stream);
    if(use_split(*attn)) return split_forward(attn->dtype, a, c.kv_blocks, workspace, st);
-   if(use_tc(*attn)) {
+   if(use_tc(*attn) && ((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(a.o_rest)) & 15) == 0) {
       if((rc = gave_up_address(&a.gave_up))) return rc;
       return tc_forward(attn->dtype, a, c.q_tiles, c.q_pairs, st);
    }
@@ -366,5 +367,11 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
       if(rc) return rc;
    }
    const Counts c = counts(*attn);
+   const bool aligned = ((reinterpret_cast< uintptr_t >(grad_o) | reinterpret_cast< uintptr_t >(dq) |
+                          reinterpret_cast< uintptr_t >(dk) | reinterpret_cast< uintptr_t >(dv)) & 15) == 0;
+   if(use_tc(*attn) && aligned && !few_rows(*attn)) {
+      if((rc = gave_up_address(&a.gave_up))) return rc;
+      return tc_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);
+   }
    return simt_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);
 }

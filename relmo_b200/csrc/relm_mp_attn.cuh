@@ -111,6 +111,8 @@ int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* work
 // Tensor cores: 2-byte types, dim a multiple of 8 up to 128, rows on 16-byte
 // boundaries (relm_mp_attn_tc.cu).
 int tc_forward(relm_mp_dtype dtype, const Args& a, int64_t tiles, int64_t pairs, cudaStream_t st);
+// (relm_mp_attn_tc_bwd.cu)
+int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace relm_mp

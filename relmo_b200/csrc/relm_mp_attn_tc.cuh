@@ -37,9 +37,10 @@ struct TcMaps {
    CUtensorMap q, k, v, go;
 };
 
-// Tensor map of [seqs, heads, rows, dim] with boxes of 128 rows by 64 columns;
+// Tensor map of [seqs, heads, rows, dim] with boxes of `box_rows` rows by 64 columns;
 // columns past dim and rows past the end read 0.
-int tc_map(CUtensorMap* map, relm_mp_dtype dtype, const void* base, const int64_t* strides, int dim, int heads, int64_t rows, int64_t seqs);
+int tc_map(CUtensorMap* map, relm_mp_dtype dtype, const void* base, const int64_t* strides, int dim, int heads, int64_t rows, int64_t seqs,
+           int box_rows = kTileRows);
 
 }  // namespace attn
 }  // namespace relm_mp

@@ -1,0 +1,574 @@
+// Cross attention on the tensor cores (tcgen05), backward: 2-byte types, head
+// dims up to 128. From the saved lse and delta = sum_d do o:
+//
+//   P = e^(scale S - lse), dS = P (dO V^T - delta)
+//   dV = P^T dO, dK = scale dS^T Q, dQ = scale dS K
+//
+// in two kernels without atomics, so that every run gives the same bits: one per
+// key tile (dK, dV summed in tensor memory over the query tiles of all heads of
+// the group) and one per query tile (dQ over the key tiles). S and dO V^T are
+// computed in both; that is 7 products for 5, and no partial sums in memory.
+//
+// P and dS are rounded to the inputs' type as they enter the second products;
+// scores, weights, differences and all sums are float32. P is held 2^8 times its
+// value (at most 2^8): over long sequences weights of 1 / length would be
+// subnormal in f16. The factor comes off dV at the end, and off dS for free
+// (dO V^T and delta are taken 2^-8 times).
+//
+// Both kernels: one thread copies tiles by tensor map, one issues products, and
+// 8 warps turn S and dO V^T into P and dS in place (two warps share 32 rows, each
+// half of the columns; each half's result stays inside its own half, so no warp
+// overwrites what another has still to read).
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "relm_mp_attn_tc.cuh"
+
+namespace relm_mp {
+namespace attn {
+namespace {
+
+using namespace tc;
+
+constexpr float kUp = 8.f, kDown = 1.f / 256.f; // log2 of P's factor, and its inverse
+constexpr int kSoftThreads = 256, kBwdThreads = kSoftThreads + 64;
+
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// A tile of `rows` rows: panels of 64 columns.
+__host__ __device__ constexpr uint32_t tile_bytes(int dp, int rows) { return (uint32_t)(dp / 64) * rows * 128; }
+
+// N columns of this thread's lane.
+template < int N >
+__device__ __forceinline__ void load_columns(uint32_t* v, uint32_t addr)
+{
+#pragma unroll
+   for(int c = 0; c < N; c += 32) tmem_ld32(v + c, addr + c);
+   wait_ld();
+   loaded< N >(v);
+}
+
+template < int N >
+__device__ __forceinline__ void store_packed(uint32_t addr, const uint32_t* v)
+{
+#pragma unroll
+   for(int c = 0; c < N; c += 16) tmem_st16(addr + c, v + c);
+}
+
+// Zeroes row `row` of a tile.
+template < int DP >
+__device__ __forceinline__ void clear_row(unsigned char* tile, int rows, int row)
+{
+#pragma unroll
+   for(int p = 0; p < DP / 64; ++p) {
+      uint4* line = reinterpret_cast< uint4* >(tile + p * rows * 128 + row * 128);
+#pragma unroll
+      for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
+   }
+}
+
+// 32 accumulator rows of a warp, times `mul`, to rows of `out` (row pitch
+// `pitch` elements) through `stage` (32 rows of DP elements, this warp's own).
+template < typename T, int DP >
+__device__ __forceinline__ void store_rows(uint32_t acc, bool any, bool ok, float mul, unsigned char* stage, T* out, int64_t pitch,
+                                           int rows, int dim)
+{
+   const int lane = threadIdx.x & 31;
+#pragma unroll
+   for(int c = 0; c < DP; c += 16) {
+      if(c >= dim) break;
+      uint32_t v[16], w[8];
+      if(any) {
+         tmem_ld16(v, acc + c);
+         wait_ld();
+         loaded< 16 >(v);
+      }
+#pragma unroll
+      for(int i = 0; i < 8; ++i) {
+         const float x = any ? __uint_as_float(v[2 * i]) * mul : 0.f, y = any ? __uint_as_float(v[2 * i + 1]) * mul : 0.f;
+         w[i] = ok ? pack2< T >(x, y) : pack2< T >(CUDART_NAN_F, CUDART_NAN_F);
+      }
+#pragma unroll
+      for(int h = 0; h < 2; ++h)
+         *reinterpret_cast< uint4* >(stage + lane * (DP * 2) + (((c >> 3) + h) ^ (lane & 7)) * 16) =
+            make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+   }
+   __syncwarp();
+   constexpr int CH = DP / 8;
+#pragma unroll 4
+   for(int i = lane; i < 32 * CH; i += 32) {
+      const int r = i / CH, c = i % CH;
+      if(r < rows && c * 8 < dim)
+         *reinterpret_cast< uint4* >(out + r * pitch + c * 8) = *reinterpret_cast< const uint4* >(stage + r * (DP * 2) + ((c ^ (r & 7)) * 16));
+   }
+   __syncwarp();
+}
+
+// ---- dK, dV: one key tile, all query tiles of the group ------------------------------
+
+template < int DP, int QN >
+struct Kv {
+   static constexpr int ST = 2;
+   static constexpr uint32_t KT = tile_bytes(DP, kTileRows), QT = tile_bytes(DP, QN);
+   static constexpr uint32_t K = 0, V = KT, Q = 2 * KT, G = Q + ST * QT, BYTES = G + ST * QT;
+   static constexpr uint32_t S = 0, P = QN, DV = 2 * QN, DK = 2 * QN + DP, COLS = 2 * (QN + DP);
+   static constexpr int RESIDENT = COLS <= 256 ? 2 : 1;
+};
+
+template < typename T, int DP, int QN >
+__global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
+   k_attn_tc_backward_kv(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                         const __grid_constant__ CUtensorMap vm, const __grid_constant__ CUtensorMap gm)
+{
+   using L = Kv< DP, QN >;
+   constexpr int HALF = QN / 2;
+   constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
+   extern __shared__ unsigned char raw[];
+   unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+   __shared__ uint64_t kv_full, q_full[L::ST], q_empty[L::ST], s_full, dp_full, p_full, ds_full, done;
+   __shared__ float4 s_lse[2][QN / 4], s_delta[2][QN / 4];
+   __shared__ uint32_t tmem_base;
+   __shared__ int gave_up;
+   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
+   const Item it = item(a.kv_tiles, a.max_kv, kTileRows, blockIdx.x);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const int key0 = it.tile * kTileRows;
+   const int q_tiles = (qs.len + QN - 1) / QN, n = q_tiles * group;
+
+   if(threadIdx.x == 0) {
+      mbar_init(&kv_full, 1);
+      for(int s = 0; s < L::ST; ++s) {
+         mbar_init(&q_full[s], 1);
+         mbar_init(&q_empty[s], 1);
+      }
+      mbar_init(&s_full, 1);
+      mbar_init(&dp_full, 1);
+      mbar_init(&p_full, kSoftThreads);
+      mbar_init(&ds_full, kSoftThreads);
+      mbar_init(&done, 1);
+      mbar_init_fence();
+      gave_up = 0;
+   }
+   if(warp == 8) tmem_alloc(&tmem_base, L::COLS);
+   fence_before();
+   __syncthreads();
+   fence_after();
+   const uint32_t tmem = tmem_base, base = smem_addr(sm);
+
+   if(warp == 9) { // copies
+      if(lane == 0 && n > 0) {
+         const int qr = (int)(a.q_off ? qs.first : 0), kr = (int)(a.kv_off ? ks.first : 0) + key0, b = a.q_off ? 0 : it.seq;
+         mbar_expect(&kv_full, 2 * L::KT);
+         for(int p = 0; p < DP / 64; ++p) {
+            tma_load(base + L::K + p * kTileRows * 128, &km, &kv_full, p * 64, kr, kv_head, b);
+            tma_load(base + L::V + p * kTileRows * 128, &vm, &kv_full, p * 64, kr, kv_head, b);
+         }
+         int issued = 0;
+         for(int i = 0; i < n; ++i) {
+            const int s = i % L::ST, round = i / L::ST;
+            if(round && !mbar_wait(&q_empty[s], (round - 1) & 1)) break;
+            const int head = kv_head * group + i / q_tiles, row = qr + (i % q_tiles) * QN;
+            mbar_expect(&q_full[s], 2 * L::QT);
+            for(int p = 0; p < DP / 64; ++p) {
+               tma_load(base + L::Q + s * L::QT + p * QN * 128, &qm, &q_full[s], p * 64, row, head, b);
+               tma_load(base + L::G + s * L::QT + p * QN * 128, &gm, &q_full[s], p * 64, row, head, b);
+            }
+            issued = i + 1;
+         }
+         if(issued < n) { // nothing may still be written to shared memory when the block ends
+            gave_up = 1;
+            mbar_wait(&kv_full, 0);
+            for(int i = issued > L::ST ? issued - L::ST : 0; i < issued; ++i) mbar_wait(&q_full[i % L::ST], (i / L::ST) & 1);
+         }
+      }
+   } else if(warp == 8) { // products
+      if(lane == 0 && n > 0) {
+         const int steps = (a.dim + 15) / 16;
+         const uint32_t out_id = instruction(BF, 128, steps * 16, true);
+         auto cols = [&](int i) { return min(QN, (qs.len - (i % q_tiles) * QN + 15) / 16 * 16); };
+         // S^T = K Q^T or dP^T = V dO^T
+         auto first = [&](uint32_t d, uint32_t left, uint32_t right, int i, uint64_t* bar) {
+            const uint32_t id = instruction(BF, 128, cols(i), false);
+            for(int k = 0; k < steps; ++k)
+               mma_ss(tmem + d, operand(base + left + (k >> 2) * kTileRows * 128 + (k & 3) * 32, 16, 1024),
+                      operand(base + right + (i % L::ST) * L::QT + (k >> 2) * QN * 128 + (k & 3) * 32, 16, 1024), id, k > 0);
+            mma_commit(bar);
+         };
+         // dV += P^T dO or dK += dS^T Q; the halves of the left operand start HALF columns apart
+         auto second = [&](uint32_t d, uint32_t left, uint32_t right, int i) {
+            const int ks16 = cols(i) / 16;
+            for(int k = 0; k < ks16; ++k) {
+               const uint32_t at = left + (k >= HALF / 16 ? HALF + (k - HALF / 16) * 8 : k * 8);
+               mma_ts(tmem + d, tmem + at, operand(base + right + (i % L::ST) * L::QT + k * 2048, QN * 128, 1024), out_id, i > 0 || k > 0);
+            }
+         };
+         bool ok = mbar_wait(&kv_full, 0) && mbar_wait(&q_full[0], 0);
+         if(ok) {
+            first(L::S, L::K, L::Q, 0, &s_full);
+            first(L::P, L::V, L::G, 0, &dp_full);
+         }
+         for(int i = 0; i < n && ok; ++i) {
+            if(!(ok = mbar_wait(&p_full, i & 1))) break;
+            fence_after();
+            second(L::DV, L::S, L::G, i);
+            if(i + 1 < n) {
+               if(!(ok = mbar_wait(&q_full[(i + 1) % L::ST], ((i + 1) / L::ST) & 1))) break;
+               first(L::S, L::K, L::Q, i + 1, &s_full);
+            }
+            if(!(ok = mbar_wait(&ds_full, i & 1))) break;
+            fence_after();
+            second(L::DK, L::P, L::Q, i);
+            mma_commit(&q_empty[i % L::ST]);
+            if(i + 1 < n) first(L::P, L::V, L::G, i + 1, &dp_full);
+         }
+         mma_commit(&done);
+         if(!ok) {
+            gave_up = 1;
+            mbar_wait(&done, 0); // products in flight read shared and tensor memory
+         }
+      }
+   } else { // lanes are keys, columns queries
+      const int half = warp >> 2, row = (warp & 3) * 32 + lane, key = key0 + row;
+      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16);
+      const uint32_t st = lanes + L::S + half * HALF, pt = lanes + L::P + half * HALF;
+      const bool in = key < ks.len && (!a.mask || a.mask[ks.first + key]);
+      const float sc = a.scale * kLog2e;
+      // What this thread puts into shared memory for iteration i: an lse (log2) or a delta.
+      const int col = threadIdx.x % QN;
+      const bool puts_lse = threadIdx.x < QN, puts = threadIdx.x < 2 * QN;
+      auto fetch = [&](int i) {
+         const int q = (i % q_tiles) * QN + col;
+         if(!puts || i >= n || q >= qs.len) return puts_lse ? CUDART_INF_F : 0.f;
+         const int64_t at = (int64_t)(kv_head * group + i / q_tiles) * a.q_rows + qs.first + q;
+         if(!puts_lse) return a.delta[at] * kDown;
+         const float v = a.lse_in[at];
+         return v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e - kUp; // a row without keys: weights 0
+      };
+      float next = n > 0 ? fetch(0) : 0.f;
+      bool ok = true;
+      for(int i = 0; i < n; ++i) {
+         const int valid = min(QN, qs.len - (i % q_tiles) * QN);
+         if(puts) reinterpret_cast< float* >(puts_lse ? s_lse[i & 1] : s_delta[i & 1])[col] = next;
+         soft_sync();
+         next = fetch(i + 1);
+         ok = ok && __all_sync(~0u, mbar_wait(&s_full, i & 1));
+         fence_after();
+         uint32_t s[HALF];
+         load_columns< HALF >(s, st);
+         const float4* lse = s_lse[i & 1] + half * (HALF / 4);
+         const bool tail = valid < QN;
+#pragma unroll
+         for(int c = 0; c < HALF / 4; ++c) {
+            const float4 v = lse[c];
+#pragma unroll
+            for(int e = 0; e < 4; ++e) {
+               const float L2 = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+               float p = exp2_fast(fmaf(__uint_as_float(s[4 * c + e]), sc, -L2));
+               if(!in || (tail && half * HALF + 4 * c + e >= valid)) p = 0.f;
+               s[4 * c + e] = __float_as_uint(p);
+            }
+         }
+         uint32_t w[HALF / 2];
+#pragma unroll
+         for(int c = 0; c < HALF / 2; ++c) w[c] = pack2< T >(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+         store_packed< HALF / 2 >(st, w);
+         if(tail) { // rows of dO and Q past the sequence: their weights are 0, so must they be
+            ok = ok && __all_sync(~0u, mbar_wait(&dp_full, i & 1));
+            const int r = threadIdx.x % QN;
+            if(puts && r >= valid) clear_row< DP >(sm + (puts_lse ? L::Q : L::G) + (i % L::ST) * L::QT, QN, r);
+            fence_async_proxy();
+         }
+         wait_st();
+         fence_before();
+         mbar_arrive(&p_full);
+         ok = ok && __all_sync(~0u, mbar_wait(&dp_full, i & 1));
+         fence_after();
+         uint32_t d[HALF];
+         load_columns< HALF >(d, pt);
+         const float4* delta = s_delta[i & 1] + half * (HALF / 4);
+#pragma unroll
+         for(int c = 0; c < HALF / 4; ++c) {
+            const float4 v = delta[c];
+            float x[4];
+#pragma unroll
+            for(int e = 0; e < 4; ++e) {
+               const float D = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
+               x[e] = __uint_as_float(s[4 * c + e]) * fmaf(__uint_as_float(d[4 * c + e]), kDown, -D);
+               if(!in || (tail && half * HALF + 4 * c + e >= valid)) x[e] = 0.f;
+            }
+            w[2 * c] = pack2< T >(x[0], x[1]);
+            w[2 * c + 1] = pack2< T >(x[2], x[3]);
+         }
+         store_packed< HALF / 2 >(pt, w);
+         wait_st();
+         fence_before();
+         mbar_arrive(&ds_full);
+      }
+      if(n > 0) ok = ok && __all_sync(~0u, mbar_wait(&done, 0));
+      fence_after();
+      if(!ok) gave_up = 1;
+      // First half of the warps: dV, second: dK; through the K and V tiles (their products are done).
+      const int k0 = key0 + (warp & 3) * 32;
+      T* out = static_cast< T* >(half ? a.dk : a.dv) + ((ks.first + k0) * a.kv_heads + kv_head) * a.dim;
+      store_rows< T, DP >(lanes + (half ? L::DK : L::DV), n > 0, ok, half ? a.scale : kDown,
+                          sm + (half ? L::V : L::K) + (warp & 3) * 32 * (DP * 2), out, (int64_t)a.kv_heads * a.dim, ks.len - k0, a.dim);
+   }
+   fence_before();
+   __syncthreads();
+   fence_after();
+   if(warp == 8) tmem_free(tmem, L::COLS);
+   if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
+}
+
+// ---- dQ: one query tile, all key tiles ------------------------------------------------
+
+template < int DP, int KN >
+struct Dq {
+   static constexpr int ST = 2;
+   static constexpr uint32_t QT = tile_bytes(DP, kTileRows), KT = tile_bytes(DP, KN);
+   static constexpr uint32_t Q = 0, G = QT, K = 2 * QT, V = K + ST * KT, BYTES = V + ST * KT;
+   static constexpr uint32_t S = 0, P = 2 * KN, DQ = 3 * KN, COLS = 3 * KN + DP; // two S tiles
+   static constexpr int RESIDENT = COLS <= 256 ? 2 : 1;
+};
+
+template < typename T, int DP, int KN >
+__global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
+   k_attn_tc_backward_q(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                        const __grid_constant__ CUtensorMap vm, const __grid_constant__ CUtensorMap gm)
+{
+   using L = Dq< DP, KN >;
+   constexpr int HALF = KN / 2;
+   constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
+   extern __shared__ unsigned char raw[];
+   unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+   __shared__ uint64_t q_full, k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], s_full[2], dp_full, ds_full, done;
+   __shared__ uint32_t tmem_base;
+   __shared__ int gave_up;
+   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const int row0 = it.tile * kTileRows, n = (ks.len + KN - 1) / KN;
+
+   if(threadIdx.x == 0) {
+      mbar_init(&q_full, 1);
+      for(int s = 0; s < L::ST; ++s) {
+         mbar_init(&k_full[s], 1);
+         mbar_init(&k_empty[s], 1);
+         mbar_init(&v_full[s], 1);
+         mbar_init(&v_empty[s], 1);
+         mbar_init(&s_full[s], 1);
+      }
+      mbar_init(&dp_full, 1);
+      mbar_init(&ds_full, kSoftThreads);
+      mbar_init(&done, 1);
+      mbar_init_fence();
+      gave_up = 0;
+   }
+   if(warp == 8) tmem_alloc(&tmem_base, L::COLS);
+   fence_before();
+   __syncthreads();
+   fence_after();
+   const uint32_t tmem = tmem_base, base = smem_addr(sm);
+
+   if(warp == 9) { // copies
+      if(lane == 0 && n > 0) {
+         const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0), b = a.q_off ? 0 : it.seq;
+         mbar_expect(&q_full, 2 * L::QT);
+         for(int p = 0; p < DP / 64; ++p) {
+            tma_load(base + L::Q + p * kTileRows * 128, &qm, &q_full, p * 64, qr, head, b);
+            tma_load(base + L::G + p * kTileRows * 128, &gm, &q_full, p * 64, qr, head, b);
+         }
+         int issued = 0;
+         for(int j = 0; j < n; ++j) {
+            const int s = j % L::ST, round = j / L::ST;
+            if(round && !(mbar_wait(&k_empty[s], (round - 1) & 1) && mbar_wait(&v_empty[s], (round - 1) & 1))) break;
+            mbar_expect(&k_full[s], L::KT);
+            for(int p = 0; p < DP / 64; ++p) tma_load(base + L::K + s * L::KT + p * KN * 128, &km, &k_full[s], p * 64, kr + j * KN, kv_head, b);
+            mbar_expect(&v_full[s], L::KT);
+            for(int p = 0; p < DP / 64; ++p) tma_load(base + L::V + s * L::KT + p * KN * 128, &vm, &v_full[s], p * 64, kr + j * KN, kv_head, b);
+            issued = j + 1;
+         }
+         if(issued < n) { // nothing may still be written to shared memory when the block ends
+            gave_up = 1;
+            mbar_wait(&q_full, 0);
+            for(int j = issued > L::ST ? issued - L::ST : 0; j < issued; ++j) {
+               mbar_wait(&k_full[j % L::ST], (j / L::ST) & 1);
+               mbar_wait(&v_full[j % L::ST], (j / L::ST) & 1);
+            }
+         }
+      }
+   } else if(warp == 8) { // products
+      if(lane == 0 && n > 0) {
+         const int steps = (a.dim + 15) / 16;
+         const uint32_t out_id = instruction(BF, 128, steps * 16, true);
+         auto cols = [&](int j) { return min(KN, (ks.len - j * KN + 15) / 16 * 16); };
+         // S = Q K^T or dP = dO V^T
+         auto first = [&](uint32_t d, uint32_t left, uint32_t right, int j, uint64_t* bar) {
+            const uint32_t id = instruction(BF, 128, cols(j), false);
+            for(int k = 0; k < steps; ++k)
+               mma_ss(tmem + d, operand(base + left + (k >> 2) * kTileRows * 128 + (k & 3) * 32, 16, 1024),
+                      operand(base + right + (j % L::ST) * L::KT + (k >> 2) * KN * 128 + (k & 3) * 32, 16, 1024), id, k > 0);
+            mma_commit(bar);
+         };
+         bool ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
+         if(ok) first(L::S, L::Q, L::K, 0, &s_full[0]);
+         ok = ok && mbar_wait(&v_full[0], 0);
+         if(ok) {
+            first(L::P, L::G, L::V, 0, &dp_full);
+            mma_commit(&v_empty[0]);
+         }
+         for(int j = 0; j < n && ok; ++j) {
+            if(j + 1 < n) { // S of the next tile while this one's dS is in the making
+               if(!(ok = mbar_wait(&k_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1))) break;
+               first(L::S + ((j + 1) & 1) * KN, L::Q, L::K, j + 1, &s_full[(j + 1) & 1]);
+            }
+            if(!(ok = mbar_wait(&ds_full, j & 1))) break;
+            fence_after();
+            const int ks16 = cols(j) / 16;
+            for(int k = 0; k < ks16; ++k) {
+               const uint32_t at = L::P + (k >= HALF / 16 ? HALF + (k - HALF / 16) * 8 : k * 8);
+               mma_ts(tmem + L::DQ, tmem + at, operand(base + L::K + (j % L::ST) * L::KT + k * 2048, KN * 128, 1024), out_id, j > 0 || k > 0);
+            }
+            mma_commit(&k_empty[j % L::ST]);
+            if(j + 1 < n) {
+               if(!(ok = mbar_wait(&v_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1))) break;
+               first(L::P, L::G, L::V, j + 1, &dp_full);
+               mma_commit(&v_empty[(j + 1) % L::ST]);
+            }
+         }
+         mma_commit(&done);
+         if(!ok) {
+            gave_up = 1;
+            mbar_wait(&done, 0); // products in flight read shared and tensor memory
+         }
+      }
+   } else { // lanes are queries, columns keys
+      const int half = warp >> 2, row = row0 + (warp & 3) * 32 + lane;
+      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16);
+      const uint32_t pt = lanes + L::P + half * HALF;
+      const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+      const float sc = a.scale * kLog2e;
+      float lse = CUDART_INF_F, delta = 0.f; // rows past the sequence or without keys: weights 0
+      if(row < qs.len) {
+         const int64_t at = (int64_t)head * a.q_rows + qs.first + row;
+         const float v = a.lse_in[at];
+         if(v != -CUDART_INF_F) lse = v * kLog2e;
+         delta = a.delta[at];
+      }
+      bool ok = true;
+      for(int j = 0; j < n; ++j) {
+         const int left = ks.len - j * KN;
+         bool all = left >= KN && !keep;
+         unsigned bits[HALF / 32];
+#pragma unroll
+         for(int c = 0; c < HALF / 32; ++c) {
+            const int key = half * HALF + c * 32 + lane;
+            bits[c] = all ? ~0u : __ballot_sync(~0u, key < left && (!keep || keep[j * KN + key]));
+         }
+         ok = ok && __all_sync(~0u, mbar_wait(&s_full[j & 1], (j >> 1) & 1));
+         fence_after();
+         uint32_t s[HALF];
+         load_columns< HALF >(s, lanes + L::S + (j & 1) * KN + half * HALF);
+#pragma unroll
+         for(int c = 0; c < HALF; ++c) {
+            float p = exp2_fast(fmaf(__uint_as_float(s[c]), sc, -lse));
+            if(!all && !(bits[c / 32] >> (c % 32) & 1)) p = 0.f;
+            s[c] = __float_as_uint(p);
+         }
+         if(!all && (warp & 3) * 32 < HALF) { // masked rows of K, read by dS K next, S is done with them
+            const int r = (warp & 3) * 32 + lane;
+            bool mine = false;
+#pragma unroll
+            for(int c = 0; c < HALF / 32; ++c)
+               if(c == (warp & 3)) mine = bits[c] >> lane & 1;
+            if(!mine) clear_row< DP >(sm + L::K + (j % L::ST) * L::KT, KN, half * HALF + r);
+            fence_async_proxy();
+         }
+         ok = ok && __all_sync(~0u, mbar_wait(&dp_full, j & 1));
+         fence_after();
+         uint32_t d[HALF], w[HALF / 2];
+         load_columns< HALF >(d, pt);
+#pragma unroll
+         for(int c = 0; c < HALF / 2; ++c) {
+            float x = __uint_as_float(s[2 * c]) * (__uint_as_float(d[2 * c]) - delta);
+            float y = __uint_as_float(s[2 * c + 1]) * (__uint_as_float(d[2 * c + 1]) - delta);
+            if(!all) { // dO V^T of a masked key may be anything
+               if(!(bits[c / 16] >> (2 * c % 32) & 1)) x = 0.f;
+               if(!(bits[c / 16] >> (2 * c % 32 + 1) & 1)) y = 0.f;
+            }
+            w[c] = pack2< T >(x, y);
+         }
+         store_packed< HALF / 2 >(pt, w);
+         wait_st();
+         fence_before();
+         mbar_arrive(&ds_full);
+      }
+      if(n > 0) ok = ok && __all_sync(~0u, mbar_wait(&done, 0));
+      fence_after();
+      if(!ok) gave_up = 1;
+      // Through the Q tile's shared memory; the two warps of 32 rows take half of the columns' work each way: the first writes.
+      const int r0 = row0 + (warp & 3) * 32;
+      if(half == 0) {
+         T* out = static_cast< T* >(a.dq) + ((qs.first + r0) * a.heads + head) * a.dim;
+         store_rows< T, DP >(lanes + L::DQ, n > 0, ok, a.scale, sm + L::Q + (warp & 3) * 32 * (DP * 2), out, (int64_t)a.heads * a.dim,
+                             qs.len - r0, a.dim);
+      }
+   }
+   fence_before();
+   __syncthreads();
+   fence_after();
+   if(warp == 8) tmem_free(tmem, L::COLS);
+   if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
+}
+
+template < typename F >
+int launch(F fn, int bytes, dim3 grid, const Args& a, const TcMaps& m, cudaStream_t st, const char* what)
+{
+   if(grid.x == 0) return RELM_MP_OK;
+   int rc = check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+   if(rc) return rc;
+   fn<<< grid, kBwdThreads, bytes, st >>>(a, m.q, m.k, m.v, m.go);
+   return check_launch(what);
+}
+
+// N: rows of the streamed tile of both kernels.
+template < typename T, int DP, int N >
+int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st)
+{
+   const bool packed = a.q_off != nullptr;
+   const int64_t qrows = packed ? a.q_rows : a.max_q, krows = packed ? a.kv_rows : a.max_kv, seqs = packed ? 1 : a.seqs;
+   const int64_t gs[3] = {a.max_q * a.heads * a.dim, (int64_t)a.heads * a.dim, a.dim};
+   auto maps = [&](TcMaps* m, int q_box, int k_box) {
+      int rc;
+      if((rc = tc_map(&m->q, dtype, a.q, a.qs, a.dim, a.heads, qrows, seqs, q_box))) return rc;
+      if((rc = tc_map(&m->go, dtype, a.go, gs, a.dim, a.heads, qrows, seqs, q_box))) return rc;
+      if((rc = tc_map(&m->k, dtype, a.k, a.ks, a.dim, a.kv_heads, krows, seqs, k_box))) return rc;
+      return tc_map(&m->v, dtype, a.v, a.vs, a.dim, a.kv_heads, krows, seqs, k_box);
+   };
+   TcMaps m;
+   int rc;
+   if((rc = maps(&m, N, kTileRows))) return rc;
+   if((rc = launch(k_attn_tc_backward_kv< T, DP, N >, (int)Kv< DP, N >::BYTES + 1024, dim3((unsigned)kv_tiles, a.kv_heads), a, m, st,
+                   "k_attn_tc_backward_kv")))
+      return rc;
+   if(N != kTileRows && (rc = maps(&m, kTileRows, N))) return rc;
+   return launch(k_attn_tc_backward_q< T, DP, N >, (int)Dq< DP, N >::BYTES + 1024, dim3((unsigned)q_tiles, a.heads), a, m, st,
+                 "k_attn_tc_backward_q");
+}
+
+}  // namespace
+
+int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st)
+{
+   if(dtype == RELM_MP_BFLOAT16)
+      return a.dim <= 64 ? backward< __nv_bfloat16, 64, 64 >(dtype, a, q_tiles, kv_tiles, st)
+                         : backward< __nv_bfloat16, 128, 128 >(dtype, a, q_tiles, kv_tiles, st);
+   return a.dim <= 64 ? backward< __half, 64, 64 >(dtype, a, q_tiles, kv_tiles, st)
+                      : backward< __half, 128, 128 >(dtype, a, q_tiles, kv_tiles, st);
+}
+
+}  // namespace attn
+}  // namespace relm_mp
