@@ -3,7 +3,8 @@
 //
 // A block owns QT tiles of 128 query rows of one head and walks the keys in
 // tiles of 128. One thread copies k and v tiles by tensor map, one thread issues
-// the products, and four warps per query tile do the softmax, a thread per row:
+// the products, two warps see to masked keys, and four warps per query tile do
+// the softmax, a thread per row:
 //
 //   S = Q K^T          both operands in shared memory, S (float32) in tensor memory
 //   P = 2^(sc S - m)   rounded to the inputs' type, written over S
@@ -30,6 +31,7 @@ namespace {
 using namespace tc;
 
 constexpr float kGrow = 8.f;
+constexpr int kBitSlots = 4;
 
 template < int DP, int QT >
 struct Fwd {
@@ -38,8 +40,41 @@ struct Fwd {
    static constexpr uint32_t PANEL = kTileRows * 128, TILE = PANELS * PANEL;
    static constexpr uint32_t Q = 0, K = QT * TILE, V = K + ST * TILE, BYTES = V + ST * TILE;
    static constexpr uint32_t COLS = QT == 2 ? 512 : 256, O = QT * 128; // tensor memory: S tiles, then O tiles
-   static constexpr int THREADS = QT * 128 + 64;
+   static constexpr int THREADS = QT * 128 + 128;
 };
+
+// Largest of 32 scores, in four independent chains.
+__device__ __forceinline__ float largest(const uint32_t* s, float top)
+{
+   float m[4] = {top, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+   for(int i = 0; i < 32; i += 8)
+#pragma unroll
+      for(int k = 0; k < 4; ++k) m[k] = fmaxf(fmaxf(m[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
+   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+__device__ __forceinline__ void hide(uint32_t* s, unsigned bits)
+{
+#pragma unroll
+   for(int i = 0; i < 32; ++i)
+      if(!(bits >> i & 1)) s[i] = 0xff800000u;
+}
+
+// 32 scores to weights 2^(sc s - ref), added to `sum` unrounded and packed.
+template < typename T >
+__device__ __forceinline__ void exponents(const uint32_t* s, uint32_t* p, uint64_t sc, uint64_t ref, uint64_t (&sum)[2])
+{
+#pragma unroll
+   for(int i = 0; i < 16; ++i) {
+      float x, y;
+      unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc, ref), x, y);
+      x = exp2_fast(x);
+      y = exp2_fast(y);
+      sum[i & 1] = add2(sum[i & 1], pair(x, y));
+      p[i] = pack2< T >(x, y);
+   }
+}
 
 template < typename T, int DP, int QT >
 __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
@@ -49,7 +84,9 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    using L = Fwd< DP, QT >;
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-   __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], s_full[QT], p_full[QT], o_full[QT];
+   __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
+   __shared__ uint64_t s_full[QT], p_full[QT][2], o_full[QT], bits_full[kBitSlots], v_last;
+   __shared__ unsigned s_bits[kBitSlots][4];
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -59,13 +96,15 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    const int row0 = it.tile * QT * kTileRows;
    const int active = QT == 1 || row0 + kTileRows >= qs.len ? 1 : QT;
    const int tiles = (ks.len + kTileRows - 1) / kTileRows;
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
    constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
 
    if(threadIdx.x == 0) {
       for(int t = 0; t < QT; ++t) {
          mbar_init(&q_full[t], 1);
          mbar_init(&s_full[t], 1);
-         mbar_init(&p_full[t], 128);
+         mbar_init(&p_full[t][0], 128);
+         mbar_init(&p_full[t][1], 128);
          mbar_init(&o_full[t], 1);
       }
       for(int s = 0; s < L::ST; ++s) {
@@ -73,7 +112,10 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          mbar_init(&k_empty[s], 1);
          mbar_init(&v_full[s], 1);
          mbar_init(&v_empty[s], 1);
+         mbar_init(&v_clean[s], 2);
       }
+      for(int s = 0; s < kBitSlots; ++s) mbar_init(&bits_full[s], 2);
+      mbar_init(&v_last, 1);
       mbar_init_fence();
       gave_up = 0;
    }
@@ -83,6 +125,9 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    fence_after();
    const uint32_t tmem = tmem_base;
    const uint32_t base = smem_addr(sm);
+   // Tiles with keys that take no part: all where there is a mask, else the last if it ends inside.
+   auto dirty = [&](int j) { return keep != nullptr || ks.len - j * kTileRows < kTileRows; };
+   auto dirty_parity = [&](int round) { return keep ? round & 1 : 0; };
 
    if(warp == QT * 4 + 1) { // copies
       if(lane == 0 && tiles > 0) {
@@ -138,14 +183,21 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          }
          if(ok) mma_commit(&k_empty[0]);
          for(int j = 0; j < tiles && ok; ++j) {
-            const int n = keys16(j) / 16;
+            const int n = keys16(j) / 16, s = j % L::ST, round = j / L::ST;
+            ok = mbar_wait(&v_full[s], round & 1);
+            if(ok && dirty(j)) {
+               if(!keep) mbar_arrive(&v_last);
+               ok = mbar_wait(&v_clean[s], dirty_parity(round));
+            }
             for(int t = 0; t < active && ok; ++t) {
-               ok = mbar_wait(&p_full[t], j & 1) && mbar_wait(&v_full[j % L::ST], (j / L::ST) & 1);
+               const uint32_t va = base + L::V + s * L::TILE;
+               for(int h = 0; h < 2 && ok; ++h) { // the weights come in two halves of 64 keys
+                  if(!(ok = mbar_wait(&p_full[t][h], j & 1))) break;
+                  fence_after();
+                  for(int i = 4 * h; i < min(n, 4 * h + 4); ++i)
+                     mma_ts(tmem + L::O + t * DP, tmem + t * 128 + i * 8, operand(va + i * 2048, L::PANEL, 1024), pv, j > 0 || i > 0);
+               }
                if(!ok) break;
-               fence_after();
-               const uint32_t va = base + L::V + (j % L::ST) * L::TILE;
-               for(int i = 0; i < n; ++i)
-                  mma_ts(tmem + L::O + t * DP, tmem + t * 128 + i * 8, operand(va + i * 2048, L::PANEL, 1024), pv, j > 0 || i > 0);
                if(j + 1 == tiles) mma_commit(&o_full[t]);
                else {
                   ok = mbar_wait(&k_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1);
@@ -153,7 +205,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                }
             }
             if(!ok) break;
-            mma_commit(&v_empty[j % L::ST]);
+            mma_commit(&v_empty[s]);
             if(j + 1 < tiles) mma_commit(&k_empty[(j + 1) % L::ST]);
          }
          if(!ok) {
@@ -163,68 +215,98 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             mbar_wait(&q_full[0], 1);
          }
       }
+   } else if(warp >= QT * 4 + 2) { // masks: 64 keys of each tile per warp
+      const int w = warp - (QT * 4 + 2);
+      for(int j = keep ? 0 : max(tiles - 1, 0); j < tiles; ++j) {
+         if(!dirty(j)) break;
+         const int left = ks.len - j * kTileRows, s = j % L::ST;
+         unsigned bits[2];
+#pragma unroll
+         for(int c = 0; c < 2; ++c) {
+            const int key = w * 64 + c * 32 + lane;
+            bits[c] = __ballot_sync(~0u, key < left && (!keep || keep[j * kTileRows + key]));
+         }
+         // The slot's last reader was tile j - 4; v of tile j - 1 arrived after the products of tile j - 3 or later.
+         if(keep && lane == 0) {
+            s_bits[j % kBitSlots][2 * w] = bits[0];
+            s_bits[j % kBitSlots][2 * w + 1] = bits[1];
+            mbar_arrive(&bits_full[j % kBitSlots]);
+         }
+         // Without a mask this warp has not followed the phases of v_full: it is called for the last tile.
+         if(!__all_sync(~0u, (keep || mbar_wait(&v_last, 0)) && mbar_wait(&v_full[s], (j / L::ST) & 1))) {
+            gave_up = 1;
+            break;
+         }
+#pragma unroll
+         for(int c = 0; c < 2; ++c)
+            if(!(bits[c] >> lane & 1))
+               for(int p = 0; p < L::PANELS; ++p) {
+                  uint4* line = reinterpret_cast< uint4* >(sm + L::V + s * L::TILE + p * L::PANEL + (w * 64 + c * 32 + lane) * 128);
+#pragma unroll
+                  for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
+               }
+         fence_async_proxy();
+         __syncwarp();
+         if(lane == 0) mbar_arrive(&v_clean[s]);
+      }
    } else { // softmax: thread = row of tile t
-      const int t = warp >> 2, row = threadIdx.x & 127;
+      const int t = warp >> 2;
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), st = lanes + t * 128, ot = lanes + L::O + t * DP;
-      const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
       const float sc = a.scale * kLog2e;
-      float m = -CUDART_INF_F, l = 0.f;
+      const uint64_t sc2 = pair(sc, sc);
+      float m = -CUDART_INF_F;
+      uint64_t sum[2] = {0, 0};
       bool ok = true;
       if(t < active) {
          for(int j = 0; j < tiles && ok; ++j) {
             const int left = ks.len - j * kTileRows, chunks = min(4, (left + 31) / 32);
-            unsigned bits[4];
-            bool all = left >= kTileRows && !keep;
+            unsigned bits[4] = {~0u, ~0u, ~0u, ~0u};
+            const bool partial = dirty(j);
+            if(keep) {
+               ok = __all_sync(~0u, mbar_wait(&bits_full[j % kBitSlots], (j / kBitSlots) & 1));
 #pragma unroll
-            for(int c = 0; c < 4; ++c) {
-               if(all) bits[c] = ~0u;
-               else {
-                  const int key = c * 32 + lane;
-                  bits[c] = __ballot_sync(~0u, key < left && (!keep || keep[j * kTileRows + key]));
-               }
-            }
-            all = all || (bits[0] & bits[1] & bits[2] & bits[3]) == ~0u;
-            if(!all && t == 0) { // rows of v that take no part
-               ok = __all_sync(~0u, mbar_wait(&v_full[j % L::ST], (j / L::ST) & 1));
-               if(!ok) break;
-               const bool in = bits[0] >> lane & 1, in1 = bits[1] >> lane & 1, in2 = bits[2] >> lane & 1, in3 = bits[3] >> lane & 1;
-               const bool mine = (warp & 3) == 0 ? in : (warp & 3) == 1 ? in1 : (warp & 3) == 2 ? in2 : in3;
-               if(!mine) {
-                  for(int p = 0; p < L::PANELS; ++p) {
-                     uint4* line = reinterpret_cast< uint4* >(sm + L::V + (j % L::ST) * L::TILE + p * L::PANEL + row * 128);
+               for(int c = 0; c < 4; ++c) bits[c] = s_bits[j % kBitSlots][c];
+            } else if(partial) {
 #pragma unroll
-                     for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
-                  }
-               }
-               fence_async_proxy();
+               for(int c = 0; c < 4; ++c) bits[c] = left >= 32 * c + 32 ? ~0u : left <= 32 * c ? 0u : (1u << (left - 32 * c)) - 1u;
             }
-            ok = __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
+            ok = ok && __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
             if(!ok) break;
             fence_after();
-            uint32_t s[128];
-#pragma unroll
-            for(int c = 0; c < 4; ++c)
-               if(c < chunks) tmem_ld32(s + c * 32, st + c * 32);
-            wait_ld();
-            loaded< 128 >(s);
+            uint32_t s[QT == 2 ? 128 : 64];
             float top = -CUDART_INF_F;
+            if constexpr(QT == 2) {
 #pragma unroll
-            for(int c = 0; c < 4; ++c) {
-               if(c >= chunks) continue;
-               if(!all) {
+               for(int c = 0; c < 4; ++c)
+                  if(c < chunks) tmem_ld32(s + c * 32, st + c * 32);
+               wait_ld();
+               loaded< 128 >(s);
 #pragma unroll
-                  for(int i = 0; i < 32; ++i)
-                     if(!(bits[c] >> i & 1)) s[c * 32 + i] = 0xff800000u;
+               for(int c = 0; c < 4; ++c) {
+                  if(c >= chunks) continue;
+                  if(partial) hide(s + c * 32, bits[c]);
+                  top = largest(s + c * 32, top);
                }
+            } else { // two blocks share the registers: the scores are read twice, 32 at a time
+               tmem_ld32(s, st);
 #pragma unroll
-               for(int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(s[c * 32 + i]));
+               for(int c = 0; c < 4; ++c) {
+                  if(c >= chunks) continue;
+                  wait_ld();
+                  loaded< 32 >(s + (c & 1) * 32);
+                  if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
+                  if(partial) hide(s + (c & 1) * 32, bits[c]);
+                  top = largest(s + (c & 1) * 32, top);
+               }
+               tmem_ld32(s, st);
             }
             top *= sc;
             float f = 1.f;
             if(top > m + kGrow || (m == -CUDART_INF_F && top > m)) {
                f = exp2_fast(m - top);
                m = top;
-               l *= f;
+               sum[0] = mul2(sum[0], pair(f, f));
+               sum[1] = mul2(sum[1], pair(f, f));
             }
             if(j > 0 && __any_sync(~0u, f != 1.f)) { // the products into O so far were done before this S
                for(int c = 0; c < a.dim; c += 16) {
@@ -238,25 +320,33 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                }
             }
             const float ref = m == -CUDART_INF_F ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t ref2 = pair(-ref, -ref);
 #pragma unroll
             for(int c = 0; c < 4; ++c) {
-               if(c >= chunks) continue;
-               uint32_t p[16];
-#pragma unroll
-               for(int i = 0; i < 16; ++i) {
-                  const float x = exp2_fast(fmaf(__uint_as_float(s[c * 32 + 2 * i]), sc, -ref));
-                  const float y = exp2_fast(fmaf(__uint_as_float(s[c * 32 + 2 * i + 1]), sc, -ref));
-                  sum[i & 3] += x + y;
-                  p[i] = pack2< T >(x, y);
+               if(c < chunks) {
+                  uint32_t p[16];
+                  if constexpr(QT == 2) {
+                     exponents< T >(s + c * 32, p, sc2, ref2, sum);
+                  } else {
+                     wait_ld();
+                     loaded< 32 >(s + (c & 1) * 32);
+                     if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
+                     if(partial) hide(s + (c & 1) * 32, bits[c]);
+                     exponents< T >(s + (c & 1) * 32, p, sc2, ref2, sum);
+                     // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
+                  }
+                  tmem_st16(st + c * 16, p);
                }
-               tmem_st16(st + c * 16, p);
+               if(c & 1) {
+                  wait_st();
+                  fence_before();
+                  mbar_arrive(&p_full[t][c >> 1]);
+               }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            wait_st();
-            fence_before();
-            mbar_arrive(&p_full[t]);
          }
+         float l, l1;
+         unpair(add2(sum[0], sum[1]), l, l1);
+         l += l1;
          if(ok && tiles > 0) ok = __all_sync(~0u, mbar_wait(&o_full[t], 0));
          fence_after();
          // Rows leave through the q tile's shared memory (its products are done), 16 bytes a lane along the rows.

@@ -265,14 +265,26 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
 #pragma unroll
             for(int e = 0; e < 4; ++e) {
                const float L2 = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
-               float p = exp2_fast(fmaf(__uint_as_float(s[4 * c + e]), sc, -L2));
-               if(!in || (tail && half * HALF + 4 * c + e >= valid)) p = 0.f;
-               s[4 * c + e] = __float_as_uint(p);
+               s[4 * c + e] = __float_as_uint(exp2_fast(fmaf(__uint_as_float(s[4 * c + e]), sc, -L2)));
             }
          }
          uint32_t w[HALF / 2];
+         // Masked keys and rows past the sequence: what was computed from them may be anything.
+         auto settle = [&] {
+#pragma unroll
+            for(int c = 0; c < HALF / 2; ++c)
+               if(!in) w[c] = 0;
+            if(tail) {
+#pragma unroll
+               for(int c = 0; c < HALF / 2; ++c) {
+                  const int q = half * HALF + 2 * c;
+                  w[c] &= q + 1 < valid ? ~0u : q < valid ? 0xffffu : 0u;
+               }
+            }
+         };
 #pragma unroll
          for(int c = 0; c < HALF / 2; ++c) w[c] = pack2< T >(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+         settle();
          store_packed< HALF / 2 >(st, w);
          if(tail) { // rows of dO and Q past the sequence: their weights are 0, so must they be
             ok = ok && __all_sync(~0u, mbar_wait(&dp_full, i & 1));
@@ -296,11 +308,11 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
             for(int e = 0; e < 4; ++e) {
                const float D = e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w;
                x[e] = __uint_as_float(s[4 * c + e]) * fmaf(__uint_as_float(d[4 * c + e]), kDown, -D);
-               if(!in || (tail && half * HALF + 4 * c + e >= valid)) x[e] = 0.f;
             }
             w[2 * c] = pack2< T >(x[0], x[1]);
             w[2 * c + 1] = pack2< T >(x[2], x[3]);
          }
+         settle();
          store_packed< HALF / 2 >(pt, w);
          wait_st();
          fence_before();
@@ -458,6 +470,7 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
          if(v != -CUDART_INF_F) lse = v * kLog2e;
          delta = a.delta[at];
       }
+      const uint64_t sc2 = pair(sc, sc), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
       bool ok = true;
       for(int j = 0; j < n; ++j) {
          const int left = ks.len - j * KN;
@@ -473,10 +486,11 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
          uint32_t s[HALF];
          load_columns< HALF >(s, lanes + L::S + (j & 1) * KN + half * HALF);
 #pragma unroll
-         for(int c = 0; c < HALF; ++c) {
-            float p = exp2_fast(fmaf(__uint_as_float(s[c]), sc, -lse));
-            if(!all && !(bits[c / 32] >> (c % 32) & 1)) p = 0.f;
-            s[c] = __float_as_uint(p);
+         for(int c = 0; c < HALF; c += 2) {
+            float x, y;
+            unpair(fma2(pair(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sc2, lse2), x, y);
+            s[c] = __float_as_uint(exp2_fast(x));
+            s[c + 1] = __float_as_uint(exp2_fast(y));
          }
          if(!all && (warp & 3) * 32 < HALF) { // masked rows of K, read by dS K next, S is done with them
             const int r = (warp & 3) * 32 + lane;
@@ -493,13 +507,18 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
          load_columns< HALF >(d, pt);
 #pragma unroll
          for(int c = 0; c < HALF / 2; ++c) {
-            float x = __uint_as_float(s[2 * c]) * (__uint_as_float(d[2 * c]) - delta);
-            float y = __uint_as_float(s[2 * c + 1]) * (__uint_as_float(d[2 * c + 1]) - delta);
-            if(!all) { // dO V^T of a masked key may be anything
-               if(!(bits[c / 16] >> (2 * c % 32) & 1)) x = 0.f;
-               if(!(bits[c / 16] >> (2 * c % 32 + 1) & 1)) y = 0.f;
-            }
+            float x, y;
+            unpair(mul2(pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])),
+                        add2(pair(__uint_as_float(d[2 * c]), __uint_as_float(d[2 * c + 1])), delta2)),
+                   x, y);
             w[c] = pack2< T >(x, y);
+         }
+         if(!all) { // scores and dO V^T of a masked key may be anything
+#pragma unroll
+            for(int c = 0; c < HALF / 2; ++c) {
+               const unsigned b = bits[c / 16] >> (2 * c % 32) & 3u;
+               w[c] &= (b & 1 ? 0xffffu : 0u) | (b & 2 ? 0xffff0000u : 0u);
+            }
          }
          store_packed< HALF / 2 >(pt, w);
          wait_st();

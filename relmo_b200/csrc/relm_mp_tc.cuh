@@ -133,6 +133,34 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v)
                 : "memory");
 }
 
+// ---- two float32 operations in one instruction --------------------------------------------
+
+__device__ __forceinline__ uint64_t pair(float x, float y)
+{
+   uint64_t v;
+   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+   return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+   uint64_t d;
+   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+   return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+   uint64_t d;
+   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+   return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+   uint64_t d;
+   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+   return d;
+}
+
 // ---- products -------------------------------------------------------------------------
 
 // Shared-memory operand of 128-byte swizzled panels (64 two-byte columns by rows):
