@@ -163,17 +163,13 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          }
       }
    } else if(warp == QT * 4) { // products
-      if(lane == 0 && tiles > 0) {
+      if(elect_one() && tiles > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t pv = instruction(BF, 128, steps * 16, true);
          auto keys16 = [&](int j) { return min(kTileRows, (ks.len - j * kTileRows + 15) / 16 * 16); };
          auto scores = [&](int t, int j) {
-            const uint32_t qa = base + L::Q + t * L::TILE, ka = base + L::K + (j % L::ST) * L::TILE;
-            const uint32_t id = instruction(BF, 128, keys16(j), false);
-            for(int i = 0; i < steps; ++i) {
-               const uint32_t off = (i >> 2) * L::PANEL + (i & 3) * 32;
-               mma_ss(tmem + t * 128, operand(qa + off, 16, 1024), operand(ka + off, 16, 1024), id, i > 0);
-            }
+            product_columns< DP, kTileRows, kTileRows >(tmem + t * 128, base + L::Q + t * L::TILE, base + L::K + (j % L::ST) * L::TILE,
+                                                        instruction(BF, 128, keys16(j), false), steps);
             mma_commit(&s_full[t]);
          };
          bool ok = mbar_wait(&k_full[0], 0);
@@ -191,13 +187,13 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             }
             for(int t = 0; t < active && ok; ++t) {
                const uint32_t va = base + L::V + s * L::TILE;
-               for(int h = 0; h < 2 && ok; ++h) { // the weights come in two halves of 64 keys
-                  if(!(ok = mbar_wait(&p_full[t][h], j & 1))) break;
-                  fence_after();
-                  for(int i = 4 * h; i < min(n, 4 * h + 4); ++i)
-                     mma_ts(tmem + L::O + t * DP, tmem + t * 128 + i * 8, operand(va + i * 2048, L::PANEL, 1024), pv, j > 0 || i > 0);
-               }
-               if(!ok) break;
+               // The weights come in two halves of 64 keys.
+               if(!(ok = mbar_wait(&p_full[t][0], j & 1))) break;
+               fence_after();
+               product_rows< 0, 4, 0, kTileRows >(tmem + L::O + t * DP, tmem + t * 128, va, pv, n, j > 0);
+               if(!(ok = mbar_wait(&p_full[t][1], j & 1))) break;
+               fence_after();
+               product_rows< 4, 4, 0, kTileRows >(tmem + L::O + t * DP, tmem + t * 128, va, pv, n, true);
                if(j + 1 == tiles) mma_commit(&o_full[t]);
                else {
                   ok = mbar_wait(&k_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1);

@@ -184,25 +184,19 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
          }
       }
    } else if(warp == 8) { // products
-      if(lane == 0 && n > 0) {
+      if(elect_one() && n > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t out_id = instruction(BF, 128, steps * 16, true);
          auto cols = [&](int i) { return min(QN, (qs.len - (i % q_tiles) * QN + 15) / 16 * 16); };
          // S^T = K Q^T or dP^T = V dO^T
          auto first = [&](uint32_t d, uint32_t left, uint32_t right, int i, uint64_t* bar) {
-            const uint32_t id = instruction(BF, 128, cols(i), false);
-            for(int k = 0; k < steps; ++k)
-               mma_ss(tmem + d, operand(base + left + (k >> 2) * kTileRows * 128 + (k & 3) * 32, 16, 1024),
-                      operand(base + right + (i % L::ST) * L::QT + (k >> 2) * QN * 128 + (k & 3) * 32, 16, 1024), id, k > 0);
+            product_columns< DP, kTileRows, QN >(tmem + d, base + left, base + right + (i % L::ST) * L::QT,
+                                                 instruction(BF, 128, cols(i), false), steps);
             mma_commit(bar);
          };
          // dV += P^T dO or dK += dS^T Q; the halves of the left operand start HALF columns apart
          auto second = [&](uint32_t d, uint32_t left, uint32_t right, int i) {
-            const int ks16 = cols(i) / 16;
-            for(int k = 0; k < ks16; ++k) {
-               const uint32_t at = left + (k >= HALF / 16 ? HALF + (k - HALF / 16) * 8 : k * 8);
-               mma_ts(tmem + d, tmem + at, operand(base + right + (i % L::ST) * L::QT + k * 2048, QN * 128, 1024), out_id, i > 0 || k > 0);
-            }
+            product_rows< 0, QN / 16, HALF, QN >(tmem + d, tmem + left, base + right + (i % L::ST) * L::QT, out_id, cols(i) / 16, i > 0);
          };
          bool ok = mbar_wait(&kv_full, 0) && mbar_wait(&q_full[0], 0);
          if(ok) {
@@ -413,16 +407,14 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
          }
       }
    } else if(warp == 8) { // products
-      if(lane == 0 && n > 0) {
+      if(elect_one() && n > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t out_id = instruction(BF, 128, steps * 16, true);
          auto cols = [&](int j) { return min(KN, (ks.len - j * KN + 15) / 16 * 16); };
          // S = Q K^T or dP = dO V^T
          auto first = [&](uint32_t d, uint32_t left, uint32_t right, int j, uint64_t* bar) {
-            const uint32_t id = instruction(BF, 128, cols(j), false);
-            for(int k = 0; k < steps; ++k)
-               mma_ss(tmem + d, operand(base + left + (k >> 2) * kTileRows * 128 + (k & 3) * 32, 16, 1024),
-                      operand(base + right + (j % L::ST) * L::KT + (k >> 2) * KN * 128 + (k & 3) * 32, 16, 1024), id, k > 0);
+            product_columns< DP, kTileRows, KN >(tmem + d, base + left, base + right + (j % L::ST) * L::KT,
+                                                 instruction(BF, 128, cols(j), false), steps);
             mma_commit(bar);
          };
          bool ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
@@ -439,11 +431,7 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
             }
             if(!(ok = mbar_wait(&ds_full, j & 1))) break;
             fence_after();
-            const int ks16 = cols(j) / 16;
-            for(int k = 0; k < ks16; ++k) {
-               const uint32_t at = L::P + (k >= HALF / 16 ? HALF + (k - HALF / 16) * 8 : k * 8);
-               mma_ts(tmem + L::DQ, tmem + at, operand(base + L::K + (j % L::ST) * L::KT + k * 2048, KN * 128, 1024), out_id, j > 0 || k > 0);
-            }
+            product_rows< 0, KN / 16, HALF, KN >(tmem + L::DQ, tmem + L::P, base + L::K + (j % L::ST) * L::KT, out_id, cols(j) / 16, j > 0);
             mma_commit(&k_empty[j % L::ST]);
             if(j + 1 < n) {
                if(!(ok = mbar_wait(&v_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1))) break;

@@ -198,5 +198,42 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar)
    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// One lane of a converged warp, the same each time.
+__device__ __forceinline__ bool elect_one()
+{
+   uint32_t one;
+   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+   return one != 0;
+}
+
+// The issuing thread is alone in its warp, so whatever it computes between two
+// products delays the second: descriptors are made once per tile, steps are
+// unrolled and add constants to them (a loop with the descriptors inside took
+// 150 cycles per 128 x 128 x 16 product, which itself takes 64).
+
+// d = a b^T over `steps` 16-column steps of two tiles of panels, both contracted along their columns.
+template < int DP, int A_ROWS, int B_ROWS >
+__device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps)
+{
+   const uint64_t da = operand(a, 16, 1024), db = operand(b, 16, 1024);
+#pragma unroll
+   for(int k = 0; k < DP / 16; ++k)
+      if(k < steps) mma_ss(d, da + ((k >> 2) * A_ROWS * 8 + (k & 3) * 2), db + ((k >> 2) * B_ROWS * 8 + (k & 3) * 2), idesc, k > 0);
+}
+
+// d (+)= a b, steps [FIRST, FIRST + N) below `steps`: a in tensor memory (two halves of HALF
+// contracted columns, HALF columns of memory apart; HALF 0: all together), b a tile of
+// B_ROWS-row panels contracted along its rows.
+template < int FIRST, int N, int HALF, int B_ROWS >
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps, bool accumulate)
+{
+   const uint64_t db = operand(b, B_ROWS * 128, 1024);
+#pragma unroll
+   for(int k = FIRST; k < FIRST + N; ++k) {
+      const int at = HALF && k >= HALF / 16 ? HALF + (k - HALF / 16) * 8 : k * 8;
+      if(k < steps) mma_ts(d, a + at, db + k * 128, idesc, accumulate || k > 0);
+   }
+}
+
 }  // namespace tc
 }  // namespace relm_mp
