@@ -530,13 +530,14 @@ RELM_MP_API int relm_mp_add_rms_norm_e4m3(relm_mp_dtype dtype, const void* x, in
                                           const void* residual, int64_t residual_stride, const void* weight,
                                           int64_t rows, int64_t width, float eps, unsigned char* q, float* scale,
                                           void* h, void* stream);
-/* Gradient of both addends (they share it) and of the weight: with n = h * inv,
+/* Gradient of both addends (they share it) and of the weight: with n = h * inv
+ * (h = x + residual again, unrounded; residual may be NULL),
  * dx = inv * (w * dy - n * mean(w * dy * n)) + dh, dweight = sum over rows of
  * dy * n (summed in a fixed order). dy, dh or dweight may be NULL. */
 RELM_MP_API size_t relm_mp_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width);
 RELM_MP_API int relm_mp_add_rms_norm_backward(relm_mp_dtype dtype, const void* dy, int64_t dy_stride,
-                                              const void* dh, int64_t dh_stride, const void* h, int64_t h_stride,
-                                              const float* inv_rms, const void* weight, int64_t rows, int64_t width,
+                                              const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
+                                              const void* residual, int64_t residual_stride, const float* inv_rms, const void* weight, int64_t rows, int64_t width,
                                               void* dx, void* dweight, void* workspace, size_t workspace_bytes,
                                               void* stream);
 

@@ -181,7 +181,7 @@ SIGNATURES: dict[str, tuple] = {
     "relm_mp_add_rms_norm_e4m3": (_INT, [_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _P, _P, _P, _P]),
     "relm_mp_add_rms_norm_backward_workspace_bytes": (_SZ, [_I64, _I64]),
     "relm_mp_add_rms_norm_backward": (
-        _INT, [_INT, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
+        _INT, [_INT, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
     "relm_mp_attn_plan_init": (_INT, [_P, _P, _I64, _P]),
     "relm_mp_attn_plan_bytes": (_SZ, [_P]),
     "relm_mp_attn_plan_fill": (_INT, [_P, _P, _P, _P, _SZ]),

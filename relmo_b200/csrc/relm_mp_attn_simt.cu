@@ -311,10 +311,10 @@ __global__ void __launch_bounds__(kBlock) k_attn_backward_q(Args a)
    }
 }
 
-int launch(const void* fn, dim3 grid, size_t smem, const Args& a, cudaStream_t st, const char* what)
+int launch(SmemLimit& limit, const void* fn, dim3 grid, size_t smem, const Args& a, cudaStream_t st, const char* what)
 {
    if(grid.x == 0 || grid.y == 0) return RELM_MP_OK;
-   int rc = check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), what);
+   int rc = limit(fn, smem, what);
    if(rc) return rc;
    Args copy = a;
    void* args[] = {&copy};
@@ -326,7 +326,8 @@ template < typename T, int DP >
 int forward(const Args& a, int64_t items, cudaStream_t st)
 {
    using S = Shape< DP >;
-   return launch((const void*)k_attn_forward< T, S >, dim3((unsigned)(items * (kTileRows / S::B)), a.heads),
+   static SmemLimit limit;
+   return launch(limit, (const void*)k_attn_forward< T, S >, dim3((unsigned)(items * (kTileRows / S::B)), a.heads),
                  3 * S::tile + S::square, a, st, "k_attn_forward");
 }
 
@@ -335,10 +336,11 @@ int backward(const Args& a, int64_t q_items, int64_t kv_items, cudaStream_t st)
 {
    using S = Shape< DP >;
    constexpr int PER = kTileRows / S::B;
-   int rc = launch((const void*)k_attn_backward_kv< T, S >, dim3((unsigned)(kv_items * PER), a.kv_heads),
+   static SmemLimit kv_limit, q_limit;
+   int rc = launch(kv_limit, (const void*)k_attn_backward_kv< T, S >, dim3((unsigned)(kv_items * PER), a.kv_heads),
                    4 * S::tile + 2 * S::square, a, st, "k_attn_backward_kv");
    if(rc) return rc;
-   return launch((const void*)k_attn_backward_q< T, S >, dim3((unsigned)(q_items * PER), a.heads),
+   return launch(q_limit, (const void*)k_attn_backward_q< T, S >, dim3((unsigned)(q_items * PER), a.heads),
                  4 * S::tile + S::square, a, st, "k_attn_backward_q");
 }
 

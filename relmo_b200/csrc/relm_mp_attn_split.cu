@@ -353,8 +353,8 @@ template < typename T, int DP >
 int launch(const SplitArgs& s, cudaStream_t st)
 {
    constexpr size_t bytes = (size_t)kWarps * kStages * 2 * kChunk * DP * 2;
-   int rc = check_cuda(cudaFuncSetAttribute(k_attn_split< T, DP >, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes),
-                       "k_attn_split");
+   static SmemLimit limit;
+   int rc = limit((const void*)k_attn_split< T, DP >, bytes, "k_attn_split");
    if(rc) return rc;
    k_attn_split< T, DP ><<< dim3(s.parts, s.a.kv_heads, s.row_groups), kThreads4, bytes, st >>>(s);
    if((rc = check_launch("k_attn_split")) || s.parts == 1) return rc;

@@ -404,7 +404,8 @@ int launch(const Args& a, const TcMaps& m, int64_t items, cudaStream_t st)
 {
    using L = Fwd< DP, QT >;
    constexpr int bytes = (int)L::BYTES + 1024;
-   int rc = check_cuda(cudaFuncSetAttribute(k_attn_tc_forward< T, DP, QT >, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "k_attn_tc_forward");
+   static SmemLimit limit;
+   int rc = limit((const void*)k_attn_tc_forward< T, DP, QT >, bytes, "k_attn_tc_forward");
    if(rc) return rc;
    k_attn_tc_forward< T, DP, QT ><<< dim3((unsigned)items, a.heads), L::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
    return check_launch("k_attn_tc_forward");
@@ -413,7 +414,7 @@ int launch(const Args& a, const TcMaps& m, int64_t items, cudaStream_t st)
 template < typename T >
 int forward(const Args& a, const TcMaps& m, int64_t tiles, int64_t pairs, cudaStream_t st)
 {
-   const bool two = a.max_q > kTileRows && pairs * a.heads >= 148;
+   const bool two = 2 * tiles >= 3 * pairs && pairs * a.heads >= 148;
    if(a.dim <= 64) return two ? launch< T, 64, 2 >(a, m, pairs, st) : launch< T, 64, 1 >(a, m, tiles, st);
    return two ? launch< T, 128, 2 >(a, m, pairs, st) : launch< T, 128, 1 >(a, m, tiles, st);
 }

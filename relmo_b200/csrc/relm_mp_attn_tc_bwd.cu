@@ -532,10 +532,10 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
 }
 
 template < typename F >
-int launch(F fn, int bytes, dim3 grid, const Args& a, const TcMaps& m, cudaStream_t st, const char* what)
+int launch(SmemLimit& limit, F fn, int bytes, dim3 grid, const Args& a, const TcMaps& m, cudaStream_t st, const char* what)
 {
    if(grid.x == 0) return RELM_MP_OK;
-   int rc = check_cuda(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+   int rc = limit((const void*)fn, bytes, what);
    if(rc) return rc;
    fn<<< grid, kBwdThreads, bytes, st >>>(a, m.q, m.k, m.v, m.go);
    return check_launch(what);
@@ -558,11 +558,12 @@ int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_til
    TcMaps m;
    int rc;
    if((rc = maps(&m, N, kTileRows))) return rc;
-   if((rc = launch(k_attn_tc_backward_kv< T, DP, N >, (int)Kv< DP, N >::BYTES + 1024, dim3((unsigned)kv_tiles, a.kv_heads), a, m, st,
+   static SmemLimit kv_limit, q_limit;
+   if((rc = launch(kv_limit, k_attn_tc_backward_kv< T, DP, N >, (int)Kv< DP, N >::BYTES + 1024, dim3((unsigned)kv_tiles, a.kv_heads), a, m, st,
                    "k_attn_tc_backward_kv")))
       return rc;
    if(N != kTileRows && (rc = maps(&m, kTileRows, N))) return rc;
-   return launch(k_attn_tc_backward_q< T, DP, N >, (int)Dq< DP, N >::BYTES + 1024, dim3((unsigned)q_tiles, a.heads), a, m, st,
+   return launch(q_limit, k_attn_tc_backward_q< T, DP, N >, (int)Dq< DP, N >::BYTES + 1024, dim3((unsigned)q_tiles, a.heads), a, m, st,
                  "k_attn_tc_backward_q");
 }
 

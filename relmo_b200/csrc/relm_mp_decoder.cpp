@@ -92,7 +92,7 @@ void check_norm(const Tensor& x, const Tensor& weight, const Tensor& residual, c
    dtype_of(x.scalar_type(), op);
 }
 
-// (y, h, inv): h is empty without a residual, inv unless it is asked for.
+// (y, h, inv): h is empty without a residual, inv undefined unless it is asked for.
 std::tuple< Tensor, Tensor, Tensor > norm_forward(const Tensor& x, const Tensor& weight, const Tensor& residual,
                                                   double eps, bool keep_inv)
 {
@@ -103,8 +103,8 @@ std::tuple< Tensor, Tensor, Tensor > norm_forward(const Tensor& x, const Tensor&
    const Tensor r2 = residual.defined() ? rows_of(residual) : Tensor();
    const int64_t rows = x2.size(0), width = x2.size(1);
    Tensor y = at::empty(x.sizes(), x.options());
-   Tensor h = residual.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
-   Tensor inv = at::empty({keep_inv ? rows : 0}, x.options().dtype(at::kFloat));
+   Tensor h = residual.defined() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options()), inv;
+   if(keep_inv) inv = at::empty({rows}, x.options().dtype(at::kFloat));
    check_rc(relm_mp_add_rms_norm(dtype_of(x.scalar_type(), op), x2.data_ptr(), row_stride(x2),
                                  r2.defined() ? r2.data_ptr() : nullptr, r2.defined() ? row_stride(r2) : 0, w.data_ptr(),
                                  rows, width, (float)eps, y.data_ptr(), residual.defined() ? h.data_ptr() : nullptr,
@@ -113,24 +113,28 @@ std::tuple< Tensor, Tensor, Tensor > norm_forward(const Tensor& x, const Tensor&
    return {y, h, inv};
 }
 
-// (dx, dweight): dweight is empty unless it is asked for.
-std::tuple< Tensor, Tensor > norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& h, const Tensor& inv,
-                                           const Tensor& weight, bool need_weight)
+// (dx, dweight): dweight is undefined unless it is asked for.
+std::tuple< Tensor, Tensor > norm_backward(const Tensor& dy, const Tensor& dh, const Tensor& x, const Tensor& residual,
+                                           const Tensor& inv, const Tensor& weight, bool need_weight)
 {
    const char* op = "add_rms_norm_backward";
-   c10::cuda::CUDAGuard guard(h.device());
-   const Tensor h2 = rows_of(h), w = weight.contiguous();
+   c10::cuda::CUDAGuard guard(x.device());
+   const Tensor x2 = rows_of(x), r2 = residual.defined() ? rows_of(residual) : Tensor(), w = weight.contiguous();
    const Tensor g = dy.defined() ? rows_of(dy) : Tensor(), gh = dh.defined() ? rows_of(dh) : Tensor();
-   const int64_t rows = h2.size(0), width = h2.size(1);
-   Tensor dx = at::empty(h.sizes(), h.options());
-   Tensor dw = at::empty({need_weight ? width : 0}, h.options());
+   const int64_t rows = x2.size(0), width = x2.size(1);
+   Tensor dx = at::empty(x.sizes(), x.options());
+   Tensor dw, ws;
    const size_t bytes = need_weight ? relm_mp_add_rms_norm_backward_workspace_bytes(rows, width) : 0;
-   const Tensor ws = bytes_like(bytes, h);
-   check_rc(relm_mp_add_rms_norm_backward(dtype_of(h.scalar_type(), op), g.defined() ? g.data_ptr() : nullptr,
+   if(need_weight) {
+      dw = at::empty({width}, x.options());
+      ws = bytes_like(bytes, x);
+   }
+   check_rc(relm_mp_add_rms_norm_backward(dtype_of(x.scalar_type(), op), g.defined() ? g.data_ptr() : nullptr,
                                           g.defined() ? row_stride(g) : 0, gh.defined() ? gh.data_ptr() : nullptr,
-                                          gh.defined() ? row_stride(gh) : 0, h2.data_ptr(), row_stride(h2),
+                                          gh.defined() ? row_stride(gh) : 0, x2.data_ptr(), row_stride(x2),
+                                          r2.defined() ? r2.data_ptr() : nullptr, r2.defined() ? row_stride(r2) : 0,
                                           inv.data_ptr< float >(), w.data_ptr(), rows, width, dx.data_ptr(),
-                                          need_weight ? dw.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(h)),
+                                          need_weight ? dw.data_ptr() : nullptr, need_weight ? ws.data_ptr() : nullptr, bytes, stream_of(x)),
             op);
    return {dx, dw};
 }
@@ -141,8 +145,7 @@ struct AddRmsNorm : torch::autograd::Function< AddRmsNorm > {
    {
       const Tensor& residual = or_none(residual_in);
       auto [y, h, inv] = norm_forward(x, weight, residual, eps, true);
-      ctx->saved_data["residual"] = residual.defined();
-      ctx->save_for_backward({residual.defined() ? h : x, inv, weight});
+      ctx->save_for_backward({x, inv, weight, residual});
       ctx->set_materialize_grads(false);
       if(!residual.defined()) ctx->mark_non_differentiable({h});
       return {y, h};
@@ -150,12 +153,12 @@ struct AddRmsNorm : torch::autograd::Function< AddRmsNorm > {
    static variable_list backward(AutogradContext* ctx, variable_list grads)
    {
       const auto saved = ctx->get_saved_variables();
-      const bool residual = ctx->saved_data["residual"].toBool();
+      const bool residual = saved[3].defined();
       const Tensor& dh = residual ? grads[1] : Tensor();
       if(!grads[0].defined() && !dh.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
       at::AutoDispatchBelowADInplaceOrView below;
-      auto [dx, dw] = norm_backward(grads[0], dh, saved[0], saved[1], saved[2], ctx->needs_input_grad(1));
-      return {dx, ctx->needs_input_grad(1) ? dw : Tensor(), residual ? dx : Tensor(), Tensor()};
+      auto [dx, dw] = norm_backward(grads[0], dh, saved[0], saved[3], saved[1], saved[2], ctx->needs_input_grad(1));
+      return {dx, dw, residual ? dx : Tensor(), Tensor()};
    }
 };
 

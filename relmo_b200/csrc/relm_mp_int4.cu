@@ -5,10 +5,17 @@
 // Bound by the weights' bytes (half a byte each), so the inner product runs on
 // the matrix instruction with the 16 weight rows as its left operand and up to
 // 8 (or 16) x rows as its right one: one instruction per 16 x 16 weights
-// whatever the number of rows. The codes become 2-byte floats by setting them
-// into the mantissa of 128 (bf16) or 1024 (f16) and subtracting 128 + z (1024
-// + z): exact. Each group's sum is float32 and is multiplied by its scale in
-// float32, so the only roundings are those of float32 sums.
+// whatever the number of rows. Turning codes into floats is then the larger
+// part of the work (an earlier form with a subtraction per pair of weights spent
+// 146 instructions per 16 x 64 weights and was bound by them: 34 us where the
+// bytes take 11), so the codes enter as they lie:
+//  - f16: the four bits in place in the mantissa of a subnormal number, c 2^-24
+//    (rows g) or c 2^-20 (rows g + 8); two masks and one shift per 4 weights;
+//  - bf16: in the mantissa of 128, as 128 + c (subnormal products would be lost);
+// and the zero point is taken off each group's sum: sum x c - z sum x, with sum x
+// from one more product with ones. Sums are float32; the cancellation costs at
+// most 5 bits of them, far below the 2-byte result's rounding. A float32 x has
+// no such room: its codes become c - z exactly (128 + c minus 128 + z).
 //
 // The right operand keeps x exact: bf16 and f16 as they are, e4m3 as f16, and
 // float32 as three bf16 columns (x = hi + mid + lo, 24 bits), which cost
@@ -86,108 +93,90 @@ __global__ void __launch_bounds__(256) k_int4_pack_groups(const __half* __restri
    if(out_z) out_z[i] = in ? zeros[row * src_groups + grp] : 0;
 }
 
-template < typename M >
-struct Magic;
-template <>
-struct Magic< __nv_bfloat16 > {
-   static constexpr uint32_t bits = 0x43004300u; // (128, 128)
-   static __device__ __forceinline__ uint32_t base(int z)
+enum Source { kSame = 0, kF32 = 1, kE4m3 = 2 };
+
+// One 32-bit word of codes as the left operand (rows g: f[0], f[2]; rows g + 8: f[1], f[3]).
+// A stored code c stands for (offset + c) * 2^-shift.
+template < typename M, int SRC >
+struct Left;
+template < int SRC >
+struct Left< __half, SRC > {
+   static constexpr bool exact = false;
+   static constexpr uint32_t ones = 0x3c003c00u;
+   static constexpr float up0 = 16777216.f, up8 = 1048576.f, offset = 0.f; // 2^24, 2^20
+   static __device__ __forceinline__ void fragments(uint32_t w, uint32_t, uint32_t, uint32_t* f)
    {
-      const __nv_bfloat162 v = __float2bfloat162_rn(128.f + (float)z);
-      return *reinterpret_cast< const uint32_t* >(&v);
+      f[0] = w & 0x000f000fu;
+      f[1] = w & 0x00f000f0u;
+      f[2] = (w >> 8) & 0x000f000fu;
+      f[3] = (w >> 8) & 0x00f000f0u;
    }
+   static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b)
+   {
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+   }
+};
+template < int SRC >
+struct Left< __nv_bfloat16, SRC > {
+   static constexpr bool exact = SRC == kF32;
+   static constexpr uint32_t ones = 0x3f803f80u;
+   static constexpr float up0 = 1.f, up8 = 1.f, offset = 128.f;
+   // (128 + z, 128 + z)
+   static __device__ __forceinline__ uint32_t base(uint32_t z) { return 0x43004300u + z * 0x00010001u; }
    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b)
    {
       const __nv_bfloat162 v = __hsub2(*reinterpret_cast< __nv_bfloat162* >(&a), *reinterpret_cast< __nv_bfloat162* >(&b));
       return *reinterpret_cast< const uint32_t* >(&v);
    }
-   static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b)
+   static __device__ __forceinline__ void fragments(uint32_t w, uint32_t z0, uint32_t z1, uint32_t* f)
    {
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                   : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-   }
-};
-template <>
-struct Magic< __half > {
-   static constexpr uint32_t bits = 0x64006400u; // (1024, 1024)
-   static __device__ __forceinline__ uint32_t base(int z)
-   {
-      const __half2 v = __float2half2_rn(1024.f + (float)z);
-      return *reinterpret_cast< const uint32_t* >(&v);
-   }
-   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b)
-   {
-      const __half2 v = __hsub2(*reinterpret_cast< __half2* >(&a), *reinterpret_cast< __half2* >(&b));
-      return *reinterpret_cast< const uint32_t* >(&v);
+#pragma unroll
+      for(int i = 0; i < 4; ++i) {
+         f[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+         if constexpr(exact) f[i] = sub(f[i], i & 1 ? z1 : z0);
+      }
    }
    static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b)
    {
-      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                   : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
    }
 };
-
-enum Source { kSame = 0, kF32 = 1, kE4m3 = 2 };
 
 // x columns of the right operand per row of x.
 template < int SRC >
 constexpr int kColumns = SRC == kF32 ? 3 : 1;
 
-__device__ __forceinline__ uint4 load_stream(const uint4* p)
+// 16 bytes, or zeros when !in (nothing is read then).
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in)
 {
-   uint4 v;
-   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                : "l"(p));
-   return v;
+   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-// 8 x values of one lane (half a column block) as 4 registers of two. `part`
-// chooses the term of a float32's split.
+// 8 x values of one lane (half a column block, in shared memory) as 4 registers
+// of two. `part` chooses the term of a float32's split.
 template < typename M, int SRC >
-__device__ __forceinline__ void load_x(const void* xrow, int64_t k0, int part, bool vec, uint32_t* b)
+__device__ __forceinline__ void load_x(const unsigned char* p, int part, uint32_t* b)
 {
    if constexpr(SRC == kSame) {
-      const M* p = static_cast< const M* >(xrow) + k0;
-      if(vec) {
-         const uint4 u = __ldg(reinterpret_cast< const uint4* >(p));
-         b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
-      } else {
-         const unsigned short* q = reinterpret_cast< const unsigned short* >(p);
-#pragma unroll
-         for(int i = 0; i < 4; ++i) b[i] = (uint32_t)q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
-      }
+      const uint4 u = *reinterpret_cast< const uint4* >(p);
+      b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
    } else if constexpr(SRC == kE4m3) {
-      const unsigned char* p = static_cast< const unsigned char* >(xrow) + k0;
-      uint32_t w[2];
-      if(vec) {
-         const uint2 u = __ldg(reinterpret_cast< const uint2* >(p));
-         w[0] = u.x, w[1] = u.y;
-      } else {
-#pragma unroll
-         for(int i = 0; i < 2; ++i)
-            w[i] = (uint32_t)p[4 * i] | (uint32_t)p[4 * i + 1] << 8 | (uint32_t)p[4 * i + 2] << 16 |
-                   (uint32_t)p[4 * i + 3] << 24;
-      }
+      const uint2 u = *reinterpret_cast< const uint2* >(p);
 #pragma unroll
       for(int i = 0; i < 4; ++i) {
-         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+         const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1))), __NV_E4M3);
          b[i] = (uint32_t)h.x | (uint32_t)h.y << 16;
       }
    } else {
-      const float* p = static_cast< const float* >(xrow) + k0;
       float f[8];
-      if(vec) {
 #pragma unroll
-         for(int i = 0; i < 2; ++i) {
-            const float4 v = __ldg(reinterpret_cast< const float4* >(p) + i);
-            f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
-         }
-      } else {
-#pragma unroll
-         for(int i = 0; i < 8; ++i) f[i] = p[i];
+      for(int i = 0; i < 2; ++i) {
+         const float4 v = reinterpret_cast< const float4* >(p)[i];
+         f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
       }
 #pragma unroll
       for(int i = 0; i < 8; ++i) {
@@ -228,15 +217,34 @@ struct MatvecArgs {
    void* y;
 };
 
+constexpr int kStages = 4;
+
+// One stage of a warp: codes of NT tiles, their scales and zero points (up to two
+// groups each), 64 columns of x.
+template < int SRC, int CT, int NT >
+struct Stage {
+   static constexpr int ES = SRC == kF32 ? 4 : SRC == kE4m3 ? 1 : 2;
+   static constexpr int ROWS = CT * 8 / kColumns< SRC >; // x rows of a launch
+   static constexpr int CODES = 0, SCALES = NT * 512, ZEROS = SCALES + NT * 64, X = ZEROS + NT * 32, BYTES = X + ROWS * 64 * ES;
+   static constexpr int PER_ROW = 64 * ES / 16, PIECES = (ROWS * PER_ROW + 31) / 32; // 16-byte pieces of x, and those of a lane
+};
+
 // A block owns 16 * NT weight rows; its warps take the 64-column blocks in turn
-// and their sums are joined in shared memory in warp order.
-template < typename M, int SRC, int CT, int NT, typename OUT >
+// and their sums are joined in shared memory in warp order. Each warp is its own
+// pipeline of asynchronous copies, three blocks ahead, without block barriers.
+// G32: groups of 32, two to a block; else a block has one scale.
+template < typename M, int SRC, int CT, int NT, bool G32, typename OUT >
 __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
 {
+   using S = Stage< SRC, CT, NT >;
+   using P = Left< M, SRC >;
    constexpr int COLS = CT * 8;
-   __shared__ float part[kWarps][NT * 16][COLS + 1];
+   extern __shared__ __align__(128) unsigned char smem[];
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-   const int64_t tile0 = (int64_t)blockIdx.x * NT;
+   const int64_t tile0 = (int64_t)blockIdx.x * NT, tiles = (a.n + 15) / 16;
+   unsigned char* const mine = smem + warp * (kStages * S::BYTES);
+   const uint32_t base = (uint32_t)__cvta_generic_to_shared(mine);
+   constexpr int halves = G32 ? 2 : 1; // groups of a block
    float total[NT][CT][4];
 #pragma unroll
    for(int n = 0; n < NT; ++n)
@@ -244,80 +252,155 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
       for(int c = 0; c < CT; ++c)
 #pragma unroll
          for(int i = 0; i < 4; ++i) total[n][c][i] = 0.f;
-   const int64_t tiles = (a.n + 15) / 16;
-#pragma unroll 4
-   for(int blk = warp; blk < a.blocks; blk += kWarps) {
-      uint4 w[NT];
+
+   // A tile past the end is read as the first one: its sums are not stored.
+   const uint4* codes[NT];
+   const __half2* scales[NT];
+   const uchar2* zeros[NT];
 #pragma unroll
-      for(int n = 0; n < NT; ++n)
-         w[n] = tile0 + n < tiles ? load_stream(a.codes + ((tile0 + n) * a.blocks + blk) * 32 + lane) : make_uint4(0, 0, 0, 0);
-      uint32_t b[CT][8];
-      const int64_t k0 = (int64_t)blk * kBlockK + 8 * t;
-      const bool second = (int64_t)blk * kBlockK + 32 < a.k; // k is a multiple of 32
+   for(int n = 0; n < NT; ++n) {
+      const int64_t tile = tile0 + n < tiles ? tile0 + n : tile0;
+      codes[n] = a.codes + tile * a.blocks * 32 + lane;
+      scales[n] = a.scales + tile * a.groups * 8 + lane * 4;
+      zeros[n] = a.zeros + tile * a.groups * 8 + lane * 8;
+   }
+   // Piece c of row r of x. The halves of odd rows change places: 8 lanes of two rows then read different banks.
+   auto x_place = [&](int r, int c) { return S::X + r * (64 * S::ES) + (SRC == kSame ? c ^ ((r & 1) << 2) : c) * 16; };
+   const char* xp[S::PIECES];
 #pragma unroll
-      for(int c = 0; c < CT; ++c) {
-         const int col = c * 8 + g, row = col / kColumns< SRC >;
-         constexpr size_t ES = SRC == kF32 ? 4 : SRC == kE4m3 ? 1 : 2;
-         const char* xrow = static_cast< const char* >(a.x) + row * a.x_stride * ES;
+   for(int i = 0; i < S::PIECES; ++i) {
+      const int r = (i * 32 + lane) / S::PER_ROW, c = (i * 32 + lane) % S::PER_ROW;
+      xp[i] = static_cast< const char* >(a.x) + (r < a.rows ? r : 0) * a.x_stride * S::ES + c * 16;
+      if(r >= a.rows && r < S::ROWS) // rows that x does not have stay zero
+         for(int st = 0; st < kStages; ++st) *reinterpret_cast< uint4* >(mine + st * S::BYTES + x_place(r, c)) = make_uint4(0, 0, 0, 0);
+   }
+   auto issue = [&](int blk, int stage) {
+      if(blk < a.blocks) {
+         const uint32_t at = base + stage * S::BYTES + lane * 16;
+         const int grp = (int)(((int64_t)blk * kBlockK) >> a.group_shift);
 #pragma unroll
-         for(int h = 0; h < 2; ++h) {
-            if(row < a.rows && (h == 0 || second)) {
-               load_x< M, SRC >(xrow, k0 + 32 * h, col % kColumns< SRC >, a.vec, b[c] + 4 * h);
+         for(int n = 0; n < NT; ++n) copy16(at + S::CODES + n * 512, codes[n] + (int64_t)blk * 32, true);
+         if(lane < 2 * halves) {
+#pragma unroll
+            for(int n = 0; n < NT; ++n) copy16(at + S::SCALES + n * 64, scales[n] + (int64_t)grp * 8, true);
+            if(a.zeros && lane < halves) {
+#pragma unroll
+               for(int n = 0; n < NT; ++n) copy16(at + S::ZEROS + n * 32, zeros[n] + (int64_t)grp * 8, true);
+            }
+         }
+#pragma unroll
+         for(int i = 0; i < S::PIECES; ++i) {
+            const int r = (i * 32 + lane) / S::PER_ROW, c = (i * 32 + lane) % S::PER_ROW;
+            if(r >= a.rows) continue;
+            // Past k (a multiple of 32, so a piece is whole or beyond it): zeros.
+            const bool in = blk * kBlockK + c * (16 / S::ES) < (int)a.k;
+            const char* from = in ? xp[i] + (int64_t)blk * (kBlockK * S::ES) : xp[i];
+            const uint32_t to = base + stage * S::BYTES + x_place(r, c);
+            if(a.vec) {
+               copy16(to, from, in);
             } else {
+               uint32_t v[4] = {0, 0, 0, 0};
+               if(in) {
 #pragma unroll
-               for(int i = 0; i < 4; ++i) b[c][4 * h + i] = 0;
+                  for(int e = 0; e < 16 / S::ES; ++e) {
+                     const uint32_t u = S::ES == 4 ? reinterpret_cast< const uint32_t* >(from)[e] : S::ES == 2 ? reinterpret_cast< const unsigned short* >(from)[e] : reinterpret_cast< const unsigned char* >(from)[e];
+                     v[e * S::ES / 4] |= u << (e * S::ES % 4 * 8);
+                  }
+               }
+               *reinterpret_cast< uint4* >(mine + (to - base)) = make_uint4(v[0], v[1], v[2], v[3]);
             }
          }
       }
-      // Groups of 64 columns or more cover the block with one scale; groups of 32 change half way.
-      const int64_t grp = ((int64_t)blk * kBlockK) >> a.group_shift;
-      const int halves = a.group_shift == 5 ? 2 : 1;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+   };
+#pragma unroll
+   for(int i = 0; i < kStages - 1; ++i) issue(warp + i * kWarps, i);
+   int stage = 0;
+   for(int blk = warp; blk < a.blocks; blk += kWarps, stage = (stage + 1) % kStages) {
+      issue(blk + (kStages - 1) * kWarps, (stage + kStages - 1) % kStages);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      const unsigned char* at = mine + stage * S::BYTES;
+      uint32_t b[CT][8];
+#pragma unroll
+      for(int c = 0; c < CT; ++c) {
+         const int col = c * 8 + g, row = col / kColumns< SRC >, part = col % kColumns< SRC >;
+#pragma unroll
+         for(int h = 0; h < 2; ++h) {
+            // A float32 row has three columns: the columns left over read the last row, their sums are not stored.
+            const int r = SRC == kF32 && row >= S::ROWS ? S::ROWS - 1 : row, half = SRC == kSame ? h ^ (r & 1) : h;
+            load_x< M, SRC >(at + S::X + (r * 64 + half * 32 + 8 * t) * S::ES, part, b[c] + 4 * h);
+         }
+      }
+      // sum x of the block's group, or of its two: a row of ones
+      float xs[2][CT][4];
+      if constexpr(!P::exact) {
+         const uint32_t ones[4] = {P::ones, P::ones, P::ones, P::ones};
+#pragma unroll
+         for(int c = 0; c < CT; ++c) {
+#pragma unroll
+            for(int h = 0; h < 2; ++h) {
+#pragma unroll
+               for(int i = 0; i < 4; ++i) xs[h][c][i] = 0.f;
+               P::mma(xs[h][c], ones, &b[c][4 * h]);
+               P::mma(xs[h][c], ones, &b[c][4 * h + 2]);
+            }
+            if constexpr(!G32) xs[0][c][0] += xs[1][c][0], xs[0][c][1] += xs[1][c][1];
+         }
+      }
 #pragma unroll
       for(int n = 0; n < NT; ++n) {
-         if(tile0 + n >= tiles) continue;
-         const uint32_t* ww = reinterpret_cast< const uint32_t* >(&w[n]);
+         const uint4 w = *reinterpret_cast< const uint4* >(at + S::CODES + n * 512 + lane * 16);
+         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
          float acc[CT][4];
          uint32_t z0 = 0, z1 = 0;
-         float s0 = 0.f, s1 = 0.f;
+         float s0 = 0.f, s1 = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
          for(int s = 0; s < 4; ++s) {
-            if(s == 0 || (s == 2 && halves == 2)) {
-               const int64_t at = ((tile0 + n) * a.groups + grp + (s >> 1)) * 8 + g;
-               const float2 sc = __half22float2(__ldg(a.scales + at));
-               s0 = sc.x, s1 = sc.y;
+            if(s == 0 || (s == 2 && G32)) {
+               const float2 sc = __half22float2(reinterpret_cast< const __half2* >(at + S::SCALES + n * 64 + (s >> 1) * 32)[g]);
                uchar2 z = make_uchar2(8, 8);
-               if(a.zeros) z = __ldg(a.zeros + at);
-               z0 = Magic< M >::base(z.x), z1 = Magic< M >::base(z.y);
+               if(a.zeros) z = reinterpret_cast< const uchar2* >(at + S::ZEROS + n * 32 + (s >> 1) * 16)[g];
+               if constexpr(P::exact) {
+                  z0 = P::base(z.x), z1 = P::base(z.y);
+               } else {
+                  o0 = -sc.x * (P::offset + (float)z.x), o1 = -sc.y * (P::offset + (float)z.y);
+               }
+               s0 = sc.x * P::up0, s1 = sc.y * P::up8;
 #pragma unroll
                for(int c = 0; c < CT; ++c)
 #pragma unroll
                   for(int i = 0; i < 4; ++i) acc[c][i] = 0.f;
             }
             uint32_t f[4];
-            f[0] = Magic< M >::sub((ww[s] & 0x000f000fu) | Magic< M >::bits, z0);
-            f[1] = Magic< M >::sub(((ww[s] >> 4) & 0x000f000fu) | Magic< M >::bits, z1);
-            f[2] = Magic< M >::sub(((ww[s] >> 8) & 0x000f000fu) | Magic< M >::bits, z0);
-            f[3] = Magic< M >::sub(((ww[s] >> 12) & 0x000f000fu) | Magic< M >::bits, z1);
+            P::fragments(ww[s], z0, z1, f);
 #pragma unroll
-            for(int c = 0; c < CT; ++c) Magic< M >::mma(acc[c], f, &b[c][2 * s]);
-            if(s == 3 || (s == 1 && halves == 2)) {
+            for(int c = 0; c < CT; ++c) P::mma(acc[c], f, &b[c][2 * s]);
+            if(s == 3 || (s == 1 && G32)) {
+               const int h = s == 3 && G32 ? 1 : 0;
 #pragma unroll
-               for(int c = 0; c < CT; ++c) {
-                  total[n][c][0] += s0 * acc[c][0];
-                  total[n][c][1] += s0 * acc[c][1];
-                  total[n][c][2] += s1 * acc[c][2];
-                  total[n][c][3] += s1 * acc[c][3];
-               }
+               for(int c = 0; c < CT; ++c)
+#pragma unroll
+                  for(int i = 0; i < 4; ++i) {
+                     total[n][c][i] = fmaf(i < 2 ? s0 : s1, acc[c][i], total[n][c][i]);
+                     if constexpr(!P::exact) total[n][c][i] = fmaf(i < 2 ? o0 : o1, xs[h][c][i & 1], total[n][c][i]);
+                  }
             }
          }
       }
+      __syncwarp(); // the stage is free for the next copies
    }
+   asm volatile("cp.async.wait_group 0;" ::: "memory");
+   __syncthreads();
+   // Sums of warp w: [w][16 NT rows][COLS + 1], over the stages.
+   float* part = reinterpret_cast< float* >(smem);
+   auto place = [&](int w, int row, int col) { return (w * (NT * 16) + row) * (COLS + 1) + col; };
 #pragma unroll
    for(int n = 0; n < NT; ++n)
 #pragma unroll
       for(int c = 0; c < CT; ++c)
 #pragma unroll
-         for(int i = 0; i < 4; ++i) part[warp][n * 16 + g + 8 * (i >> 1)][c * 8 + 2 * t + (i & 1)] = total[n][c][i];
+         for(int i = 0; i < 4; ++i) part[place(warp, n * 16 + g + 8 * (i >> 1), c * 8 + 2 * t + (i & 1))] = total[n][c][i];
    __syncthreads();
    constexpr int PER = kColumns< SRC >;
    for(int i = threadIdx.x; i < a.rows * NT * 16; i += kWarps * 32) {
@@ -328,17 +411,35 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
 #pragma unroll
       for(int w = 0; w < kWarps; ++w)
 #pragma unroll
-         for(int p = 0; p < PER; ++p) v += part[w][j][r * PER + p];
+         for(int p = 0; p < PER; ++p) v += part[place(w, j, r * PER + p)];
       if(a.x_scale) v *= a.x_scale[r];
       static_cast< OUT* >(a.y)[(int64_t)r * a.n + out] = store_as< OUT >(v);
    }
 }
 
+template < typename M, int SRC, int CT, int NT, typename OUT >
+int launch_tiles(const MatvecArgs& a, cudaStream_t st)
+{
+   constexpr int stages = kWarps * kStages * Stage< SRC, CT, NT >::BYTES, sums = kWarps * NT * 16 * (CT * 8 + 1) * 4;
+   constexpr int bytes = stages > sums ? stages : sums;
+   const bool g32 = a.group_shift == 5;
+   const auto kernel = g32 ? k_int4_matvec< M, SRC, CT, NT, true, OUT > : k_int4_matvec< M, SRC, CT, NT, false, OUT >;
+   static SmemLimit limit[2];
+   const int rc = limit[g32]((const void*)kernel, bytes, "k_int4_matvec");
+   if(rc) return rc;
+   const int64_t tiles = (a.n + 15) / 16;
+   kernel<<< (unsigned)((tiles + NT - 1) / NT), kWarps * 32, bytes, st >>>(a);
+   return check_launch("k_int4_matvec");
+}
+
+// Each block reads all of x: wide weights give a block several tiles, as long as every SM keeps two blocks.
 template < typename M, int SRC, int CT, typename OUT >
-void launch(const MatvecArgs& a, cudaStream_t st)
+int launch(const MatvecArgs& a, cudaStream_t st)
 {
    const int64_t tiles = (a.n + 15) / 16;
-   k_int4_matvec< M, SRC, CT, 1, OUT ><<< (unsigned)tiles, kWarps * 32, 0, st >>>(a);
+   if(CT <= 2 && tiles >= 3 * 296) return launch_tiles< M, SRC, CT, CT <= 2 ? 4 : 2, OUT >(a, st);
+   if(tiles >= 2 * 296) return launch_tiles< M, SRC, CT, 2, OUT >(a, st);
+   return launch_tiles< M, SRC, CT, 1, OUT >(a, st);
 }
 
 template < typename M, int SRC, typename OUT >
@@ -353,9 +454,7 @@ int matvec(MatvecArgs a, int64_t rows, cudaStream_t st)
       b.x = static_cast< const char* >(a.x) + lo * a.x_stride * es;
       b.y = static_cast< OUT* >(a.y) + lo * a.n;
       if(a.x_scale) b.x_scale = a.x_scale + lo;
-      if(b.rows <= FEW) launch< M, SRC, 1, OUT >(b, st);
-      else launch< M, SRC, MANY * kColumns< SRC > / 8, OUT >(b, st);
-      const int rc = check_launch("k_int4_matvec");
+      const int rc = b.rows <= FEW ? launch< M, SRC, 1, OUT >(b, st) : launch< M, SRC, MANY * kColumns< SRC > / 8, OUT >(b, st);
       if(rc) return rc;
    }
    return RELM_MP_OK;

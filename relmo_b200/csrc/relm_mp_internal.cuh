@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -81,6 +82,26 @@ int fill_rows(relm_mp_dtype dtype, void* out, int64_t count, bool neg_inf, cudaS
 int fill_value(relm_mp_dtype dtype, void* out, int64_t count, double value, cudaStream_t stream);
 
 size_t dtype_size(relm_mp_dtype dtype);
+
+// Lets one kernel have `bytes` of dynamic shared memory, once per device: the
+// call costs about 4 us, a launch 3.
+class SmemLimit {
+   std::atomic< uint64_t > done_{0};
+
+  public:
+   int operator()(const void* kernel, size_t bytes, const char* what)
+   {
+      if(bytes <= 32 * 1024) return RELM_MP_OK; // with up to 16 KB of static shared memory, within the default
+      int dev = 0;
+      const int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+      if(rc) return rc;
+      const uint64_t bit = 1ull << (dev & 63);
+      if(dev < 64 && (done_.load(std::memory_order_acquire) & bit)) return RELM_MP_OK;
+      const int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+      if(!e && dev < 64) done_.fetch_or(bit, std::memory_order_release);
+      return e;
+   }
+};
 
 // Stable LSD radix sort of (key, value) pairs by key bits [0, end_bit)
 // (relm_mp_sort.cu). The pairs start in (keys, vals) and end in them, or in

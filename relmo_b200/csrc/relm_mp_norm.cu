@@ -8,8 +8,10 @@
 // TPR threads, each NV chunks of VEC elements), reduced by shuffles (and a few
 // words of shared memory when the group is wider than a warp) and written once.
 // Sums and the norm are float32. The norm uses the unrounded float32 sum
-// x + r; h is rounded to the storage type only as it is written, so the
-// backward's n comes from the rounded h and the saved float32 inv.
+// x + r; h is rounded to the storage type only as it is written. The backward
+// adds x and r again instead of reading h (one more read of 8): with the rounded
+// h the weight's gradient, a sum of terms of either sign, was 1.6 times as far
+// from its 64-bit value.
 #include <cuda_fp8.h>
 
 #include "relm_mp_internal.cuh"
@@ -243,8 +245,8 @@ __global__ void __launch_bounds__(1024) k_add_rms_norm_long(FwdArgs a)
 }
 
 struct BwdArgs {
-   const void *dy, *dh, *h, *weight;
-   int64_t dy_stride, dh_stride, h_stride, rows;
+   const void *dy, *dh, *x, *residual, *weight;
+   int64_t dy_stride, dh_stride, x_stride, r_stride, rows;
    const float* inv;
    int width;
    void* dx;
@@ -270,22 +272,34 @@ __global__ void __launch_bounds__(kBlock< TPR >) k_add_rms_norm_bwd(BwdArgs a)
       const int64_t row = row0 + sub;
       const bool live = row < a.rows;
       const float inv = live ? a.inv[row] : 0.f;
-      float n[NV * VEC], g[NV * VEC];
+      float n[NV * VEC], g[NV * VEC], o[NV * VEC]; // o: dh, loaded with the rest so that the row's reduction hides it
       float dot = 0.f;
 #pragma unroll
       for(int c = 0; c < NV; ++c) {
          const int col = (c * TPR + lane) * VEC;
          if(live && col < a.width) {
-            load_once< T, VEC >(static_cast< const T* >(a.h) + row * a.h_stride + col, n + c * VEC);
+            load_once< T, VEC >(static_cast< const T* >(a.x) + row * a.x_stride + col, n + c * VEC);
+            if(a.residual) {
+               float r[VEC];
+               load_once< T, VEC >(static_cast< const T* >(a.residual) + row * a.r_stride + col, r);
+#pragma unroll
+               for(int i = 0; i < VEC; ++i) n[c * VEC + i] += r[i];
+            }
             if(a.dy) {
                load_once< T, VEC >(static_cast< const T* >(a.dy) + row * a.dy_stride + col, g + c * VEC);
             } else {
 #pragma unroll
                for(int i = 0; i < VEC; ++i) g[c * VEC + i] = 0.f;
             }
+            if(a.dh) {
+               load_once< T, VEC >(static_cast< const T* >(a.dh) + row * a.dh_stride + col, o + c * VEC);
+            } else {
+#pragma unroll
+               for(int i = 0; i < VEC; ++i) o[c * VEC + i] = 0.f;
+            }
          } else {
 #pragma unroll
-            for(int i = 0; i < VEC; ++i) n[c * VEC + i] = g[c * VEC + i] = 0.f;
+            for(int i = 0; i < VEC; ++i) n[c * VEC + i] = g[c * VEC + i] = o[c * VEC + i] = 0.f;
          }
       }
 #pragma unroll
@@ -312,16 +326,9 @@ __global__ void __launch_bounds__(kBlock< TPR >) k_add_rms_norm_bwd(BwdArgs a)
       for(int c = 0; c < NV; ++c) {
          const int col = (c * TPR + lane) * VEC;
          if(!live || col >= a.width) continue;
-         float o[VEC];
-         if(a.dh) {
-            load_once< T, VEC >(static_cast< const T* >(a.dh) + row * a.dh_stride + col, o);
-         } else {
 #pragma unroll
-            for(int i = 0; i < VEC; ++i) o[i] = 0.f;
-         }
-#pragma unroll
-         for(int i = 0; i < VEC; ++i) o[i] += inv * (g[c * VEC + i] - n[c * VEC + i] * dot);
-         store_vec< T, VEC >(static_cast< T* >(a.dx) + row * a.width + col, o);
+         for(int i = 0; i < VEC; ++i) o[c * VEC + i] += inv * (g[c * VEC + i] - n[c * VEC + i] * dot);
+         store_vec< T, VEC >(static_cast< T* >(a.dx) + row * a.width + col, o + c * VEC);
       }
    }
    if(!a.partial) return;
@@ -360,19 +367,21 @@ __global__ void __launch_bounds__(1024) k_add_rms_norm_bwd_long(BwdArgs a)
    if(out)
       for(int c = threadIdx.x; c < a.width; c += 1024) out[c] = 0.f;
    for(int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, phase ^= 1) {
-      const T* h = static_cast< const T* >(a.h) + row * a.h_stride;
+      const T* x = static_cast< const T* >(a.x) + row * a.x_stride;
+      const T* r = static_cast< const T* >(a.residual) + row * a.r_stride;
+      auto h = [&](int c) { return to_f32(x[c]) + (a.residual ? to_f32(r[c]) : 0.f); };
       const T* dy = static_cast< const T* >(a.dy) + row * a.dy_stride;
       const T* dh = static_cast< const T* >(a.dh) + row * a.dh_stride;
       const float inv = a.inv[row];
       float dot = 0.f;
       for(int c = threadIdx.x; c < a.width; c += 1024) {
-         const float n = to_f32(h[c]) * inv, g = a.dy ? to_f32(dy[c]) : 0.f;
+         const float n = h(c) * inv, g = a.dy ? to_f32(dy[c]) : 0.f;
          if(out) out[c] += g * n;
          dot += g * to_f32(w[c]) * n;
       }
       dot = reduce_row< 1024 >(dot, red[phase], Sum()) / (float)a.width;
       for(int c = threadIdx.x; c < a.width; c += 1024) {
-         const float n = to_f32(h[c]) * inv, g = a.dy ? to_f32(dy[c]) * to_f32(w[c]) : 0.f;
+         const float n = h(c) * inv, g = a.dy ? to_f32(dy[c]) * to_f32(w[c]) : 0.f;
          static_cast< T* >(a.dx)[row * a.width + c] = from_f32< T >(inv * (g - n * dot) + (a.dh ? to_f32(dh[c]) : 0.f));
       }
    }
@@ -487,10 +496,10 @@ template < int TPR >
 int64_t backward_blocks(int64_t rows)
 {
    const int64_t blocks = (rows + kBlockRows< TPR > - 1) / kBlockRows< TPR >;
-   const int64_t cap = (int64_t)kSms * (kBlock< TPR > >= 1024 ? 1 : kBlock< TPR > == 512 ? 2 : 4);
+   const int64_t cap = (int64_t)kSms * (kBlock< TPR > >= 1024 ? 1 : kBlock< TPR > == 512 ? 2 : kBlock< TPR > == 256 ? 5 : 8);
    return blocks < cap ? blocks : cap;
 }
-constexpr int64_t kMaxPartials = kSms * 4;
+constexpr int64_t kMaxPartials = kSms * 8;
 
 template < typename T, int VEC >
 int64_t launch_backward(const BwdArgs& a, cudaStream_t st)
@@ -514,8 +523,8 @@ int backward(const BwdArgs& a, void* dweight, cudaStream_t st)
 {
    auto fits = [&](int vec) {
       const size_t b = vec * sizeof(T);
-      return a.width % vec == 0 && a.h_stride % vec == 0 && (!a.dy || a.dy_stride % vec == 0) &&
-             (!a.dh || a.dh_stride % vec == 0) && aligned(a.dy, b) && aligned(a.dh, b) && aligned(a.h, b) &&
+      return a.width % vec == 0 && a.x_stride % vec == 0 && (!a.residual || a.r_stride % vec == 0) && (!a.dy || a.dy_stride % vec == 0) &&
+             (!a.dh || a.dh_stride % vec == 0) && aligned(a.dy, b) && aligned(a.dh, b) && aligned(a.x, b) && aligned(a.residual, b) &&
              aligned(a.weight, b) && aligned(a.dx, b);
    };
    constexpr int FULL = 16 / sizeof(T);
@@ -563,19 +572,19 @@ size_t relm_mp_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t width
 }
 
 int relm_mp_add_rms_norm_backward(relm_mp_dtype dtype, const void* dy, int64_t dy_stride, const void* dh,
-                                  int64_t dh_stride, const void* h, int64_t h_stride, const float* inv_rms,
-                                  const void* weight, int64_t rows, int64_t width, void* dx, void* dweight,
+                                  int64_t dh_stride, const void* x, int64_t x_stride, const void* residual,
+                                  int64_t residual_stride, const float* inv_rms, const void* weight, int64_t rows, int64_t width, void* dx, void* dweight,
                                   void* workspace, size_t workspace_bytes, void* stream)
 {
    int rc;
    if((rc = check_norm(dtype, rows, width, "add_rms_norm_backward"))) return rc;
    cudaStream_t st = static_cast< cudaStream_t >(stream);
    if(rows == 0) return dweight ? check_cuda(cudaMemsetAsync(dweight, 0, width * dtype_size(dtype), st), "memset") : RELM_MP_OK;
-   if(!h || !inv_rms || !weight || !dx)
+   if(!x || !inv_rms || !weight || !dx)
       return fail(RELM_MP_ERR_INVALID_ARGUMENT, "add_rms_norm_backward: pointers must not be NULL.");
    if(dweight && (!workspace || workspace_bytes < relm_mp_add_rms_norm_backward_workspace_bytes(rows, width)))
       return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "add_rms_norm_backward: workspace too small.");
-   const BwdArgs a{dy, dh, h, weight, dy_stride, dh_stride, h_stride, rows, inv_rms, (int)width, dx,
+   const BwdArgs a{dy, dh, x, residual, weight, dy_stride, dh_stride, x_stride, residual_stride, rows, inv_rms, (int)width, dx,
                    dweight ? static_cast< float* >(workspace) : nullptr};
    switch(dtype) {
       case RELM_MP_FLOAT32: return backward< float >(a, dweight, st);

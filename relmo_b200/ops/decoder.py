@@ -26,23 +26,33 @@ import math
 import os
 from dataclasses import dataclass, field
 
-from .mp_dispatch import CUSTOM, route
+from .mp_dispatch import route
 from .mp_runtime import _OFF_WORDS, require_torch, torch
 
 E4M3_MAX = 448.0
 
-_loaded = False
+_ops = None  # torch.ops.relm_mp_b200 once the library is loaded
 
 
 def _on_cuda(op_name: str, tensor) -> bool:
     """Whether ``tensor``'s call runs the kernels; raises where it should but cannot."""
 
-    global _loaded
+    global _ops
     if not tensor.is_cuda:
         return False
-    if not _loaded or os.environ.get("RELM_MP_ENABLE", "1").strip().lower() in _OFF_WORDS:
-        _loaded = route(op_name, tensor) == CUSTOM
+    if _ops is None or os.environ.get("RELM_MP_ENABLE", "1").strip().lower() in _OFF_WORDS:
+        route(op_name, tensor)
+        _ops = _Ops()
     return True
+
+
+class _Ops:
+    """The operators' overloads, looked up once: a lookup through ``torch.ops``
+    costs a microsecond or two of a call that takes ten."""
+
+    def __init__(self):
+        for name in ("add_rms_norm", "add_rms_norm_e4m3", "cross_attention", "int4_pack", "int4_matvec"):
+            setattr(self, name, getattr(torch.ops.relm_mp_b200, name).default)
 
 
 # ---- add + RMS norm ----------------------------------------------------------------
@@ -70,9 +80,8 @@ def add_rms_norm(x, weight, residual=None, *, eps: float = 1e-6):
     before it is rounded to ``x``'s dtype). Differentiable in x, weight and
     residual; weight and residual share x's dtype."""
 
-    require_torch("add_rms_norm")
     if _on_cuda("add_rms_norm", x):
-        y, h = torch.ops.relm_mp_b200.add_rms_norm(x, weight, residual, eps)
+        y, h = _ops.add_rms_norm(x, weight, residual, eps)
         return y, (x if residual is None else h)
     y, h = _norm_parts(x, weight, residual, eps, "add_rms_norm")
     return y.to(x.dtype), (x if residual is None else h.to(x.dtype))
@@ -83,10 +92,8 @@ def add_rms_norm_e4m3(x, weight, residual=None, *, eps: float = 1e-6):
     float8_e4m3fn, ``scale`` float32 of one value per row (``max|y| / 448``, 1 for
     a row of zeros), ``y = q * scale``. For inference: no gradient."""
 
-    require_torch("add_rms_norm_e4m3")
     if _on_cuda("add_rms_norm_e4m3", x):
-        with torch.no_grad():
-            q, scale, h = torch.ops.relm_mp_b200.add_rms_norm_e4m3(x, weight, residual, eps)
+        q, scale, h = _ops.add_rms_norm_e4m3(x, weight, residual, eps)
         return q, scale, (x if residual is None else h)
     with torch.no_grad():
         y, h = _norm_parts(x, weight, residual, eps, "add_rms_norm_e4m3")
@@ -153,15 +160,14 @@ def cross_attention(q, k, v, plan: AttentionPlan | None = None, *, scale: float 
     gradient. Returns q's shape and dtype; differentiable in q, k and v, with
     the same bits on every run."""
 
-    require_torch("cross_attention")
     if scale is None:
         scale = q.size(-1) ** -0.5
     if _on_cuda("cross_attention", q):
         if plan is None:
-            return torch.ops.relm_mp_b200.cross_attention(q, k, v, None, [], scale, key_mask)
+            return _ops.cross_attention(q, k, v, None, [], scale, key_mask)
         if plan.memory is None:
             raise RuntimeError("cross_attention: the plan was made for the CPU.")
-        return torch.ops.relm_mp_b200.cross_attention(q, k, v, plan.memory, plan.sizes, scale, key_mask)
+        return _ops.cross_attention(q, k, v, plan.memory, plan.sizes, scale, key_mask)
     return _cross_attention_formula(q, k, v, plan, scale, key_mask)
 
 
@@ -231,7 +237,7 @@ class Int4Weight:
         self.has_zeros = zeros is not None
         self.packed = self._plain = None
         if _on_cuda("int4_pack", codes):
-            self.packed = torch.ops.relm_mp_b200.int4_pack(codes, scales, zeros)
+            self.packed = _ops.int4_pack(codes, scales, zeros)
         else:
             self._plain = (codes, scales, zeros)
 
@@ -280,17 +286,13 @@ def int4_matvec(x, weight: Int4Weight, *, x_scale=None, out_dtype=None):
     bfloat16). x enters the products exactly and sums are float32. For inference:
     no gradient."""
 
-    require_torch("int4_matvec")
     low = x.dtype == torch.float8_e4m3fn
     if out_dtype is None:
         out_dtype = torch.bfloat16 if low else x.dtype
     if _on_cuda("int4_matvec", x):
         if weight.packed is None:
             raise RuntimeError("int4_matvec: the weight is on the CPU.")
-        with torch.no_grad():
-            return torch.ops.relm_mp_b200.int4_matvec(
-                x, weight.packed, weight.n, weight.k, weight.group, weight.has_zeros, x_scale, out_dtype
-            )
+        return _ops.int4_matvec(x, weight.packed, weight.n, weight.k, weight.group, weight.has_zeros, x_scale, out_dtype)
     if x.size(-1) != weight.k:
         raise RuntimeError(f"int4_matvec: x must be [..., {weight.k}], got {tuple(x.shape)}.")
     if not low and out_dtype != x.dtype:
