@@ -2,9 +2,9 @@
 // 128, forward.
 //
 // A block owns QT tiles of 128 query rows of one head and walks the keys in
-// tiles of 128. One thread copies k and v tiles by tensor map, one thread issues
-// the products, two warps see to masked keys, and four warps per query tile do
-// the softmax, a thread per row:
+// tiles of 128. One thread copies k and v tiles by tensor map, one per query tile
+// issues products, a warp sees to masked keys, and four warps per query tile do the
+// softmax, a thread per row:
 //
 //   S = Q K^T          both operands in shared memory, S (float32) in tensor memory
 //   P = 2^(sc S - m)   rounded to the inputs' type, written over S
@@ -16,8 +16,9 @@
 // float32. With two tiles per block the products of one overlap the softmax of
 // the other, and both read the same k and v from shared memory.
 //
-// Keys outside the sequence or masked get weight 0; their rows of v are zeroed
-// in shared memory first, as 0 times an infinity or NaN would not be 0.
+// Keys outside the sequence or masked get weight 0 by a bias of -inf on their
+// scores. Their rows of k and v are zeroed in shared memory first: what they hold
+// may be an infinity or NaN, which neither a bias nor a weight of 0 would hide.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -31,7 +32,7 @@ namespace {
 using namespace tc;
 
 constexpr float kGrow = 8.f;
-constexpr int kBitSlots = 4;
+constexpr int kBiasSlots = 4;
 
 template < int DP, int QT >
 struct Fwd {
@@ -39,9 +40,19 @@ struct Fwd {
    static constexpr int PANELS = DP / 64;
    static constexpr uint32_t PANEL = kTileRows * 128, TILE = PANELS * PANEL;
    static constexpr uint32_t Q = 0, K = QT * TILE, V = K + ST * TILE, BYTES = V + ST * TILE;
-   static constexpr uint32_t COLS = QT == 2 ? 512 : 256, O = QT * 128; // tensor memory: S tiles, then O tiles
-   static constexpr int THREADS = QT * 128 + 128;
+   // Tensor memory: S tiles, O tiles and, where there is room, weights of their own
+   // (the next S can then be computed while this one is turned into weights).
+   static constexpr bool APART = QT == 2 && DP == 64;
+   static constexpr uint32_t COLS = QT == 2 ? 512 : 256, O = QT * 128, P = APART ? O + QT * DP : 0;
+   static constexpr int MMA_WARP = QT * 4, COPY_WARP = MMA_WARP + QT, MASK_WARP = COPY_WARP + 1, THREADS = (MASK_WARP + 1) * 32;
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+   float d;
+   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+   return d;
+}
 
 // Largest of 32 scores, in four independent chains.
 __device__ __forceinline__ float largest(const uint32_t* s, float top)
@@ -50,30 +61,39 @@ __device__ __forceinline__ float largest(const uint32_t* s, float top)
 #pragma unroll
    for(int i = 0; i < 32; i += 8)
 #pragma unroll
-      for(int k = 0; k < 4; ++k) m[k] = fmaxf(fmaxf(m[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
-   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      for(int k = 0; k < 4; ++k) m[k] = max3(m[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+   return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
-__device__ __forceinline__ void hide(uint32_t* s, unsigned bits)
+// s = s sc + bias: masked keys (bias -inf) fall out. Their k rows are zeros, so s is finite.
+__device__ __forceinline__ void apply_bias(uint32_t* s, const float4* bias, uint64_t sc)
 {
 #pragma unroll
-   for(int i = 0; i < 32; ++i)
-      if(!(bits >> i & 1)) s[i] = 0xff800000u;
-}
-
-// 32 scores to weights 2^(sc s - ref), added to `sum` unrounded and packed.
-template < typename T >
-__device__ __forceinline__ void exponents(const uint32_t* s, uint32_t* p, uint64_t sc, uint64_t ref, uint64_t (&sum)[2])
-{
-#pragma unroll
-   for(int i = 0; i < 16; ++i) {
+   for(int i = 0; i < 8; ++i) {
+      const float4 b = bias[i];
       float x, y;
-      unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc, ref), x, y);
-      x = exp2_fast(x);
-      y = exp2_fast(y);
-      sum[i & 1] = add2(sum[i & 1], pair(x, y));
-      p[i] = pack2< T >(x, y);
+      unpair(fma2(pair(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), sc, pair(b.x, b.y)), x, y);
+      s[4 * i] = __float_as_uint(x), s[4 * i + 1] = __float_as_uint(y);
+      unpair(fma2(pair(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), sc, pair(b.z, b.w)), x, y);
+      s[4 * i + 2] = __float_as_uint(x), s[4 * i + 3] = __float_as_uint(y);
    }
+}
+
+// 32 scores to weights 2^(sc s - ref), added to `sum` unrounded and packed. Each
+// step runs over all of them before the next, in place: with two warps per
+// scheduler a warp that waits for each of its results in turn leaves the units idle.
+template < typename T >
+__device__ __forceinline__ void exponents(uint32_t* s, uint32_t* p, uint64_t sc, uint64_t ref, uint64_t (&sum)[2])
+{
+   float x[32];
+#pragma unroll
+   for(int i = 0; i < 16; ++i) unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc, ref), x[2 * i], x[2 * i + 1]);
+#pragma unroll
+   for(int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
+#pragma unroll
+   for(int i = 0; i < 16; ++i) p[i] = pack2< T >(x[2 * i], x[2 * i + 1]);
+#pragma unroll
+   for(int i = 0; i < 16; ++i) sum[i & 1] = add2(sum[i & 1], pair(x[2 * i], x[2 * i + 1]));
 }
 
 template < typename T, int DP, int QT >
@@ -84,9 +104,9 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    using L = Fwd< DP, QT >;
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-   __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
-   __shared__ uint64_t s_full[QT], p_full[QT][2], o_full[QT], bits_full[kBitSlots], v_last;
-   __shared__ unsigned s_bits[kBitSlots][4];
+   __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], k_clean[L::ST], v_clean[L::ST];
+   __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], bias_full[kBiasSlots], stagger;
+   __shared__ float4 s_bias[kBiasSlots][kTileRows / 4];
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -103,23 +123,26 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       for(int t = 0; t < QT; ++t) {
          mbar_init(&q_full[t], 1);
          mbar_init(&s_full[t], 1);
+         mbar_init(&s_free[t], 128);
          mbar_init(&p_full[t][0], 128);
          mbar_init(&p_full[t][1], 128);
-         mbar_init(&o_full[t], 1);
+         mbar_init(&pv_done[t], 1);
+         mbar_init(&drain[t], 1);
       }
       for(int s = 0; s < L::ST; ++s) {
          mbar_init(&k_full[s], 1);
-         mbar_init(&k_empty[s], 1);
          mbar_init(&v_full[s], 1);
-         mbar_init(&v_empty[s], 1);
-         mbar_init(&v_clean[s], 2);
+         mbar_init(&k_clean[s], 1);
+         mbar_init(&v_clean[s], 1);
+         mbar_init(&k_empty[s], active + 1); // each query tile's products, and the mask warp
+         mbar_init(&v_empty[s], active + 1);
       }
-      for(int s = 0; s < kBitSlots; ++s) mbar_init(&bits_full[s], 2);
-      mbar_init(&v_last, 1);
+      for(int s = 0; s < kBiasSlots; ++s) mbar_init(&bias_full[s], 1);
+      mbar_init(&stagger, 1);
       mbar_init_fence();
       gave_up = 0;
    }
-   if(warp == QT * 4) tmem_alloc(&tmem_base, L::COLS);
+   if(warp == L::MMA_WARP) tmem_alloc(&tmem_base, L::COLS);
    fence_before();
    __syncthreads();
    fence_after();
@@ -127,9 +150,9 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    const uint32_t base = smem_addr(sm);
    // Tiles with keys that take no part: all where there is a mask, else the last if it ends inside.
    auto dirty = [&](int j) { return keep != nullptr || ks.len - j * kTileRows < kTileRows; };
-   auto dirty_parity = [&](int round) { return keep ? round & 1 : 0; };
+   auto dirty_round = [&](int j, int ring) { return keep ? j / ring & 1 : 0; };
 
-   if(warp == QT * 4 + 1) { // copies
+   if(warp == L::COPY_WARP) {
       if(lane == 0 && tiles > 0) {
          const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0);
          const int b = a.q_off ? 0 : it.seq;
@@ -162,110 +185,120 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             }
          }
       }
-   } else if(warp == QT * 4) { // products
-      if(elect_one() && tiles > 0) {
+   } else if(warp >= L::MMA_WARP && warp < L::COPY_WARP) { // products of one query tile
+      const int t = warp - L::MMA_WARP;
+      if(elect_one() && tiles > 0 && t < active) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t pv = instruction(BF, 128, steps * 16, true);
-         auto keys16 = [&](int j) { return min(kTileRows, (ks.len - j * kTileRows + 15) / 16 * 16); };
-         auto scores = [&](int t, int j) {
-            product_columns< DP, kTileRows, kTileRows >(tmem + t * 128, base + L::Q + t * L::TILE, base + L::K + (j % L::ST) * L::TILE,
-                                                        instruction(BF, 128, keys16(j), false), steps);
-            mma_commit(&s_full[t]);
+         const uint32_t pt = tmem + (L::APART ? L::P + t * 64 : t * 128), ot = tmem + L::O + t * DP;
+         // Keys of tile j: S for whole chunks of 32 (the softmax reads those), the second product in steps of 16.
+         auto keys = [&](int j, int unit) { return min(kTileRows, (ks.len - j * kTileRows + unit - 1) / unit * unit); };
+         auto ready = [&](uint64_t* full, uint64_t* clean, int j) {
+            return mbar_wait(&full[j % L::ST], (j / L::ST) & 1) && (!dirty(j) || mbar_wait(&clean[j % L::ST], dirty_round(j, L::ST)));
          };
-         bool ok = mbar_wait(&k_full[0], 0);
-         for(int t = 0; t < active && ok; ++t) {
-            ok = mbar_wait(&q_full[t], 0);
-            if(ok) scores(t, 0);
-         }
-         if(ok) mma_commit(&k_empty[0]);
+         auto scores = [&](int j) {
+            product_columns< DP, kTileRows, kTileRows >(tmem + t * 128, base + L::Q + t * L::TILE, base + L::K + (j % L::ST) * L::TILE,
+                                                        instruction(BF, 128, keys(j, 32), false), steps);
+            mma_commit(&s_full[t]);
+            mma_commit(&k_empty[j % L::ST]);
+         };
+         // The second tile starts half an iteration after the first and stays there: in step, both would take
+         // the exponential unit at once and leave it idle at once (D = 128: 370 us in step, STAGGERED apart).
+         const bool apart = active == 2 && tiles >= 4;
+         bool ok = mbar_wait(&q_full[t], 0) && ready(k_full, k_clean, 0) && (!apart || t == 0 || mbar_wait(&stagger, 0));
+         if(ok) scores(0);
          for(int j = 0; j < tiles && ok; ++j) {
-            const int n = keys16(j) / 16, s = j % L::ST, round = j / L::ST;
-            ok = mbar_wait(&v_full[s], round & 1);
-            if(ok && dirty(j)) {
-               if(!keep) mbar_arrive(&v_last);
-               ok = mbar_wait(&v_clean[s], dirty_parity(round));
-            }
-            for(int t = 0; t < active && ok; ++t) {
-               const uint32_t va = base + L::V + s * L::TILE;
-               // The weights come in two halves of 64 keys.
-               if(!(ok = mbar_wait(&p_full[t][0], j & 1))) break;
+            if(L::APART && j + 1 < tiles) { // the scores have been read: the next ones
+               if(!(ok = mbar_wait(&s_free[t], j & 1) && ready(k_full, k_clean, j + 1))) break;
                fence_after();
-               product_rows< 0, 4, 0, kTileRows >(tmem + L::O + t * DP, tmem + t * 128, va, pv, n, j > 0);
-               if(!(ok = mbar_wait(&p_full[t][1], j & 1))) break;
-               fence_after();
-               product_rows< 4, 4, 0, kTileRows >(tmem + L::O + t * DP, tmem + t * 128, va, pv, n, true);
-               if(j + 1 == tiles) mma_commit(&o_full[t]);
-               else {
-                  ok = mbar_wait(&k_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1);
-                  if(ok) scores(t, j + 1);
-               }
+               scores(j + 1);
             }
-            if(!ok) break;
-            mma_commit(&v_empty[s]);
-            if(j + 1 < tiles) mma_commit(&k_empty[(j + 1) % L::ST]);
+            const int n = keys(j, 16) / 16;
+            const uint32_t va = base + L::V + (j % L::ST) * L::TILE;
+            // The weights come in two halves of 64 keys.
+            if(!(ok = ready(v_full, v_clean, j) && mbar_wait(&p_full[t][0], j & 1))) break;
+            fence_after();
+            product_rows< 0, 4, 0, kTileRows >(ot, pt, va, pv, n, j > 0);
+            if(!(ok = mbar_wait(&p_full[t][1], j & 1))) break;
+            fence_after();
+            product_rows< 4, 4, 0, kTileRows >(ot, pt, va, pv, n, true);
+            mma_commit(&pv_done[t]);
+            mma_commit(&v_empty[j % L::ST]);
+            if(!L::APART && j + 1 < tiles) {
+               if(!(ok = ready(k_full, k_clean, j + 1))) break;
+               scores(j + 1);
+            }
          }
          if(!ok) {
             gave_up = 1;
-            // Products in flight read shared and tensor memory: wait for them before the block ends.
-            mma_commit(&q_full[0]);
-            mbar_wait(&q_full[0], 1);
+            mma_commit(&drain[t]); // products in flight read shared and tensor memory: wait for them before the block ends
+            mbar_wait(&drain[t], 0);
          }
       }
-   } else if(warp >= QT * 4 + 2) { // masks: 64 keys of each tile per warp
-      const int w = warp - (QT * 4 + 2);
-      for(int j = keep ? 0 : max(tiles - 1, 0); j < tiles; ++j) {
-         if(!dirty(j)) break;
-         const int left = ks.len - j * kTileRows, s = j % L::ST;
-         unsigned bits[2];
+   } else if(warp == L::MASK_WARP) {
+      // Follows every tile (so that it never falls a phase behind) and works on those with keys that take
+      // no part: a bias of -inf for them, and zeros in their rows of k and v, whatever these held.
+      auto clear = [&](uint32_t tile, const unsigned(&bits)[4]) {
 #pragma unroll
-         for(int c = 0; c < 2; ++c) {
-            const int key = w * 64 + c * 32 + lane;
-            bits[c] = __ballot_sync(~0u, key < left && (!keep || keep[j * kTileRows + key]));
-         }
-         // The slot's last reader was tile j - 4; v of tile j - 1 arrived after the products of tile j - 3 or later.
-         if(keep && lane == 0) {
-            s_bits[j % kBitSlots][2 * w] = bits[0];
-            s_bits[j % kBitSlots][2 * w + 1] = bits[1];
-            mbar_arrive(&bits_full[j % kBitSlots]);
-         }
-         // Without a mask this warp has not followed the phases of v_full: it is called for the last tile.
-         if(!__all_sync(~0u, (keep || mbar_wait(&v_last, 0)) && mbar_wait(&v_full[s], (j / L::ST) & 1))) {
-            gave_up = 1;
-            break;
-         }
-#pragma unroll
-         for(int c = 0; c < 2; ++c)
+         for(int c = 0; c < 4; ++c)
             if(!(bits[c] >> lane & 1))
                for(int p = 0; p < L::PANELS; ++p) {
-                  uint4* line = reinterpret_cast< uint4* >(sm + L::V + s * L::TILE + p * L::PANEL + (w * 64 + c * 32 + lane) * 128);
+                  uint4* line = reinterpret_cast< uint4* >(sm + tile + p * L::PANEL + (c * 32 + lane) * 128);
 #pragma unroll
                   for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
                }
          fence_async_proxy();
          __syncwarp();
-         if(lane == 0) mbar_arrive(&v_clean[s]);
+      };
+      for(int j = 0; j < tiles; ++j) {
+         const int left = ks.len - j * kTileRows, s = j % L::ST;
+         const bool work = dirty(j);
+         unsigned bits[4];
+         if(work) {
+            // The slot was last read for tile j - 4, whose weights were done before v of tile j - 1 arrived.
+            const int slot = keep ? j % kBiasSlots : 0;
+#pragma unroll
+            for(int c = 0; c < 4; ++c) {
+               const int key = c * 32 + lane;
+               const bool in = key < left && (!keep || keep[j * kTileRows + key]);
+               bits[c] = __ballot_sync(~0u, in);
+               reinterpret_cast< float* >(s_bias[slot])[key] = in ? 0.f : -CUDART_INF_F;
+            }
+            __syncwarp();
+            if(lane == 0) mbar_arrive(&bias_full[slot]);
+         }
+         bool ok = __all_sync(~0u, mbar_wait(&k_full[s], (j / L::ST) & 1));
+         if(ok && work) clear(L::K + s * L::TILE, bits);
+         if(ok && lane == 0) {
+            if(work) mbar_arrive(&k_clean[s]);
+            mbar_arrive(&k_empty[s]);
+         }
+         ok = ok && __all_sync(~0u, mbar_wait(&v_full[s], (j / L::ST) & 1));
+         if(ok && work) clear(L::V + s * L::TILE, bits);
+         if(ok && lane == 0) {
+            if(work) mbar_arrive(&v_clean[s]);
+            mbar_arrive(&v_empty[s]);
+         }
+         if(!ok) {
+            gave_up = 1;
+            break;
+         }
       }
    } else { // softmax: thread = row of tile t
       const int t = warp >> 2;
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), st = lanes + t * 128, ot = lanes + L::O + t * DP;
+      const uint32_t pt = L::APART ? lanes + L::P + t * 64 : st;
       const float sc = a.scale * kLog2e;
-      const uint64_t sc2 = pair(sc, sc);
+      const uint64_t sc2 = pair(sc, sc), one2 = pair(1.f, 1.f);
       float m = -CUDART_INF_F;
       uint64_t sum[2] = {0, 0};
       bool ok = true;
       if(t < active) {
          for(int j = 0; j < tiles && ok; ++j) {
-            const int left = ks.len - j * kTileRows, chunks = min(4, (left + 31) / 32);
-            unsigned bits[4] = {~0u, ~0u, ~0u, ~0u};
+            const int chunks = min(4, (ks.len - j * kTileRows + 31) / 32);
             const bool partial = dirty(j);
-            if(keep) {
-               ok = __all_sync(~0u, mbar_wait(&bits_full[j % kBitSlots], (j / kBitSlots) & 1));
-#pragma unroll
-               for(int c = 0; c < 4; ++c) bits[c] = s_bits[j % kBitSlots][c];
-            } else if(partial) {
-#pragma unroll
-               for(int c = 0; c < 4; ++c) bits[c] = left >= 32 * c + 32 ? ~0u : left <= 32 * c ? 0u : (1u << (left - 32 * c)) - 1u;
-            }
+            const float4* bias = s_bias[keep ? j % kBiasSlots : 0];
+            if(partial) ok = __all_sync(~0u, mbar_wait(&bias_full[keep ? j % kBiasSlots : 0], dirty_round(j, kBiasSlots)));
             ok = ok && __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
             if(!ok) break;
             fence_after();
@@ -277,12 +310,18 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   if(c < chunks) tmem_ld32(s + c * 32, st + c * 32);
                wait_ld();
                loaded< 128 >(s);
-#pragma unroll
-               for(int c = 0; c < 4; ++c) {
-                  if(c >= chunks) continue;
-                  if(partial) hide(s + c * 32, bits[c]);
-                  top = largest(s + c * 32, top);
+               if constexpr(L::APART) {
+                  fence_before();
+                  mbar_arrive(&s_free[t]);
                }
+               if(partial) {
+#pragma unroll
+                  for(int c = 0; c < 4; ++c)
+                     if(c < chunks) apply_bias(s + c * 32, bias + c * 8, sc2);
+               }
+#pragma unroll
+               for(int c = 0; c < 4; ++c)
+                  if(c < chunks) top = largest(s + c * 32, top);
             } else { // two blocks share the registers: the scores are read twice, 32 at a time
                tmem_ld32(s, st);
 #pragma unroll
@@ -291,12 +330,14 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   wait_ld();
                   loaded< 32 >(s + (c & 1) * 32);
                   if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
-                  if(partial) hide(s + (c & 1) * 32, bits[c]);
+                  if(partial) apply_bias(s + (c & 1) * 32, bias + c * 8, sc2);
                   top = largest(s + (c & 1) * 32, top);
                }
                tmem_ld32(s, st);
             }
-            top *= sc;
+            if(!partial) top *= sc;
+            if constexpr(L::APART) // the last weights have been used
+               if(j > 0 && !(ok = __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1)))) break;
             float f = 1.f;
             if(top > m + kGrow || (m == -CUDART_INF_F && top > m)) {
                f = exp2_fast(m - top);
@@ -304,7 +345,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                sum[0] = mul2(sum[0], pair(f, f));
                sum[1] = mul2(sum[1], pair(f, f));
             }
-            if(j > 0 && __any_sync(~0u, f != 1.f)) { // the products into O so far were done before this S
+            if(j > 0 && __any_sync(~0u, f != 1.f)) { // the products into O so far are done (before this S, or waited for above)
                for(int c = 0; c < a.dim; c += 16) {
                   uint32_t o[16];
                   tmem_ld16(o, ot + c);
@@ -315,23 +356,24 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   tmem_st16(ot + c, o);
                }
             }
+            if(QT == 2 && j == 0 && threadIdx.x == 0) mbar_arrive(&stagger); // this tile's exponentials begin
             const float ref = m == -CUDART_INF_F ? 0.f : m;
-            const uint64_t ref2 = pair(-ref, -ref);
+            const uint64_t ref2 = pair(-ref, -ref), by = partial ? one2 : sc2;
 #pragma unroll
             for(int c = 0; c < 4; ++c) {
                if(c < chunks) {
                   uint32_t p[16];
                   if constexpr(QT == 2) {
-                     exponents< T >(s + c * 32, p, sc2, ref2, sum);
+                     exponents< T >(s + c * 32, p, by, ref2, sum);
                   } else {
                      wait_ld();
                      loaded< 32 >(s + (c & 1) * 32);
                      if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
-                     if(partial) hide(s + (c & 1) * 32, bits[c]);
-                     exponents< T >(s + (c & 1) * 32, p, sc2, ref2, sum);
+                     if(partial) apply_bias(s + (c & 1) * 32, bias + c * 8, sc2);
+                     exponents< T >(s + (c & 1) * 32, p, by, ref2, sum);
                      // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
                   }
-                  tmem_st16(st + c * 16, p);
+                  tmem_st16(pt + c * 16, p);
                }
                if(c & 1) {
                   wait_st();
@@ -343,7 +385,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          float l, l1;
          unpair(add2(sum[0], sum[1]), l, l1);
          l += l1;
-         if(ok && tiles > 0) ok = __all_sync(~0u, mbar_wait(&o_full[t], 0));
+         if(ok && tiles > 0) ok = __all_sync(~0u, mbar_wait(&pv_done[t], (tiles - 1) & 1));
          fence_after();
          // Rows leave through the q tile's shared memory (its products are done), 16 bytes a lane along the rows.
          const bool none = l == 0.f;
@@ -395,7 +437,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    fence_before();
    __syncthreads();
    fence_after();
-   if(warp == QT * 4) tmem_free(tmem, L::COLS);
+   if(warp == L::MMA_WARP) tmem_free(tmem, L::COLS);
    if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
 }
 
