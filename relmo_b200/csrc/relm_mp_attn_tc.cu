@@ -16,9 +16,9 @@
 // float32. With two tiles per block the products of one overlap the softmax of
 // the other, and both read the same k and v from shared memory.
 //
-// Keys outside the sequence or masked get weight 0 by a bias of -inf on their
-// scores. Their rows of k and v are zeroed in shared memory first: what they hold
-// may be an infinity or NaN, which neither a bias nor a weight of 0 would hide.
+// Keys outside the sequence or masked get a score of -inf, so weight 0. Their rows
+// of v are zeroed in shared memory first: what they hold may be an infinity or NaN,
+// which a weight of 0 would not hide.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -32,7 +32,7 @@ namespace {
 using namespace tc;
 
 constexpr float kGrow = 8.f;
-constexpr int kBiasSlots = 4;
+constexpr int kLimitSlots = 4;
 
 template < int DP, int QT >
 struct Fwd {
@@ -65,17 +65,18 @@ __device__ __forceinline__ float largest(const uint32_t* s, float top)
    return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
-// s = s sc + bias: masked keys (bias -inf) fall out. Their k rows are zeros, so s is finite.
-__device__ __forceinline__ void apply_bias(uint32_t* s, const float4* bias, uint64_t sc)
+// Masked keys (limit -inf) fall out, the others (limit +inf) stay: the smaller of
+// score and limit is right even for a masked score that is NaN. (A kept one that
+// is NaN becomes +inf, and NaN again when the row's maximum is taken off it.)
+__device__ __forceinline__ void apply_limit(uint32_t* s, const float4* limit)
 {
 #pragma unroll
    for(int i = 0; i < 8; ++i) {
-      const float4 b = bias[i];
-      float x, y;
-      unpair(fma2(pair(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), sc, pair(b.x, b.y)), x, y);
-      s[4 * i] = __float_as_uint(x), s[4 * i + 1] = __float_as_uint(y);
-      unpair(fma2(pair(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), sc, pair(b.z, b.w)), x, y);
-      s[4 * i + 2] = __float_as_uint(x), s[4 * i + 3] = __float_as_uint(y);
+      const float4 b = limit[i];
+      s[4 * i] = __float_as_uint(fminf(__uint_as_float(s[4 * i]), b.x));
+      s[4 * i + 1] = __float_as_uint(fminf(__uint_as_float(s[4 * i + 1]), b.y));
+      s[4 * i + 2] = __float_as_uint(fminf(__uint_as_float(s[4 * i + 2]), b.z));
+      s[4 * i + 3] = __float_as_uint(fminf(__uint_as_float(s[4 * i + 3]), b.w));
    }
 }
 
@@ -104,9 +105,9 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    using L = Fwd< DP, QT >;
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-   __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], k_clean[L::ST], v_clean[L::ST];
-   __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], bias_full[kBiasSlots], stagger;
-   __shared__ float4 s_bias[kBiasSlots][kTileRows / 4];
+   __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
+   __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], limit_full[kLimitSlots], stagger;
+   __shared__ float4 s_limit[kLimitSlots][kTileRows / 4];
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -132,12 +133,11 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       for(int s = 0; s < L::ST; ++s) {
          mbar_init(&k_full[s], 1);
          mbar_init(&v_full[s], 1);
-         mbar_init(&k_clean[s], 1);
          mbar_init(&v_clean[s], 1);
-         mbar_init(&k_empty[s], active + 1); // each query tile's products, and the mask warp
-         mbar_init(&v_empty[s], active + 1);
+         mbar_init(&k_empty[s], active);     // each query tile's products
+         mbar_init(&v_empty[s], active + 1); // and the mask warp
       }
-      for(int s = 0; s < kBiasSlots; ++s) mbar_init(&bias_full[s], 1);
+      for(int s = 0; s < kLimitSlots; ++s) mbar_init(&limit_full[s], 1);
       mbar_init(&stagger, 1);
       mbar_init_fence();
       gave_up = 0;
@@ -191,32 +191,32 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          const int steps = (a.dim + 15) / 16;
          const uint32_t pv = instruction(BF, 128, steps * 16, true);
          const uint32_t pt = tmem + (L::APART ? L::P + t * 64 : t * 128), ot = tmem + L::O + t * DP;
-         // Keys of tile j: S for whole chunks of 32 (the softmax reads those), the second product in steps of 16.
-         auto keys = [&](int j, int unit) { return min(kTileRows, (ks.len - j * kTileRows + unit - 1) / unit * unit); };
-         auto ready = [&](uint64_t* full, uint64_t* clean, int j) {
-            return mbar_wait(&full[j % L::ST], (j / L::ST) & 1) && (!dirty(j) || mbar_wait(&clean[j % L::ST], dirty_round(j, L::ST)));
+         auto keys16 = [&](int j) { return min(kTileRows, (ks.len - j * kTileRows + 15) / 16 * 16); };
+         auto k_ready = [&](int j) { return mbar_wait(&k_full[j % L::ST], (j / L::ST) & 1); };
+         auto v_ready = [&](int j) {
+            return mbar_wait(&v_full[j % L::ST], (j / L::ST) & 1) && (!dirty(j) || mbar_wait(&v_clean[j % L::ST], dirty_round(j, L::ST)));
          };
          auto scores = [&](int j) {
             product_columns< DP, kTileRows, kTileRows >(tmem + t * 128, base + L::Q + t * L::TILE, base + L::K + (j % L::ST) * L::TILE,
-                                                        instruction(BF, 128, keys(j, 32), false), steps);
+                                                        instruction(BF, 128, keys16(j), false), steps);
             mma_commit(&s_full[t]);
             mma_commit(&k_empty[j % L::ST]);
          };
          // The second tile starts half an iteration after the first and stays there: in step, both would take
          // the exponential unit at once and leave it idle at once (D = 128: 370 us in step, STAGGERED apart).
          const bool apart = active == 2 && tiles >= 4;
-         bool ok = mbar_wait(&q_full[t], 0) && ready(k_full, k_clean, 0) && (!apart || t == 0 || mbar_wait(&stagger, 0));
+         bool ok = mbar_wait(&q_full[t], 0) && k_ready(0) && (!apart || t == 0 || mbar_wait(&stagger, 0));
          if(ok) scores(0);
          for(int j = 0; j < tiles && ok; ++j) {
             if(L::APART && j + 1 < tiles) { // the scores have been read: the next ones
-               if(!(ok = mbar_wait(&s_free[t], j & 1) && ready(k_full, k_clean, j + 1))) break;
+               if(!(ok = mbar_wait(&s_free[t], j & 1) && k_ready(j + 1))) break;
                fence_after();
                scores(j + 1);
             }
-            const int n = keys(j, 16) / 16;
+            const int n = keys16(j) / 16;
             const uint32_t va = base + L::V + (j % L::ST) * L::TILE;
             // The weights come in two halves of 64 keys.
-            if(!(ok = ready(v_full, v_clean, j) && mbar_wait(&p_full[t][0], j & 1))) break;
+            if(!(ok = v_ready(j) && mbar_wait(&p_full[t][0], j & 1))) break;
             fence_after();
             product_rows< 0, 4, 0, kTileRows >(ot, pt, va, pv, n, j > 0);
             if(!(ok = mbar_wait(&p_full[t][1], j & 1))) break;
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             mma_commit(&pv_done[t]);
             mma_commit(&v_empty[j % L::ST]);
             if(!L::APART && j + 1 < tiles) {
-               if(!(ok = ready(k_full, k_clean, j + 1))) break;
+               if(!(ok = k_ready(j + 1))) break;
                scores(j + 1);
             }
          }
@@ -236,52 +236,53 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          }
       }
    } else if(warp == L::MASK_WARP) {
-      // Follows every tile (so that it never falls a phase behind) and works on those with keys that take
-      // no part: a bias of -inf for them, and zeros in their rows of k and v, whatever these held.
-      auto clear = [&](uint32_t tile, const unsigned(&bits)[4]) {
+      // Follows every tile (so that it never falls a phase behind) and works on those with keys that take no
+      // part: limits for their scores, and zeros in their rows of v, whatever these held.
+      bool next[4];
+      auto kept = [&](int j) {
 #pragma unroll
-         for(int c = 0; c < 4; ++c)
-            if(!(bits[c] >> lane & 1))
-               for(int p = 0; p < L::PANELS; ++p) {
-                  uint4* line = reinterpret_cast< uint4* >(sm + tile + p * L::PANEL + (c * 32 + lane) * 128);
-#pragma unroll
-                  for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
-               }
-         fence_async_proxy();
-         __syncwarp();
+         for(int c = 0; c < 4; ++c) {
+            const int key = j * kTileRows + c * 32 + lane;
+            next[c] = key < ks.len && (!keep || keep[key]);
+         }
       };
+      kept(0);
       for(int j = 0; j < tiles; ++j) {
-         const int left = ks.len - j * kTileRows, s = j % L::ST;
+         const int s = j % L::ST;
          const bool work = dirty(j);
          unsigned bits[4];
          if(work) {
             // The slot was last read for tile j - 4, whose weights were done before v of tile j - 1 arrived.
-            const int slot = keep ? j % kBiasSlots : 0;
+            const int slot = keep ? j % kLimitSlots : 0;
 #pragma unroll
             for(int c = 0; c < 4; ++c) {
-               const int key = c * 32 + lane;
-               const bool in = key < left && (!keep || keep[j * kTileRows + key]);
-               bits[c] = __ballot_sync(~0u, in);
-               reinterpret_cast< float* >(s_bias[slot])[key] = in ? 0.f : -CUDART_INF_F;
+               bits[c] = __ballot_sync(~0u, next[c]);
+               reinterpret_cast< float* >(s_limit[slot])[c * 32 + lane] = next[c] ? CUDART_INF_F : -CUDART_INF_F;
             }
             __syncwarp();
-            if(lane == 0) mbar_arrive(&bias_full[slot]);
+            if(lane == 0) mbar_arrive(&limit_full[slot]);
          }
-         bool ok = __all_sync(~0u, mbar_wait(&k_full[s], (j / L::ST) & 1));
-         if(ok && work) clear(L::K + s * L::TILE, bits);
-         if(ok && lane == 0) {
-            if(work) mbar_arrive(&k_clean[s]);
-            mbar_arrive(&k_empty[s]);
-         }
-         ok = ok && __all_sync(~0u, mbar_wait(&v_full[s], (j / L::ST) & 1));
-         if(ok && work) clear(L::V + s * L::TILE, bits);
-         if(ok && lane == 0) {
-            if(work) mbar_arrive(&v_clean[s]);
-            mbar_arrive(&v_empty[s]);
-         }
+         kept(j + 1); // on its way while v is waited for
+         const bool ok = __all_sync(~0u, mbar_wait(&v_full[s], (j / L::ST) & 1));
          if(!ok) {
             gave_up = 1;
             break;
+         }
+         if(work) {
+#pragma unroll
+            for(int c = 0; c < 4; ++c)
+               if(!(bits[c] >> lane & 1))
+                  for(int p = 0; p < L::PANELS; ++p) {
+                     uint4* line = reinterpret_cast< uint4* >(sm + L::V + s * L::TILE + p * L::PANEL + (c * 32 + lane) * 128);
+#pragma unroll
+                     for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
+                  }
+            fence_async_proxy();
+            __syncwarp();
+         }
+         if(lane == 0) {
+            if(work) mbar_arrive(&v_clean[s]);
+            mbar_arrive(&v_empty[s]);
          }
       }
    } else { // softmax: thread = row of tile t
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), st = lanes + t * 128, ot = lanes + L::O + t * DP;
       const uint32_t pt = L::APART ? lanes + L::P + t * 64 : st;
       const float sc = a.scale * kLog2e;
-      const uint64_t sc2 = pair(sc, sc), one2 = pair(1.f, 1.f);
+      const uint64_t sc2 = pair(sc, sc);
       float m = -CUDART_INF_F;
       uint64_t sum[2] = {0, 0};
       bool ok = true;
@@ -297,8 +298,8 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          for(int j = 0; j < tiles && ok; ++j) {
             const int chunks = min(4, (ks.len - j * kTileRows + 31) / 32);
             const bool partial = dirty(j);
-            const float4* bias = s_bias[keep ? j % kBiasSlots : 0];
-            if(partial) ok = __all_sync(~0u, mbar_wait(&bias_full[keep ? j % kBiasSlots : 0], dirty_round(j, kBiasSlots)));
+            const float4* limit = s_limit[keep ? j % kLimitSlots : 0];
+            if(partial) ok = __all_sync(~0u, mbar_wait(&limit_full[keep ? j % kLimitSlots : 0], dirty_round(j, kLimitSlots)));
             ok = ok && __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
             if(!ok) break;
             fence_after();
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                if(partial) {
 #pragma unroll
                   for(int c = 0; c < 4; ++c)
-                     if(c < chunks) apply_bias(s + c * 32, bias + c * 8, sc2);
+                     if(c < chunks) apply_limit(s + c * 32, limit + c * 8);
                }
 #pragma unroll
                for(int c = 0; c < 4; ++c)
@@ -330,12 +331,12 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   wait_ld();
                   loaded< 32 >(s + (c & 1) * 32);
                   if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
-                  if(partial) apply_bias(s + (c & 1) * 32, bias + c * 8, sc2);
+                  if(partial) apply_limit(s + (c & 1) * 32, limit + c * 8);
                   top = largest(s + (c & 1) * 32, top);
                }
                tmem_ld32(s, st);
             }
-            if(!partial) top *= sc;
+            top *= sc;
             if constexpr(L::APART) // the last weights have been used
                if(j > 0 && !(ok = __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1)))) break;
             float f = 1.f;
@@ -358,19 +359,19 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             }
             if(QT == 2 && j == 0 && threadIdx.x == 0) mbar_arrive(&stagger); // this tile's exponentials begin
             const float ref = m == -CUDART_INF_F ? 0.f : m;
-            const uint64_t ref2 = pair(-ref, -ref), by = partial ? one2 : sc2;
+            const uint64_t ref2 = pair(-ref, -ref);
 #pragma unroll
             for(int c = 0; c < 4; ++c) {
                if(c < chunks) {
                   uint32_t p[16];
                   if constexpr(QT == 2) {
-                     exponents< T >(s + c * 32, p, by, ref2, sum);
+                     exponents< T >(s + c * 32, p, sc2, ref2, sum);
                   } else {
                      wait_ld();
                      loaded< 32 >(s + (c & 1) * 32);
                      if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
-                     if(partial) apply_bias(s + (c & 1) * 32, bias + c * 8, sc2);
-                     exponents< T >(s + (c & 1) * 32, p, by, ref2, sum);
+                     if(partial) apply_limit(s + (c & 1) * 32, limit + c * 8);
+                     exponents< T >(s + (c & 1) * 32, p, sc2, ref2, sum);
                      // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
                   }
                   tmem_st16(pt + c * 16, p);
