@@ -44,7 +44,10 @@ struct Fwd {
    // (the next S can then be computed while this one is turned into weights).
    static constexpr bool APART = QT == 2 && DP == 64;
    static constexpr uint32_t COLS = QT == 2 ? 512 : 256, O = QT * 128, P = APART ? O + QT * DP : 0;
-   static constexpr int MMA_WARP = QT * 4, COPY_WARP = MMA_WARP + QT, MASK_WARP = COPY_WARP + 1, THREADS = (MASK_WARP + 1) * 32;
+   // Threads of a row: two tiles have the registers for a thread per half row, and with four
+   // softmax warps per scheduler the waits of one are filled by others.
+   static constexpr int HALVES = QT == 2 ? 2 : 1, SOFT = 128 * HALVES;
+   static constexpr int MMA_WARP = QT * 4 * HALVES, COPY_WARP = MMA_WARP + QT, MASK_WARP = COPY_WARP + 1, THREADS = (MASK_WARP + 1) * 32;
 };
 
 __device__ __forceinline__ float max3(float a, float b, float c)
@@ -108,6 +111,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
    __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], limit_full[kLimitSlots], stagger;
    __shared__ float4 s_limit[kLimitSlots][kTileRows / 4];
+   __shared__ float s_top[2][QT][L::HALVES][L::HALVES == 2 ? kTileRows : 1]; // of the two halves of a row, by iteration parity
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       for(int t = 0; t < QT; ++t) {
          mbar_init(&q_full[t], 1);
          mbar_init(&s_full[t], 1);
-         mbar_init(&s_free[t], 128);
+         mbar_init(&s_free[t], L::SOFT);
          mbar_init(&p_full[t][0], 128);
          mbar_init(&p_full[t][1], 128);
          mbar_init(&pv_done[t], 1);
@@ -285,8 +289,8 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             mbar_arrive(&v_empty[s]);
          }
       }
-   } else { // softmax: thread = row of tile t
-      const int t = warp >> 2;
+   } else { // softmax: thread = row of tile t, or half h of its keys
+      const int t = warp / (4 * L::HALVES), h = L::HALVES == 2 ? warp >> 2 & 1 : 0, row = threadIdx.x & 127;
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), st = lanes + t * 128, ot = lanes + L::O + t * DP;
       const uint32_t pt = L::APART ? lanes + L::P + t * 64 : st;
       const float sc = a.scale * kLog2e;
@@ -294,35 +298,38 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       float m = -CUDART_INF_F;
       uint64_t sum[2] = {0, 0};
       bool ok = true;
+      // The two warps that share 32 rows.
+      auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
       if(t < active) {
-         for(int j = 0; j < tiles && ok; ++j) {
+         for(int j = 0; j < tiles; ++j) {
             const int chunks = min(4, (ks.len - j * kTileRows + 31) / 32);
             const bool partial = dirty(j);
             const float4* limit = s_limit[keep ? j % kLimitSlots : 0];
-            if(partial) ok = __all_sync(~0u, mbar_wait(&limit_full[keep ? j % kLimitSlots : 0], dirty_round(j, kLimitSlots)));
+            if(partial) ok = ok && __all_sync(~0u, mbar_wait(&limit_full[keep ? j % kLimitSlots : 0], dirty_round(j, kLimitSlots)));
             ok = ok && __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
-            if(!ok) break;
+            // (Where a wait gave up the loop runs on without waits: the two halves of a row meet at barriers.)
             fence_after();
-            uint32_t s[QT == 2 ? 128 : 64];
+            uint32_t s[64];
             float top = -CUDART_INF_F;
-            if constexpr(QT == 2) {
+            if constexpr(L::HALVES == 2) {
 #pragma unroll
-               for(int c = 0; c < 4; ++c)
-                  if(c < chunks) tmem_ld32(s + c * 32, st + c * 32);
+               for(int c = 0; c < 2; ++c)
+                  if(2 * h + c < chunks) tmem_ld32(s + c * 32, st + (2 * h + c) * 32);
                wait_ld();
-               loaded< 128 >(s);
-               if constexpr(L::APART) {
-                  fence_before();
-                  mbar_arrive(&s_free[t]);
-               }
-               if(partial) {
+               loaded< 64 >(s);
+               fence_before();
+               if constexpr(L::APART) mbar_arrive(&s_free[t]);
 #pragma unroll
-                  for(int c = 0; c < 4; ++c)
-                     if(c < chunks) apply_limit(s + c * 32, limit + c * 8);
+               for(int c = 0; c < 2; ++c) {
+                  if(2 * h + c >= chunks) continue;
+                  if(partial) apply_limit(s + c * 32, limit + (2 * h + c) * 8);
+                  top = largest(s + c * 32, top);
                }
-#pragma unroll
-               for(int c = 0; c < 4; ++c)
-                  if(c < chunks) top = largest(s + c * 32, top);
+               // A NaN is left out of the maximum here and of the exchange: it shows in its own weights.
+               s_top[j & 1][t][h][row] = top;
+               pair_sync(); // both halves' scores are in registers: their place may take weights
+               fence_after();
+               top = fmaxf(top, s_top[j & 1][t][h ^ 1][row]);
             } else { // two blocks share the registers: the scores are read twice, 32 at a time
                tmem_ld32(s, st);
 #pragma unroll
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             }
             top *= sc;
             if constexpr(L::APART) // the last weights have been used
-               if(j > 0 && !(ok = __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1)))) break;
+               if(j > 0) ok = ok && __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1));
             float f = 1.f;
             if(top > m + kGrow || (m == -CUDART_INF_F && top > m)) {
                f = exp2_fast(m - top);
@@ -347,7 +354,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                sum[1] = mul2(sum[1], pair(f, f));
             }
             if(j > 0 && __any_sync(~0u, f != 1.f)) { // the products into O so far are done (before this S, or waited for above)
-               for(int c = 0; c < a.dim; c += 16) {
+               for(int c = h * 16; c < a.dim; c += 16 * L::HALVES) {
                   uint32_t o[16];
                   tmem_ld16(o, ot + c);
                   wait_ld();
@@ -360,26 +367,35 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             if(QT == 2 && j == 0 && threadIdx.x == 0) mbar_arrive(&stagger); // this tile's exponentials begin
             const float ref = m == -CUDART_INF_F ? 0.f : m;
             const uint64_t ref2 = pair(-ref, -ref);
+            if constexpr(L::HALVES == 2) {
 #pragma unroll
-            for(int c = 0; c < 4; ++c) {
-               if(c < chunks) {
+               for(int c = 0; c < 2; ++c) {
+                  if(2 * h + c >= chunks) continue;
                   uint32_t p[16];
-                  if constexpr(QT == 2) {
-                     exponents< T >(s + c * 32, p, sc2, ref2, sum);
-                  } else {
+                  exponents< T >(s + c * 32, p, sc2, ref2, sum);
+                  tmem_st16(pt + (2 * h + c) * 16, p);
+               }
+               wait_st();
+               fence_before();
+               mbar_arrive(&p_full[t][h]);
+            } else {
+#pragma unroll
+               for(int c = 0; c < 4; ++c) {
+                  if(c < chunks) {
+                     uint32_t p[16];
                      wait_ld();
                      loaded< 32 >(s + (c & 1) * 32);
                      if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
                      if(partial) apply_limit(s + (c & 1) * 32, limit + c * 8);
                      exponents< T >(s + (c & 1) * 32, p, sc2, ref2, sum);
                      // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
+                     tmem_st16(pt + c * 16, p);
                   }
-                  tmem_st16(pt + c * 16, p);
-               }
-               if(c & 1) {
-                  wait_st();
-                  fence_before();
-                  mbar_arrive(&p_full[t][c >> 1]);
+                  if(c & 1) {
+                     wait_st();
+                     fence_before();
+                     mbar_arrive(&p_full[t][c >> 1]);
+                  }
                }
             }
          }
@@ -388,6 +404,14 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          l += l1;
          if(ok && tiles > 0) ok = __all_sync(~0u, mbar_wait(&pv_done[t], (tiles - 1) & 1));
          fence_after();
+         if constexpr(L::HALVES == 2) {
+            pair_sync();
+            s_top[0][t][h][row] = l;
+            s_top[1][t][h][row] = ok ? 1.f : 0.f;
+            pair_sync();
+            l += s_top[0][t][h ^ 1][row];
+            ok = ok && s_top[1][t][h ^ 1][row] == 1.f;
+         }
          // Rows leave through the q tile's shared memory (its products are done), 16 bytes a lane along the rows.
          const bool none = l == 0.f;
          const float inv = none ? 0.f : 1.f / l;
@@ -395,7 +419,8 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          unsigned char* stage = sm + L::Q + t * L::TILE + (warp & 3) * 32 * (DP * 2);
          for(int pass = 0; pass < (a.o_rest ? 2 : 1); ++pass) {
 #pragma unroll
-            for(int c = 0; c < DP; c += 16) {
+            for(int c0 = 0; c0 < DP; c0 += 16 * L::HALVES) {
+               const int c = c0 + 16 * h;
                if(c >= a.dim) break;
                uint32_t o[16];
                if(tiles > 0) {
@@ -412,23 +437,25 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   if(pass) w[i] = pack2< T >(x - low2< T >(w[i]), y - high2< T >(w[i]));
                }
 #pragma unroll
-               for(int h = 0; h < 2; ++h)
-                  *reinterpret_cast< uint4* >(stage + lane * (DP * 2) + (((c >> 3) + h) ^ (lane & 7)) * 16) =
-                     make_uint4(w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]);
+               for(int k = 0; k < 2; ++k)
+                  *reinterpret_cast< uint4* >(stage + lane * (DP * 2) + (((c >> 3) + k) ^ (lane & 7)) * 16) =
+                     make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
             }
-            __syncwarp();
+            if constexpr(L::HALVES == 2) pair_sync();
+            else __syncwarp();
             T* out = static_cast< T* >(pass ? a.o_rest : a.o);
             constexpr int CH = DP / 8;
 #pragma unroll 4
-            for(int i = lane; i < 32 * CH; i += 32) {
+            for(int i = h * 32 + lane; i < 32 * CH; i += 32 * L::HALVES) {
                const int r = i / CH, c = i % CH;
                if(r0 + r < qs.len && c * 8 < a.dim)
                   *reinterpret_cast< uint4* >(out + ((qs.first + r0 + r) * a.heads + head) * a.dim + c * 8) =
                      *reinterpret_cast< const uint4* >(stage + r * (DP * 2) + ((c ^ (r & 7)) * 16));
             }
-            __syncwarp();
+            if constexpr(L::HALVES == 2) pair_sync();
+            else __syncwarp();
          }
-         if(a.lse && r0 + lane < qs.len) {
+         if(a.lse && h == 0 && r0 + lane < qs.len) {
             float v = none ? -CUDART_INF_F : m * kLn2 + logf(l);
             a.lse[(int64_t)head * a.q_rows + qs.first + r0 + lane] = ok ? v : CUDART_NAN_F;
          }
