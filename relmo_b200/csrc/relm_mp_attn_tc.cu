@@ -83,21 +83,24 @@ __device__ __forceinline__ void apply_limit(uint32_t* s, const float4* limit)
    }
 }
 
-// 32 scores to weights 2^(sc s - ref), added to `sum` unrounded and packed. Each
-// step runs over all of them before the next, in place: with two warps per
-// scheduler a warp that waits for each of its results in turn leaves the units idle.
+// 32 scores to weights 2^(sc s - ref), added to `sum` unrounded and packed into
+// the first 16 registers. Eight at a time and in place: the registers are full,
+// and a spilled score costs more than all of this.
 template < typename T >
-__device__ __forceinline__ void exponents(uint32_t* s, uint32_t* p, uint64_t sc, uint64_t ref, uint64_t (&sum)[2])
+__device__ __forceinline__ void exponents(uint32_t* s, uint64_t sc, uint64_t ref, uint64_t (&sum)[2])
 {
-   float x[32];
 #pragma unroll
-   for(int i = 0; i < 16; ++i) unpair(fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), sc, ref), x[2 * i], x[2 * i + 1]);
+   for(int k = 0; k < 32; k += 8) {
+      float x[8];
 #pragma unroll
-   for(int i = 0; i < 32; ++i) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x[i]));
+      for(int i = 0; i < 8; i += 2) unpair(fma2(pair(__uint_as_float(s[k + i]), __uint_as_float(s[k + i + 1])), sc, ref), x[i], x[i + 1]);
 #pragma unroll
-   for(int i = 0; i < 16; ++i) p[i] = pack2< T >(x[2 * i], x[2 * i + 1]);
+      for(int i = 0; i < 8; ++i) x[i] = exp2_fast(x[i]);
 #pragma unroll
-   for(int i = 0; i < 16; ++i) sum[i & 1] = add2(sum[i & 1], pair(x[2 * i], x[2 * i + 1]));
+      for(int i = 0; i < 8; i += 2) sum[i / 2 & 1] = add2(sum[i / 2 & 1], pair(x[i], x[i + 1]));
+#pragma unroll
+      for(int i = 0; i < 8; i += 2) s[(k + i) / 2] = pack2< T >(x[i], x[i + 1]);
+   }
 }
 
 template < typename T, int DP, int QT >
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
    __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], limit_full[kLimitSlots], stagger;
    __shared__ float4 s_limit[kLimitSlots][kTileRows / 4];
-   __shared__ float s_top[2][QT][L::HALVES][L::HALVES == 2 ? kTileRows : 1]; // of the two halves of a row, by iteration parity
+   __shared__ float s_top[QT][2][L::HALVES == 2 ? kTileRows : 1]; // of the two halves of a row
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -300,6 +303,15 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       bool ok = true;
       // The two warps that share 32 rows.
       auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+      auto pair_any = [&](bool x) {
+         if constexpr(L::HALVES == 1) return __any_sync(~0u, x) != 0;
+         uint32_t any;
+         asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+                      : "=r"(any)
+                      : "r"((uint32_t)x), "r"(1 + t * 4 + (warp & 3))
+                      : "memory");
+         return any != 0;
+      };
       if(t < active) {
          for(int j = 0; j < tiles; ++j) {
             const int chunks = min(4, (ks.len - j * kTileRows + 31) / 32);
@@ -325,11 +337,6 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   if(partial) apply_limit(s + c * 32, limit + (2 * h + c) * 8);
                   top = largest(s + c * 32, top);
                }
-               // A NaN is left out of the maximum here and of the exchange: it shows in its own weights.
-               s_top[j & 1][t][h][row] = top;
-               pair_sync(); // both halves' scores are in registers: their place may take weights
-               fence_after();
-               top = fmaxf(top, s_top[j & 1][t][h ^ 1][row]);
             } else { // two blocks share the registers: the scores are read twice, 32 at a time
                tmem_ld32(s, st);
 #pragma unroll
@@ -344,36 +351,48 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                tmem_ld32(s, st);
             }
             top *= sc;
-            if constexpr(L::APART) // the last weights have been used
-               if(j > 0) ok = ok && __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1));
-            float f = 1.f;
-            if(top > m + kGrow || (m == -CUDART_INF_F && top > m)) {
-               f = exp2_fast(m - top);
-               m = top;
-               sum[0] = mul2(sum[0], pair(f, f));
-               sum[1] = mul2(sum[1], pair(f, f));
-            }
-            if(j > 0 && __any_sync(~0u, f != 1.f)) { // the products into O so far are done (before this S, or waited for above)
-               for(int c = h * 16; c < a.dim; c += 16 * L::HALVES) {
-                  uint32_t o[16];
-                  tmem_ld16(o, ot + c);
-                  wait_ld();
-                  loaded< 16 >(o);
+            // Most tiles leave the reference alone; only that is agreed on here (which also says that both
+            // halves' scores are in registers: their place may take weights).
+            if(pair_any(top > m + kGrow || (m == -CUDART_INF_F && top > m))) {
+               if constexpr(L::HALVES == 2) {
+                  s_top[t][h][row] = top;
+                  pair_sync();
+                  top = fmaxf(top, s_top[t][h ^ 1][row]);
+                  pair_sync();
+               }
+               float f = 1.f;
+               if(top > m + kGrow || (m == -CUDART_INF_F && top > m)) {
+                  f = exp2_fast(m - top);
+                  m = top;
+                  sum[0] = mul2(sum[0], pair(f, f));
+                  sum[1] = mul2(sum[1], pair(f, f));
+               }
+               if(j > 0) { // the products into O so far were done before this S, or are waited for
+                  if constexpr(L::APART) ok = ok && __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1));
+                  fence_after();
+                  for(int c = h * 16; c < a.dim; c += 16 * L::HALVES) {
+                     uint32_t o[16];
+                     tmem_ld16(o, ot + c);
+                     wait_ld();
+                     loaded< 16 >(o);
 #pragma unroll
-                  for(int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  tmem_st16(ot + c, o);
+                     for(int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                     tmem_st16(ot + c, o);
+                  }
                }
             }
+            if constexpr(L::HALVES == 2) fence_after();
             if(QT == 2 && j == 0 && threadIdx.x == 0) mbar_arrive(&stagger); // this tile's exponentials begin
             const float ref = m == -CUDART_INF_F ? 0.f : m;
             const uint64_t ref2 = pair(-ref, -ref);
             if constexpr(L::HALVES == 2) {
+               if constexpr(L::APART) // the last weights have been used
+                  if(j > 0) ok = ok && __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1));
 #pragma unroll
                for(int c = 0; c < 2; ++c) {
                   if(2 * h + c >= chunks) continue;
-                  uint32_t p[16];
-                  exponents< T >(s + c * 32, p, sc2, ref2, sum);
-                  tmem_st16(pt + (2 * h + c) * 16, p);
+                  exponents< T >(s + c * 32, sc2, ref2, sum);
+                  tmem_st16(pt + (2 * h + c) * 16, s + c * 32);
                }
                wait_st();
                fence_before();
@@ -382,14 +401,13 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
 #pragma unroll
                for(int c = 0; c < 4; ++c) {
                   if(c < chunks) {
-                     uint32_t p[16];
                      wait_ld();
                      loaded< 32 >(s + (c & 1) * 32);
                      if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
                      if(partial) apply_limit(s + (c & 1) * 32, limit + c * 8);
-                     exponents< T >(s + (c & 1) * 32, p, sc2, ref2, sum);
+                     exponents< T >(s + (c & 1) * 32, sc2, ref2, sum);
                      // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
-                     tmem_st16(pt + c * 16, p);
+                     tmem_st16(pt + c * 16, s + (c & 1) * 32);
                   }
                   if(c & 1) {
                      wait_st();
@@ -405,12 +423,9 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          if(ok && tiles > 0) ok = __all_sync(~0u, mbar_wait(&pv_done[t], (tiles - 1) & 1));
          fence_after();
          if constexpr(L::HALVES == 2) {
-            pair_sync();
-            s_top[0][t][h][row] = l;
-            s_top[1][t][h][row] = ok ? 1.f : 0.f;
-            pair_sync();
-            l += s_top[0][t][h ^ 1][row];
-            ok = ok && s_top[1][t][h ^ 1][row] == 1.f;
+            s_top[t][h][row] = l;
+            ok = !pair_any(!ok);
+            l += s_top[t][h ^ 1][row];
          }
          // Rows leave through the q tile's shared memory (its products are done), 16 bytes a lane along the rows.
          const bool none = l == 0.f;
