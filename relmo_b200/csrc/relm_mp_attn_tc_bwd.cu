@@ -15,10 +15,10 @@
 // subnormal in f16. The factor comes off dV at the end, and off dS for free
 // (dO V^T and delta are taken 2^-8 times).
 //
-// Both kernels: one thread copies tiles by tensor map, one issues products, and
-// 8 warps turn S and dO V^T into P and dS in place (two warps share 32 rows, each
-// half of the columns; each half's result stays inside its own half, so no warp
-// overwrites what another has still to read).
+// Both kernels: one thread copies tiles by tensor map, one issues products, and a
+// group of four warps for each 32 columns turns S and dO V^T into P and dS in
+// place (a thread per row; a group's result stays inside its own columns, so no
+// warp overwrites what another has still to read).
 #include <math_constants.h>
 
 #include <type_traits>
@@ -32,9 +32,10 @@ namespace {
 using namespace tc;
 
 constexpr float kUp = 8.f, kDown = 1.f / 256.f; // log2 of P's factor, and its inverse
-constexpr int kSoftThreads = 256, kBwdThreads = kSoftThreads + 64;
+constexpr int kGroup = 32; // columns of a group of four warps
 
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+template < int THREADS >
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
 
 // A tile of `rows` rows: panels of 64 columns.
 __host__ __device__ constexpr uint32_t tile_bytes(int dp, int rows) { return (uint32_t)(dp / 64) * rows * 128; }
@@ -113,16 +114,17 @@ struct Kv {
    static constexpr uint32_t KT = tile_bytes(DP, kTileRows), QT = tile_bytes(DP, QN);
    static constexpr uint32_t K = 0, V = KT, Q = 2 * KT, G = Q + ST * QT, BYTES = G + ST * QT;
    static constexpr uint32_t S = 0, P = QN, DV = 2 * QN, DK = 2 * QN + DP, COLS = 2 * (QN + DP);
+   static constexpr int SOFT = QN / kGroup * 128, MMA_WARP = SOFT / 32, THREADS = SOFT + 64;
    static constexpr int RESIDENT = COLS <= 256 ? 2 : 1;
 };
 
 template < typename T, int DP, int QN >
-__global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
+__global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
    k_attn_tc_backward_kv(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
                          const __grid_constant__ CUtensorMap vm, const __grid_constant__ CUtensorMap gm)
 {
    using L = Kv< DP, QN >;
-   constexpr int HALF = QN / 2;
+   constexpr int HALF = kGroup;
    constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
@@ -145,19 +147,19 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
       }
       mbar_init(&s_full, 1);
       mbar_init(&dp_full, 1);
-      mbar_init(&p_full, kSoftThreads);
-      mbar_init(&ds_full, kSoftThreads);
+      mbar_init(&p_full, L::SOFT);
+      mbar_init(&ds_full, L::SOFT);
       mbar_init(&done, 1);
       mbar_init_fence();
       gave_up = 0;
    }
-   if(warp == 8) tmem_alloc(&tmem_base, L::COLS);
+   if(warp == L::MMA_WARP) tmem_alloc(&tmem_base, L::COLS);
    fence_before();
    __syncthreads();
    fence_after();
    const uint32_t tmem = tmem_base, base = smem_addr(sm);
 
-   if(warp == 9) { // copies
+   if(warp == L::MMA_WARP + 1) { // copies
       if(lane == 0 && n > 0) {
          const int qr = (int)(a.q_off ? qs.first : 0), kr = (int)(a.kv_off ? ks.first : 0) + key0, b = a.q_off ? 0 : it.seq;
          mbar_expect(&kv_full, 2 * L::KT);
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
             for(int i = issued > L::ST ? issued - L::ST : 0; i < issued; ++i) mbar_wait(&q_full[i % L::ST], (i / L::ST) & 1);
          }
       }
-   } else if(warp == 8) { // products
+   } else if(warp == L::MMA_WARP) { // products
       if(elect_one() && n > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t out_id = instruction(BF, 128, steps * 16, true);
@@ -245,7 +247,7 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
       for(int i = 0; i < n; ++i) {
          const int valid = min(QN, qs.len - (i % q_tiles) * QN);
          if(puts) reinterpret_cast< float* >(puts_lse ? s_lse[i & 1] : s_delta[i & 1])[col] = next;
-         soft_sync();
+         soft_sync< L::SOFT >();
          next = fetch(i + 1);
          ok = ok && __all_sync(~0u, mbar_wait(&s_full, i & 1));
          fence_after();
@@ -315,16 +317,16 @@ __global__ void __launch_bounds__(kBwdThreads, Kv< DP, QN >::RESIDENT)
       if(n > 0) ok = ok && __all_sync(~0u, mbar_wait(&done, 0));
       fence_after();
       if(!ok) gave_up = 1;
-      // First half of the warps: dV, second: dK; through the K and V tiles (their products are done).
+      // One group writes dV, one dK, through the K and V tiles (their products are done).
       const int k0 = key0 + (warp & 3) * 32;
       T* out = static_cast< T* >(half ? a.dk : a.dv) + ((ks.first + k0) * a.kv_heads + kv_head) * a.dim;
-      store_rows< T, DP >(lanes + (half ? L::DK : L::DV), n > 0, ok, half ? a.scale : kDown,
+      if(half < 2) store_rows< T, DP >(lanes + (half ? L::DK : L::DV), n > 0, ok, half ? a.scale : kDown,
                           sm + (half ? L::V : L::K) + (warp & 3) * 32 * (DP * 2), out, (int64_t)a.kv_heads * a.dim, ks.len - k0, a.dim);
    }
    fence_before();
    __syncthreads();
    fence_after();
-   if(warp == 8) tmem_free(tmem, L::COLS);
+   if(warp == L::MMA_WARP) tmem_free(tmem, L::COLS);
    if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
 }
 
@@ -336,16 +338,17 @@ struct Dq {
    static constexpr uint32_t QT = tile_bytes(DP, kTileRows), KT = tile_bytes(DP, KN);
    static constexpr uint32_t Q = 0, G = QT, K = 2 * QT, V = K + ST * KT, BYTES = V + ST * KT;
    static constexpr uint32_t S = 0, P = 2 * KN, DQ = 3 * KN, COLS = 3 * KN + DP; // two S tiles
+   static constexpr int SOFT = KN / kGroup * 128, MMA_WARP = SOFT / 32, THREADS = SOFT + 64;
    static constexpr int RESIDENT = COLS <= 256 ? 2 : 1;
 };
 
 template < typename T, int DP, int KN >
-__global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
+__global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
    k_attn_tc_backward_q(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
                         const __grid_constant__ CUtensorMap vm, const __grid_constant__ CUtensorMap gm)
 {
    using L = Dq< DP, KN >;
-   constexpr int HALF = KN / 2;
+   constexpr int HALF = kGroup;
    constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
@@ -368,18 +371,18 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
          mbar_init(&s_full[s], 1);
       }
       mbar_init(&dp_full, 1);
-      mbar_init(&ds_full, kSoftThreads);
+      mbar_init(&ds_full, L::SOFT);
       mbar_init(&done, 1);
       mbar_init_fence();
       gave_up = 0;
    }
-   if(warp == 8) tmem_alloc(&tmem_base, L::COLS);
+   if(warp == L::MMA_WARP) tmem_alloc(&tmem_base, L::COLS);
    fence_before();
    __syncthreads();
    fence_after();
    const uint32_t tmem = tmem_base, base = smem_addr(sm);
 
-   if(warp == 9) { // copies
+   if(warp == L::MMA_WARP + 1) { // copies
       if(lane == 0 && n > 0) {
          const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0), b = a.q_off ? 0 : it.seq;
          mbar_expect(&q_full, 2 * L::QT);
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
             }
          }
       }
-   } else if(warp == 8) { // products
+   } else if(warp == L::MMA_WARP) { // products
       if(elect_one() && n > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t out_id = instruction(BF, 128, steps * 16, true);
@@ -480,13 +483,8 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
             s[c] = __float_as_uint(exp2_fast(x));
             s[c + 1] = __float_as_uint(exp2_fast(y));
          }
-         if(!all && (warp & 3) * 32 < HALF) { // masked rows of K, read by dS K next, S is done with them
-            const int r = (warp & 3) * 32 + lane;
-            bool mine = false;
-#pragma unroll
-            for(int c = 0; c < HALF / 32; ++c)
-               if(c == (warp & 3)) mine = bits[c] >> lane & 1;
-            if(!mine) clear_row< DP >(sm + L::K + (j % L::ST) * L::KT, KN, half * HALF + r);
+         if(!all && (warp & 3) == 0) { // masked rows of K, read by dS K next, S is done with them
+            if(!(bits[0] >> lane & 1)) clear_row< DP >(sm + L::K + (j % L::ST) * L::KT, KN, half * HALF + lane);
             fence_async_proxy();
          }
          ok = ok && __all_sync(~0u, mbar_wait(&dp_full, j & 1));
@@ -516,7 +514,7 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
       if(n > 0) ok = ok && __all_sync(~0u, mbar_wait(&done, 0));
       fence_after();
       if(!ok) gave_up = 1;
-      // Through the Q tile's shared memory; the two warps of 32 rows take half of the columns' work each way: the first writes.
+      // Through the Q tile's shared memory; the first group writes.
       const int r0 = row0 + (warp & 3) * 32;
       if(half == 0) {
          T* out = static_cast< T* >(a.dq) + ((qs.first + r0) * a.heads + head) * a.dim;
@@ -527,17 +525,17 @@ __global__ void __launch_bounds__(kBwdThreads, Dq< DP, KN >::RESIDENT)
    fence_before();
    __syncthreads();
    fence_after();
-   if(warp == 8) tmem_free(tmem, L::COLS);
+   if(warp == L::MMA_WARP) tmem_free(tmem, L::COLS);
    if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
 }
 
 template < typename F >
-int launch(SmemLimit& limit, F fn, int bytes, dim3 grid, const Args& a, const TcMaps& m, cudaStream_t st, const char* what)
+int launch(SmemLimit& limit, F fn, int threads, int bytes, dim3 grid, const Args& a, const TcMaps& m, cudaStream_t st, const char* what)
 {
    if(grid.x == 0) return RELM_MP_OK;
    int rc = limit((const void*)fn, bytes, what);
    if(rc) return rc;
-   fn<<< grid, kBwdThreads, bytes, st >>>(a, m.q, m.k, m.v, m.go);
+   fn<<< grid, threads, bytes, st >>>(a, m.q, m.k, m.v, m.go);
    return check_launch(what);
 }
 
@@ -559,11 +557,11 @@ int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_til
    int rc;
    if((rc = maps(&m, N, kTileRows))) return rc;
    static SmemLimit kv_limit, q_limit;
-   if((rc = launch(kv_limit, k_attn_tc_backward_kv< T, DP, N >, (int)Kv< DP, N >::BYTES + 1024, dim3((unsigned)kv_tiles, a.kv_heads), a, m, st,
+   if((rc = launch(kv_limit, k_attn_tc_backward_kv< T, DP, N >, Kv< DP, N >::THREADS, (int)Kv< DP, N >::BYTES + 1024, dim3((unsigned)kv_tiles, a.kv_heads), a, m, st,
                    "k_attn_tc_backward_kv")))
       return rc;
    if(N != kTileRows && (rc = maps(&m, kTileRows, N))) return rc;
-   return launch(q_limit, k_attn_tc_backward_q< T, DP, N >, (int)Dq< DP, N >::BYTES + 1024, dim3((unsigned)q_tiles, a.heads), a, m, st,
+   return launch(q_limit, k_attn_tc_backward_q< T, DP, N >, Dq< DP, N >::THREADS, (int)Dq< DP, N >::BYTES + 1024, dim3((unsigned)q_tiles, a.heads), a, m, st,
                  "k_attn_tc_backward_q");
 }
 

@@ -221,16 +221,17 @@ __device__ __forceinline__ void product_columns(uint32_t d, uint32_t a, uint32_t
       if(k < steps) mma_ss(d, da + ((k >> 2) * A_ROWS * 8 + (k & 3) * 2), db + ((k >> 2) * B_ROWS * 8 + (k & 3) * 2), idesc, k > 0);
 }
 
-// d (+)= a b, steps [FIRST, FIRST + N) below `steps`: a in tensor memory (two halves of HALF
-// contracted columns, HALF columns of memory apart; HALF 0: all together), b a tile of
+// d (+)= a b, steps [FIRST, FIRST + N) below `steps`: a in tensor memory (groups of GROUP
+// contracted columns, GROUP columns of memory apart; GROUP 0: all together), b a tile of
 // B_ROWS-row panels contracted along its rows.
-template < int FIRST, int N, int HALF, int B_ROWS >
+template < int FIRST, int N, int GROUP, int B_ROWS >
 __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int steps, bool accumulate)
 {
    const uint64_t db = operand(b, B_ROWS * 128, 1024);
 #pragma unroll
    for(int k = FIRST; k < FIRST + N; ++k) {
-      const int at = HALF && k >= HALF / 16 ? HALF + (k - HALF / 16) * 8 : k * 8;
+      constexpr int PER = GROUP ? GROUP / 16 : N + FIRST;
+      const int at = k / PER * GROUP + k % PER * 8;
       if(k < steps) mma_ts(d, a + at, db + k * 128, idesc, accumulate || k > 0);
    }
 }
