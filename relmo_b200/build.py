@@ -47,11 +47,12 @@ CUDA_SOURCES = [
     "relm_mp_attn.cu",
     "relm_mp_attn_simt.cu",
     "relm_mp_attn_split.cu",
+    "relm_mp_attn_short.cu",
     "relm_mp_attn_tc.cu",
     "relm_mp_attn_tc_bwd.cu",
 ]
 TORCH_SOURCES = ["relm_mp_torch.cpp", "relm_mp_cpu.cpp", "relm_mp_decoder.cpp"]
-HEADERS = ["relm_mp_internal.cuh", "relm_mp_segment.cuh", "relm_mp_seg_impl.cuh", "relm_mp_attn.cuh", "relm_mp_attn_tc.cuh", "relm_mp_tc.cuh"]
+HEADERS = ["relm_mp_internal.cuh", "relm_mp_segment.cuh", "relm_mp_seg_impl.cuh", "relm_mp_attn.cuh", "relm_mp_attn_mma.cuh", "relm_mp_attn_tc.cuh", "relm_mp_tc.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -134,6 +134,9 @@ bool use_tc(const relm_mp_attn& in)
           ok(in.v_stride, in.kv_rows, in.max_kv, in.kv_heads);
 }
 
+// All keys of a sequence fit one block of the kernels for short sequences.
+bool short_keys(const relm_mp_attn& in) { return aligned_rows(in) && in.max_kv <= 128 && in.dim <= 64 && in.seqs <= 65535 * 32; }
+
 // Few query rows (tokens x heads of a group) per sequence: a tile of 128 would be mostly empty.
 bool few_rows(const relm_mp_attn& in) { return in.max_q * (in.heads / in.kv_heads) <= 16; }
 
@@ -331,6 +334,8 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
    const Counts c = counts(*attn);
    cudaStream_t st = static_cast< cudaStream_t >(stream);
    if(use_split(*attn)) return split_forward(attn->dtype, a, c.kv_blocks, workspace, st);
+   if(short_keys(*attn) && ((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(a.o_rest)) & 3) == 0)
+      return short_forward(attn->dtype, a, c.q_tiles, st);
    if(use_tc(*attn) && ((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(a.o_rest)) & 15) == 0) {
       if((rc = gave_up_address(&a.gave_up))) return rc;
       return tc_forward(attn->dtype, a, c.q_tiles, c.q_pairs, st);
@@ -357,7 +362,15 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
    cudaStream_t st = static_cast< cudaStream_t >(stream);
    Args a = make_args(*attn);
    float* delta = static_cast< float* >(workspace);
+   a.o = const_cast< void* >(o), a.o_rest = const_cast< void* >(o_rest);
    a.go = grad_o, a.lse_in = lse, a.delta = delta, a.dq = dq, a.dk = dk, a.dv = dv;
+   const Counts c = counts(*attn);
+   const bool aligned = ((reinterpret_cast< uintptr_t >(grad_o) | reinterpret_cast< uintptr_t >(dq) |
+                          reinterpret_cast< uintptr_t >(dk) | reinterpret_cast< uintptr_t >(dv)) & 15) == 0;
+   // One block per sequence and key head walks all its query rows: not for long queries of few sequences.
+   const bool many = attn->seqs * a.kv_heads >= 296 || attn->max_q * (a.heads / a.kv_heads) <= 256;
+   if(short_keys(*attn) && aligned && many && (((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(o_rest)) & 15) == 0))
+      return short_backward(attn->dtype, a, st);
    if(attn->q_rows) {
       switch(attn->dtype) {
          case RELM_MP_FLOAT32: rc = launch_delta< float >(grad_o, o, o_rest, attn->q_rows, a.heads, a.dim, delta, st); break;
@@ -366,9 +379,6 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
       }
       if(rc) return rc;
    }
-   const Counts c = counts(*attn);
-   const bool aligned = ((reinterpret_cast< uintptr_t >(grad_o) | reinterpret_cast< uintptr_t >(dq) |
-                          reinterpret_cast< uintptr_t >(dk) | reinterpret_cast< uintptr_t >(dv)) & 15) == 0;
    if(use_tc(*attn) && aligned && !few_rows(*attn)) {
       if((rc = gave_up_address(&a.gave_up))) return rc;
       return tc_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);

@@ -28,7 +28,7 @@ struct Args {
    void *o, *o_rest; // o_rest may be NULL
    float* lse;       // may be NULL
    // backward
-   const void *go;
+   const void* go; // (o and o_rest are inputs then)
    const float *lse_in, *delta;
    void *dq, *dk, *dv;
    int* gave_up; // set by a kernel that gave up waiting
@@ -107,6 +107,10 @@ struct SplitPlan {
 };
 SplitPlan split_plan(const Args& a, int64_t blocks);
 int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* workspace, cudaStream_t st);
+
+// Up to 128 keys a sequence, dim up to 64, 2-byte types, aligned rows (relm_mp_attn_short.cu).
+int short_forward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, cudaStream_t st);
+int short_backward(relm_mp_dtype dtype, const Args& a, cudaStream_t st);
 
 // Tensor cores: 2-byte types, dim a multiple of 8 up to 128, rows on 16-byte
 // boundaries (relm_mp_attn_tc.cu).

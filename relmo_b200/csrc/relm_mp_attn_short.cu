@@ -1,0 +1,411 @@
+// Cross attention over short key sequences (up to 128 keys, head dims up to 64,
+// 2-byte types): the objects of one state, say. Thousands of small problems, so
+// what counts is how many are in flight per SM. Tiles of 64 query rows on the
+// warp-level matrix instruction need no tensor memory, no barriers with other
+// roles and 16 to 80 KB of shared memory: three to eight blocks share an SM where
+// the tcgen05 kernels fit two, and all keys of a sequence are in one block:
+//
+//  - forward: the softmax sees all its scores at once, no running maximum;
+//  - backward: one kernel. Query rows first: each warp has 16, computes P and dS
+//    against all keys, leaves both in shared memory and has its rows of dQ = dS K
+//    complete. Then keys: each warp has 32 and adds P^T dO and dS^T Q to its dV and
+//    dK, kept in registers over the query tiles of the group. Five products, no
+//    atomics, delta = do . o on the way.
+//
+// Keys outside the sequence or masked are zeros in shared memory (their rows are
+// never read) and get weight 0.
+#include <math_constants.h>
+
+#include "relm_mp_attn_mma.cuh"
+
+namespace relm_mp {
+namespace attn {
+namespace {
+
+constexpr int kKeys = 128, kTile = 64, kShortThreads = 128;
+
+// Rows [row0, row0 + rows) of one head, 16 bytes a copy; rows past `len` or not kept are zeros.
+template < typename T, int DP >
+__device__ __forceinline__ void copy_rows(uint32_t dst, const T* src, int64_t stride, int rows, int row0, int len, int dim,
+                                          const unsigned char* keep)
+{
+   constexpr int CH = DP / 8;
+   for(int i = threadIdx.x; i < rows * CH; i += kShortThreads) {
+      const int r = i / CH, c = i % CH;
+      const bool in = row0 + r < len && c * 8 < dim && (!keep || keep[row0 + r]);
+      copy16(dst + swizzled< DP >(r, c), in ? src + (int64_t)(row0 + r) * stride + c * 8 : src, in);
+   }
+}
+__device__ __forceinline__ void copies_done()
+{
+   asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
+   __syncthreads();
+}
+
+// Which of the 128 keys take part, as four words, in every warp.
+__device__ __forceinline__ void key_bits(unsigned (&bits)[4], int len, const unsigned char* keep)
+{
+#pragma unroll
+   for(int c = 0; c < 4; ++c) {
+      const int key = c * 32 + (threadIdx.x & 31);
+      bits[c] = __ballot_sync(~0u, key < len && (!keep || keep[key]));
+   }
+}
+
+// The left operand's 16 x 16 block: rows row0.., 16-byte pieces c, c + 1 of a tile.
+template < int DP >
+__device__ __forceinline__ void load_left(uint32_t* f, uint32_t tile, int row0, int c)
+{
+   const int lane = threadIdx.x & 31;
+   ldmatrix4(f, tile + swizzled< DP >(row0 + (lane & 15), c + (lane >> 4)));
+}
+// Two right operands (16 rows key0.. of a [keys][dim] tile as columns n, pieces c, c + 1 contracted).
+template < int DP >
+__device__ __forceinline__ void load_right(uint32_t* b, uint32_t tile, int key0, int c)
+{
+   const int lane = threadIdx.x & 31;
+   ldmatrix4(b, tile + swizzled< DP >(key0 + (lane >> 4) * 8 + (lane & 7), c + (lane >> 3 & 1)));
+}
+// Two right operands (rows row0.. contracted, pieces c, c + 1 as columns n).
+template < int DP >
+__device__ __forceinline__ void load_right_rows(uint32_t* b, uint32_t tile, int row0, int c)
+{
+   const int lane = threadIdx.x & 31;
+   ldmatrix4_trans(b, tile + swizzled< DP >(row0 + (lane >> 3 & 1) * 8 + (lane & 7), c + (lane >> 4)));
+}
+
+template < typename T >
+__device__ __forceinline__ void store2(T* p, float x, float y)
+{
+   *reinterpret_cast< uint32_t* >(p) = Mma< T >::pack(x, y);
+}
+
+template < typename T, int DP >
+__global__ void __launch_bounds__(kShortThreads) k_attn_short_forward(Args a)
+{
+   constexpr int KS = DP / 16;
+   extern __shared__ __align__(128) unsigned char smem[];
+   const uint32_t sk = (uint32_t)__cvta_generic_to_shared(smem), sv = sk + kKeys * DP * 2;
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x / 2);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
+   const int row0 = it.tile * kTileRows + (blockIdx.x & 1) * kTile;
+   if(row0 >= qs.len) return;
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   const int n16 = (ks.len + 15) / 16; // 16-key steps
+   copy_rows< T, DP >(sk, static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2], a.ks[1], n16 * 16, 0, ks.len, a.dim, keep);
+   copy_rows< T, DP >(sv, static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2], a.vs[1], n16 * 16, 0, ks.len, a.dim, keep);
+   uint32_t qf[KS][4];
+#pragma unroll
+   for(int half = 0; half < 2; ++half) {
+      const int r = row0 + warp * 16 + g + 8 * half;
+      const T* q = static_cast< const T* >(a.q) + qs.base + (int64_t)r * a.qs[1] + head * a.qs[2];
+#pragma unroll
+      for(int kk = 0; kk < KS; ++kk)
+#pragma unroll
+         for(int c = 0; c < 2; ++c) {
+            const int d = kk * 16 + c * 8 + 2 * t4;
+            qf[kk][half + 2 * c] = r < qs.len && d < a.dim ? *reinterpret_cast< const uint32_t* >(q + d) : 0u;
+         }
+   }
+   unsigned bits[4];
+   key_bits(bits, ks.len, keep);
+   copies_done();
+   const float sc = a.scale * kLog2e;
+   float s[kKeys / 8][4];
+   float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+   for(int n = 0; n < kKeys / 16; ++n) {
+      if(n >= n16) continue;
+#pragma unroll
+      for(int e = 0; e < 2; ++e) s[2 * n + e][0] = s[2 * n + e][1] = s[2 * n + e][2] = s[2 * n + e][3] = 0.f;
+#pragma unroll
+      for(int kk = 0; kk < KS; ++kk) {
+         uint32_t b[4];
+         load_right< DP >(b, sk, n * 16, kk * 2);
+         Mma< T >::run(s[2 * n], qf[kk], b[0], b[1]);
+         Mma< T >::run(s[2 * n + 1], qf[kk], b[2], b[3]);
+      }
+      const unsigned w = bits[n / 2] >> (n % 2 * 16) >> (2 * t4);
+#pragma unroll
+      for(int e = 0; e < 2; ++e)
+#pragma unroll
+         for(int i = 0; i < 4; ++i) {
+            s[2 * n + e][i] = w >> (e * 8 + (i & 1)) & 1 ? s[2 * n + e][i] * sc : -CUDART_INF_F;
+            top[i >> 1] = fmaxf(top[i >> 1], s[2 * n + e][i]);
+         }
+   }
+   float l[2] = {0.f, 0.f}, ref[2];
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+      ref[h] = top[h] == -CUDART_INF_F ? 0.f : top[h];
+   }
+   float o[DP / 8][4];
+#pragma unroll
+   for(int d = 0; d < DP / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+#pragma unroll
+   for(int n = 0; n < kKeys / 16; ++n) {
+      if(n >= n16) continue;
+#pragma unroll
+      for(int e = 0; e < 2; ++e)
+#pragma unroll
+         for(int i = 0; i < 4; ++i) {
+            s[2 * n + e][i] = exp2_fast(s[2 * n + e][i] - ref[i >> 1]);
+            l[i >> 1] += s[2 * n + e][i];
+         }
+      // The weights enter the second product in the inputs' type, their sum l stays float32.
+      const uint32_t p[4] = {Mma< T >::pack(s[2 * n][0], s[2 * n][1]), Mma< T >::pack(s[2 * n][2], s[2 * n][3]),
+                             Mma< T >::pack(s[2 * n + 1][0], s[2 * n + 1][1]), Mma< T >::pack(s[2 * n + 1][2], s[2 * n + 1][3])};
+#pragma unroll
+      for(int d = 0; d < DP / 16; ++d) {
+         uint32_t b[4];
+         load_right_rows< DP >(b, sv, n * 16, d * 2);
+         Mma< T >::run(o[2 * d], p, b[0], b[1]);
+         Mma< T >::run(o[2 * d + 1], p, b[2], b[3]);
+      }
+   }
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(~0u, l[h], 1);
+      l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      const int row = row0 + warp * 16 + g + 8 * h;
+      if(row >= qs.len) continue;
+      const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+      const int64_t at = ((qs.first + row) * a.heads + head) * a.dim;
+#pragma unroll
+      for(int d = 0; d < DP / 8; ++d) {
+         const int c = d * 8 + 2 * t4;
+         if(c >= a.dim) continue;
+         const float x = o[d][2 * h] * inv, y = o[d][2 * h + 1] * inv;
+         const uint32_t w = Mma< T >::pack(x, y);
+         *reinterpret_cast< uint32_t* >(static_cast< T* >(a.o) + at + c) = w;
+         if(a.o_rest) {
+            const T* r = reinterpret_cast< const T* >(&w);
+            store2(static_cast< T* >(a.o_rest) + at + c, x - to_f32(r[0]), y - to_f32(r[1]));
+         }
+      }
+      if(a.lse && t4 == 0)
+         a.lse[(int64_t)head * a.q_rows + qs.first + row] = l[h] == 0.f ? -CUDART_INF_F : top[h] * kLn2 + logf(l[h]);
+   }
+}
+
+// Rows of 128 weights (256 bytes): piece c of row r.
+__device__ __forceinline__ uint32_t weight_at(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) * 16)); }
+
+template < int DP >
+struct Bwd {
+   static constexpr int K = 0, V = kKeys * DP * 2, Q = 2 * V, G = Q + kTile * DP * 2, P = G + kTile * DP * 2, DS = P + kTile * 256,
+                        BYTES = DS + kTile * 256;
+};
+
+template < typename T, int DP >
+__global__ void __launch_bounds__(kShortThreads) k_attn_short_backward(Args a)
+{
+   using L = Bwd< DP >;
+   extern __shared__ __align__(128) unsigned char smem[];
+   __shared__ float s_lse[kTile], s_delta[kTile];
+   const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, seq = blockIdx.x;
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, seq), ks = locate(a.kv_off, a.max_kv, a.ks, seq);
+   const Seq vs = locate(a.kv_off, a.max_kv, a.vs, seq);
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   const int n16 = (ks.len + 15) / 16;
+   copy_rows< T, DP >(base + L::K, static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2], a.ks[1], n16 * 16, 0, ks.len, a.dim, keep);
+   copy_rows< T, DP >(base + L::V, static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2], a.vs[1], n16 * 16, 0, ks.len, a.dim, keep);
+   unsigned bits[4];
+   key_bits(bits, ks.len, keep);
+   const float sc = a.scale * kLog2e;
+   float dk[2][DP / 8][4], dv[2][DP / 8][4];
+#pragma unroll
+   for(int i = 0; i < 2; ++i)
+#pragma unroll
+      for(int d = 0; d < DP / 8; ++d)
+#pragma unroll
+         for(int e = 0; e < 4; ++e) dk[i][d][e] = dv[i][d][e] = 0.f;
+
+   for(int head = kv_head * group; head < (kv_head + 1) * group; ++head)
+      for(int q0 = 0; q0 < qs.len; q0 += kTile) {
+         const int64_t go_row = (int64_t)a.heads * a.dim, go0 = (qs.first * a.heads + head) * a.dim;
+         const T* go = static_cast< const T* >(a.go) + go0;
+         const int m16 = (min(kTile, qs.len - q0) + 15) / 16; // 16-row steps
+         copy_rows< T, DP >(base + L::Q, static_cast< const T* >(a.q) + qs.base + head * a.qs[2], a.qs[1], m16 * 16, q0, qs.len, a.dim, nullptr);
+         copy_rows< T, DP >(base + L::G, go, go_row, m16 * 16, q0, qs.len, a.dim, nullptr);
+         { // delta = do . (o + o_rest): two threads a row
+            const int r = threadIdx.x >> 1, row = q0 + r;
+            float s = 0.f;
+            if(row < qs.len) {
+               const T* x = go + row * go_row;
+               const T* y = static_cast< const T* >(a.o) + go0 + row * go_row;
+               const T* z = a.o_rest ? static_cast< const T* >(a.o_rest) + go0 + row * go_row : nullptr;
+#pragma unroll
+               for(int d = (threadIdx.x & 1) * 8; d < DP; d += 16) {
+                  if(d >= a.dim) continue;
+                  const uint4 u = *reinterpret_cast< const uint4* >(x + d), v = *reinterpret_cast< const uint4* >(y + d);
+                  const T *xe = reinterpret_cast< const T* >(&u), *ye = reinterpret_cast< const T* >(&v);
+#pragma unroll
+                  for(int e = 0; e < 8; ++e) s = fmaf(to_f32(xe[e]), to_f32(ye[e]), s);
+                  if(z) {
+                     const uint4 w = *reinterpret_cast< const uint4* >(z + d);
+                     const T* ze = reinterpret_cast< const T* >(&w);
+#pragma unroll
+                     for(int e = 0; e < 8; ++e) s = fmaf(to_f32(xe[e]), to_f32(ze[e]), s);
+                  }
+               }
+            }
+            s += __shfl_xor_sync(~0u, s, 1);
+            if((threadIdx.x & 1) == 0) {
+               const float v = row < qs.len ? a.lse_in[(int64_t)head * a.q_rows + qs.first + row] : -CUDART_INF_F;
+               s_lse[r] = v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e; // no such row, or a row without keys: weights 0
+               s_delta[r] = s;
+            }
+         }
+         copies_done();
+
+         // Query rows: warp has 16. Weights and score gradients of 32 keys at a time.
+         if(warp < m16) {
+            const int r0 = warp * 16;
+            const float lse[2] = {s_lse[r0 + g], s_lse[r0 + g + 8]}, delta[2] = {s_delta[r0 + g], s_delta[r0 + g + 8]};
+            float dq[DP / 8][4];
+#pragma unroll
+            for(int d = 0; d < DP / 8; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.f;
+            for(int n = 0; n < n16; ++n) {
+               float s[2][4], dp[2][4];
+#pragma unroll
+               for(int e = 0; e < 2; ++e)
+#pragma unroll
+                  for(int i = 0; i < 4; ++i) s[e][i] = dp[e][i] = 0.f;
+#pragma unroll
+               for(int kk = 0; kk < DP / 16; ++kk) {
+                  uint32_t f[4], b[4];
+                  load_left< DP >(f, base + L::Q, r0, kk * 2);
+                  load_right< DP >(b, base + L::K, n * 16, kk * 2);
+                  Mma< T >::run(s[0], f, b[0], b[1]);
+                  Mma< T >::run(s[1], f, b[2], b[3]);
+                  load_left< DP >(f, base + L::G, r0, kk * 2);
+                  load_right< DP >(b, base + L::V, n * 16, kk * 2);
+                  Mma< T >::run(dp[0], f, b[0], b[1]);
+                  Mma< T >::run(dp[1], f, b[2], b[3]);
+               }
+               const unsigned word = n < 2 ? bits[0] : n < 4 ? bits[1] : n < 6 ? bits[2] : bits[3];
+               const unsigned w = word >> (n % 2 * 16) >> (2 * t4);
+               uint32_t df[4];
+#pragma unroll
+               for(int e = 0; e < 2; ++e)
+#pragma unroll
+                  for(int h = 0; h < 2; ++h) {
+                     float p[2], x[2];
+#pragma unroll
+                     for(int i = 0; i < 2; ++i) {
+                        p[i] = w >> (e * 8 + i) & 1 ? exp2_fast(fmaf(s[e][2 * h + i], sc, -lse[h])) : 0.f;
+                        x[i] = p[i] * (dp[e][2 * h + i] - delta[h]);
+                     }
+                     // Rounded to the inputs' type for the products that follow.
+                     const uint32_t pw = Mma< T >::pack(p[0], p[1]);
+                     df[e * 2 + h] = Mma< T >::pack(x[0], x[1]);
+                     const uint32_t at = weight_at(r0 + g + 8 * h, n * 2 + e) + t4 * 4;
+                     *reinterpret_cast< uint32_t* >(smem + L::P + at) = pw;
+                     *reinterpret_cast< uint32_t* >(smem + L::DS + at) = df[e * 2 + h];
+                  }
+#pragma unroll
+               for(int d = 0; d < DP / 16; ++d) {
+                  uint32_t b[4];
+                  load_right_rows< DP >(b, base + L::K, n * 16, d * 2);
+                  Mma< T >::run(dq[2 * d], df, b[0], b[1]);
+                  Mma< T >::run(dq[2 * d + 1], df, b[2], b[3]);
+               }
+            }
+#pragma unroll
+            for(int h = 0; h < 2; ++h) {
+               const int row = q0 + r0 + g + 8 * h;
+               if(row >= qs.len) continue;
+               T* out = static_cast< T* >(a.dq) + go0 + row * go_row;
+#pragma unroll
+               for(int d = 0; d < DP / 8; ++d)
+                  if(d * 8 + 2 * t4 < a.dim) store2(out + d * 8 + 2 * t4, dq[d][2 * h] * a.scale, dq[d][2 * h + 1] * a.scale);
+            }
+         }
+         __syncthreads();
+
+         // Keys: warp has 32, over the tile's query rows.
+         if(warp * 32 < n16 * 16)
+            for(int m = 0; m < m16; ++m) {
+               uint32_t pf[2][4], df[2][4];
+#pragma unroll
+               for(int i = 0; i < 2; ++i) {
+                  const uint32_t at = weight_at(m * 16 + (lane >> 4) * 8 + (lane & 7), warp * 4 + i * 2 + (lane >> 3 & 1));
+                  ldmatrix4_trans(pf[i], base + L::P + at);
+                  ldmatrix4_trans(df[i], base + L::DS + at);
+               }
+#pragma unroll
+               for(int d = 0; d < DP / 16; ++d) {
+                  uint32_t b[4], c[4];
+                  load_right_rows< DP >(b, base + L::G, m * 16, d * 2);
+                  load_right_rows< DP >(c, base + L::Q, m * 16, d * 2);
+#pragma unroll
+                  for(int i = 0; i < 2; ++i) {
+                     Mma< T >::run(dv[i][2 * d], pf[i], b[0], b[1]);
+                     Mma< T >::run(dv[i][2 * d + 1], pf[i], b[2], b[3]);
+                     Mma< T >::run(dk[i][2 * d], df[i], c[0], c[1]);
+                     Mma< T >::run(dk[i][2 * d + 1], df[i], c[2], c[3]);
+                  }
+               }
+            }
+         __syncthreads(); // the tiles are free for the next copies
+      }
+   // (A sequence without queries leaves its copies in flight until here.)
+   asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+   for(int i = 0; i < 2; ++i)
+#pragma unroll
+      for(int h = 0; h < 2; ++h) {
+         const int key = warp * 32 + i * 16 + g + 8 * h;
+         if(key >= ks.len) continue;
+         const int64_t at = ((ks.first + key) * a.kv_heads + kv_head) * a.dim;
+#pragma unroll
+         for(int d = 0; d < DP / 8; ++d) {
+            const int c = d * 8 + 2 * t4;
+            if(c >= a.dim) continue;
+            store2(static_cast< T* >(a.dk) + at + c, dk[i][d][2 * h] * a.scale, dk[i][d][2 * h + 1] * a.scale);
+            store2(static_cast< T* >(a.dv) + at + c, dv[i][d][2 * h], dv[i][d][2 * h + 1]);
+         }
+      }
+}
+
+template < typename T, int DP >
+int forward(const Args& a, int64_t q_tiles, cudaStream_t st)
+{
+   k_attn_short_forward< T, DP ><<< dim3((unsigned)(2 * q_tiles), a.heads), kShortThreads, 2 * kKeys * DP * 2, st >>>(a);
+   return check_launch("k_attn_short_forward");
+}
+
+template < typename T, int DP >
+int backward(const Args& a, cudaStream_t st)
+{
+   static SmemLimit limit;
+   const int rc = limit((const void*)k_attn_short_backward< T, DP >, Bwd< DP >::BYTES, "k_attn_short_backward");
+   if(rc) return rc;
+   k_attn_short_backward< T, DP ><<< dim3((unsigned)a.seqs, a.kv_heads), kShortThreads, Bwd< DP >::BYTES, st >>>(a);
+   return check_launch("k_attn_short_backward");
+}
+
+}  // namespace
+
+int short_forward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, cudaStream_t st)
+{
+   if(dtype == RELM_MP_BFLOAT16) return a.dim <= 32 ? forward< __nv_bfloat16, 32 >(a, q_tiles, st) : forward< __nv_bfloat16, 64 >(a, q_tiles, st);
+   return a.dim <= 32 ? forward< __half, 32 >(a, q_tiles, st) : forward< __half, 64 >(a, q_tiles, st);
+}
+
+int short_backward(relm_mp_dtype dtype, const Args& a, cudaStream_t st)
+{
+   if(dtype == RELM_MP_BFLOAT16) return a.dim <= 32 ? backward< __nv_bfloat16, 32 >(a, st) : backward< __nv_bfloat16, 64 >(a, st);
+   return a.dim <= 32 ? backward< __half, 32 >(a, st) : backward< __half, 64 >(a, st);
+}
+
+}  // namespace attn
+}  // namespace relm_mp
