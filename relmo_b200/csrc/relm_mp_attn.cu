@@ -111,16 +111,18 @@ Counts counts(const relm_mp_attn& in)
            in.seqs * ceil_div(in.max_kv, kTileRows), in.seqs * ceil_div(in.max_kv, kBlockKeys)};
 }
 
-// 16-byte copies of k and v rows: every row of every head starts on a 16-byte boundary.
-bool aligned_rows(const relm_mp_attn& in)
+// 16-byte copies of rows: every row of every head starts on a 16-byte boundary.
+bool aligned_any(const relm_mp_attn& in)
 {
    if(!in.q || !in.k || !in.v) return false;
-   if(in.dtype == RELM_MP_FLOAT32 || in.dim % 8) return false;
+   const int64_t unit = in.dtype == RELM_MP_FLOAT32 ? 4 : 8;
+   if(in.dim % unit) return false;
    auto ok = [&](const void* p, const int64_t* s) {
-      return (reinterpret_cast< uintptr_t >(p) & 15) == 0 && (in.plan || s[0] % 8 == 0) && s[1] % 8 == 0 && s[2] % 8 == 0;
+      return (reinterpret_cast< uintptr_t >(p) & 15) == 0 && (in.plan || s[0] % unit == 0) && s[1] % unit == 0 && s[2] % unit == 0;
    };
    return ok(in.k, in.k_stride) && ok(in.v, in.v_stride) && ok(in.q, in.q_stride);
 }
+bool aligned_rows(const relm_mp_attn& in) { return in.dtype != RELM_MP_FLOAT32 && aligned_any(in); }
 
 // Tensor maps hold these strides and coordinates.
 bool use_tc(const relm_mp_attn& in)
@@ -141,7 +143,7 @@ bool short_keys(const relm_mp_attn& in) { return aligned_rows(in) && in.max_kv <
 bool few_rows(const relm_mp_attn& in) { return in.max_q * (in.heads / in.kv_heads) <= 16; }
 
 // The form split over the keys.
-bool use_split(const relm_mp_attn& in) { return aligned_rows(in) && few_rows(in); }
+bool use_split(const relm_mp_attn& in) { return few_rows(in); }
 
 // delta[head, row] = sum over dim of go * (o + o_rest), in float32; 8 lanes per row and head.
 template < typename T, int VEC >
@@ -317,7 +319,7 @@ int relm_mp_attn_plan_fill(const int64_t* q_lengths, const int64_t* kv_lengths, 
 size_t relm_mp_cross_attention_workspace_bytes(const relm_mp_attn* attn)
 {
    if(check_attn(attn, "cross_attention") || attn->q_rows == 0) return 0;
-   return use_split(*attn) ? split_plan(make_args(*attn), counts(*attn).kv_blocks).bytes : 0;
+   return use_split(*attn) ? split_plan(make_args(*attn), counts(*attn).kv_blocks, aligned_rows(*attn)).bytes : 0;
 }
 
 int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void* o_rest, void* workspace,
@@ -333,7 +335,7 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
    a.o = o, a.lse = lse, a.o_rest = attn->dtype == RELM_MP_FLOAT32 ? nullptr : o_rest;
    const Counts c = counts(*attn);
    cudaStream_t st = static_cast< cudaStream_t >(stream);
-   if(use_split(*attn)) return split_forward(attn->dtype, a, c.kv_blocks, workspace, st);
+   if(use_split(*attn)) return split_forward(attn->dtype, a, c.kv_blocks, aligned_any(*attn), workspace, st);
    if(short_keys(*attn) && ((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(a.o_rest)) & 3) == 0)
       return short_forward(attn->dtype, a, c.q_tiles, st);
    if(use_tc(*attn) && ((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(a.o_rest)) & 15) == 0) {

@@ -100,13 +100,14 @@ __device__ __forceinline__ float exp2_fast(float x)
 int simt_forward(relm_mp_dtype dtype, const Args& a, int64_t items, cudaStream_t st);
 int simt_backward(relm_mp_dtype dtype, const Args& a, int64_t q_items, int64_t kv_items, cudaStream_t st);
 
-// Few query rows per sequence, 2-byte types, work split over the keys (relm_mp_attn_split.cu).
+// Few query rows per sequence, work split over the keys (relm_mp_attn_split.cu). `aligned`: every row of
+// every head starts on a 16-byte boundary; `two_bytes`: of an aligned 2-byte type.
 struct SplitPlan {
    int parts, row_groups;
    size_t part_o, part_ml, bytes; // workspace
 };
-SplitPlan split_plan(const Args& a, int64_t blocks);
-int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* workspace, cudaStream_t st);
+SplitPlan split_plan(const Args& a, int64_t blocks, bool two_bytes);
+int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, bool aligned, void* workspace, cudaStream_t st);
 
 // Up to 128 keys a sequence, dim up to 64, 2-byte types, aligned rows (relm_mp_attn_short.cu).
 int short_forward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, cudaStream_t st);

@@ -17,6 +17,8 @@
 // end of a segment. No block-wide barrier is in the loop.
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "relm_mp_attn_mma.cuh"
 
 namespace relm_mp {
@@ -243,6 +245,193 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split(SplitArgs s)
    }
 }
 
+// The same on the CUDA cores, in float32 throughout: float32 inputs, and 2-byte
+// ones whose rows are not on 16-byte boundaries. 16 keys a step and warp: two
+// lanes per key for the scores (each half of the row, from shared memory; the
+// query rows are broadcast), then the lanes share the output's columns. R: query
+// rows held in registers.
+template < typename T, int DP, int R >
+__global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool aligned)
+{
+   const Args& a = s.a;
+   constexpr int VEC = DP / 32, LD = DP + 4; // output columns of a lane; floats of a row in shared memory
+   constexpr uint32_t TILE = kChunk * LD * 4, STAGE = 2 * TILE;
+   constexpr int STAGES = DP > 128 ? 1 : 3; // (wide rows: what shared memory holds)
+   extern __shared__ __align__(128) unsigned char smem[];
+   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_p[kWarps][R][kChunk], sm_q[R][DP];
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, key_lane = lane >> 1, half = lane & 1;
+   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, row0 = blockIdx.z * R;
+   unsigned char* const mine = smem + warp * (STAGES * STAGE);
+   const uint32_t base = (uint32_t)__cvta_generic_to_shared(mine);
+   const int64_t first = part_start(s.blocks, s.parts, blockIdx.x), last = part_start(s.blocks, s.parts, blockIdx.x + 1);
+   const float sc = a.scale * kLog2e;
+   int64_t seq = 0;
+   for(int64_t b0 = 0; b0 < a.seqs; b0 += kThreads4) {
+      const int64_t b = b0 + threadIdx.x;
+      const int n = __syncthreads_count(b < a.seqs && block_of(a, b) < first && block_of(a, b + 1) <= first);
+      seq += n;
+      if(n < kThreads4) break;
+   }
+   for(; seq < a.seqs; ++seq) {
+      const int64_t blk0 = block_of(a, seq), blk1 = block_of(a, seq + 1);
+      if(blk0 >= last && blockIdx.x != s.parts - 1) break;
+      const Seq qs = locate(a.q_off, a.max_q, a.qs, (int)seq);
+      const int rows = qs.len * group;
+      if(row0 >= rows) continue;
+      const Seq ks = locate(a.kv_off, a.max_kv, a.ks, (int)seq), vs = locate(a.kv_off, a.max_kv, a.vs, (int)seq);
+      const int64_t lo = blk0 > first ? blk0 : first, hi = blk1 < last ? blk1 : last;
+      const bool whole = lo == blk0 && hi == blk1;
+      const int key_lo = (int)(lo - blk0) * kBlockKeys;
+      const int key_hi = whole || hi == blk1 ? ks.len : (int)(hi - blk0) * kBlockKeys;
+      const T* kp = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
+      const T* vp = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
+      const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+      for(int i = threadIdx.x; i < R * DP; i += kThreads4) {
+         const int r = row0 + i / DP, d = i % DP;
+         const T* q = static_cast< const T* >(a.q) + qs.base + (int64_t)(r / group) * a.qs[1] + (kv_head * group + r % group) * a.qs[2];
+         sm_q[i / DP][d] = r < rows && d < a.dim ? to_f32(q[d]) : 0.f;
+      }
+      __syncthreads();
+      float o[R][VEC], m[R], l[R];
+#pragma unroll
+      for(int r = 0; r < R; ++r) {
+         m[r] = -CUDART_INF_F, l[r] = 0.f;
+#pragma unroll
+         for(int v = 0; v < VEC; ++v) o[r][v] = 0.f;
+      }
+      const int steps = key_hi > key_lo + warp * kChunk ? (key_hi - key_lo - warp * kChunk + kChunk * kWarps - 1) / (kChunk * kWarps) : 0;
+      auto issue = [&](int step, int stage) {
+         if(step < steps) {
+            const int key0 = key_lo + (step * kWarps + warp) * kChunk;
+            if(std::is_same< T, float >::value && aligned) {
+               constexpr int CH = DP / 4;
+               for(int i = lane; i < kChunk * CH; i += 32) {
+                  const int r = i / CH, c = i % CH;
+                  const bool in = key0 + r < key_hi && c * 4 < a.dim;
+                  const int64_t key = in ? key0 + r : 0;
+                  const uint32_t to = base + stage * STAGE + (r * LD + c * 4) * 4;
+                  copy16(to, in ? kp + key * a.ks[1] + c * 4 : kp, in);
+                  copy16(to + TILE, in ? vp + key * a.vs[1] + c * 4 : vp, in);
+               }
+            } else {
+               float* to = reinterpret_cast< float* >(mine + stage * STAGE);
+               for(int i = lane; i < kChunk * DP; i += 32) {
+                  const int r = i / DP, c = i % DP;
+                  const bool in = key0 + r < key_hi && c < a.dim;
+                  to[r * LD + c] = in ? to_f32(kp[(int64_t)(key0 + r) * a.ks[1] + c]) : 0.f;
+                  to[TILE / 4 + r * LD + c] = in ? to_f32(vp[(int64_t)(key0 + r) * a.vs[1] + c]) : 0.f;
+               }
+            }
+         }
+         asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      for(int i = 0; i < STAGES - 1; ++i) issue(i, i);
+      for(int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+         issue(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+         __syncwarp();
+         const float* sk = reinterpret_cast< const float* >(mine + stage * STAGE);
+         const float* sv = sk + TILE / 4;
+         const int key = key_lo + (step * kWarps + warp) * kChunk + key_lane;
+         const bool in = key < key_hi && (!keep || keep[key]);
+         float c[R];
+#pragma unroll
+         for(int r = 0; r < R; ++r) c[r] = 0.f;
+#pragma unroll 4
+         for(int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 4) {
+            const float4 k = *reinterpret_cast< const float4* >(sk + key_lane * LD + d);
+#pragma unroll
+            for(int r = 0; r < R; ++r) {
+               const float4 q = *reinterpret_cast< const float4* >(&sm_q[r][d]);
+               c[r] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, c[r]))));
+            }
+         }
+         const unsigned bits = __ballot_sync(~0u, in); // bit 2 j: key j
+#pragma unroll
+         for(int r = 0; r < R; ++r) {
+            c[r] += __shfl_xor_sync(~0u, c[r], 1);
+            c[r] = in ? c[r] * sc : -CUDART_INF_F;
+            float top = c[r];
+#pragma unroll
+            for(int x = 2; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+            if(top > m[r]) {
+               const float f = exp2_fast(m[r] - top);
+               m[r] = top;
+               l[r] *= f;
+#pragma unroll
+               for(int v = 0; v < VEC; ++v) o[r][v] *= f;
+            }
+            const float p = exp2_fast(c[r] - (m[r] == -CUDART_INF_F ? 0.f : m[r]));
+            if(half == 0) {
+               l[r] += p;
+               sm_p[warp][r][key_lane] = p;
+            }
+         }
+         __syncwarp();
+#pragma unroll 4
+         for(int j = 0; j < kChunk; ++j) {
+            if(!(bits >> (2 * j) & 1)) continue; // what a masked row holds is not read
+            float v[VEC];
+#pragma unroll
+            for(int e = 0; e < VEC; ++e) v[e] = sv[j * LD + e * 32 + lane];
+#pragma unroll
+            for(int r = 0; r < R; ++r) {
+               const float p = sm_p[warp][r][j];
+#pragma unroll
+               for(int e = 0; e < VEC; ++e) o[r][e] = fmaf(p, v[e], o[r][e]);
+            }
+         }
+         __syncwarp(); // the stage and the weights are free
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      // Join the warps: each leaves its output in its own buffer.
+      __syncwarp();
+      float* out = reinterpret_cast< float* >(mine);
+#pragma unroll
+      for(int r = 0; r < R; ++r) {
+#pragma unroll
+         for(int x = 1; x < 32; x <<= 1) l[r] += __shfl_xor_sync(~0u, l[r], x);
+         if(lane == 0) sm_m[warp][r] = m[r], sm_l[warp][r] = l[r];
+#pragma unroll
+         for(int e = 0; e < VEC; ++e) out[r * DP + e * 32 + lane] = o[r][e];
+      }
+      __syncthreads();
+      const int64_t slot = ((int64_t)blockIdx.x + seq) * a.kv_heads + kv_head;
+      for(int i = threadIdx.x; i < R * DP; i += kThreads4) {
+         const int r = i / DP, d = i % DP;
+         if(row0 + r >= rows) break;
+         float M = -CUDART_INF_F;
+#pragma unroll
+         for(int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][r]);
+         const float ref = M == -CUDART_INF_F ? 0.f : M;
+         float L = 0.f, v = 0.f;
+#pragma unroll
+         for(int w = 0; w < kWarps; ++w) {
+            const float f = exp2_fast(sm_m[w][r] - ref);
+            L += sm_l[w][r] * f;
+            v += reinterpret_cast< const float* >(smem + w * (STAGES * STAGE))[i] * f;
+         }
+         if(whole) {
+            const int tok = (row0 + r) / group, head = kv_head * group + (row0 + r) % group;
+            if(d < a.dim) {
+               const int64_t at = ((qs.first + tok) * a.heads + head) * a.dim + d;
+               const float x = L == 0.f ? 0.f : v / L;
+               const T y = from_f32< T >(x);
+               static_cast< T* >(a.o)[at] = y;
+               if(a.o_rest) static_cast< T* >(a.o_rest)[at] = from_f32< T >(x - to_f32(y));
+            }
+            if(d == 0 && a.lse)
+               a.lse[(int64_t)head * a.q_rows + qs.first + tok] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
+         } else {
+            const int64_t at = slot * s.row_groups * kRows + row0 + r;
+            s.part_o[at * DP + d] = v;
+            if(d == 0) s.part_ml[at] = make_float2(M, L);
+         }
+      }
+      __syncthreads();
+   }
+}
+
 // Rows of sequences that more than one part worked on: a warp per row.
 template < typename T, int DP >
 __global__ void __launch_bounds__(128) k_attn_join(SplitArgs s)
@@ -293,6 +482,15 @@ __global__ void __launch_bounds__(128) k_attn_join(SplitArgs s)
 int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 template < typename T, int DP >
+int launch_join(const SplitArgs& s, cudaStream_t st)
+{
+   if(s.parts == 1) return RELM_MP_OK;
+   const int64_t y = ceil_div(s.a.max_q * s.a.heads, 4);
+   k_attn_join< T, DP ><<< dim3((unsigned)s.a.seqs, (unsigned)(y < 64 ? y : 64)), 128, 0, st >>>(s);
+   return check_launch("k_attn_join");
+}
+
+template < typename T, int DP >
 int launch(const SplitArgs& s, cudaStream_t st)
 {
    constexpr size_t bytes = (size_t)kWarps * kStages * 2 * kChunk * DP * 2;
@@ -300,34 +498,55 @@ int launch(const SplitArgs& s, cudaStream_t st)
    int rc = limit((const void*)k_attn_split< T, DP >, bytes, "k_attn_split");
    if(rc) return rc;
    k_attn_split< T, DP ><<< dim3(s.parts, s.a.kv_heads, s.row_groups), kThreads4, bytes, st >>>(s);
-   if((rc = check_launch("k_attn_split")) || s.parts == 1) return rc;
-   const int64_t rows = s.a.max_q * s.a.heads;
-   const int64_t y = ceil_div(rows, 4);
-   k_attn_join< T, DP ><<< dim3((unsigned)s.a.seqs, (unsigned)(y < 64 ? y : 64)), 128, 0, st >>>(s);
-   return check_launch("k_attn_join");
+   rc = check_launch("k_attn_split");
+   return rc ? rc : launch_join< T, DP >(s, st);
+}
+
+template < typename T, int DP, int R >
+int launch_wide(const SplitArgs& s, bool aligned, cudaStream_t st)
+{
+   constexpr size_t bytes = (size_t)kWarps * (DP > 128 ? 1 : 3) * 2 * kChunk * (DP + 4) * 4;
+   static SmemLimit limit;
+   int rc = limit((const void*)k_attn_split_wide< T, DP, R >, bytes, "k_attn_split_wide");
+   if(rc) return rc;
+   const int groups = (int)ceil_div(s.a.max_q * (s.a.heads / s.a.kv_heads), R);
+   k_attn_split_wide< T, DP, R ><<< dim3(s.parts, s.a.kv_heads, groups), kThreads4, bytes, st >>>(s, aligned);
+   rc = check_launch("k_attn_split_wide");
+   return rc ? rc : launch_join< T, DP >(s, st);
+}
+
+template < typename T, int DP >
+int launch_rows(const SplitArgs& s, bool aligned, cudaStream_t st)
+{
+   const int64_t rows = s.a.max_q * (s.a.heads / s.a.kv_heads);
+   if(rows == 1) return launch_wide< T, DP, 1 >(s, aligned, st);
+   return rows <= 4 ? launch_wide< T, DP, 4 >(s, aligned, st) : launch_wide< T, DP, 8 >(s, aligned, st);
 }
 
 template < typename T >
-int launch_dim(const SplitArgs& s, cudaStream_t st)
+int launch_dim(const SplitArgs& s, bool aligned, cudaStream_t st)
 {
-   switch(padded_dim(s.a.dim)) {
-      case 32: return launch< T, 32 >(s, st);
-      case 64: return launch< T, 64 >(s, st);
-      case 128: return launch< T, 128 >(s, st);
-      default: return launch< T, 256 >(s, st);
+   const int dp = padded_dim(s.a.dim);
+   if constexpr(!std::is_same< T, float >::value) {
+      if(aligned) return dp == 32 ? launch< T, 32 >(s, st) : dp == 64 ? launch< T, 64 >(s, st) : dp == 128 ? launch< T, 128 >(s, st) : launch< T, 256 >(s, st);
    }
+   return dp == 32    ? launch_rows< T, 32 >(s, aligned, st)
+          : dp == 64  ? launch_rows< T, 64 >(s, aligned, st)
+          : dp == 128 ? launch_rows< T, 128 >(s, aligned, st)
+                      : launch_rows< T, 256 >(s, aligned, st);
 }
 
 }  // namespace
 
 // Parts: one wave of resident blocks (shared memory allows about 200 KB per SM),
 // but at least 4 key blocks each, so that a part has work for every warp's pipeline.
-SplitPlan split_plan(const Args& a, int64_t blocks)
+SplitPlan split_plan(const Args& a, int64_t blocks, bool two_bytes)
 {
    const int dp = padded_dim(a.dim);
    SplitPlan p;
    p.row_groups = (int)ceil_div(a.max_q * (a.heads / a.kv_heads), kRows);
-   const int64_t resident = std::max< int64_t >(1, std::min< int64_t >(8, 200 * 1024 / (kWarps * kStages * 2 * kChunk * dp * 2)));
+   const int64_t row = two_bytes ? dp * 2 : (dp + 4) * 4, stages = !two_bytes && dp > 128 ? 1 : kStages;
+   const int64_t resident = std::max< int64_t >(1, std::min< int64_t >(8, 200 * 1024 / (kWarps * stages * 2 * kChunk * row)));
    const int64_t slots = 148 * resident / (a.kv_heads * p.row_groups);
    p.parts = (int)std::max< int64_t >(1, std::min(slots, ceil_div(blocks, 4)));
    const size_t rows = p.parts == 1 ? 0 : (size_t)(p.parts + a.seqs) * a.kv_heads * p.row_groups * kRows;
@@ -337,13 +556,17 @@ SplitPlan split_plan(const Args& a, int64_t blocks)
    return p;
 }
 
-int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, void* workspace, cudaStream_t st)
+int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, bool aligned, void* workspace, cudaStream_t st)
 {
-   const SplitPlan p = split_plan(a, blocks);
+   const SplitPlan p = split_plan(a, blocks, dtype != RELM_MP_FLOAT32 && aligned);
    char* w = static_cast< char* >(workspace);
    const SplitArgs s{a, blocks, p.parts, reinterpret_cast< float* >(w + p.part_o), reinterpret_cast< float2* >(w + p.part_ml),
                      p.row_groups};
-   return dtype == RELM_MP_BFLOAT16 ? launch_dim< __nv_bfloat16 >(s, st) : launch_dim< __half >(s, st);
+   switch(dtype) {
+      case RELM_MP_FLOAT32: return launch_dim< float >(s, aligned, st);
+      case RELM_MP_BFLOAT16: return launch_dim< __nv_bfloat16 >(s, aligned, st);
+      default: return launch_dim< __half >(s, aligned, st);
+   }
 }
 
 }  // namespace attn
