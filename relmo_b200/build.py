@@ -45,7 +45,7 @@ CUDA_SOURCES = [
     "relm_mp_norm.cu",
     "relm_mp_int4.cu",
     "relm_mp_attn.cu",
-    "relm_mp_attn_simt.cu",
+    "relm_mp_attn_warp.cu",
     "relm_mp_attn_split.cu",
     "relm_mp_attn_short.cu",
     "relm_mp_attn_tc.cu",

@@ -342,13 +342,16 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
       if((rc = gave_up_address(&a.gave_up))) return rc;
       return tc_forward(attn->dtype, a, c.q_tiles, c.q_pairs, st);
    }
-   return simt_forward(attn->dtype, a, c.q_tiles, st);
+   return warp_forward(attn->dtype, a, c.q_tiles, aligned_any(*attn), st);
 }
+
+static size_t delta_bytes(const relm_mp_attn& in) { return align_up((size_t)in.heads * in.q_rows * sizeof(float)); }
 
 size_t relm_mp_cross_attention_backward_workspace_bytes(const relm_mp_attn* attn)
 {
    if(check_attn(attn, "cross_attention_backward")) return 0;
-   return align_up((size_t)attn->heads * attn->q_rows * sizeof(float));
+   const int few = few_rows(*attn) ? warp_few_parts(make_args(*attn)) : 0;
+   return delta_bytes(*attn) + (few > 1 ? align_up((size_t)few * attn->q_rows * attn->heads * attn->dim * sizeof(float)) : 0);
 }
 
 int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_o, const void* o, const void* o_rest,
@@ -385,5 +388,7 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
       if((rc = gave_up_address(&a.gave_up))) return rc;
       return tc_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);
    }
-   return simt_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);
+   const int few = few_rows(*attn) ? warp_few_parts(a) : 0;
+   return warp_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, aligned_any(*attn) && aligned, few, static_cast< char* >(workspace) + delta_bytes(*attn),
+                        st);
 }

@@ -96,9 +96,12 @@ __device__ __forceinline__ float exp2_fast(float x)
    return y;
 }
 
-// Kernels on the CUDA cores, for every type, dim and stride (relm_mp_attn_simt.cu).
-int simt_forward(relm_mp_dtype dtype, const Args& a, int64_t items, cudaStream_t st);
-int simt_backward(relm_mp_dtype dtype, const Args& a, int64_t q_items, int64_t kv_items, cudaStream_t st);
+// Every type, dim and stride, on the warp-level matrix instructions (relm_mp_attn_warp.cu). `aligned`: every
+// row starts on a 16-byte boundary. few_parts > 0: the backward of few query rows, dQ in so many parts
+// (more than one: summed through `parts`, float32 [few_parts, q rows, heads, dim]).
+int warp_forward(relm_mp_dtype dtype, const Args& a, int64_t items, bool aligned, cudaStream_t st);
+int warp_few_parts(const Args& a);
+int warp_backward(relm_mp_dtype dtype, const Args& a, int64_t q_items, int64_t kv_items, bool aligned, int few_parts, void* parts, cudaStream_t st);
 
 // Few query rows per sequence, work split over the keys (relm_mp_attn_split.cu). `aligned`: every row of
 // every head starts on a 16-byte boundary; `two_bytes`: of an aligned 2-byte type.

@@ -1,0 +1,626 @@
+// Cross attention on the warp-level matrix instructions, for what the tcgen05
+// kernels do not take: float32, head dims above 128 or that are no multiple of 8,
+// rows off 16-byte boundaries, and the backward of few query rows.
+//
+// A warp owns 16 rows (queries, or keys for dK and dV) and walks the other side in
+// tiles that the block shares. Scores come out in the layout in which the weights
+// enter the second product, so weights never leave the registers:
+//
+//   forward  S = Q K^T, running maximum and sum per row, O = O c + P V
+//   dK, dV   rows are keys: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q
+//   dQ       S = Q K^T, dP = dO V^T, dQ += dS K
+//
+// No atomics: every output row has one owner. Float32 products are exact to about
+// 22 bits: each factor is the sum of two tf32 numbers (x = hi + lo, rounded to
+// nearest) and hi hi + hi lo + lo hi is summed in float32 (m16n8k8); the dropped
+// lo lo is below 2^-22. The instruction cuts its sums instead of rounding them (a
+// sum over 4 097 keys was 3e-5 off that way), so at most 32 terms are summed in one
+// accumulator, the small products in another, and both are added to the rest by
+// ordinary additions. Bound by those products
+// (float32) or by the tile copies.
+//
+// Rows that are masked or outside the sequence are zeros in shared memory (never
+// read) and get weight 0.
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "relm_mp_attn_mma.cuh"
+
+namespace relm_mp {
+namespace attn {
+namespace {
+
+// Row pitch in elements: 16 bytes more than the row, so that 8 rows lie in different banks.
+template < typename T, int DP >
+constexpr int kPitch = DP + 16 / (int)sizeof(T);
+template < typename T, int DP >
+constexpr size_t kRowBytes = kPitch< T, DP > * sizeof(T);
+
+// `rows` rows from row0 on into shared memory; rows past `len` or not kept, and columns past dim, are zeros.
+template < typename T, int DP >
+__device__ __forceinline__ void fill_tile(T* dst, const T* src, int64_t stride, int rows, int row0, int len, int dim,
+                                          const unsigned char* keep, bool aligned)
+{
+   if(aligned) {
+      constexpr int PER = 16 / sizeof(T), CH = DP / PER;
+      for(int i = threadIdx.x; i < rows * CH; i += blockDim.x) {
+         const int r = i / CH, c = i % CH;
+         const bool in = row0 + r < len && c * PER < dim && (!keep || keep[row0 + r]);
+         copy16((uint32_t)__cvta_generic_to_shared(dst + r * kPitch< T, DP > + c * PER), in ? src + (int64_t)(row0 + r) * stride + c * PER : src, in);
+      }
+   } else {
+      for(int i = threadIdx.x; i < rows * DP; i += blockDim.x) {
+         const int r = i / DP, c = i % DP;
+         const bool in = row0 + r < len && c < dim && (!keep || keep[row0 + r]);
+         dst[r * kPitch< T, DP > + c] = in ? src[(int64_t)(row0 + r) * stride + c] : from_f32< T >(0.f);
+      }
+   }
+}
+__device__ __forceinline__ void tiles_done()
+{
+   asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
+   __syncthreads();
+}
+
+__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, const uint32_t* b)
+{
+   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// x = hi + lo in tf32 (lo is cut to tf32 by the product).
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo)
+{
+   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+   lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+// c (16 x 8 NT) += a (16 rows from a_row) b^T (8 NT rows from b_row), over the tiles' columns.
+template < typename T, int DP, int NT >
+__device__ __forceinline__ void product_t(float (&c)[NT][4], const T* a, int a_row, const T* b, int b_row)
+{
+   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+   constexpr int LD = kPitch< T, DP >;
+   if constexpr(std::is_same< T, float >::value) {
+      for(int k0 = 0; k0 < DP; k0 += 32) {
+         float s[NT][4], e[NT][4];
+#pragma unroll
+         for(int n = 0; n < NT; ++n)
+#pragma unroll
+            for(int i = 0; i < 4; ++i) s[n][i] = e[n][i] = 0.f;
+#pragma unroll
+         for(int k = k0; k < k0 + 32; k += 8) {
+            uint32_t ah[4], al[4];
+#pragma unroll
+            for(int i = 0; i < 4; ++i) split(a[(a_row + g + 8 * (i & 1)) * LD + k + t4 + 4 * (i >> 1)], ah[i], al[i]);
+#pragma unroll
+            for(int n = 0; n < NT; ++n) {
+               uint32_t bh[2], bl[2];
+#pragma unroll
+               for(int i = 0; i < 2; ++i) split(b[(b_row + n * 8 + g) * LD + k + t4 + 4 * i], bh[i], bl[i]);
+               mma_tf32(e[n], al, bh);
+               mma_tf32(e[n], ah, bl);
+               mma_tf32(s[n], ah, bh);
+            }
+         }
+#pragma unroll
+         for(int n = 0; n < NT; ++n)
+#pragma unroll
+            for(int i = 0; i < 4; ++i) c[n][i] += s[n][i] + e[n][i];
+      }
+   } else {
+#pragma unroll 4
+      for(int k = 0; k < DP; k += 16) {
+         uint32_t f[4];
+         ldmatrix4(f, (uint32_t)__cvta_generic_to_shared(a + (a_row + (lane & 15)) * LD + k + (lane >> 4) * 8));
+#pragma unroll
+         for(int n = 0; n < NT; n += 2) {
+            uint32_t w[4];
+            ldmatrix4(w, (uint32_t)__cvta_generic_to_shared(b + (b_row + n * 8 + (lane >> 4) * 8 + (lane & 7)) * LD + k + (lane >> 3 & 1) * 8));
+            Mma< T >::run(c[n], f, w[0], w[1]);
+            Mma< T >::run(c[n + 1], f, w[2], w[3]);
+         }
+      }
+   }
+}
+
+// c (16 x 8 ND) += w (16 x 8 NT) b (8 NT rows from b_row; columns from col). FINE: 2-byte
+// weights as the sum of two, so that their rounding does not count.
+template < typename T, int DP, int NT, int ND, bool FINE >
+__device__ __forceinline__ void product(float (&c)[ND][4], const float (&w)[NT][4], const T* b, int b_row, int col)
+{
+   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+   constexpr int LD = kPitch< T, DP >;
+   if constexpr(std::is_same< T, float >::value) {
+      // The order of the contracted rows is free: slots t and t + 4 take rows 2 t and 2 t + 1, as w holds them.
+      uint32_t ah[NT][4], al[NT][4];
+#pragma unroll
+      for(int n = 0; n < NT; ++n)
+#pragma unroll
+         for(int i = 0; i < 4; ++i) split(w[n][(i & 1) * 2 + (i >> 1)], ah[n][i], al[n][i]);
+#pragma unroll
+      for(int d = 0; d < ND; ++d) {
+         float s[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+         for(int n = 0; n < NT; ++n) {
+            uint32_t bh[2], bl[2];
+#pragma unroll
+            for(int i = 0; i < 2; ++i) split(b[(b_row + n * 8 + 2 * t4 + i) * LD + col + d * 8 + g], bh[i], bl[i]);
+            mma_tf32(e, al[n], bh);
+            mma_tf32(e, ah[n], bl);
+            mma_tf32(s, ah[n], bh);
+         }
+#pragma unroll
+         for(int i = 0; i < 4; ++i) c[d][i] += s[i] + e[i];
+      }
+   } else {
+#pragma unroll
+      for(int n = 0; n < NT; n += 2) {
+         const uint32_t f[4] = {Mma< T >::pack(w[n][0], w[n][1]), Mma< T >::pack(w[n][2], w[n][3]), Mma< T >::pack(w[n + 1][0], w[n + 1][1]),
+                                Mma< T >::pack(w[n + 1][2], w[n + 1][3])};
+         uint32_t r[4];
+         if constexpr(FINE) {
+#pragma unroll
+            for(int i = 0; i < 4; ++i) {
+               const T* e = reinterpret_cast< const T* >(&f[i]);
+               r[i] = Mma< T >::pack(w[n + (i >> 1)][2 * (i & 1)] - to_f32(e[0]), w[n + (i >> 1)][2 * (i & 1) + 1] - to_f32(e[1]));
+            }
+         }
+#pragma unroll
+         for(int d = 0; d < ND; d += 2) {
+            uint32_t v[4];
+            ldmatrix4_trans(v, (uint32_t)__cvta_generic_to_shared(b + (b_row + n * 8 + (lane >> 3 & 1) * 8 + (lane & 7)) * LD + col + d * 8 + (lane >> 4) * 8));
+            Mma< T >::run(c[d], f, v[0], v[1]);
+            Mma< T >::run(c[d + 1], f, v[2], v[3]);
+            if constexpr(FINE) {
+               Mma< T >::run(c[d], r, v[0], v[1]);
+               Mma< T >::run(c[d + 1], r, v[2], v[3]);
+            }
+         }
+      }
+   }
+}
+
+template < int N >
+__device__ __forceinline__ void zero(float (&c)[N][4])
+{
+#pragma unroll
+   for(int n = 0; n < N; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+}
+
+// Sizes of the owned and the streamed tiles: what fits shared memory twice where it can.
+template < typename T, int DP_ >
+struct Shape {
+   static constexpr int WARPS = sizeof(T) == 4 && DP_ > 128 ? 4 : 8, OWN = WARPS * 16, STREAM = 32;
+   static constexpr size_t own = OWN * kRowBytes< T, DP_ >, stream = STREAM * kRowBytes< T, DP_ >;
+};
+
+template < typename T, int DP >
+__global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_forward(Args a, bool aligned)
+{
+   using S = Shape< T, DP >;
+   constexpr int NT = S::STREAM / 8, ND = DP / 8, PER = kTileRows / S::OWN;
+   extern __shared__ __align__(128) unsigned char smem[];
+   T *sq = reinterpret_cast< T* >(smem), *sk = reinterpret_cast< T* >(smem + S::own), *sv = reinterpret_cast< T* >(smem + S::own + S::stream);
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x / PER);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
+   const int row0 = it.tile * kTileRows + (blockIdx.x % PER) * S::OWN;
+   if(row0 >= qs.len) return;
+   const T* k = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
+   const T* v = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   fill_tile< T, DP >(sq, static_cast< const T* >(a.q) + qs.base + head * a.qs[2], a.qs[1], S::OWN, row0, qs.len, a.dim, nullptr, aligned);
+   float o[ND][4], m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};
+   zero(o);
+   const float sc = a.scale * kLog2e;
+   for(int key0 = 0; key0 < ks.len; key0 += S::STREAM) {
+      fill_tile< T, DP >(sk, k, a.ks[1], S::STREAM, key0, ks.len, a.dim, keep, aligned);
+      fill_tile< T, DP >(sv, v, a.vs[1], S::STREAM, key0, ks.len, a.dim, keep, aligned);
+      const unsigned bits = __ballot_sync(~0u, key0 + lane < ks.len && (!keep || keep[key0 + lane]));
+      tiles_done();
+      float s[NT][4];
+      zero(s);
+      product_t< T, DP, NT >(s, sq, warp * 16, sk, 0);
+      float top[2] = {m[0], m[1]};
+#pragma unroll
+      for(int n = 0; n < NT; ++n)
+#pragma unroll
+         for(int i = 0; i < 4; ++i) {
+            s[n][i] = bits >> (n * 8 + 2 * t4 + (i & 1)) & 1 ? s[n][i] * sc : -CUDART_INF_F;
+            top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
+         }
+      float f[2], ref[2];
+#pragma unroll
+      for(int h = 0; h < 2; ++h) {
+         top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
+         top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
+         // No kept key so far: every score is -inf and every weight 0, whatever the reference.
+         ref[h] = top[h] == -CUDART_INF_F ? 0.f : top[h];
+         f[h] = exp2_fast(m[h] - ref[h]);
+         m[h] = top[h];
+         l[h] *= f[h];
+      }
+      if(__any_sync(~0u, f[0] != 1.f || f[1] != 1.f)) {
+#pragma unroll
+         for(int d = 0; d < ND; ++d)
+#pragma unroll
+            for(int i = 0; i < 4; ++i) o[d][i] *= f[i >> 1];
+      }
+#pragma unroll
+      for(int n = 0; n < NT; ++n)
+#pragma unroll
+         for(int i = 0; i < 4; ++i) {
+            s[n][i] = exp2_fast(s[n][i] - ref[i >> 1]);
+            l[i >> 1] += s[n][i];
+         }
+      product< T, DP, NT, ND, false >(o, s, sv, 0, 0);
+      __syncthreads();
+   }
+   T* out = static_cast< T* >(a.o);
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(~0u, l[h], 1);
+      l[h] += __shfl_xor_sync(~0u, l[h], 2);
+      const int row = row0 + warp * 16 + g + 8 * h;
+      if(row >= qs.len) continue;
+      const bool none = l[h] == 0.f; // no kept key (a NaN score leaves l NaN)
+      const float inv = none ? 0.f : 1.f / l[h];
+      const int64_t at = ((qs.first + row) * a.heads + head) * a.dim;
+#pragma unroll
+      for(int d = 0; d < ND; ++d)
+#pragma unroll
+         for(int e = 0; e < 2; ++e) {
+            const int c = d * 8 + 2 * t4 + e;
+            if(c >= a.dim) continue;
+            const float x = none ? 0.f : o[d][2 * h + e] * inv;
+            const T y = from_f32< T >(x);
+            out[at + c] = y;
+            if(a.o_rest) static_cast< T* >(a.o_rest)[at + c] = from_f32< T >(x - to_f32(y));
+         }
+      if(a.lse && t4 == 0) a.lse[(int64_t)head * a.q_rows + qs.first + row] = none ? -CUDART_INF_F : m[h] * kLn2 + logf(l[h]);
+   }
+   asm volatile("cp.async.wait_all;" ::: "memory"); // (the query tile's copies, where there was no key)
+}
+
+// Weights and score gradients in place of S and dP: 0 where !keep bit. `row` statistics are per row
+// (i >> 1) or, TRANS, per column.
+template < int NT, bool TRANS >
+__device__ __forceinline__ void weigh(float (&s)[NT][4], float (&dp)[NT][4], float sc, const float* lse, const float* delta, unsigned bits,
+                                      const bool (&in)[2])
+{
+   const int t4 = threadIdx.x & 3;
+#pragma unroll
+   for(int n = 0; n < NT; ++n)
+#pragma unroll
+      for(int i = 0; i < 4; ++i) {
+         const int c = n * 8 + 2 * t4 + (i & 1), at = TRANS ? c : i >> 1;
+         const bool kept = TRANS ? in[i >> 1] : (bits >> c & 1) != 0;
+         const float p = kept ? exp2_fast(fmaf(s[n][i], sc, -lse[at])) : 0.f;
+         s[n][i] = p;
+         dp[n][i] = kept ? p * (dp[n][i] - delta[at]) : 0.f;
+      }
+}
+
+// dK and dV of OWN keys and, for wide heads, of 128 columns (blockIdx.z). QN query rows at a time.
+template < typename T, int DP, int QN, bool FINE >
+__global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_backward_kv(Args a, bool aligned)
+{
+   using S = Shape< T, DP >;
+   constexpr int NT = QN / 8, DC = DP > 128 ? 128 : DP, ND = DC / 8, PER = kTileRows / S::OWN;
+   constexpr size_t STREAM = QN * kRowBytes< T, DP >;
+   extern __shared__ __align__(128) unsigned char smem[];
+   __shared__ float s_lse[QN], s_delta[QN];
+   T *sk = reinterpret_cast< T* >(smem), *sv = reinterpret_cast< T* >(smem + S::own), *sq = reinterpret_cast< T* >(smem + 2 * S::own),
+     *sg = reinterpret_cast< T* >(smem + 2 * S::own + STREAM);
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, col = blockIdx.z * DC;
+   const Item it = item(a.kv_tiles, a.max_kv, kTileRows, blockIdx.x / PER);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
+   const int key0 = it.tile * kTileRows + (blockIdx.x % PER) * S::OWN;
+   if(key0 >= ks.len) return;
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   fill_tile< T, DP >(sk, static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2], a.ks[1], S::OWN, key0, ks.len, a.dim, keep, aligned);
+   fill_tile< T, DP >(sv, static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2], a.vs[1], S::OWN, key0, ks.len, a.dim, keep, aligned);
+   float dk[ND][4], dv[ND][4];
+   zero(dk);
+   zero(dv);
+   bool in[2];
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      const int key = key0 + warp * 16 + g + 8 * h;
+      in[h] = key < ks.len && (!keep || keep[key]);
+   }
+   const float sc = a.scale * kLog2e;
+   for(int head = kv_head * group; head < (kv_head + 1) * group; ++head) {
+      const T* q = static_cast< const T* >(a.q) + qs.base + head * a.qs[2];
+      const T* go = static_cast< const T* >(a.go) + (qs.first * a.heads + head) * a.dim;
+      for(int q0 = 0; q0 < qs.len; q0 += QN) {
+         fill_tile< T, DP >(sq, q, a.qs[1], QN, q0, qs.len, a.dim, nullptr, aligned);
+         fill_tile< T, DP >(sg, go, (int64_t)a.heads * a.dim, QN, q0, qs.len, a.dim, nullptr, aligned);
+         if(threadIdx.x < QN) {
+            const int row = q0 + threadIdx.x;
+            const int64_t at = (int64_t)head * a.q_rows + qs.first + row;
+            const float v = row < qs.len ? a.lse_in[at] : -CUDART_INF_F;
+            s_lse[threadIdx.x] = v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e; // no such row, or a row without keys: weights 0
+            s_delta[threadIdx.x] = row < qs.len ? a.delta[at] : 0.f;
+         }
+         tiles_done();
+         float s[NT][4], dp[NT][4];
+         zero(s);
+         zero(dp);
+         product_t< T, DP, NT >(s, sk, warp * 16, sq, 0);
+         product_t< T, DP, NT >(dp, sv, warp * 16, sg, 0);
+         weigh< NT, true >(s, dp, sc, s_lse, s_delta, 0, in);
+         product< T, DP, NT, ND, FINE >(dv, s, sg, 0, col);
+         product< T, DP, NT, ND, FINE >(dk, dp, sq, 0, col);
+         __syncthreads();
+      }
+   }
+   asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      const int key = key0 + warp * 16 + g + 8 * h;
+      if(key >= ks.len) continue;
+      const int64_t at = ((ks.first + key) * a.kv_heads + kv_head) * a.dim;
+#pragma unroll
+      for(int d = 0; d < ND; ++d)
+#pragma unroll
+         for(int e = 0; e < 2; ++e) {
+            const int c = col + d * 8 + 2 * t4 + e;
+            if(c >= a.dim) continue;
+            static_cast< T* >(a.dk)[at + c] = from_f32< T >(dk[d][2 * h + e] * a.scale);
+            static_cast< T* >(a.dv)[at + c] = from_f32< T >(dv[d][2 * h + e]);
+         }
+   }
+}
+
+template < typename T, int DP >
+__global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_backward_q(Args a, bool aligned)
+{
+   using S = Shape< T, DP >;
+   constexpr int NT = S::STREAM / 8, ND = DP / 8, PER = kTileRows / S::OWN;
+   extern __shared__ __align__(128) unsigned char smem[];
+   T *sq = reinterpret_cast< T* >(smem), *sg = reinterpret_cast< T* >(smem + S::own), *sk = reinterpret_cast< T* >(smem + 2 * S::own),
+     *sv = reinterpret_cast< T* >(smem + 2 * S::own + S::stream);
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x / PER);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
+   const int row0 = it.tile * kTileRows + (blockIdx.x % PER) * S::OWN;
+   if(row0 >= qs.len) return;
+   const T* k = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
+   const T* v = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   fill_tile< T, DP >(sq, static_cast< const T* >(a.q) + qs.base + head * a.qs[2], a.qs[1], S::OWN, row0, qs.len, a.dim, nullptr, aligned);
+   fill_tile< T, DP >(sg, static_cast< const T* >(a.go) + (qs.first * a.heads + head) * a.dim, (int64_t)a.heads * a.dim, S::OWN, row0, qs.len,
+                      a.dim, nullptr, aligned);
+   float dq[ND][4], lse[2], delta[2];
+   zero(dq);
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      const int row = row0 + warp * 16 + g + 8 * h;
+      const int64_t at = (int64_t)head * a.q_rows + qs.first + row;
+      const float v = row < qs.len ? a.lse_in[at] : -CUDART_INF_F;
+      lse[h] = v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e;
+      delta[h] = row < qs.len ? a.delta[at] : 0.f;
+   }
+   const float sc = a.scale * kLog2e;
+   const bool in[2] = {true, true};
+   for(int key0 = 0; key0 < ks.len; key0 += S::STREAM) {
+      fill_tile< T, DP >(sk, k, a.ks[1], S::STREAM, key0, ks.len, a.dim, keep, aligned);
+      fill_tile< T, DP >(sv, v, a.vs[1], S::STREAM, key0, ks.len, a.dim, keep, aligned);
+      const unsigned bits = __ballot_sync(~0u, key0 + lane < ks.len && (!keep || keep[key0 + lane]));
+      tiles_done();
+      float s[NT][4], dp[NT][4];
+      zero(s);
+      zero(dp);
+      product_t< T, DP, NT >(s, sq, warp * 16, sk, 0);
+      product_t< T, DP, NT >(dp, sg, warp * 16, sv, 0);
+      weigh< NT, false >(s, dp, sc, lse, delta, bits, in);
+      product< T, DP, NT, ND, false >(dq, dp, sk, 0, 0);
+      __syncthreads();
+   }
+   asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      const int row = row0 + warp * 16 + g + 8 * h;
+      if(row >= qs.len) continue;
+      T* out = static_cast< T* >(a.dq) + ((qs.first + row) * a.heads + head) * a.dim;
+#pragma unroll
+      for(int d = 0; d < ND; ++d)
+#pragma unroll
+         for(int e = 0; e < 2; ++e)
+            if(d * 8 + 2 * t4 + e < a.dim) out[d * 8 + 2 * t4 + e] = from_f32< T >(dq[d][2 * h + e] * a.scale);
+   }
+}
+
+// dQ of few rows (tokens x heads of a group, up to 16): the block's four warps take different keys, and
+// blockIdx.z a part of them; partial sums go to `parts` ([z][query row, head, dim]) and are added in order.
+constexpr int kFewWarps = 4, kFewKeys = kFewWarps * 16;
+template < typename T, int DP >
+__global__ void __launch_bounds__(kFewWarps * 32) k_attn_warp_backward_q_few(Args a, bool aligned, float* parts, int part_keys)
+{
+   constexpr int ND = DP / 8, LD = kPitch< T, DP >;
+   constexpr size_t ROWS = 16 * kRowBytes< T, DP >, KEYS = kFewKeys * kRowBytes< T, DP >;
+   extern __shared__ __align__(128) unsigned char smem[];
+   T *sq = reinterpret_cast< T* >(smem), *sg = reinterpret_cast< T* >(smem + ROWS), *sk = reinterpret_cast< T* >(smem + 2 * ROWS),
+     *sv = reinterpret_cast< T* >(smem + 2 * ROWS + KEYS);
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+   const int seq = blockIdx.x, kv_head = blockIdx.y, group = a.heads / a.kv_heads;
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, seq), ks = locate(a.kv_off, a.max_kv, a.ks, seq);
+   const Seq vs = locate(a.kv_off, a.max_kv, a.vs, seq);
+   const int rows = qs.len * group;
+   if(rows == 0) return;
+   const T* k = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
+   const T* v = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   for(int i = threadIdx.x; i < 16 * DP; i += kFewWarps * 32) {
+      const int r = i / DP, c = i % DP, head = kv_head * group + r % group;
+      const bool in = r < rows && c < a.dim;
+      sq[r * LD + c] = in ? static_cast< const T* >(a.q)[qs.base + (int64_t)(r / group) * a.qs[1] + head * a.qs[2] + c] : from_f32< T >(0.f);
+      sg[r * LD + c] = in ? static_cast< const T* >(a.go)[((qs.first + r / group) * a.heads + head) * a.dim + c] : from_f32< T >(0.f);
+   }
+   float dq[ND][4], lse[2], delta[2];
+   zero(dq);
+#pragma unroll
+   for(int h = 0; h < 2; ++h) {
+      const int r = g + 8 * h;
+      const int64_t at = (int64_t)(kv_head * group + r % group) * a.q_rows + qs.first + r / group;
+      const float x = r < rows ? a.lse_in[at] : -CUDART_INF_F;
+      lse[h] = x == -CUDART_INF_F ? CUDART_INF_F : x * kLog2e;
+      delta[h] = r < rows ? a.delta[at] : 0.f;
+   }
+   const float sc = a.scale * kLog2e;
+   const bool in[2] = {true, true};
+   const int lo = blockIdx.z * part_keys, hi = min(ks.len, lo + part_keys);
+   for(int key0 = lo; key0 < hi; key0 += kFewKeys) {
+      fill_tile< T, DP >(sk, k, a.ks[1], kFewKeys, key0, hi, a.dim, keep, aligned);
+      fill_tile< T, DP >(sv, v, a.vs[1], kFewKeys, key0, hi, a.dim, keep, aligned);
+      const int key = key0 + warp * 16 + lane;
+      const unsigned bits = __ballot_sync(~0u, lane < 16 && key < hi && (!keep || keep[key]));
+      tiles_done();
+      float s[2][4], dp[2][4];
+      zero(s);
+      zero(dp);
+      product_t< T, DP, 2 >(s, sq, 0, sk, warp * 16);
+      product_t< T, DP, 2 >(dp, sg, 0, sv, warp * 16);
+      weigh< 2, false >(s, dp, sc, lse, delta, bits, in);
+      product< T, DP, 2, ND, true >(dq, dp, sk, warp * 16, 0);
+      __syncthreads();
+   }
+   // Join the warps in order.
+   __syncthreads();
+   float* sum = reinterpret_cast< float* >(smem);
+   for(int w = 0; w < kFewWarps; ++w) {
+      if(warp == w) {
+#pragma unroll
+         for(int d = 0; d < ND; ++d)
+#pragma unroll
+            for(int i = 0; i < 4; ++i) {
+               float* at = sum + (g + 8 * (i >> 1)) * DP + d * 8 + 2 * t4 + (i & 1);
+               *at = w ? *at + dq[d][i] : dq[d][i];
+            }
+      }
+      __syncthreads();
+   }
+   for(int i = threadIdx.x; i < rows * DP; i += kFewWarps * 32) {
+      const int r = i / DP, c = i % DP;
+      if(c >= a.dim) continue;
+      const int64_t at = ((qs.first + r / group) * a.heads + kv_head * group + r % group) * a.dim + c;
+      if(parts) parts[(int64_t)blockIdx.z * a.q_rows * a.heads * a.dim + at] = sum[i];
+      else static_cast< T* >(a.dq)[at] = from_f32< T >(sum[i] * a.scale);
+   }
+}
+
+template < typename T >
+__global__ void __launch_bounds__(256) k_attn_sum_parts(const float* __restrict__ parts, int count, int64_t n, float scale, T* __restrict__ out)
+{
+   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+   if(i >= n) return;
+   float s = 0.f;
+   for(int p = 0; p < count; ++p) s += parts[p * n + i];
+   out[i] = from_f32< T >(s * scale);
+}
+
+template < typename F, typename... X >
+int launch(SmemLimit& limit, F fn, dim3 grid, int threads, size_t bytes, cudaStream_t st, const char* what, X... args)
+{
+   if(grid.x == 0) return RELM_MP_OK;
+   const int rc = limit((const void*)fn, bytes, what);
+   if(rc) return rc;
+   fn<<< grid, threads, bytes, st >>>(args...);
+   return check_launch(what);
+}
+
+template < typename T, int DP >
+int forward(const Args& a, int64_t items, bool aligned, cudaStream_t st)
+{
+   using S = Shape< T, DP >;
+   static SmemLimit limit;
+   return launch(limit, k_attn_warp_forward< T, DP >, dim3((unsigned)(items * (kTileRows / S::OWN)), a.heads), S::WARPS * 32, S::own + 2 * S::stream,
+                 st, "k_attn_warp_forward", a, aligned);
+}
+
+template < typename T, int DP >
+int backward(const Args& a, int64_t q_items, int64_t kv_items, bool aligned, int few_parts, void* parts, cudaStream_t st)
+{
+   using S = Shape< T, DP >;
+   static SmemLimit kv_limit, kv_few_limit, q_limit, q_few_limit;
+   const dim3 kv_grid((unsigned)(kv_items * (kTileRows / S::OWN)), a.kv_heads, DP > 128 ? 2 : 1);
+   int rc;
+   if(few_parts == 0) {
+      rc = launch(kv_limit, k_attn_warp_backward_kv< T, DP, 32, false >, kv_grid, S::WARPS * 32, 2 * S::own + 2 * S::stream, st,
+                  "k_attn_warp_backward_kv", a, aligned);
+      return rc ? rc
+                : launch(q_limit, k_attn_warp_backward_q< T, DP >, dim3((unsigned)(q_items * (kTileRows / S::OWN)), a.heads), S::WARPS * 32,
+                         2 * S::own + 2 * S::stream, st, "k_attn_warp_backward_q", a, aligned);
+   }
+   if((rc = launch(kv_few_limit, k_attn_warp_backward_kv< T, DP, 16, true >, kv_grid, S::WARPS * 32, 2 * S::own + 32 * kRowBytes< T, DP >, st,
+                   "k_attn_warp_backward_kv", a, aligned)) ||
+      a.q_rows == 0)
+      return rc;
+   float* p = few_parts > 1 ? static_cast< float* >(parts) : nullptr;
+   const int part_keys = (int)(ceil_div(ceil_div(std::max< int64_t >(a.max_kv, 1), few_parts), kFewKeys) * kFewKeys);
+   const size_t bytes = std::max((32 + 2 * kFewKeys) * kRowBytes< T, DP >, (size_t)16 * DP * 4);
+   if((rc = launch(q_few_limit, k_attn_warp_backward_q_few< T, DP >, dim3((unsigned)a.seqs, a.kv_heads, few_parts), kFewWarps * 32, bytes, st,
+                   "k_attn_warp_backward_q_few", a, aligned, p, part_keys)) ||
+      !p)
+      return rc;
+   const int64_t n = a.q_rows * a.heads * a.dim;
+   k_attn_sum_parts< T ><<< (unsigned)ceil_div(n, 256), 256, 0, st >>>(p, few_parts, n, a.scale, static_cast< T* >(a.dq));
+   return check_launch("k_attn_sum_parts");
+}
+
+template < typename T >
+int forward_dim(const Args& a, int64_t items, bool aligned, cudaStream_t st)
+{
+   return a.dim <= 32    ? forward< T, 32 >(a, items, aligned, st)
+          : a.dim <= 64  ? forward< T, 64 >(a, items, aligned, st)
+          : a.dim <= 128 ? forward< T, 128 >(a, items, aligned, st)
+                         : forward< T, 256 >(a, items, aligned, st);
+}
+
+template < typename T >
+int backward_dim(const Args& a, int64_t qi, int64_t ki, bool aligned, int few, void* parts, cudaStream_t st)
+{
+   return a.dim <= 32    ? backward< T, 32 >(a, qi, ki, aligned, few, parts, st)
+          : a.dim <= 64  ? backward< T, 64 >(a, qi, ki, aligned, few, parts, st)
+          : a.dim <= 128 ? backward< T, 128 >(a, qi, ki, aligned, few, parts, st)
+                         : backward< T, 256 >(a, qi, ki, aligned, few, parts, st);
+}
+
+}  // namespace
+
+// Parts of the keys for the dQ of few rows: two blocks per SM, at least 256 keys each.
+int warp_few_parts(const Args& a)
+{
+   const int64_t blocks = std::max< int64_t >(a.seqs * a.kv_heads, 1);
+   return (int)std::max< int64_t >(1, std::min< int64_t >(ceil_div(a.max_kv, 256), 296 / blocks));
+}
+
+int warp_forward(relm_mp_dtype dtype, const Args& a, int64_t items, bool aligned, cudaStream_t st)
+{
+   switch(dtype) {
+      case RELM_MP_FLOAT32: return forward_dim< float >(a, items, aligned, st);
+      case RELM_MP_BFLOAT16: return forward_dim< __nv_bfloat16 >(a, items, aligned, st);
+      default: return forward_dim< __half >(a, items, aligned, st);
+   }
+}
+
+int warp_backward(relm_mp_dtype dtype, const Args& a, int64_t q_items, int64_t kv_items, bool aligned, int few_parts, void* parts, cudaStream_t st)
+{
+   switch(dtype) {
+      case RELM_MP_FLOAT32: return backward_dim< float >(a, q_items, kv_items, aligned, few_parts, parts, st);
+      case RELM_MP_BFLOAT16: return backward_dim< __nv_bfloat16 >(a, q_items, kv_items, aligned, few_parts, parts, st);
+      default: return backward_dim< __half >(a, q_items, kv_items, aligned, few_parts, parts, st);
+   }
+}
+
+}  // namespace attn
+}  // namespace relm_mp
