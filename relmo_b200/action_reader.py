@@ -1,0 +1,215 @@
+"""A decoder that scores candidate actions of planning states from their object embeddings.
+
+relmo's relational models end in object embeddings, one row per object, states
+one after another (:class:`relmo_b200.relational_gnn.RelationalGNN`). An
+:class:`ActionReader` reads them: the candidate actions of a state (any number
+per state, described by a feature row each) attend to the objects of that state
+(any number per state) through pre-norm blocks
+
+    x, h = add_rms_norm(last sublayer's output, w, h)
+    q = x Wq;  k, v = objects Wkv;  y = cross_attention(q, k, v) Wo
+    x, h = add_rms_norm(y, w, h)
+    y = act(x Wup) Wdown
+
+and get a score each. :class:`RelationalPolicy` puts it behind a relational model
+and trains both. :meth:`ActionReader.served` is the same decoder for inference on
+few rows: 4-bit projections, rows in 8 bits out of the norms, keys and values of
+the objects kept between calls.
+
+``python -m relmo_b200.action_reader`` trains a small policy on synthetic states
+and compares its served form with it.
+"""
+
+from __future__ import annotations
+
+import argparse
+from dataclasses import dataclass
+
+import torch
+import torch.nn.functional as F
+from torch import nn
+
+from .nn import Linear, activation
+from .ops import decoder
+from .workloads import RelationalBatch
+
+EPS = 1e-6
+
+
+def objects_per_state(batch: RelationalBatch) -> list[int]:
+    """Host counts of the batch's objects (they are stored state-major)."""
+
+    return torch.bincount(batch.object_state, minlength=batch.num_states).tolist()
+
+
+def reading_plan(batch: RelationalBatch, actions_per_state) -> decoder.AttentionPlan:
+    """The plan of one batch: made once, beside its routing, for all layers and the backward."""
+
+    return decoder.attention_plan(actions_per_state, objects_per_state(batch), batch.object_state.device)
+
+
+class ReaderBlock(nn.Module):
+    def __init__(self, width: int, object_width: int, heads: int, kv_heads: int, hidden: int, act: str = "silu"):
+        super().__init__()
+        if width % heads or heads % kv_heads:
+            raise ValueError(f"width {width} must divide into {heads} heads, and heads into {kv_heads} key/value heads.")
+        self.heads, self.kv_heads, self.dim = int(heads), int(kv_heads), width // heads
+        self.norm_read = nn.Parameter(torch.ones(width))
+        self.norm_mix = nn.Parameter(torch.ones(width))
+        self.query = Linear(width, width, bias=False)
+        self.key_value = Linear(object_width, 2 * self.kv_heads * self.dim, bias=False)
+        self.out = Linear(width, width, bias=False)
+        self.up = Linear(width, hidden, bias=False)
+        self.down = Linear(hidden, width, bias=False)
+        self.act = activation(act)
+
+    def keys_values(self, objects):
+        kv = self.key_value(objects).view(-1, 2, self.kv_heads, self.dim)
+        return kv[:, 0], kv[:, 1]
+
+    def forward(self, y, h, objects, plan, object_mask=None):
+        x, h = decoder.add_rms_norm(y, self.norm_read.to(y.dtype), h, eps=EPS)
+        q = self.query(x).view(-1, self.heads, self.dim)
+        k, v = self.keys_values(objects)
+        o = decoder.cross_attention(q, k, v, plan, key_mask=object_mask)
+        x, h = decoder.add_rms_norm(self.out(o.reshape(x.shape)), self.norm_mix.to(y.dtype), h, eps=EPS)
+        return self.down(self.act(self.up(x))), h
+
+
+class ActionReader(nn.Module):
+    """Scores ``[actions]`` from action features ``[actions, features]`` and object embeddings
+    ``[objects, object_width]``, both packed by state as the plan says. Objects where
+    ``object_mask`` is False are not read."""
+
+    def __init__(self, features: int, object_width: int, width: int = 128, num_layers: int = 2, heads: int = 4,
+                 kv_heads: int | None = None, hidden: int | None = None, act: str = "silu"):
+        super().__init__()
+        kv_heads = heads if kv_heads is None else kv_heads
+        hidden = 4 * width if hidden is None else hidden
+        self.embed = Linear(features, width)
+        self.blocks = nn.ModuleList(
+            ReaderBlock(width, object_width, heads, kv_heads, hidden, act) for _ in range(num_layers)
+        )
+        self.norm_out = nn.Parameter(torch.ones(width))
+        self.score = Linear(width, 1, bias=False)  # scores are compared within a state: a common bias says nothing
+
+    def forward(self, actions, objects, plan, object_mask=None):
+        y = self.embed(actions)
+        h = torch.zeros_like(y)
+        for block in self.blocks:
+            y, h = block(y, h, objects, plan, object_mask)
+        x, _ = decoder.add_rms_norm(y, self.norm_out.to(y.dtype), h, eps=EPS)
+        return self.score(x).squeeze(-1)
+
+    def served(self, group: int = 32, dtype: torch.dtype | None = None) -> "ServedActionReader":
+        return ServedActionReader(self, group, dtype)
+
+
+@dataclass(frozen=True)
+class StateMemory:
+    """Keys and values of a batch of states, one pair per block, and how many objects each state has."""
+
+    keys_values: list
+    objects: list[int]
+    object_mask: object = None
+
+
+class ServedActionReader:
+    """An :class:`ActionReader` for inference. ``remember`` reads the objects once;
+    ``score`` then takes a few actions per state at a time."""
+
+    def __init__(self, reader: ActionReader, group: int = 32, dtype: torch.dtype | None = None):
+        self.dtype = dtype or reader.embed.weight.dtype
+        cast = lambda p: p.detach().to(self.dtype).contiguous()  # noqa: E731
+        pack = lambda linear: decoder.quantize_int4(linear.weight, group)  # noqa: E731
+        self.reader = reader
+        self.blocks = [
+            {"norm_read": cast(b.norm_read), "norm_mix": cast(b.norm_mix), "query": pack(b.query), "out": pack(b.out),
+             "up": pack(b.up), "down": pack(b.down)}
+            for b in reader.blocks
+        ]
+        self.norm_out = cast(reader.norm_out)
+
+    @torch.no_grad()
+    def remember(self, objects, objects_per_state, object_mask=None) -> StateMemory:
+        kv = []
+        for b in self.reader.blocks:
+            k, v = b.keys_values(objects.to(b.key_value.weight.dtype))
+            kv.append((k.to(self.dtype), v.to(self.dtype)))
+        return StateMemory(kv, list(objects_per_state), object_mask)
+
+    @torch.no_grad()
+    def score(self, actions, actions_per_state, memory: StateMemory):
+        r = self.reader
+        plan = decoder.attention_plan(actions_per_state, memory.objects, actions.device)
+        y = r.embed(actions.to(r.embed.weight.dtype)).to(self.dtype)
+        h = torch.zeros_like(y)
+        for block, w, (k, v) in zip(r.blocks, self.blocks, memory.keys_values):
+            x, scale, h = decoder.add_rms_norm_e4m3(y, w["norm_read"], h, eps=EPS)
+            q = decoder.int4_matvec(x, w["query"], x_scale=scale, out_dtype=self.dtype).view(-1, block.heads, block.dim)
+            o = decoder.cross_attention(q, k, v, plan, key_mask=memory.object_mask)
+            y = decoder.int4_matvec(o.reshape(h.shape), w["out"])
+            x, scale, h = decoder.add_rms_norm_e4m3(y, w["norm_mix"], h, eps=EPS)
+            u = block.act(decoder.int4_matvec(x, w["up"], x_scale=scale, out_dtype=self.dtype))
+            y = decoder.int4_matvec(u, w["down"])
+        x, _ = decoder.add_rms_norm(y, self.norm_out, h, eps=EPS)
+        return F.linear(x.to(r.score.weight.dtype), r.score.weight).squeeze(-1)
+
+
+class RelationalPolicy(nn.Module):
+    """A relational model and the reader of its object embeddings."""
+
+    def __init__(self, model: nn.Module, reader: ActionReader):
+        super().__init__()
+        self.model, self.reader = model, reader
+
+    def forward(self, batch: RelationalBatch, actions, plan, object_mask=None):
+        objects, _ = self.model(batch)
+        return self.reader(actions, objects.to(actions.dtype), plan, object_mask)
+
+
+def state_log_probabilities(scores, actions_per_state):
+    """Log softmax of the scores over each state's own actions."""
+
+    parts = [p.log_softmax(0) for p in scores.float().split(list(actions_per_state))]
+    return torch.cat(parts) if parts else scores
+
+
+def main() -> int:
+    from .relational_gnn import RelationalGNN
+    from .workloads import relational_batch
+
+    parser = argparse.ArgumentParser(description=main.__doc__ or __doc__)
+    parser.add_argument("--states", type=int, default=64)
+    parser.add_argument("--steps", type=int, default=30)
+    parser.add_argument("--device", default="cuda" if torch.cuda.is_available() else "cpu")
+    args = parser.parse_args()
+    torch.manual_seed(0)
+    arities = {"p0": 1, "p1": 2, "p2": 3}
+    batch = relational_batch(args.states, 20, arities, 30, seed=0, device=args.device)
+    counts = [3 + (7 * s) % 11 for s in range(args.states)]  # candidate actions of each state
+    actions = torch.randn(sum(counts), 16, device=args.device)
+    best = torch.tensor([sum(counts[:s]) + s % n for s, n in enumerate(counts)], device=args.device)
+    policy = RelationalPolicy(RelationalGNN(64, 3, "sum", arities), ActionReader(16, 64, width=128)).to(args.device)
+    plan = reading_plan(batch, counts)
+    optimizer = torch.optim.AdamW(policy.parameters(), lr=1e-3)
+    for step in range(args.steps):
+        optimizer.zero_grad(set_to_none=True)
+        loss = -state_log_probabilities(policy(batch, actions, plan), counts)[best].mean()
+        loss.backward()
+        optimizer.step()
+        if step % 10 == 0 or step == args.steps - 1:
+            print(f"step {step:3d}  loss {loss.item():.4f}")
+    with torch.no_grad():
+        objects, _ = policy.model(batch)
+        full = policy.reader(actions, objects, plan)
+        served = policy.reader.served()
+        memory = served.remember(objects, objects_per_state(batch))
+        quick = served.score(actions, counts, memory)
+    agree = sum(int(a.argmax() == b.argmax()) for a, b in zip(full.split(counts), quick.split(counts)))
+    print(f"served in 4 and 8 bits: {agree} of {args.states} states choose the same action")
+    return 0
+
+
+if __name__ == "__main__":
+    raise SystemExit(main())

@@ -1,0 +1,145 @@
+"""The action reader: the decoder operators together, in training and served."""
+
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+from relmo_b200 import action_reader as ar
+from relmo_b200.ops import decoder
+from relmo_b200.relational_gnn import RelationalGNN
+from relmo_b200.workloads import relational_batch
+from tests import _decoder_ref as ref
+
+ARITIES = {"p0": 1, "p1": 2}
+COUNTS = [3, 0, 5, 1]
+
+
+def setup(device, dtype=torch.float32):
+    torch.manual_seed(0)
+    batch = relational_batch(4, 9, ARITIES, 12, seed=1, device=device)
+    reader = ar.ActionReader(6, 32, width=64, num_layers=2, heads=4, kv_heads=2, hidden=96).to(device, dtype)
+    actions = torch.randn(sum(COUNTS), 6, generator=torch.Generator().manual_seed(2)).to(device, dtype)
+    objects = torch.randn(36, 32, generator=torch.Generator().manual_seed(3)).to(device, dtype)
+    return batch, reader, actions, objects
+
+
+def plain(reader, actions, objects, counts, per_state, mask=None):
+    """The same model from the formulas, in the parameters' type."""
+
+    y = reader.embed(actions)
+    h = torch.zeros_like(y)
+    for b in reader.blocks:
+        x, h = ref.norm(y, b.norm_read, h, ar.EPS)
+        k, v = b.keys_values(objects)
+        o = ref.attention(b.query(x).view(-1, b.heads, b.dim), k, v, counts, per_state, b.dim**-0.5, mask)
+        x, h = ref.norm(b.out(o.reshape(x.shape)), b.norm_mix, h, ar.EPS)
+        y = b.down(b.act(b.up(x)))
+    return reader.score(ref.norm(y, reader.norm_out, h, ar.EPS)[0]).squeeze(-1)
+
+
+def check_training(device):
+    batch, reader, actions, objects = setup(device)
+    plan = ar.reading_plan(batch, COUNTS)
+    assert ar.objects_per_state(batch) == [9] * 4
+    mask = torch.ones(36, dtype=torch.bool, device=device)
+    mask[::4] = False
+    mask[18:27] = False  # all objects of the third state
+    wide = copy.deepcopy(reader).double()
+    objects.requires_grad_()
+    wide_objects = objects.detach().double().requires_grad_()
+    scores = reader(actions, objects, plan, mask)
+    want = plain(wide, actions.double(), wide_objects, COUNTS, [9] * 4, mask)
+    ref.close(scores.detach(), want.detach(), what="scores")
+    ar.state_log_probabilities(scores, COUNTS)[[0, 4, 8]].sum().backward()
+    torch.cat([p.log_softmax(0) for p in want.split(COUNTS)])[[0, 4, 8]].sum().backward()
+    # float32 through two blocks of four products each: a few times the error of one
+    for (name, p), q in zip(reader.named_parameters(), wide.parameters()):
+        if q.grad is None:
+            continue
+        assert (p.grad.double() - q.grad).norm() <= 1e-4 * max(q.grad.norm(), 1e-3), name
+    assert (objects.grad.double() - wide_objects.grad).norm() <= 1e-4 * wide_objects.grad.norm()
+    assert bool((objects.grad[~mask] == 0).all())
+
+
+def check_served(device, dtype):
+    batch, reader, actions, objects = setup(device, dtype)
+    served = reader.served(32)
+    memory = served.remember(objects, [9] * 4)
+    got = served.score(actions, COUNTS, memory)
+    # few at a time: the same scores
+    parts = [served.score(actions[i:i + 1], [1 if s == b else 0 for b in range(4)], memory)
+             for i, s in enumerate([0, 0, 0, 2, 2, 2, 2, 2, 3])]
+    tol = 0.02  # an 8-bit step more or less in a few of 64 places per norm, and the type's own rounding
+    assert (torch.cat(parts).double() - got.double()).norm() <= tol * got.double().norm()
+    # the same products with the weights that the 4-bit codes stand for, rows in full precision
+    wide = copy.deepcopy(reader).double()
+    eye = lambda k: torch.eye(k, device=device)  # noqa: E731
+    for b, w in zip(wide.blocks, served.blocks):
+        for name, p in (("query", b.query), ("out", b.out), ("up", b.up), ("down", b.down)):
+            p.weight.data = decoder.int4_matvec(eye(w[name].k), w[name]).t().double()
+    want = plain(wide, actions.double(), objects.double(), COUNTS, [9] * 4)
+    # rows in 8 bits: relative steps of 2^-4, half of them at most, some 2^-6 in the root mean square of a row's
+    # products; four such roundings add up to 2^-5 in the sublayers' outputs
+    assert (got.double() - want).norm() <= 2**-4 * want.norm()
+
+
+def test_training_cpu():
+    check_training("cpu")
+
+
+def test_served_cpu():
+    check_served("cpu", torch.float32)
+
+
+def test_policy_learns_cpu():
+    batch, _, actions, _ = setup("cpu")
+    policy = ar.RelationalPolicy(RelationalGNN(32, 2, "sum", ARITIES), ar.ActionReader(6, 32, width=32, num_layers=1, heads=2))
+    plan = ar.reading_plan(batch, COUNTS)
+    opt = torch.optim.AdamW(policy.parameters(), lr=1e-2)
+    losses = []
+    for _ in range(20):
+        opt.zero_grad()
+        loss = -ar.state_log_probabilities(policy(batch, actions, plan), COUNTS)[[1, 4, 8]].mean()
+        loss.backward()
+        opt.step()
+        losses.append(loss.item())
+    assert losses[-1] < 0.5 * losses[0]
+
+
+def test_refusals():
+    with pytest.raises(ValueError, match="must divide"):
+        ar.ReaderBlock(30, 8, 4, 4, 64)
+    with pytest.raises(RuntimeError, match="multiple of group"):
+        ar.ActionReader(4, 8, width=24, heads=2, num_layers=1).served()
+
+
+@pytest.mark.gpu
+def test_training_gpu():
+    check_training("cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_served_gpu(dtype):
+    check_served("cuda", dtype)
+
+
+@pytest.mark.gpu
+def test_policy_step_bf16_autocast():
+    batch, _, actions, _ = setup("cuda")
+    policy = ar.RelationalPolicy(RelationalGNN(32, 2, "sum", ARITIES), ar.ActionReader(6, 32, width=64, num_layers=2)).cuda()
+    plan = ar.reading_plan(batch, COUNTS)
+    opt = torch.optim.AdamW(policy.parameters(), lr=1e-2)
+    losses = []
+    for _ in range(15):
+        opt.zero_grad()
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            scores = policy(batch, actions, plan)
+        loss = -ar.state_log_probabilities(scores, COUNTS)[[1, 4, 8]].mean()
+        loss.backward()
+        opt.step()
+        losses.append(loss.item())
+    assert losses[-1] < 0.7 * losses[0]
