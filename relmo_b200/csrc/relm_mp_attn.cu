@@ -319,7 +319,9 @@ int relm_mp_attn_plan_fill(const int64_t* q_lengths, const int64_t* kv_lengths, 
 size_t relm_mp_cross_attention_workspace_bytes(const relm_mp_attn* attn)
 {
    if(check_attn(attn, "cross_attention") || attn->q_rows == 0) return 0;
-   return use_split(*attn) ? split_plan(make_args(*attn), counts(*attn).kv_blocks, aligned_rows(*attn)).bytes : 0;
+   const Args a = make_args(*attn);
+   if(use_split(*attn)) return split_plan(a, counts(*attn).kv_blocks, aligned_rows(*attn)).bytes;
+   return use_tc(*attn) && !short_keys(*attn) ? tc_parts_bytes(a, tc_parts(a, counts(*attn).q_tiles)) : 0;
 }
 
 int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void* o_rest, void* workspace,
@@ -340,7 +342,7 @@ int relm_mp_cross_attention(const relm_mp_attn* attn, void* o, float* lse, void*
       return short_forward(attn->dtype, a, c.q_tiles, st);
    if(use_tc(*attn) && ((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(a.o_rest)) & 15) == 0) {
       if((rc = gave_up_address(&a.gave_up))) return rc;
-      return tc_forward(attn->dtype, a, c.q_tiles, c.q_pairs, st);
+      return tc_forward(attn->dtype, a, c.q_tiles, c.q_pairs, tc_parts(a, c.q_tiles), workspace, st);
    }
    return warp_forward(attn->dtype, a, c.q_tiles, aligned_any(*attn), st);
 }

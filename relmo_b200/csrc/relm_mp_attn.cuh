@@ -31,6 +31,9 @@ struct Args {
    const void* go; // (o and o_rest are inputs then)
    const float *lse_in, *delta;
    void *dq, *dk, *dv;
+   // forward with the keys in several parts: unnormalised outputs [part, q row, head, dim], (max, sum) [part, head, q row]
+   float* part_o;
+   float2* part_ml;
    int* gave_up; // set by a kernel that gave up waiting
 };
 
@@ -118,7 +121,9 @@ int short_backward(relm_mp_dtype dtype, const Args& a, cudaStream_t st);
 
 // Tensor cores: 2-byte types, dim a multiple of 8 up to 128, rows on 16-byte
 // boundaries (relm_mp_attn_tc.cu).
-int tc_forward(relm_mp_dtype dtype, const Args& a, int64_t tiles, int64_t pairs, cudaStream_t st);
+int tc_parts(const Args& a, int64_t tiles);
+size_t tc_parts_bytes(const Args& a, int parts);
+int tc_forward(relm_mp_dtype dtype, Args a, int64_t tiles, int64_t pairs, int parts, void* workspace, cudaStream_t st);
 // (relm_mp_attn_tc_bwd.cu)
 int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st);
 

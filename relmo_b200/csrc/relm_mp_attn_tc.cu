@@ -123,8 +123,13 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const int row0 = it.tile * QT * kTileRows;
    const int active = QT == 1 || row0 + kTileRows >= qs.len ? 1 : QT;
-   const int tiles = (ks.len + kTileRows - 1) / kTileRows;
-   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+   // This block's part of the keys: whole tiles, all of them where there is one part (always, with two query tiles).
+   const bool whole = QT == 2 || gridDim.z == 1;
+   const int every = (ks.len + kTileRows - 1) / kTileRows;
+   const int tile0 = whole ? 0 : (int)((int64_t)every * blockIdx.z / gridDim.z);
+   const int tiles = whole ? every : (int)((int64_t)every * (blockIdx.z + 1) / gridDim.z) - tile0;
+   const int key0 = tile0 * kTileRows, klen = whole ? ks.len : min(ks.len - key0, tiles * kTileRows);
+   const unsigned char* keep = a.mask ? a.mask + ks.first + key0 : nullptr;
    constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
 
    if(threadIdx.x == 0) {
@@ -156,12 +161,12 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    const uint32_t tmem = tmem_base;
    const uint32_t base = smem_addr(sm);
    // Tiles with keys that take no part: all where there is a mask, else the last if it ends inside.
-   auto dirty = [&](int j) { return keep != nullptr || ks.len - j * kTileRows < kTileRows; };
+   auto dirty = [&](int j) { return keep != nullptr || klen - j * kTileRows < kTileRows; };
    auto dirty_round = [&](int j, int ring) { return keep ? j / ring & 1 : 0; };
 
    if(warp == L::COPY_WARP) {
       if(lane == 0 && tiles > 0) {
-         const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0);
+         const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0) + key0;
          const int b = a.q_off ? 0 : it.seq;
          auto load = [&](uint32_t dst, const CUtensorMap* m, uint64_t* bar, int row, int h) {
             mbar_expect(bar, L::TILE);
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          const int steps = (a.dim + 15) / 16;
          const uint32_t pv = instruction(BF, 128, steps * 16, true);
          const uint32_t pt = tmem + (L::APART ? L::P + t * 64 : t * 128), ot = tmem + L::O + t * DP;
-         auto keys16 = [&](int j) { return min(kTileRows, (ks.len - j * kTileRows + 15) / 16 * 16); };
+         auto keys16 = [&](int j) { return min(kTileRows, (klen - j * kTileRows + 15) / 16 * 16); };
          auto k_ready = [&](int j) { return mbar_wait(&k_full[j % L::ST], (j / L::ST) & 1); };
          auto v_ready = [&](int j) {
             return mbar_wait(&v_full[j % L::ST], (j / L::ST) & 1) && (!dirty(j) || mbar_wait(&v_clean[j % L::ST], dirty_round(j, L::ST)));
@@ -210,7 +215,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             mma_commit(&k_empty[j % L::ST]);
          };
          // The second tile starts half an iteration after the first and stays there: in step, both would take
-         // the exponential unit at once and leave it idle at once (D = 128: 370 us in step, STAGGERED apart).
+         // the exponential unit at once and leave it idle at once (4 x 2048 x 4096, 16 heads of 128: 370 us in step, 331 us half an iteration apart).
          const bool apart = active == 2 && tiles >= 4;
          bool ok = mbar_wait(&q_full[t], 0) && k_ready(0) && (!apart || t == 0 || mbar_wait(&stagger, 0));
          if(ok) scores(0);
@@ -250,7 +255,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
 #pragma unroll
          for(int c = 0; c < 4; ++c) {
             const int key = j * kTileRows + c * 32 + lane;
-            next[c] = key < ks.len && (!keep || keep[key]);
+            next[c] = key < klen && (!keep || keep[key]);
          }
       };
       kept(0);
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       };
       if(t < active) {
          for(int j = 0; j < tiles; ++j) {
-            const int chunks = min(4, (ks.len - j * kTileRows + 31) / 32);
+            const int chunks = min(4, (klen - j * kTileRows + 31) / 32);
             const bool partial = dirty(j);
             const float4* limit = s_limit[keep ? j % kLimitSlots : 0];
             if(partial) ok = ok && __all_sync(~0u, mbar_wait(&limit_full[keep ? j % kLimitSlots : 0], dirty_round(j, kLimitSlots)));
@@ -427,12 +432,32 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             ok = !pair_any(!ok);
             l += s_top[t][h ^ 1][row];
          }
+         const int row_at = row0 + t * kTileRows + row;
+         if(!whole) { // a part: k_attn_tc_join does the rest
+            if(row_at < qs.len) {
+               const int64_t at = (int64_t)blockIdx.z * a.q_rows + qs.first + row_at;
+               if(h == 0) a.part_ml[((int64_t)blockIdx.z * a.heads + head) * a.q_rows + qs.first + row_at] = make_float2(m, ok ? l : CUDART_NAN_F);
+               a.part_o += (at * a.heads + head) * a.dim;
+            }
+            for(int c = 16 * h; c < a.dim; c += 16 * L::HALVES) {
+               uint32_t o[16];
+               if(tiles > 0) {
+                  tmem_ld16(o, ot + c);
+                  wait_ld();
+                  loaded< 16 >(o);
+               }
+#pragma unroll
+               for(int i = 0; i < 16; i += 4)
+                  if(row_at < qs.len && c + i < a.dim)
+                     *reinterpret_cast< uint4* >(a.part_o + c + i) = tiles > 0 ? make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_uint4(0, 0, 0, 0);
+            }
+         }
          // Rows leave through the q tile's shared memory (its products are done), 16 bytes a lane along the rows.
          const bool none = l == 0.f;
          const float inv = none ? 0.f : 1.f / l;
          const int r0 = row0 + t * kTileRows + (warp & 3) * 32;
          unsigned char* stage = sm + L::Q + t * L::TILE + (warp & 3) * 32 * (DP * 2);
-         for(int pass = 0; pass < (a.o_rest ? 2 : 1); ++pass) {
+         for(int pass = 0; whole && pass < (a.o_rest ? 2 : 1); ++pass) {
 #pragma unroll
             for(int c0 = 0; c0 < DP; c0 += 16 * L::HALVES) {
                const int c = c0 + 16 * h;
@@ -470,7 +495,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             if constexpr(L::HALVES == 2) pair_sync();
             else __syncwarp();
          }
-         if(a.lse && h == 0 && r0 + lane < qs.len) {
+         if(whole && a.lse && h == 0 && r0 + lane < qs.len) {
             float v = none ? -CUDART_INF_F : m * kLn2 + logf(l);
             a.lse[(int64_t)head * a.q_rows + qs.first + r0 + lane] = ok ? v : CUDART_NAN_F;
          }
@@ -484,29 +509,82 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
 }
 
+// The parts of a row joined in key order: a warp per row and head.
+template < typename T >
+__global__ void __launch_bounds__(256) k_attn_tc_join(Args a, int parts)
+{
+   const int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), n = a.q_rows * a.heads;
+   const int lane = threadIdx.x & 31;
+   if(i >= n) return;
+   const int64_t row = i / a.heads;
+   const int head = (int)(i % a.heads);
+   auto ml = [&](int p) { return a.part_ml[((int64_t)p * a.heads + head) * a.q_rows + row]; };
+   float M = -CUDART_INF_F, L = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+   for(int p = 0; p < parts; ++p) M = fmaxf(M, ml(p).x);
+   const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll 4
+   for(int p = 0; p < parts; ++p) {
+      const float2 x = ml(p);
+      const float f = exp2_fast(x.x - ref);
+      L += x.y * f;
+#pragma unroll
+      for(int e = 0; e < 4; ++e)
+         if(e * 32 + lane < a.dim) v[e] = fmaf(a.part_o[(p * n + i) * a.dim + e * 32 + lane], f, v[e]);
+   }
+#pragma unroll
+   for(int e = 0; e < 4; ++e) {
+      const int c = e * 32 + lane;
+      if(c >= a.dim) continue;
+      const float x = L == 0.f ? 0.f : v[e] / L;
+      const T y = from_f32< T >(x);
+      static_cast< T* >(a.o)[i * a.dim + c] = y;
+      if(a.o_rest) static_cast< T* >(a.o_rest)[i * a.dim + c] = from_f32< T >(x - to_f32(y));
+   }
+   if(lane == 0 && a.lse) a.lse[(int64_t)head * a.q_rows + row] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
+}
+
 template < typename T, int DP, int QT >
-int launch(const Args& a, const TcMaps& m, int64_t items, cudaStream_t st)
+int launch(const Args& a, const TcMaps& m, int64_t items, int parts, cudaStream_t st)
 {
    using L = Fwd< DP, QT >;
    constexpr int bytes = (int)L::BYTES + 1024;
    static SmemLimit limit;
    int rc = limit((const void*)k_attn_tc_forward< T, DP, QT >, bytes, "k_attn_tc_forward");
    if(rc) return rc;
-   k_attn_tc_forward< T, DP, QT ><<< dim3((unsigned)items, a.heads), L::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
+   k_attn_tc_forward< T, DP, QT ><<< dim3((unsigned)items, a.heads, parts), L::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
    return check_launch("k_attn_tc_forward");
 }
 
 template < typename T >
-int forward(const Args& a, const TcMaps& m, int64_t tiles, int64_t pairs, cudaStream_t st)
+int forward(const Args& a, const TcMaps& m, int64_t tiles, int64_t pairs, int parts, cudaStream_t st)
 {
+   // Two tiles per block share k and v and overlap; one tile per block, two blocks per SM, where most second
+   // tiles would be empty (512 ragged states: 105 us paired, 75 us single) or the pairs leave SMs idle.
    const bool two = 2 * tiles >= 3 * pairs && pairs * a.heads >= 148;
-   if(a.dim <= 64) return two ? launch< T, 64, 2 >(a, m, pairs, st) : launch< T, 64, 1 >(a, m, tiles, st);
-   return two ? launch< T, 128, 2 >(a, m, pairs, st) : launch< T, 128, 1 >(a, m, tiles, st);
+   int rc;
+   if(a.dim <= 64) rc = two ? launch< T, 64, 2 >(a, m, pairs, 1, st) : launch< T, 64, 1 >(a, m, tiles, parts, st);
+   else rc = two ? launch< T, 128, 2 >(a, m, pairs, 1, st) : launch< T, 128, 1 >(a, m, tiles, parts, st);
+   if(rc || two || parts == 1) return rc;
+   k_attn_tc_join< T ><<< (unsigned)ceil_div(a.q_rows * a.heads, 8), 256, 0, st >>>(a, parts);
+   return check_launch("k_attn_tc_join");
 }
 
 }  // namespace
 
-int tc_forward(relm_mp_dtype dtype, const Args& a, int64_t tiles, int64_t pairs, cudaStream_t st)
+// Parts of the keys where the query tiles alone leave most SMs idle: up to two blocks per SM, four tiles each at least.
+int tc_parts(const Args& a, int64_t tiles)
+{
+   const int64_t blocks = std::max< int64_t >(tiles * a.heads, 1);
+   if(blocks >= 148) return 1;
+   return (int)std::max< int64_t >(1, std::min< int64_t >(296 / blocks, ceil_div(a.max_kv, 4 * kTileRows)));
+}
+
+size_t tc_parts_bytes(const Args& a, int parts)
+{
+   return parts == 1 ? 0 : align_up((size_t)parts * a.q_rows * a.heads * 8) + align_up((size_t)parts * a.q_rows * a.heads * a.dim * 4);
+}
+
+int tc_forward(relm_mp_dtype dtype, Args a, int64_t tiles, int64_t pairs, int parts, void* workspace, cudaStream_t st)
 {
    TcMaps m;
    int rc;
@@ -514,7 +592,9 @@ int tc_forward(relm_mp_dtype dtype, const Args& a, int64_t tiles, int64_t pairs,
       (rc = tc_map(&m.k, dtype, a.k, a.ks, a.dim, a.kv_heads, a.kv_off ? a.kv_rows : a.max_kv, a.kv_off ? 1 : a.seqs)) ||
       (rc = tc_map(&m.v, dtype, a.v, a.vs, a.dim, a.kv_heads, a.kv_off ? a.kv_rows : a.max_kv, a.kv_off ? 1 : a.seqs)))
       return rc;
-   return dtype == RELM_MP_BFLOAT16 ? forward< __nv_bfloat16 >(a, m, tiles, pairs, st) : forward< __half >(a, m, tiles, pairs, st);
+   a.part_ml = static_cast< float2* >(workspace);
+   a.part_o = reinterpret_cast< float* >(static_cast< char* >(workspace) + align_up((size_t)parts * a.q_rows * a.heads * 8));
+   return dtype == RELM_MP_BFLOAT16 ? forward< __nv_bfloat16 >(a, m, tiles, pairs, parts, st) : forward< __half >(a, m, tiles, pairs, parts, st);
 }
 
 }  // namespace attn
