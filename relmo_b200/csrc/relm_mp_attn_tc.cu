@@ -32,7 +32,7 @@ namespace {
 using namespace tc;
 
 constexpr float kGrow = 8.f;
-constexpr int kLimitSlots = 4;
+constexpr int kBitSlots = 4;
 
 template < int DP, int QT >
 struct Fwd {
@@ -68,19 +68,12 @@ __device__ __forceinline__ float largest(const uint32_t* s, float top)
    return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
 
-// Masked keys (limit -inf) fall out, the others (limit +inf) stay: the smaller of
-// score and limit is right even for a masked score that is NaN. (A kept one that
-// is NaN becomes +inf, and NaN again when the row's maximum is taken off it.)
-__device__ __forceinline__ void apply_limit(uint32_t* s, const float4* limit)
+// Scores of keys that take no part become -inf, whatever they were.
+__device__ __forceinline__ void hide(uint32_t* s, unsigned bits)
 {
 #pragma unroll
-   for(int i = 0; i < 8; ++i) {
-      const float4 b = limit[i];
-      s[4 * i] = __float_as_uint(fminf(__uint_as_float(s[4 * i]), b.x));
-      s[4 * i + 1] = __float_as_uint(fminf(__uint_as_float(s[4 * i + 1]), b.y));
-      s[4 * i + 2] = __float_as_uint(fminf(__uint_as_float(s[4 * i + 2]), b.z));
-      s[4 * i + 3] = __float_as_uint(fminf(__uint_as_float(s[4 * i + 3]), b.w));
-   }
+   for(int i = 0; i < 32; ++i)
+      if(!(bits >> i & 1)) s[i] = 0xff800000u;
 }
 
 // 32 scores to weights 2^(sc s - ref), added to `sum` unrounded and packed into
@@ -112,8 +105,8 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
    __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
-   __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], limit_full[kLimitSlots], stagger;
-   __shared__ float4 s_limit[kLimitSlots][kTileRows / 4];
+   __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], bits_full[kBitSlots], stagger;
+   __shared__ unsigned s_bits[kBitSlots][4]; // a tile's keys that take part
    __shared__ float s_top[QT][2][L::HALVES == 2 ? kTileRows : 1]; // of the two halves of a row
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
@@ -149,7 +142,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          mbar_init(&k_empty[s], active);     // each query tile's products
          mbar_init(&v_empty[s], active + 1); // and the mask warp
       }
-      for(int s = 0; s < kLimitSlots; ++s) mbar_init(&limit_full[s], 1);
+      for(int s = 0; s < kBitSlots; ++s) mbar_init(&bits_full[s], 1);
       mbar_init(&stagger, 1);
       mbar_init_fence();
       gave_up = 0;
@@ -249,7 +242,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       }
    } else if(warp == L::MASK_WARP) {
       // Follows every tile (so that it never falls a phase behind) and works on those with keys that take no
-      // part: limits for their scores, and zeros in their rows of v, whatever these held.
+      // part: their bits for the softmax, and zeros in their rows of v, whatever these held.
       bool next[4];
       auto kept = [&](int j) {
 #pragma unroll
@@ -265,14 +258,13 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          unsigned bits[4];
          if(work) {
             // The slot was last read for tile j - 4, whose weights were done before v of tile j - 1 arrived.
-            const int slot = keep ? j % kLimitSlots : 0;
+            const int slot = keep ? j % kBitSlots : 0;
 #pragma unroll
             for(int c = 0; c < 4; ++c) {
                bits[c] = __ballot_sync(~0u, next[c]);
-               reinterpret_cast< float* >(s_limit[slot])[c * 32 + lane] = next[c] ? CUDART_INF_F : -CUDART_INF_F;
+               if(lane == 0) s_bits[slot][c] = bits[c];
             }
-            __syncwarp();
-            if(lane == 0) mbar_arrive(&limit_full[slot]);
+            if(lane == 0) mbar_arrive(&bits_full[slot]);
          }
          kept(j + 1); // on its way while v is waited for
          const bool ok = __all_sync(~0u, mbar_wait(&v_full[s], (j / L::ST) & 1));
@@ -321,8 +313,8 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          for(int j = 0; j < tiles; ++j) {
             const int chunks = min(4, (klen - j * kTileRows + 31) / 32);
             const bool partial = dirty(j);
-            const float4* limit = s_limit[keep ? j % kLimitSlots : 0];
-            if(partial) ok = ok && __all_sync(~0u, mbar_wait(&limit_full[keep ? j % kLimitSlots : 0], dirty_round(j, kLimitSlots)));
+            const unsigned* bits = s_bits[keep ? j % kBitSlots : 0];
+            if(partial) ok = ok && __all_sync(~0u, mbar_wait(&bits_full[keep ? j % kBitSlots : 0], dirty_round(j, kBitSlots)));
             ok = ok && __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
             // (Where a wait gave up the loop runs on without waits: the two halves of a row meet at barriers.)
             fence_after();
@@ -339,7 +331,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
 #pragma unroll
                for(int c = 0; c < 2; ++c) {
                   if(2 * h + c >= chunks) continue;
-                  if(partial) apply_limit(s + c * 32, limit + (2 * h + c) * 8);
+                  if(partial) hide(s + c * 32, bits[2 * h + c]);
                   top = largest(s + c * 32, top);
                }
             } else { // two blocks share the registers: the scores are read twice, 32 at a time
@@ -350,7 +342,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   wait_ld();
                   loaded< 32 >(s + (c & 1) * 32);
                   if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
-                  if(partial) apply_limit(s + (c & 1) * 32, limit + c * 8);
+                  if(partial) hide(s + (c & 1) * 32, bits[c]);
                   top = largest(s + (c & 1) * 32, top);
                }
                tmem_ld32(s, st);
@@ -409,7 +401,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                      wait_ld();
                      loaded< 32 >(s + (c & 1) * 32);
                      if(c + 1 < chunks) tmem_ld32(s + (~c & 1) * 32, st + (c + 1) * 32);
-                     if(partial) apply_limit(s + (c & 1) * 32, limit + c * 8);
+                     if(partial) hide(s + (c & 1) * 32, bits[c]);
                      exponents< T >(s + (c & 1) * 32, sc2, ref2, sum);
                      // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
                      tmem_st16(pt + c * 16, s + (c & 1) * 32);
