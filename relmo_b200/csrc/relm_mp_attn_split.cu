@@ -246,20 +246,27 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split(SplitArgs s)
 }
 
 // The same on the CUDA cores, in float32 throughout: float32 inputs, and 2-byte
-// ones whose rows are not on 16-byte boundaries. 16 keys a step and warp: two
-// lanes per key for the scores (each half of the row, from shared memory; the
-// query rows are broadcast), then the lanes share the output's columns. R: query
-// rows held in registers.
+// ones whose rows are not on 16-byte boundaries. Each step and warp has 16 (wide
+// rows: 8) keys: two (four) lanes per key for the scores, in turn over the row's
+// 16-byte pieces (row pitch such that 8 lanes read different banks; the query rows
+// are broadcast), then the lanes share the output's columns. R: query rows held in
+// registers.
+template < int DP >
+struct Wide {
+   static constexpr int CHUNK = DP > 64 ? 8 : 16, PER = 32 / CHUNK, LD = DP + 4 * PER, STAGES = DP > 32 ? 2 : 3;
+   static constexpr uint32_t TILE = CHUNK * LD * 4, STAGE = 2 * TILE;
+   static constexpr size_t BYTES = (size_t)kWarps * STAGES * STAGE;
+};
 template < typename T, int DP, int R >
 __global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool aligned)
 {
    const Args& a = s.a;
-   constexpr int VEC = DP / 32, LD = DP + 4; // output columns of a lane; floats of a row in shared memory
-   constexpr uint32_t TILE = kChunk * LD * 4, STAGE = 2 * TILE;
-   constexpr int STAGES = DP > 128 ? 1 : 3; // (wide rows: what shared memory holds)
+   using W = Wide< DP >;
+   constexpr int VEC = DP / 32, LD = W::LD, STAGES = W::STAGES, CHUNK = W::CHUNK, PER = W::PER; // VEC: output columns of a lane
+   constexpr uint32_t TILE = W::TILE, STAGE = W::STAGE;
    extern __shared__ __align__(128) unsigned char smem[];
-   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_p[kWarps][R][kChunk], sm_q[R][DP];
-   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, key_lane = lane >> 1, half = lane & 1;
+   __shared__ float sm_m[kWarps][R], sm_l[kWarps][R], sm_p[kWarps][R][CHUNK], sm_q[R][DP];
+   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, key_lane = lane / PER, part = lane % PER;
    const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, row0 = blockIdx.z * R;
    unsigned char* const mine = smem + warp * (STAGES * STAGE);
    const uint32_t base = (uint32_t)__cvta_generic_to_shared(mine);
@@ -299,13 +306,13 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool
 #pragma unroll
          for(int v = 0; v < VEC; ++v) o[r][v] = 0.f;
       }
-      const int steps = key_hi > key_lo + warp * kChunk ? (key_hi - key_lo - warp * kChunk + kChunk * kWarps - 1) / (kChunk * kWarps) : 0;
+      const int steps = key_hi > key_lo + warp * CHUNK ? (key_hi - key_lo - warp * CHUNK + CHUNK * kWarps - 1) / (CHUNK * kWarps) : 0;
       auto issue = [&](int step, int stage) {
          if(step < steps) {
-            const int key0 = key_lo + (step * kWarps + warp) * kChunk;
+            const int key0 = key_lo + (step * kWarps + warp) * CHUNK;
             if(std::is_same< T, float >::value && aligned) {
                constexpr int CH = DP / 4;
-               for(int i = lane; i < kChunk * CH; i += 32) {
+               for(int i = lane; i < CHUNK * CH; i += 32) {
                   const int r = i / CH, c = i % CH;
                   const bool in = key0 + r < key_hi && c * 4 < a.dim;
                   const int64_t key = in ? key0 + r : 0;
@@ -315,7 +322,7 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool
                }
             } else {
                float* to = reinterpret_cast< float* >(mine + stage * STAGE);
-               for(int i = lane; i < kChunk * DP; i += 32) {
+               for(int i = lane; i < CHUNK * DP; i += 32) {
                   const int r = i / DP, c = i % DP;
                   const bool in = key0 + r < key_hi && c < a.dim;
                   to[r * LD + c] = in ? to_f32(kp[(int64_t)(key0 + r) * a.ks[1] + c]) : 0.f;
@@ -332,13 +339,13 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool
          __syncwarp();
          const float* sk = reinterpret_cast< const float* >(mine + stage * STAGE);
          const float* sv = sk + TILE / 4;
-         const int key = key_lo + (step * kWarps + warp) * kChunk + key_lane;
+         const int key = key_lo + (step * kWarps + warp) * CHUNK + key_lane;
          const bool in = key < key_hi && (!keep || keep[key]);
          float c[R];
 #pragma unroll
          for(int r = 0; r < R; ++r) c[r] = 0.f;
 #pragma unroll 4
-         for(int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 4) {
+         for(int d = part * 4; d < DP; d += 4 * PER) {
             const float4 k = *reinterpret_cast< const float4* >(sk + key_lane * LD + d);
 #pragma unroll
             for(int r = 0; r < R; ++r) {
@@ -346,14 +353,15 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool
                c[r] = fmaf(k.x, q.x, fmaf(k.y, q.y, fmaf(k.z, q.z, fmaf(k.w, q.w, c[r]))));
             }
          }
-         const unsigned bits = __ballot_sync(~0u, in); // bit 2 j: key j
+         const unsigned bits = __ballot_sync(~0u, in); // bit PER j: key j
 #pragma unroll
          for(int r = 0; r < R; ++r) {
-            c[r] += __shfl_xor_sync(~0u, c[r], 1);
+#pragma unroll
+            for(int x = 1; x < PER; x <<= 1) c[r] += __shfl_xor_sync(~0u, c[r], x);
             c[r] = in ? c[r] * sc : -CUDART_INF_F;
             float top = c[r];
 #pragma unroll
-            for(int x = 2; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+            for(int x = PER; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
             if(top > m[r]) {
                const float f = exp2_fast(m[r] - top);
                m[r] = top;
@@ -362,15 +370,15 @@ __global__ void __launch_bounds__(kThreads4) k_attn_split_wide(SplitArgs s, bool
                for(int v = 0; v < VEC; ++v) o[r][v] *= f;
             }
             const float p = exp2_fast(c[r] - (m[r] == -CUDART_INF_F ? 0.f : m[r]));
-            if(half == 0) {
+            if(part == 0) {
                l[r] += p;
                sm_p[warp][r][key_lane] = p;
             }
          }
          __syncwarp();
 #pragma unroll 4
-         for(int j = 0; j < kChunk; ++j) {
-            if(!(bits >> (2 * j) & 1)) continue; // what a masked row holds is not read
+         for(int j = 0; j < CHUNK; ++j) {
+            if(!(bits >> (PER * j) & 1)) continue; // what a masked row holds is not read
             float v[VEC];
 #pragma unroll
             for(int e = 0; e < VEC; ++e) v[e] = sv[j * LD + e * 32 + lane];
@@ -505,7 +513,7 @@ int launch(const SplitArgs& s, cudaStream_t st)
 template < typename T, int DP, int R >
 int launch_wide(const SplitArgs& s, bool aligned, cudaStream_t st)
 {
-   constexpr size_t bytes = (size_t)kWarps * (DP > 128 ? 1 : 3) * 2 * kChunk * (DP + 4) * 4;
+   constexpr size_t bytes = Wide< DP >::BYTES;
    static SmemLimit limit;
    int rc = limit((const void*)k_attn_split_wide< T, DP, R >, bytes, "k_attn_split_wide");
    if(rc) return rc;
@@ -538,15 +546,16 @@ int launch_dim(const SplitArgs& s, bool aligned, cudaStream_t st)
 
 }  // namespace
 
-// Parts: one wave of resident blocks (shared memory allows about 200 KB per SM),
+// Parts: one wave of resident blocks (shared memory allows about 224 KB per SM),
 // but at least 4 key blocks each, so that a part has work for every warp's pipeline.
 SplitPlan split_plan(const Args& a, int64_t blocks, bool two_bytes)
 {
    const int dp = padded_dim(a.dim);
    SplitPlan p;
    p.row_groups = (int)ceil_div(a.max_q * (a.heads / a.kv_heads), kRows);
-   const int64_t row = two_bytes ? dp * 2 : (dp + 4) * 4, stages = !two_bytes && dp > 128 ? 1 : kStages;
-   const int64_t resident = std::max< int64_t >(1, std::min< int64_t >(8, 200 * 1024 / (kWarps * stages * 2 * kChunk * row)));
+   const int64_t wide = dp == 32 ? Wide< 32 >::BYTES : dp == 64 ? Wide< 64 >::BYTES : dp == 128 ? Wide< 128 >::BYTES : Wide< 256 >::BYTES;
+   const int64_t bytes = two_bytes ? kWarps * kStages * 2 * kChunk * dp * 2 : wide;
+   const int64_t resident = std::max< int64_t >(1, std::min< int64_t >(8, 224 * 1024 / bytes));
    const int64_t slots = 148 * resident / (a.kv_heads * p.row_groups);
    p.parts = (int)std::max< int64_t >(1, std::min(slots, ceil_div(blocks, 4)));
    const size_t rows = p.parts == 1 ? 0 : (size_t)(p.parts + a.seqs) * a.kv_heads * p.row_groups * kRows;
