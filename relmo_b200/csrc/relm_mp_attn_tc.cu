@@ -96,6 +96,49 @@ __device__ __forceinline__ void exponents(uint32_t* s, uint64_t sc, uint64_t ref
    }
 }
 
+// 32 rows of O, one per lane (TMEM `acc`), divided and rounded, to o (and what rounding took, to o_rest)
+// through `stage`, 16 bytes a lane along the rows.
+template < typename T, int DP >
+__device__ __forceinline__ void store_output(uint32_t acc, bool any, bool ok, float inv, bool none, unsigned char* stage, const Args& a,
+                                             const Seq& qs, int head, int r0)
+{
+   const int lane = threadIdx.x & 31;
+   for(int pass = 0; pass < (a.o_rest ? 2 : 1); ++pass) {
+#pragma unroll
+      for(int c = 0; c < DP; c += 16) {
+         if(c >= a.dim) break;
+         uint32_t o[16], w[8];
+         if(any) {
+            tmem_ld16(o, acc + c);
+            wait_ld();
+            loaded< 16 >(o);
+         }
+#pragma unroll
+         for(int i = 0; i < 8; ++i) {
+            float x = !any || none ? 0.f : __uint_as_float(o[2 * i]) * inv, y = !any || none ? 0.f : __uint_as_float(o[2 * i + 1]) * inv;
+            if(!ok) x = y = CUDART_NAN_F; // a wait gave up: nothing here is a result
+            w[i] = pack2< T >(x, y);
+            if(pass) w[i] = pack2< T >(x - low2< T >(w[i]), y - high2< T >(w[i]));
+         }
+#pragma unroll
+         for(int k = 0; k < 2; ++k)
+            *reinterpret_cast< uint4* >(stage + lane * (DP * 2) + (((c >> 3) + k) ^ (lane & 7)) * 16) =
+               make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+      }
+      __syncwarp();
+      T* out = static_cast< T* >(pass ? a.o_rest : a.o);
+      constexpr int CH = DP / 8;
+#pragma unroll 4
+      for(int i = lane; i < 32 * CH; i += 32) {
+         const int r = i / CH, c = i % CH;
+         if(r0 + r < qs.len && c * 8 < a.dim)
+            *reinterpret_cast< uint4* >(out + ((qs.first + r0 + r) * a.heads + head) * a.dim + c * 8) =
+               *reinterpret_cast< const uint4* >(stage + r * (DP * 2) + ((c ^ (r & 7)) * 16));
+      }
+      __syncwarp();
+   }
+}
+
 template < typename T, int DP, int QT >
 __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    k_attn_tc_forward(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
@@ -501,6 +544,269 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
 }
 
+// Head dims up to 64: four query tiles per block against key tiles of 64. Per score
+// there is half the product work of wider heads and the same softmax, so the waits
+// of a tile's chain (scores, load, weights, store, product) are what costs; four
+// chains, started in turn by one products thread, fill them, and with 64 keys a
+// thread has a whole row: nothing is exchanged between threads. Tensor memory:
+// four S tiles (weights over their first half) and four O tiles.
+struct Quad {
+   static constexpr int QT = 4, KN = 64, ST = 4, BITS = 8; // stages of k and of v; slots of mask bits
+   static constexpr uint32_t Q_TILE = kTileRows * 128, K_TILE = KN * 128;
+   static constexpr uint32_t Q = 0, K = QT * Q_TILE, V = K + ST * K_TILE, BYTES = V + ST * K_TILE;
+   static constexpr uint32_t COLS = 512, O = QT * KN;
+   static constexpr int MMA_WARP = QT * 4, COPY_WARP = MMA_WARP + 1, MASK_WARP = COPY_WARP + 1, THREADS = (MASK_WARP + 1) * 32;
+};
+
+template < typename T >
+__global__ void __launch_bounds__(Quad::THREADS, 1)
+   k_attn_tc_forward_quad(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                          const __grid_constant__ CUtensorMap vm)
+{
+   using L = Quad;
+   constexpr int DP = 64, KN = L::KN;
+   constexpr bool BF = std::is_same< T, __nv_bfloat16 >::value;
+   extern __shared__ unsigned char raw[];
+   __shared__ uint64_t q_full[L::QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
+   __shared__ uint64_t s_full[L::QT], p_full[L::QT], pv_done[L::QT], drain, bits_full[L::BITS];
+   __shared__ unsigned s_bits[L::BITS][2];
+   __shared__ uint32_t tmem_base;
+   __shared__ int gave_up;
+   // The pairs' list serves: the n tiles of a sequence go evenly to the first ceil(n / 4) of its ceil(n / 2) items.
+   const Item it = item(a.q_pairs, a.max_q, 2 * kTileRows, blockIdx.x);
+   const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
+   const int q_tiles = (qs.len + kTileRows - 1) / kTileRows, blocks = (q_tiles + L::QT - 1) / L::QT;
+   if(it.tile >= blocks) return;
+   const int tile0 = (int)((int64_t)q_tiles * it.tile / blocks), active = (int)((int64_t)q_tiles * (it.tile + 1) / blocks) - tile0;
+   const int row0 = tile0 * kTileRows;
+   unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+   const int tiles = (ks.len + KN - 1) / KN;
+   const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+
+   if(threadIdx.x == 0) {
+      for(int t = 0; t < L::QT; ++t) {
+         mbar_init(&q_full[t], 1);
+         mbar_init(&s_full[t], 1);
+         mbar_init(&p_full[t], 128);
+         mbar_init(&pv_done[t], 1);
+      }
+      for(int s = 0; s < L::ST; ++s) {
+         mbar_init(&k_full[s], 1);
+         mbar_init(&k_empty[s], 1);
+         mbar_init(&v_full[s], 1);
+         mbar_init(&v_empty[s], 2); // products and the mask warp
+         mbar_init(&v_clean[s], 1);
+      }
+      for(int s = 0; s < L::BITS; ++s) mbar_init(&bits_full[s], 1);
+      mbar_init(&drain, 1);
+      mbar_init_fence();
+      gave_up = 0;
+   }
+   if(warp == L::MMA_WARP) tmem_alloc(&tmem_base, L::COLS);
+   fence_before();
+   __syncthreads();
+   fence_after();
+   const uint32_t tmem = tmem_base, base = smem_addr(sm);
+   // Tiles with keys that take no part: all where there is a mask, else the last if it ends inside.
+   auto dirty = [&](int j) { return keep != nullptr || ks.len - j * KN < KN; };
+   auto dirty_round = [&](int j, int ring) { return keep ? j / ring & 1 : 0; };
+
+   if(warp == L::COPY_WARP) {
+      if(lane == 0 && tiles > 0) {
+         const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0), b = a.q_off ? 0 : it.seq;
+         for(int t = 0; t < active; ++t) {
+            mbar_expect(&q_full[t], L::Q_TILE);
+            tma_load(base + L::Q + t * L::Q_TILE, &qm, &q_full[t], 0, qr + t * kTileRows, head, b);
+         }
+         bool ok = true;
+         int issued = 0;
+         for(int j = 0; j < tiles; ++j) {
+            const int s = j % L::ST, round = j / L::ST;
+            if(round && !(ok = mbar_wait(&k_empty[s], (round - 1) & 1) && mbar_wait(&v_empty[s], (round - 1) & 1))) break;
+            mbar_expect(&k_full[s], L::K_TILE);
+            tma_load(base + L::K + s * L::K_TILE, &km, &k_full[s], 0, kr + j * KN, kv_head, b);
+            mbar_expect(&v_full[s], L::K_TILE);
+            tma_load(base + L::V + s * L::K_TILE, &vm, &v_full[s], 0, kr + j * KN, kv_head, b);
+            issued = j + 1;
+         }
+         if(!ok) { // nothing may still be written to shared memory when the block ends
+            gave_up = 1;
+            for(int t = 0; t < active; ++t) mbar_wait(&q_full[t], 0);
+            for(int j = issued > L::ST ? issued - L::ST : 0; j < issued; ++j) {
+               mbar_wait(&k_full[j % L::ST], (j / L::ST) & 1);
+               mbar_wait(&v_full[j % L::ST], (j / L::ST) & 1);
+            }
+         }
+      }
+   } else if(warp == L::MMA_WARP) {
+      if(elect_one() && tiles > 0) {
+         const int steps = (a.dim + 15) / 16;
+         const uint32_t pv = instruction(BF, 128, steps * 16, true);
+         auto keys16 = [&](int j) { return min(KN, (ks.len - j * KN + 15) / 16 * 16); };
+         auto scores = [&](int t, int j) {
+            product_columns< DP, kTileRows, KN >(tmem + t * KN, base + L::Q + t * L::Q_TILE, base + L::K + (j % L::ST) * L::K_TILE,
+                                                 instruction(BF, 128, keys16(j), false), steps);
+            mma_commit(&s_full[t]);
+         };
+         bool ok = mbar_wait(&k_full[0], 0);
+         for(int t = 0; t < active && ok; ++t) {
+            ok = mbar_wait(&q_full[t], 0);
+            if(ok) scores(t, 0);
+         }
+         if(ok) mma_commit(&k_empty[0]);
+         for(int j = 0; j < tiles && ok; ++j) {
+            const int s = j % L::ST, n = keys16(j) / 16;
+            if(!(ok = mbar_wait(&v_full[s], (j / L::ST) & 1) && (!dirty(j) || mbar_wait(&v_clean[s], dirty_round(j, L::ST))))) break;
+            if(j + 1 < tiles && !(ok = mbar_wait(&k_full[(j + 1) % L::ST], ((j + 1) / L::ST) & 1))) break;
+            for(int t = 0; t < active; ++t) {
+               if(!(ok = mbar_wait(&p_full[t], j & 1))) break;
+               fence_after();
+               product_rows< 0, 4, 0, KN >(tmem + L::O + t * DP, tmem + t * KN, base + L::V + s * L::K_TILE, pv, n, j > 0);
+               if(j + 1 < tiles) scores(t, j + 1);
+               else mma_commit(&pv_done[t]);
+            }
+            if(!ok) break;
+            mma_commit(&v_empty[s]);
+            if(j + 1 < tiles) mma_commit(&k_empty[(j + 1) % L::ST]);
+         }
+         if(!ok) {
+            gave_up = 1;
+            mma_commit(&drain); // products in flight read shared and tensor memory: wait for them before the block ends
+            mbar_wait(&drain, 0);
+         }
+      }
+   } else if(warp == L::MASK_WARP) {
+      // Follows every tile (so that it never falls a phase behind) and works on those with keys that take no
+      // part: their bits for the softmax, and zeros in their rows of v, whatever these held.
+      bool next[2];
+      auto kept = [&](int j) {
+#pragma unroll
+         for(int c = 0; c < 2; ++c) {
+            const int key = j * KN + c * 32 + lane;
+            next[c] = key < ks.len && (!keep || keep[key]);
+         }
+      };
+      kept(0);
+      for(int j = 0; j < tiles; ++j) {
+         const int s = j % L::ST;
+         const bool work = dirty(j);
+         unsigned bits[2] = {0, 0};
+         if(work) {
+            // The slot was last read for tile j - 8, whose weights were done before v of tile j - 1 arrived.
+            const int slot = keep ? j % L::BITS : 0;
+#pragma unroll
+            for(int c = 0; c < 2; ++c) {
+               bits[c] = __ballot_sync(~0u, next[c]);
+               if(lane == 0) s_bits[slot][c] = bits[c];
+            }
+            if(lane == 0) mbar_arrive(&bits_full[slot]);
+         }
+         kept(j + 1); // on its way while v is waited for
+         if(!__all_sync(~0u, mbar_wait(&v_full[s], (j / L::ST) & 1))) {
+            gave_up = 1;
+            break;
+         }
+         if(work) {
+#pragma unroll
+            for(int c = 0; c < 2; ++c)
+               if(!(bits[c] >> lane & 1)) {
+                  uint4* line = reinterpret_cast< uint4* >(sm + L::V + s * L::K_TILE + (c * 32 + lane) * 128);
+#pragma unroll
+                  for(int i = 0; i < 8; ++i) line[i] = make_uint4(0, 0, 0, 0);
+               }
+            fence_async_proxy();
+            __syncwarp();
+         }
+         if(lane == 0) {
+            if(work) mbar_arrive(&v_clean[s]);
+            mbar_arrive(&v_empty[s]);
+         }
+      }
+   } else if(warp >> 2 < active) { // softmax: thread = row of tile t
+      const int t = warp >> 2;
+      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), st = lanes + t * KN, ot = lanes + L::O + t * DP;
+      const float sc = a.scale * kLog2e;
+      const uint64_t sc2 = pair(sc, sc);
+      float m = -CUDART_INF_F;
+      uint64_t sum[2] = {0, 0};
+      bool ok = true;
+      for(int j = 0; j < tiles && ok; ++j) {
+         const int left = ks.len - j * KN;
+         const bool partial = dirty(j);
+         const int slot = keep ? j % L::BITS : 0;
+         if(partial) ok = __all_sync(~0u, mbar_wait(&bits_full[slot], dirty_round(j, L::BITS)));
+         ok = ok && __all_sync(~0u, mbar_wait(&s_full[t], j & 1));
+         if(!ok) break;
+         fence_after();
+         uint32_t s[64];
+         float top = -CUDART_INF_F;
+#pragma unroll
+         for(int c = 0; c < 2; ++c)
+            if(c * 32 < left) tmem_ld32(s + c * 32, st + c * 32);
+         wait_ld();
+         loaded< 64 >(s);
+#pragma unroll
+         for(int c = 0; c < 2; ++c) {
+            if(c * 32 >= left) continue;
+            if(partial) hide(s + c * 32, s_bits[slot][c]);
+            top = largest(s + c * 32, top);
+         }
+         top *= sc;
+         const bool grew = top > m + kGrow || (m == -CUDART_INF_F && top > m);
+         if(__any_sync(~0u, grew)) {
+            float f = 1.f;
+            if(grew) {
+               f = exp2_fast(m - top);
+               m = top;
+               sum[0] = mul2(sum[0], pair(f, f));
+               sum[1] = mul2(sum[1], pair(f, f));
+            }
+            if(j > 0) { // the products into O so far were done before this S
+               for(int c = 0; c < a.dim; c += 16) {
+                  uint32_t o[16];
+                  tmem_ld16(o, ot + c);
+                  wait_ld();
+                  loaded< 16 >(o);
+#pragma unroll
+                  for(int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_st16(ot + c, o);
+               }
+            }
+         }
+         const float ref = m == -CUDART_INF_F ? 0.f : m;
+         const uint64_t ref2 = pair(-ref, -ref);
+#pragma unroll
+         for(int c = 0; c < 2; ++c) {
+            if(c * 32 >= left) continue;
+            exponents< T >(s + c * 32, sc2, ref2, sum);
+            tmem_st16(st + c * 16, s + c * 32);
+         }
+         wait_st();
+         fence_before();
+         mbar_arrive(&p_full[t]);
+      }
+      float l, l1;
+      unpair(add2(sum[0], sum[1]), l, l1);
+      l += l1;
+      if(ok && tiles > 0) ok = __all_sync(~0u, mbar_wait(&pv_done[t], 0));
+      fence_after();
+      const bool none = l == 0.f;
+      const int r0 = row0 + t * kTileRows + (warp & 3) * 32;
+      unsigned char* stage = sm + L::Q + t * L::Q_TILE + (warp & 3) * 32 * 128;
+      store_output< T, DP >(ot, tiles > 0, ok, none ? 0.f : 1.f / l, none, stage, a, qs, head, r0);
+      if(a.lse && r0 + lane < qs.len)
+         a.lse[(int64_t)head * a.q_rows + qs.first + r0 + lane] = !ok ? CUDART_NAN_F : none ? -CUDART_INF_F : m * kLn2 + logf(l);
+      if(!ok) gave_up = 1;
+   }
+   fence_before();
+   __syncthreads();
+   fence_after();
+   if(warp == L::MMA_WARP) tmem_free(tmem, L::COLS);
+   if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
+}
+
 // The parts of a row joined in key order: a warp per row and head.
 template < typename T >
 __global__ void __launch_bounds__(256) k_attn_tc_join(Args a, int parts)
@@ -535,6 +841,17 @@ __global__ void __launch_bounds__(256) k_attn_tc_join(Args a, int parts)
    if(lane == 0 && a.lse) a.lse[(int64_t)head * a.q_rows + row] = L == 0.f ? -CUDART_INF_F : M * kLn2 + logf(L);
 }
 
+template < typename T >
+int launch_quad(const Args& a, const TcMaps& m, int64_t pairs, cudaStream_t st)
+{
+   constexpr int bytes = (int)Quad::BYTES + 1024;
+   static SmemLimit limit;
+   const int rc = limit((const void*)k_attn_tc_forward_quad< T >, bytes, "k_attn_tc_forward_quad");
+   if(rc) return rc;
+   k_attn_tc_forward_quad< T ><<< dim3((unsigned)pairs, a.heads), Quad::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
+   return check_launch("k_attn_tc_forward_quad");
+}
+
 template < typename T, int DP, int QT >
 int launch(const Args& a, const TcMaps& m, int64_t items, int parts, cudaStream_t st)
 {
@@ -548,13 +865,10 @@ int launch(const Args& a, const TcMaps& m, int64_t items, int parts, cudaStream_
 }
 
 template < typename T >
-int forward(const Args& a, const TcMaps& m, int64_t tiles, int64_t pairs, int parts, cudaStream_t st)
+int forward(const Args& a, const TcMaps& m, int64_t tiles, int64_t pairs, int parts, bool two, cudaStream_t st)
 {
-   // Two tiles per block share k and v and overlap; one tile per block, two blocks per SM, where most second
-   // tiles would be empty (512 ragged states: 105 us paired, 75 us single) or the pairs leave SMs idle.
-   const bool two = 2 * tiles >= 3 * pairs && pairs * a.heads >= 148;
    int rc;
-   if(a.dim <= 64) rc = two ? launch< T, 64, 2 >(a, m, pairs, 1, st) : launch< T, 64, 1 >(a, m, tiles, parts, st);
+   if(a.dim <= 64) rc = two ? launch_quad< T >(a, m, pairs, st) : launch< T, 64, 1 >(a, m, tiles, parts, st);
    else rc = two ? launch< T, 128, 2 >(a, m, pairs, 1, st) : launch< T, 128, 1 >(a, m, tiles, parts, st);
    if(rc || two || parts == 1) return rc;
    k_attn_tc_join< T ><<< (unsigned)ceil_div(a.q_rows * a.heads, 8), 256, 0, st >>>(a, parts);
@@ -578,15 +892,19 @@ size_t tc_parts_bytes(const Args& a, int parts)
 
 int tc_forward(relm_mp_dtype dtype, Args a, int64_t tiles, int64_t pairs, int parts, void* workspace, cudaStream_t st)
 {
+   // Two tiles per block share k and v and overlap; one tile per block, two blocks per SM, where most second
+   // tiles would be empty (512 ragged states: 105 us paired, 75 us single) or the pairs leave SMs idle.
+   const bool two = 2 * tiles >= 3 * pairs && pairs * a.heads >= 148;
+   const int key_box = two && a.dim <= 64 ? Quad::KN : kTileRows;
    TcMaps m;
    int rc;
    if((rc = tc_map(&m.q, dtype, a.q, a.qs, a.dim, a.heads, a.q_off ? a.q_rows : a.max_q, a.q_off ? 1 : a.seqs)) ||
-      (rc = tc_map(&m.k, dtype, a.k, a.ks, a.dim, a.kv_heads, a.kv_off ? a.kv_rows : a.max_kv, a.kv_off ? 1 : a.seqs)) ||
-      (rc = tc_map(&m.v, dtype, a.v, a.vs, a.dim, a.kv_heads, a.kv_off ? a.kv_rows : a.max_kv, a.kv_off ? 1 : a.seqs)))
+      (rc = tc_map(&m.k, dtype, a.k, a.ks, a.dim, a.kv_heads, a.kv_off ? a.kv_rows : a.max_kv, a.kv_off ? 1 : a.seqs, key_box)) ||
+      (rc = tc_map(&m.v, dtype, a.v, a.vs, a.dim, a.kv_heads, a.kv_off ? a.kv_rows : a.max_kv, a.kv_off ? 1 : a.seqs, key_box)))
       return rc;
    a.part_ml = static_cast< float2* >(workspace);
    a.part_o = reinterpret_cast< float* >(static_cast< char* >(workspace) + align_up((size_t)parts * a.q_rows * a.heads * 8));
-   return dtype == RELM_MP_BFLOAT16 ? forward< __nv_bfloat16 >(a, m, tiles, pairs, parts, st) : forward< __half >(a, m, tiles, pairs, parts, st);
+   return dtype == RELM_MP_BFLOAT16 ? forward< __nv_bfloat16 >(a, m, tiles, pairs, parts, two, st) : forward< __half >(a, m, tiles, pairs, parts, two, st);
 }
 
 }  // namespace attn
