@@ -40,13 +40,10 @@ struct Fwd {
    static constexpr int PANELS = DP / 64;
    static constexpr uint32_t PANEL = kTileRows * 128, TILE = PANELS * PANEL;
    static constexpr uint32_t Q = 0, K = QT * TILE, V = K + ST * TILE, BYTES = V + ST * TILE;
-   // Tensor memory: S tiles, O tiles and, where there is room, weights of their own
-   // (the next S can then be computed while this one is turned into weights).
-   static constexpr bool APART = QT == 2 && DP == 64;
-   static constexpr uint32_t COLS = QT == 2 ? 512 : 256, O = QT * 128, P = APART ? O + QT * DP : 0;
+   static constexpr uint32_t COLS = QT == 2 ? 512 : 256, O = QT * 128; // tensor memory: S tiles, then O tiles
    // Threads of a row: two tiles have the registers for a thread per half row, and with four
    // softmax warps per scheduler the waits of one are filled by others.
-   static constexpr int HALVES = QT == 2 ? 2 : 1, SOFT = 128 * HALVES;
+   static constexpr int HALVES = QT == 2 ? 2 : 1;
    static constexpr int MMA_WARP = QT * 4 * HALVES, COPY_WARP = MMA_WARP + QT, MASK_WARP = COPY_WARP + 1, THREADS = (MASK_WARP + 1) * 32;
 };
 
@@ -148,7 +145,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    extern __shared__ unsigned char raw[];
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
    __shared__ uint64_t q_full[QT], k_full[L::ST], k_empty[L::ST], v_full[L::ST], v_empty[L::ST], v_clean[L::ST];
-   __shared__ uint64_t s_full[QT], s_free[QT], p_full[QT][2], pv_done[QT], drain[QT], bits_full[kBitSlots], stagger;
+   __shared__ uint64_t s_full[QT], p_full[QT][2], pv_done[QT], drain[QT], bits_full[kBitSlots], stagger;
    __shared__ unsigned s_bits[kBitSlots][4]; // a tile's keys that take part
    __shared__ float s_top[QT][2][L::HALVES == 2 ? kTileRows : 1]; // of the two halves of a row
    __shared__ uint32_t tmem_base;
@@ -172,7 +169,6 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       for(int t = 0; t < QT; ++t) {
          mbar_init(&q_full[t], 1);
          mbar_init(&s_full[t], 1);
-         mbar_init(&s_free[t], L::SOFT);
          mbar_init(&p_full[t][0], 128);
          mbar_init(&p_full[t][1], 128);
          mbar_init(&pv_done[t], 1);
@@ -238,7 +234,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
       if(elect_one() && tiles > 0 && t < active) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t pv = instruction(BF, 128, steps * 16, true);
-         const uint32_t pt = tmem + (L::APART ? L::P + t * 64 : t * 128), ot = tmem + L::O + t * DP;
+         const uint32_t pt = tmem + t * 128, ot = tmem + L::O + t * DP;
          auto keys16 = [&](int j) { return min(kTileRows, (klen - j * kTileRows + 15) / 16 * 16); };
          auto k_ready = [&](int j) { return mbar_wait(&k_full[j % L::ST], (j / L::ST) & 1); };
          auto v_ready = [&](int j) {
@@ -252,15 +248,10 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
          };
          // The second tile starts half an iteration after the first and stays there: in step, both would take
          // the exponential unit at once and leave it idle at once (4 x 2048 x 4096, 16 heads of 128: 370 us in step, 331 us half an iteration apart).
-         const bool apart = active == 2 && tiles >= 4;
+         const bool apart = active == 2 && tiles >= 4; // (the barrier is for them alone)
          bool ok = mbar_wait(&q_full[t], 0) && k_ready(0) && (!apart || t == 0 || mbar_wait(&stagger, 0));
          if(ok) scores(0);
          for(int j = 0; j < tiles && ok; ++j) {
-            if(L::APART && j + 1 < tiles) { // the scores have been read: the next ones
-               if(!(ok = mbar_wait(&s_free[t], j & 1) && k_ready(j + 1))) break;
-               fence_after();
-               scores(j + 1);
-            }
             const int n = keys16(j) / 16;
             const uint32_t va = base + L::V + (j % L::ST) * L::TILE;
             // The weights come in two halves of 64 keys.
@@ -272,7 +263,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             product_rows< 4, 4, 0, kTileRows >(ot, pt, va, pv, n, true);
             mma_commit(&pv_done[t]);
             mma_commit(&v_empty[j % L::ST]);
-            if(!L::APART && j + 1 < tiles) {
+            if(j + 1 < tiles) {
                if(!(ok = k_ready(j + 1))) break;
                scores(j + 1);
             }
@@ -335,7 +326,6 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    } else { // softmax: thread = row of tile t, or half h of its keys
       const int t = warp / (4 * L::HALVES), h = L::HALVES == 2 ? warp >> 2 & 1 : 0, row = threadIdx.x & 127;
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16), st = lanes + t * 128, ot = lanes + L::O + t * DP;
-      const uint32_t pt = L::APART ? lanes + L::P + t * 64 : st;
       const float sc = a.scale * kLog2e;
       const uint64_t sc2 = pair(sc, sc);
       float m = -CUDART_INF_F;
@@ -370,7 +360,6 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                wait_ld();
                loaded< 64 >(s);
                fence_before();
-               if constexpr(L::APART) mbar_arrive(&s_free[t]);
 #pragma unroll
                for(int c = 0; c < 2; ++c) {
                   if(2 * h + c >= chunks) continue;
@@ -407,8 +396,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                   sum[0] = mul2(sum[0], pair(f, f));
                   sum[1] = mul2(sum[1], pair(f, f));
                }
-               if(j > 0) { // the products into O so far were done before this S, or are waited for
-                  if constexpr(L::APART) ok = ok && __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1));
+               if(j > 0) { // the products into O so far were done before this S
                   fence_after();
                   for(int c = h * 16; c < a.dim; c += 16 * L::HALVES) {
                      uint32_t o[16];
@@ -426,13 +414,11 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
             const float ref = m == -CUDART_INF_F ? 0.f : m;
             const uint64_t ref2 = pair(-ref, -ref);
             if constexpr(L::HALVES == 2) {
-               if constexpr(L::APART) // the last weights have been used
-                  if(j > 0) ok = ok && __all_sync(~0u, mbar_wait(&pv_done[t], (j - 1) & 1));
 #pragma unroll
                for(int c = 0; c < 2; ++c) {
                   if(2 * h + c >= chunks) continue;
                   exponents< T >(s + c * 32, sc2, ref2, sum);
-                  tmem_st16(pt + (2 * h + c) * 16, s + c * 32);
+                  tmem_st16(st + (2 * h + c) * 16, s + c * 32);
                }
                wait_st();
                fence_before();
@@ -447,7 +433,7 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
                      if(partial) hide(s + (c & 1) * 32, bits[c]);
                      exponents< T >(s + (c & 1) * 32, sc2, ref2, sum);
                      // The next scores lie from column 32 (c + 1) on, these weights before column 16 (c + 1).
-                     tmem_st16(pt + c * 16, s + (c & 1) * 32);
+                     tmem_st16(st + c * 16, s + (c & 1) * 32);
                   }
                   if(c & 1) {
                      wait_st();
@@ -894,7 +880,9 @@ int tc_forward(relm_mp_dtype dtype, Args a, int64_t tiles, int64_t pairs, int pa
 {
    // Two tiles per block share k and v and overlap; one tile per block, two blocks per SM, where most second
    // tiles would be empty (512 ragged states: 105 us paired, 75 us single) or the pairs leave SMs idle.
-   const bool two = 2 * tiles >= 3 * pairs && pairs * a.heads >= 148;
+   // Four tiles (dims up to 64) go to a block where the pairs would: 4 x 2048 x 4096, 16 heads of 64, 230 us against
+   // 235 us in pairs, masked 293 against 336; they need more pairs to fill the SMs.
+   const bool two = 2 * tiles >= 3 * pairs && pairs * a.heads >= (a.dim <= 64 ? 222 : 148);
    const int key_box = two && a.dim <= 64 ? Quad::KN : kTileRows;
    TcMaps m;
    int rc;
