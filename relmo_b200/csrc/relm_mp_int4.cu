@@ -6,14 +6,15 @@
 // the matrix instruction with the 16 weight rows as its left operand and up to
 // 8 (or 16) x rows as its right one: one instruction per 16 x 16 weights
 // whatever the number of rows. Turning codes into floats is then the larger
-// part of the work (an earlier form with a subtraction per pair of weights spent
-// 146 instructions per 16 x 64 weights and was bound by them: 34 us where the
-// bytes take 11), so the codes enter as they lie:
+// part of the work (a form with a subtraction per pair of weights spent 146
+// instructions per 16 x 64 weights and was bound by them: 34 us for 7 rows by
+// 16384 x 8192, whose bytes take 11; this one spends 98 and takes 21 us), so the
+// codes enter as they lie:
 //  - f16: the four bits in place in the mantissa of a subnormal number, c 2^-24
 //    (rows g) or c 2^-20 (rows g + 8); two masks and one shift per 4 weights;
 //  - bf16: in the mantissa of 128, as 128 + c (subnormal products would be lost);
-// and the zero point is taken off each group's sum: sum x c - z sum x, with sum x
-// from one more product with ones. Sums are float32; the cancellation costs at
+// and the zero point is taken off each group's sum: the accumulator starts at
+// -z sum x, with -sum x from one more product, with minus ones. Sums are float32; the cancellation costs at
 // most 5 bits of them, far below the 2-byte result's rounding. A float32 x has
 // no such room: its codes become c - z exactly (128 + c minus 128 + z).
 //
@@ -28,6 +29,8 @@
 // never crosses a group of 32.
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "relm_mp_internal.cuh"
 
 using namespace relm_mp;
@@ -39,7 +42,7 @@ constexpr int kBlockK = 64; // columns of one packed word row
 
 struct Layout {
    int64_t tiles, blocks, groups; // 16-row tiles, 64-column blocks, groups (padded to whole blocks)
-   size_t scales, zeros, bytes;
+   size_t table, bytes;           // scales (and zero points) by tile, group and row pair
 };
 
 Layout layout(int64_t n, int64_t k, int64_t group, bool zeros)
@@ -48,9 +51,8 @@ Layout layout(int64_t n, int64_t k, int64_t group, bool zeros)
    l.tiles = (n + 15) / 16;
    l.blocks = (k + kBlockK - 1) / kBlockK;
    l.groups = (l.blocks * kBlockK + group - 1) / group;
-   l.scales = align_up((size_t)l.tiles * l.blocks * 512);
-   l.zeros = l.scales + align_up((size_t)l.tiles * l.groups * 32);
-   l.bytes = l.zeros + (zeros ? align_up((size_t)l.tiles * l.groups * 16) : 0);
+   l.table = align_up((size_t)l.tiles * l.blocks * 512);
+   l.bytes = l.table + align_up((size_t)l.tiles * l.groups * (zeros ? 64 : 32));
    return l;
 }
 
@@ -77,34 +79,40 @@ __global__ void __launch_bounds__(256) k_int4_pack(const unsigned char* __restri
    out[w] = v;
 }
 
-// Per (tile, group): scales (and zero points) of rows (g, g + 8) side by side.
-__global__ void __launch_bounds__(256) k_int4_pack_groups(const __half* __restrict__ scales,
+// Per (tile, group), for rows (g, g + 8): their scales and, with zero points, a word of z (g) and 16 z (g + 8):
+// as f16 those are the zero points in the units of the f16 product's rows, z 2^-24 and z 2^-20.
+__global__ void __launch_bounds__(256) k_int4_pack_groups(const unsigned short* __restrict__ scales,
                                                           const unsigned char* __restrict__ zeros, int64_t n,
                                                           int64_t src_groups, int64_t groups, int64_t total,
-                                                          __half* __restrict__ out_s, unsigned char* __restrict__ out_z)
+                                                          uint32_t* __restrict__ out)
 {
    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
    if(i >= total) return;
-   const int64_t tile = (i >> 4) / groups, grp = (i >> 4) % groups;
-   const int e = i & 15;
-   const int64_t row = tile * 16 + (e >> 1) + 8 * (e & 1);
-   const bool in = row < n && grp < src_groups;
-   out_s[i] = in ? scales[row * src_groups + grp] : __float2half_rn(0.f);
-   if(out_z) out_z[i] = in ? zeros[row * src_groups + grp] : 0;
+   const int64_t tile = (i >> 3) / groups, grp = (i >> 3) % groups;
+   uint32_t s = 0, z = 0;
+   for(int h = 0; h < 2; ++h) {
+      const int64_t row = tile * 16 + (i & 7) + 8 * h;
+      if(row >= n || grp >= src_groups) continue; // padding: scale 0
+      s |= (uint32_t)scales[row * src_groups + grp] << (16 * h);
+      if(zeros) z |= (uint32_t)zeros[row * src_groups + grp] << (h ? 20 : 0);
+   }
+   if(zeros) out[2 * i] = s, out[2 * i + 1] = z;
+   else out[i] = s;
 }
 
 enum Source { kSame = 0, kF32 = 1, kE4m3 = 2 };
 
-// One 32-bit word of codes as the left operand (rows g: f[0], f[2]; rows g + 8: f[1], f[3]).
-// A stored code c stands for (offset + c) * 2^-shift.
+// One 32-bit word of codes as the left operand (rows g: f[0], f[2]; rows g + 8: f[1], f[3]),
+// and what is taken off a group's sum per sum x: the zero points (`z`, as packed) in the operand's units.
 template < typename M, int SRC >
 struct Left;
 template < int SRC >
 struct Left< __half, SRC > {
    static constexpr bool exact = false;
    static constexpr uint32_t ones = 0x3c003c00u;
-   static constexpr float up0 = 16777216.f, up8 = 1048576.f, offset = 0.f; // 2^24, 2^20
-   static __device__ __forceinline__ void fragments(uint32_t w, uint32_t, uint32_t, uint32_t* f)
+   static constexpr float up0 = 16777216.f, up8 = 1048576.f; // 2^24, 2^20: the sums' units
+   static __device__ __forceinline__ float2 offsets(uint32_t z) { return __half22float2(*reinterpret_cast< const __half2* >(&z)); }
+   static __device__ __forceinline__ void fragments(uint32_t w, uint32_t, uint32_t* f)
    {
       f[0] = w & 0x000f000fu;
       f[1] = w & 0x00f000f0u;
@@ -121,21 +129,24 @@ struct Left< __half, SRC > {
 template < int SRC >
 struct Left< __nv_bfloat16, SRC > {
    static constexpr bool exact = SRC == kF32;
-   static constexpr uint32_t ones = 0x3f803f80u;
-   static constexpr float up0 = 1.f, up8 = 1.f, offset = 128.f;
-   // (128 + z, 128 + z)
-   static __device__ __forceinline__ uint32_t base(uint32_t z) { return 0x43004300u + z * 0x00010001u; }
+   [[maybe_unused]] static constexpr uint32_t ones = 0x3f803f80u;
+   static constexpr float up0 = 1.f, up8 = 1.f;
+   // 2^23 + z as a float has z in its low bits
+   static __device__ __forceinline__ float2 offsets(uint32_t z)
+   {
+      return make_float2(__uint_as_float(0x4b000000u | (z & 0xffffu)) - 8388480.f, __uint_as_float(0x4b000000u | z >> 20) - 8388480.f);
+   }
    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b)
    {
       const __nv_bfloat162 v = __hsub2(*reinterpret_cast< __nv_bfloat162* >(&a), *reinterpret_cast< __nv_bfloat162* >(&b));
       return *reinterpret_cast< const uint32_t* >(&v);
    }
-   static __device__ __forceinline__ void fragments(uint32_t w, uint32_t z0, uint32_t z1, uint32_t* f)
+   static __device__ __forceinline__ void fragments(uint32_t w, uint32_t z, uint32_t* f)
    {
 #pragma unroll
       for(int i = 0; i < 4; ++i) {
          f[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-         if constexpr(exact) f[i] = sub(f[i], i & 1 ? z1 : z0);
+         if constexpr(exact) f[i] = sub(f[i], 0x43004300u + (i & 1 ? z >> 20 : z & 0xffffu) * 0x00010001u); // minus (128 + z, 128 + z)
       }
    }
    static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b)
@@ -145,6 +156,7 @@ struct Left< __nv_bfloat16, SRC > {
           : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
    }
 };
+constexpr uint32_t kZero8 = 8u | 128u << 16; // the packed word of zero points 8, 8
 
 // x columns of the right operand per row of x.
 template < int SRC >
@@ -209,23 +221,22 @@ struct MatvecArgs {
    const float* x_scale;
    int rows;
    const uint4* codes;
-   const __half2* scales;
-   const uchar2* zeros; // NULL: 8
+   const uint4* table;
    int64_t n, k, groups;
-   int blocks, group_shift;
-   bool vec;
+   int blocks, group_shift, wide; // wide: blocks with all of their tiles
+   bool vec, zeros;
    void* y;
 };
 
 constexpr int kStages = 4;
 
-// One stage of a warp: codes of NT tiles, their scales and zero points (up to two
-// groups each), 64 columns of x.
+// One stage of a warp: codes of NT tiles, their table entries (up to two groups
+// each), 64 columns of x.
 template < int SRC, int CT, int NT >
 struct Stage {
    static constexpr int ES = SRC == kF32 ? 4 : SRC == kE4m3 ? 1 : 2;
    static constexpr int ROWS = CT * 8 / kColumns< SRC >; // x rows of a launch
-   static constexpr int CODES = 0, SCALES = NT * 512, ZEROS = SCALES + NT * 64, X = ZEROS + NT * 32, BYTES = X + ROWS * 64 * ES;
+   static constexpr int CODES = 0, TABLE = NT * 512, X = TABLE + NT * 128, BYTES = X + ROWS * 64 * ES;
    static constexpr int PER_ROW = 64 * ES / 16, PIECES = (ROWS * PER_ROW + 31) / 32; // 16-byte pieces of x, and those of a lane
 };
 
@@ -233,7 +244,7 @@ struct Stage {
 // and their sums are joined in shared memory in warp order. Each warp is its own
 // pipeline of asynchronous copies, three blocks ahead, without block barriers.
 // G32: groups of 32, two to a block; else a block has one scale.
-template < typename M, int SRC, int CT, int NT, bool G32, typename OUT >
+template < typename M, int SRC, int CT, int NT, bool G32, bool ZEROS, typename OUT >
 __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
 {
    using S = Stage< SRC, CT, NT >;
@@ -241,7 +252,10 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
    constexpr int COLS = CT * 8;
    extern __shared__ __align__(128) unsigned char smem[];
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-   const int64_t tile0 = (int64_t)blockIdx.x * NT, tiles = (a.n + 15) / 16;
+   const int64_t tiles = (a.n + 15) / 16;
+   // Blocks from a.wide on have a tile less.
+   const int64_t tile0 = (int64_t)blockIdx.x * NT - ((int)blockIdx.x > a.wide ? (int)blockIdx.x - a.wide : 0);
+   const int mine_n = (int)blockIdx.x >= a.wide ? NT - 1 : NT;
    unsigned char* const mine = smem + warp * (kStages * S::BYTES);
    const uint32_t base = (uint32_t)__cvta_generic_to_shared(mine);
    constexpr int halves = G32 ? 2 : 1; // groups of a block
@@ -255,14 +269,13 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
 
    // A tile past the end is read as the first one: its sums are not stored.
    const uint4* codes[NT];
-   const __half2* scales[NT];
-   const uchar2* zeros[NT];
+   const uint4* table[NT];
+   constexpr int ENTRY = ZEROS ? 4 : 2; // 16-byte pieces of a (tile, group)
 #pragma unroll
    for(int n = 0; n < NT; ++n) {
       const int64_t tile = tile0 + n < tiles ? tile0 + n : tile0;
       codes[n] = a.codes + tile * a.blocks * 32 + lane;
-      scales[n] = a.scales + tile * a.groups * 8 + lane * 4;
-      zeros[n] = a.zeros + tile * a.groups * 8 + lane * 8;
+      table[n] = a.table + tile * a.groups * ENTRY + lane;
    }
    // Piece c of row r of x. The halves of odd rows change places: 8 lanes of two rows then read different banks.
    auto x_place = [&](int r, int c) { return S::X + r * (64 * S::ES) + (SRC == kSame ? c ^ ((r & 1) << 2) : c) * 16; };
@@ -279,14 +292,12 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
          const uint32_t at = base + stage * S::BYTES + lane * 16;
          const int grp = (int)(((int64_t)blk * kBlockK) >> a.group_shift);
 #pragma unroll
-         for(int n = 0; n < NT; ++n) copy16(at + S::CODES + n * 512, codes[n] + (int64_t)blk * 32, true);
-         if(lane < 2 * halves) {
+         for(int n = 0; n < NT; ++n)
+            if(NT == 1 || n < mine_n) copy16(at + S::CODES + n * 512, codes[n] + (int64_t)blk * 32, true);
+         if(lane < ENTRY * halves) {
 #pragma unroll
-            for(int n = 0; n < NT; ++n) copy16(at + S::SCALES + n * 64, scales[n] + (int64_t)grp * 8, true);
-            if(a.zeros && lane < halves) {
-#pragma unroll
-               for(int n = 0; n < NT; ++n) copy16(at + S::ZEROS + n * 32, zeros[n] + (int64_t)grp * 8, true);
-            }
+            for(int n = 0; n < NT; ++n)
+               if(NT == 1 || n < mine_n) copy16(at + S::TABLE + n * 128, table[n] + (int64_t)grp * ENTRY, true);
          }
 #pragma unroll
          for(int i = 0; i < S::PIECES; ++i) {
@@ -332,59 +343,59 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
             load_x< M, SRC >(at + S::X + (r * 64 + half * 32 + 8 * t) * S::ES, part, b[c] + 4 * h);
          }
       }
-      // sum x of the block's group, or of its two: a row of ones
+      // Minus sum x of the block's group, or of its two: a row of minus ones
       float xs[2][CT][4];
       if constexpr(!P::exact) {
-         const uint32_t ones[4] = {P::ones, P::ones, P::ones, P::ones};
+         const uint32_t ones[4] = {P::ones ^ 0x80008000u, P::ones ^ 0x80008000u, P::ones ^ 0x80008000u, P::ones ^ 0x80008000u};
 #pragma unroll
          for(int c = 0; c < CT; ++c) {
 #pragma unroll
-            for(int h = 0; h < 2; ++h) {
+            for(int i = 0; i < 4; ++i) xs[0][c][i] = xs[1][c][i] = 0.f;
 #pragma unroll
-               for(int i = 0; i < 4; ++i) xs[h][c][i] = 0.f;
-               P::mma(xs[h][c], ones, &b[c][4 * h]);
-               P::mma(xs[h][c], ones, &b[c][4 * h + 2]);
-            }
-            if constexpr(!G32) xs[0][c][0] += xs[1][c][0], xs[0][c][1] += xs[1][c][1];
+            for(int k = 0; k < 4; ++k) P::mma(xs[G32 ? k >> 1 : 0][c], ones, &b[c][2 * k]);
          }
       }
 #pragma unroll
       for(int n = 0; n < NT; ++n) {
+         if(NT > 1 && n >= mine_n) break;
          const uint4 w = *reinterpret_cast< const uint4* >(at + S::CODES + n * 512 + lane * 16);
          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
          float acc[CT][4];
-         uint32_t z0 = 0, z1 = 0;
-         float s0 = 0.f, s1 = 0.f, o0 = 0.f, o1 = 0.f;
+         uint32_t z = kZero8;
+         float2 scale = make_float2(0.f, 0.f);
 #pragma unroll
          for(int s = 0; s < 4; ++s) {
+            // Groups of 64 columns or more cover the block with one scale; groups of 32 change half way.
             if(s == 0 || (s == 2 && G32)) {
-               const float2 sc = __half22float2(reinterpret_cast< const __half2* >(at + S::SCALES + n * 64 + (s >> 1) * 32)[g]);
-               uchar2 z = make_uchar2(8, 8);
-               if(a.zeros) z = reinterpret_cast< const uchar2* >(at + S::ZEROS + n * 32 + (s >> 1) * 16)[g];
-               if constexpr(P::exact) {
-                  z0 = P::base(z.x), z1 = P::base(z.y);
+               const unsigned char* e = at + S::TABLE + n * 128 + (s >> 1) * (ENTRY * 16) + g * (ENTRY * 2);
+               uint32_t sc;
+               if constexpr(ZEROS) {
+                  const uint2 v = *reinterpret_cast< const uint2* >(e);
+                  sc = v.x, z = v.y;
                } else {
-                  o0 = -sc.x * (P::offset + (float)z.x), o1 = -sc.y * (P::offset + (float)z.y);
+                  sc = *reinterpret_cast< const uint32_t* >(e);
                }
-               s0 = sc.x * P::up0, s1 = sc.y * P::up8;
+               scale = __half22float2(*reinterpret_cast< const __half2* >(&sc));
+               if constexpr(P::exact) {
 #pragma unroll
-               for(int c = 0; c < CT; ++c)
+                  for(int c = 0; c < CT; ++c) acc[c][0] = acc[c][1] = acc[c][2] = acc[c][3] = 0.f;
+               } else {
+                  const float2 o = P::offsets(z);
 #pragma unroll
-                  for(int i = 0; i < 4; ++i) acc[c][i] = 0.f;
+                  for(int c = 0; c < CT; ++c)
+#pragma unroll
+                     for(int i = 0; i < 4; ++i) acc[c][i] = (i < 2 ? o.x : o.y) * xs[s >> 1][c][i & 1];
+               }
             }
             uint32_t f[4];
-            P::fragments(ww[s], z0, z1, f);
+            P::fragments(ww[s], z, f);
 #pragma unroll
             for(int c = 0; c < CT; ++c) P::mma(acc[c], f, &b[c][2 * s]);
             if(s == 3 || (s == 1 && G32)) {
-               const int h = s == 3 && G32 ? 1 : 0;
 #pragma unroll
                for(int c = 0; c < CT; ++c)
 #pragma unroll
-                  for(int i = 0; i < 4; ++i) {
-                     total[n][c][i] = fmaf(i < 2 ? s0 : s1, acc[c][i], total[n][c][i]);
-                     if constexpr(!P::exact) total[n][c][i] = fmaf(i < 2 ? o0 : o1, xs[h][c][i & 1], total[n][c][i]);
-                  }
+                  for(int i = 0; i < 4; ++i) total[n][c][i] = fmaf(i < 2 ? scale.x : scale.y, acc[c][i], total[n][c][i]);
             }
          }
       }
@@ -400,13 +411,13 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
 #pragma unroll
       for(int c = 0; c < CT; ++c)
 #pragma unroll
-         for(int i = 0; i < 4; ++i) part[place(warp, n * 16 + g + 8 * (i >> 1), c * 8 + 2 * t + (i & 1))] = total[n][c][i];
+         for(int i = 0; i < 4; ++i) part[place(warp, n * 16 + g + 8 * (i >> 1), c * 8 + 2 * t + (i & 1))] = total[n][c][i] * (i < 2 ? P::up0 : P::up8);
    __syncthreads();
    constexpr int PER = kColumns< SRC >;
    for(int i = threadIdx.x; i < a.rows * NT * 16; i += kWarps * 32) {
       const int r = i / (NT * 16), j = i % (NT * 16);
       const int64_t out = tile0 * 16 + j;
-      if(out >= a.n) continue;
+      if(out >= a.n || j >= mine_n * 16) continue;
       float v = 0.f;
 #pragma unroll
       for(int w = 0; w < kWarps; ++w)
@@ -418,28 +429,42 @@ __global__ void __launch_bounds__(kWarps * 32) k_int4_matvec(MatvecArgs a)
 }
 
 template < typename M, int SRC, int CT, int NT, typename OUT >
-int launch_tiles(const MatvecArgs& a, cudaStream_t st)
+int launch_tiles(MatvecArgs a, unsigned blocks, int64_t wide, cudaStream_t st)
 {
+   a.wide = (int)wide;
    constexpr int stages = kWarps * kStages * Stage< SRC, CT, NT >::BYTES, sums = kWarps * NT * 16 * (CT * 8 + 1) * 4;
    constexpr int bytes = stages > sums ? stages : sums;
    const bool g32 = a.group_shift == 5;
-   const auto kernel = g32 ? k_int4_matvec< M, SRC, CT, NT, true, OUT > : k_int4_matvec< M, SRC, CT, NT, false, OUT >;
-   static SmemLimit limit[2];
-   const int rc = limit[g32]((const void*)kernel, bytes, "k_int4_matvec");
+   const auto kernel = g32 ? (a.zeros ? k_int4_matvec< M, SRC, CT, NT, true, true, OUT > : k_int4_matvec< M, SRC, CT, NT, true, false, OUT >)
+                           : (a.zeros ? k_int4_matvec< M, SRC, CT, NT, false, true, OUT > : k_int4_matvec< M, SRC, CT, NT, false, false, OUT >);
+   static SmemLimit limit[4];
+   const int rc = limit[2 * g32 + a.zeros]((const void*)kernel, bytes, "k_int4_matvec");
    if(rc) return rc;
-   const int64_t tiles = (a.n + 15) / 16;
-   kernel<<< (unsigned)((tiles + NT - 1) / NT), kWarps * 32, bytes, st >>>(a);
+   kernel<<< blocks, kWarps * 32, bytes, st >>>(a);
    return check_launch("k_int4_matvec");
 }
 
-// Each block reads all of x: wide weights give a block several tiles, as long as every SM keeps two blocks.
+// Each block reads all of x, so wide weights give a block several tiles. Up to eight tiles per SM are dealt to two
+// blocks per SM, the first 148 with the larger half: every SM has as many tiles as any other, or one fewer.
 template < typename M, int SRC, int CT, typename OUT >
 int launch(const MatvecArgs& a, cudaStream_t st)
 {
-   const int64_t tiles = (a.n + 15) / 16;
-   if(CT <= 2 && tiles >= 3 * 296) return launch_tiles< M, SRC, CT, CT <= 2 ? 4 : 2, OUT >(a, st);
-   if(tiles >= 2 * 296) return launch_tiles< M, SRC, CT, 2, OUT >(a, st);
-   return launch_tiles< M, SRC, CT, 1, OUT >(a, st);
+   constexpr int64_t SMS = 148;
+   const int64_t tiles = (a.n + 15) / 16, per_sm = (tiles + SMS - 1) / SMS;
+   constexpr int MOST = CT <= 2 ? 4 : 2;
+   auto dealt = [&](auto nt) { // blocks of NT tiles, and of NT - 1 where per_sm is odd
+      constexpr int NT = decltype(nt)::value;
+      const int64_t wide = per_sm % 2 ? SMS : 2 * SMS, done = wide * NT;
+      const int64_t blocks = tiles <= done ? (tiles + NT - 1) / NT : wide + (tiles - done + NT - 2) / (NT - 1);
+      return launch_tiles< M, SRC, CT, NT, OUT >(a, (unsigned)blocks, wide, st);
+   };
+   if(per_sm <= 2) return launch_tiles< M, SRC, CT, 1, OUT >(a, (unsigned)tiles, tiles, st);
+   if(per_sm <= 4) return dealt(std::integral_constant< int, 2 >());
+   if constexpr(MOST == 4) {
+      if(per_sm <= 6) return dealt(std::integral_constant< int, 3 >());
+      if(per_sm <= 8) return dealt(std::integral_constant< int, 4 >());
+   }
+   return launch_tiles< M, SRC, CT, MOST, OUT >(a, (unsigned)((tiles + MOST - 1) / MOST), tiles, st);
 }
 
 template < typename M, int SRC, typename OUT >
@@ -487,12 +512,11 @@ int relm_mp_int4_pack(const unsigned char* codes, const void* scales, const unsi
    if(packed_bytes < l.bytes) return fail(RELM_MP_ERR_WORKSPACE_TOO_SMALL, "int4_pack: packed buffer too small.");
    cudaStream_t st = static_cast< cudaStream_t >(stream);
    char* base = static_cast< char* >(packed);
-   const int64_t words = l.tiles * l.blocks * 128, entries = l.tiles * l.groups * 16;
+   const int64_t words = l.tiles * l.blocks * 128, entries = l.tiles * l.groups * 8;
    k_int4_pack<<< (unsigned)((words + 255) / 256), 256, 0, st >>>(codes, n, k, l.blocks, words, reinterpret_cast< uint32_t* >(base));
    if((rc = check_launch("k_int4_pack"))) return rc;
-   k_int4_pack_groups<<< (unsigned)((entries + 255) / 256), 256, 0, st >>>(
-      static_cast< const __half* >(scales), zeros, n, k / group, l.groups, entries,
-      reinterpret_cast< __half* >(base + l.scales), zeros ? reinterpret_cast< unsigned char* >(base + l.zeros) : nullptr);
+   k_int4_pack_groups<<< (unsigned)((entries + 255) / 256), 256, 0, st >>>(static_cast< const unsigned short* >(scales), zeros, n, k / group,
+                                                                            l.groups, entries, reinterpret_cast< uint32_t* >(base + l.table));
    return check_launch("k_int4_pack_groups");
 }
 
@@ -513,8 +537,8 @@ int relm_mp_int4_matvec(relm_mp_dtype dtype, int x_e4m3, const void* x, int64_t 
    MatvecArgs a{};
    a.x = x, a.x_stride = x_stride, a.x_scale = x_scale;
    a.codes = reinterpret_cast< const uint4* >(base);
-   a.scales = reinterpret_cast< const __half2* >(base + l.scales);
-   a.zeros = has_zeros ? reinterpret_cast< const uchar2* >(base + l.zeros) : nullptr;
+   a.table = reinterpret_cast< const uint4* >(base + l.table);
+   a.zeros = has_zeros != 0;
    a.n = n, a.k = k, a.groups = l.groups, a.blocks = (int)l.blocks;
    a.group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
    a.vec = (reinterpret_cast< uintptr_t >(x) & 15) == 0 && (x_stride * es) % 16 == 0;
