@@ -152,6 +152,7 @@ struct AddRmsNorm : torch::autograd::Function< AddRmsNorm > {
    }
    static variable_list backward(AutogradContext* ctx, variable_list grads)
    {
+      TORCH_CHECK(!at::GradMode::is_enabled(), "add_rms_norm: its gradient cannot be differentiated (create_graph).");
       const auto saved = ctx->get_saved_variables();
       const bool residual = saved[3].defined();
       const Tensor& dh = residual ? grads[1] : Tensor();
@@ -337,6 +338,7 @@ struct CrossAttention : torch::autograd::Function< CrossAttention > {
    static variable_list backward(AutogradContext* ctx, variable_list grads)
    {
       const char* op = "cross_attention_backward";
+      TORCH_CHECK(!at::GradMode::is_enabled(), "cross_attention: its gradient cannot be differentiated (create_graph).");
       const auto s = ctx->get_saved_variables();
       const auto meta = ctx->saved_data["meta"].toIntVector();
       at::AutoDispatchBelowADInplaceOrView below;

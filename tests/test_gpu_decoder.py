@@ -301,6 +301,77 @@ def test_attention_packed_strides_broadcast_heads_and_unaligned(dtype):
     ref.close(decoder.cross_attention(odd, k, v, plan).detach(), want.detach())
 
 
+# Enough tiles and heads for the kernels that give a block two or four query tiles.
+MANY = ([520, 130, 1, 700], [300, 65, 640, 129])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(40, 8, 64), (40, 40, 128), (48, 8, 96), (40, 10, 32), (40, 8, 40)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_many_tiles(dtype, heads, kv_heads, dim, masked):
+    ql, kl = MANY
+    q, k, v, do = make(dtype, ql, kl, heads, kv_heads, dim)
+    mask = None
+    if masked:
+        mask = torch.rand(sum(kl), generator=torch.Generator().manual_seed(5)).cuda() < 0.8
+        mask[300:365] = False         # nothing left of the second sequence
+        mask[365 + 64:365 + 192] = False  # whole tiles of the third
+        k[~mask], v[~mask] = math.nan, math.inf
+    check(q, k, v, do, ql, kl, mask)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_many_tiles_neighbours_and_growing_scores(dim):
+    ql, kl = [300, 300, 300], [400, 200, 1000]
+    q, k, v, _ = make(BF16, ql, kl, 40, 40, dim)
+    k = k * torch.linspace(0.1, 8, k.size(0), device="cuda")[:, None, None].to(BF16)  # maxima that keep growing
+    want = ref.attention(q[600:].double(), k[600:].double(), v[600:].double(), ql[2:], kl[2:], dim**-0.5)
+    q[300:600], k[400:600], v[400:600] = math.nan, math.inf, math.nan
+    o = decoder.cross_attention(q, k, v, decoder.attention_plan(ql, kl))
+    assert bool(torch.isfinite(o[:300]).all()) and bool(torch.isfinite(o[600:]).all())
+    # float32 scores of up to 60 have errors of 60 * 2^-24 * a few: far below the type's rounding
+    assert (o[600:].double() - want).norm() <= 3 * ref.U[BF16] * want.norm()
+    same = decoder.cross_attention(q, k, v, decoder.attention_plan(ql, kl))
+    assert torch.equal(o[600:], same[600:])
+
+
+def test_operators_in_a_cuda_graph():
+    ql, kl = [200, 31, 300], [333, 64, 500]
+    runs = []
+    for dtype, dim in ((BF16, 64), (F16, 128), (F32, 32)):
+        q, k, v, _ = make(dtype, ql, kl, 8, 4, dim)
+        plan = decoder.attention_plan(ql, kl)
+        runs.append((lambda q=q, k=k, v=v, plan=plan: decoder.cross_attention(q, k, v, plan), q))
+        one = decoder.attention_plan([1, 1, 1], kl)
+        runs.append((lambda q=q, k=k, v=v, one=one: decoder.cross_attention(q[:3], k, v, one), q))
+        x, w = rnd((50, 128), dtype, 7), rnd((128,), dtype, 8)
+        runs.append((lambda x=x, w=w: torch.cat([t.float() for t in decoder.add_rms_norm(x, w, x)]), x))
+        weight = decoder.Int4Weight(*make_int4(96, 128, 32, True))
+        runs.append((lambda x=x, weight=weight: decoder.int4_matvec(x, weight), x))
+    for call, value in runs:
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        value.copy_(rnd(value.shape, value.dtype, 99))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call())
+
+
+def test_gradients_of_gradients_are_refused():
+    x, w = rnd((4, 32), F32, 1).requires_grad_(), rnd((32,), F32, 2).requires_grad_()
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        torch.autograd.grad(decoder.add_rms_norm(x, w)[0].sum(), x, create_graph=True)
+    q, k, v, do = (t.requires_grad_() for t in make(F32, [3], [4], 2, 2, 16))
+    o = decoder.cross_attention(q, k, v, decoder.attention_plan([3], [4]))
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        torch.autograd.grad(o, q, do.detach(), create_graph=True)
+
+
 def test_attention_same_bits_other_stream_and_plan_reuse():
     ql, kl = [200, 31, 1], [333, 64, 500]
     for dtype in (BF16, F32):
