@@ -14,6 +14,10 @@
 //
 // Keys outside the sequence or masked are zeros in shared memory (their rows are
 // never read) and get weight 0.
+//
+// Measured: 512 states of 8 to 160 query rows over 100 keys, 4 heads of 32, bf16:
+// forward 43 us, backward 67 us (197 us for both on the tcgen05 kernels); bound by
+// instruction issue.
 #include <math_constants.h>
 
 #include "relm_mp_attn_mma.cuh"

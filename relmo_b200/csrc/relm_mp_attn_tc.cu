@@ -1,10 +1,11 @@
 // Cross attention on the tensor cores (tcgen05): 2-byte types, head dims up to
 // 128, forward.
 //
-// A block owns QT tiles of 128 query rows of one head and walks the keys in
-// tiles of 128. One thread copies k and v tiles by tensor map, one per query tile
-// issues products, a warp sees to masked keys, and four warps per query tile do the
-// softmax, a thread per row:
+// A block owns QT tiles of 128 query rows of one head (one or two; dims up to 64
+// have a form with four, further down) and walks the keys in tiles of 128. One
+// thread copies k and v tiles by tensor map, one per query tile issues products, a
+// warp sees to masked keys, and four or eight warps per query tile do the softmax, a
+// thread per row or half row:
 //
 //   S = Q K^T          both operands in shared memory, S (float32) in tensor memory
 //   P = 2^(sc S - m)   rounded to the inputs' type, written over S
@@ -19,6 +20,11 @@
 // Keys outside the sequence or masked get a score of -inf, so weight 0. Their rows
 // of v are zeroed in shared memory first: what they hold may be an infinity or NaN,
 // which a weight of 0 would not hide.
+//
+// Measured: 4 sequences of 2 048 queries over 4 001 to 4 096 keys, 16 heads of 128
+// over 4, bf16: 300 us (0.91 PFLOP/s), bound by the latency of a tile's chain; 16
+// sequences of 100 to 3 001 queries over 301 to 6 000 masked keys, 16 heads of 64,
+// f16: 0.83 ms (0.42 PFLOP/s, half as many products per score).
 #include <math_constants.h>
 
 #include <type_traits>

@@ -5,18 +5,19 @@
 // Bound by the weights' bytes (half a byte each), so the inner product runs on
 // the matrix instruction with the 16 weight rows as its left operand and up to
 // 8 (or 16) x rows as its right one: one instruction per 16 x 16 weights
-// whatever the number of rows. Turning codes into floats is then the larger
-// part of the work (a form with a subtraction per pair of weights spent 146
-// instructions per 16 x 64 weights and was bound by them: 34 us for 7 rows by
-// 16384 x 8192, whose bytes take 11; this one spends 98 and takes 21 us), so the
-// codes enter as they lie:
+// whatever the number of rows. Turning codes into floats is then the larger part
+// of the work: a form with a subtraction per pair of weights spent 146 instructions
+// per 16 x 64 weights and was bound by them (34 us for 7 rows by 16384 x 8192,
+// whose bytes take 11; this one spends 98 and takes 21 us). So the codes enter as
+// they lie:
 //  - f16: the four bits in place in the mantissa of a subnormal number, c 2^-24
 //    (rows g) or c 2^-20 (rows g + 8); two masks and one shift per 4 weights;
 //  - bf16: in the mantissa of 128, as 128 + c (subnormal products would be lost);
 // and the zero point is taken off each group's sum: the accumulator starts at
-// -z sum x, with -sum x from one more product, with minus ones. Sums are float32; the cancellation costs at
-// most 5 bits of them, far below the 2-byte result's rounding. A float32 x has
-// no such room: its codes become c - z exactly (128 + c minus 128 + z).
+// -z sum x, with -sum x from one more product, with minus ones. Sums are float32;
+// the cancellation costs at most 5 bits of them, far below the 2-byte result's
+// rounding. A float32 x has no such room: its codes become c - z exactly (128 + c
+// minus 128 + z).
 //
 // The right operand keeps x exact: bf16 and f16 as they are, e4m3 as f16, and
 // float32 as three bf16 columns (x = hi + mid + lo, 24 bits), which cost

@@ -12,6 +12,10 @@
 // adds x and r again instead of reading h (one more read of 8): with the rounded
 // h the weight's gradient, a sum of terms of either sign, was 1.6 times as far
 // from its 64-bit value.
+//
+// Measured: 16384 x 8192 bf16 forward with residual 185 us (5.8 TB/s, 88% of the
+// copy rate); 51200 x 128 bf16 forward and backward 26 us of kernels, float32 rows
+// of an odd length (no 16-byte chunks) 63 us for 43 at the copy rate.
 #include <cuda_fp8.h>
 
 #include "relm_mp_internal.cuh"
