@@ -352,7 +352,12 @@ static size_t delta_bytes(const relm_mp_attn& in) { return align_up((size_t)in.h
 size_t relm_mp_cross_attention_backward_workspace_bytes(const relm_mp_attn* attn)
 {
    if(check_attn(attn, "cross_attention_backward")) return 0;
-   const int few = few_rows(*attn) ? warp_few_parts(make_args(*attn)) : 0;
+   const Args a = make_args(*attn);
+   if(use_tc(*attn) && !few_rows(*attn)) {
+      const Counts c = counts(*attn);
+      return delta_bytes(*attn) + align_up(tc_backward_bytes(a, c.q_tiles, c.kv_tiles));
+   }
+   const int few = few_rows(*attn) ? warp_few_parts(a) : 0;
    return delta_bytes(*attn) + (few > 1 ? align_up((size_t)few * attn->q_rows * attn->heads * attn->dim * sizeof(float)) : 0);
 }
 
@@ -388,7 +393,7 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
    }
    if(use_tc(*attn) && aligned && !few_rows(*attn)) {
       if((rc = gave_up_address(&a.gave_up))) return rc;
-      return tc_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, st);
+      return tc_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, static_cast< char* >(workspace) + delta_bytes(*attn), st);
    }
    const int few = few_rows(*attn) ? warp_few_parts(a) : 0;
    return warp_backward(attn->dtype, a, c.q_tiles, c.kv_tiles, aligned_any(*attn) && aligned, few, static_cast< char* >(workspace) + delta_bytes(*attn),

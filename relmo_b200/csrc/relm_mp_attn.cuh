@@ -125,7 +125,8 @@ int tc_parts(const Args& a, int64_t tiles);
 size_t tc_parts_bytes(const Args& a, int parts);
 int tc_forward(relm_mp_dtype dtype, Args a, int64_t tiles, int64_t pairs, int parts, void* workspace, cudaStream_t st);
 // (relm_mp_attn_tc_bwd.cu)
-int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st);
+size_t tc_backward_bytes(const Args& a, int64_t q_tiles, int64_t kv_tiles);
+int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, void* workspace, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace relm_mp

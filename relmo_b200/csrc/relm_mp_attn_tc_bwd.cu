@@ -19,8 +19,16 @@
 // group of four warps for each 32 columns turns S and dO V^T into P and dS in
 // place (a thread per row; a group's result stays inside its own columns, so no
 // warp overwrites what another has still to read).
+//
+// Measured: 4 sequences of 2 048 queries over 4 001 to 4 096 keys, 16 heads of 128
+// over 4, bf16: dK/dV 502 us (3 040 cycles per iteration of four 128 x 128 x 128
+// products), dQ 362 us (2 505 for three). The
+// tensor pipe is busy for about nine tenths of that: with an operand or two in
+// shared memory such a product takes some 720 cycles, 512 by its arithmetic.
 #include <math_constants.h>
 
+#include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "relm_mp_attn_tc.cuh"
@@ -106,6 +114,86 @@ __device__ __forceinline__ void store_rows(uint32_t acc, bool any, bool ok, floa
    __syncwarp();
 }
 
+// ---- work in parts ---------------------------------------------------------------------
+
+// A job is a tile of one head. The jobs of the last, partial wave of blocks are cut
+// into `parts` along the other side; their sums go to the workspace in float32 and
+// k_attn_tc_backward_join adds them in order. parts == 1: the grid is (tiles, heads).
+struct Share {
+   int tiles, full, rest, parts; // `full` jobs whole, then `rest` in parts
+   float* sums;                  // [rest * parts][outputs][DP / 4][kTileRows][4]
+};
+
+struct Job {
+   int tile, head, part; // part: -1 for a whole job
+};
+
+__device__ __forceinline__ Job job_of(const Share& w)
+{
+   if(w.parts == 1) return Job{(int)blockIdx.x, (int)blockIdx.y, -1};
+   const int past = (int)blockIdx.x - w.full;
+   const int job = past < 0 ? (int)blockIdx.x : w.full + past / w.parts;
+   return Job{job % w.tiles, job / w.tiles, past < 0 ? -1 : past % w.parts};
+}
+
+// Iterations [begin, end) of `n`.
+__device__ __forceinline__ void part_of(const Share& w, int part, int n, int& begin, int& end)
+{
+   begin = part < 0 ? 0 : (int)((int64_t)n * part / w.parts);
+   end = part < 0 ? n : (int)((int64_t)n * (part + 1) / w.parts);
+}
+
+// The number of this block's part, -1 for a whole job (worked out again at a kernel's end, not held through it).
+__device__ __forceinline__ int part_block(const Share& w) { return w.parts == 1 ? -1 : (int)blockIdx.x - w.full; }
+
+// This thread's accumulator row to `out` ([DP / 4][kTileRows][4], row `row`).
+template < int DP >
+__device__ __forceinline__ void store_sums(uint32_t acc, bool any, bool ok, float* out, int row, int dim)
+{
+#pragma unroll
+   for(int c = 0; c < DP; c += 16) {
+      if(c >= dim) break;
+      uint32_t v[16];
+      if(any) {
+         tmem_ld16(v, acc + c);
+         wait_ld();
+         loaded< 16 >(v);
+      }
+#pragma unroll
+      for(int i = 0; i < 16; ++i) v[i] = !ok ? __float_as_uint(CUDART_NAN_F) : any ? v[i] : 0;
+#pragma unroll
+      for(int i = 0; i < 16; i += 4)
+         *reinterpret_cast< uint4* >(out + ((int64_t)((c + i) / 4) * kTileRows + row) * 4) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+   }
+}
+
+// Block (job, 16 columns, output), a thread per row. KV: outputs dV and dK of a key tile, else dQ of a query tile.
+template < typename T, int DP, bool KV >
+__global__ void __launch_bounds__(kTileRows) k_attn_tc_backward_join(Args a, Share w)
+{
+   const int job = w.full + blockIdx.x, tile = job % w.tiles, head = job / w.tiles, c = blockIdx.y * 16, which = blockIdx.z;
+   const Item it = KV ? item(a.kv_tiles, a.max_kv, kTileRows, tile) : item(a.q_tiles, a.max_q, kTileRows, tile);
+   const Seq s = KV ? locate(a.kv_off, a.max_kv, a.ks, it.seq) : locate(a.q_off, a.max_q, a.qs, it.seq);
+   const int row = it.tile * kTileRows + threadIdx.x, heads = KV ? a.kv_heads : a.heads;
+   if(row >= s.len || c >= a.dim) return;
+   constexpr int OUTPUTS = KV ? 2 : 1, SIZE = kTileRows * DP / 4; // float4 of an output
+   const float4* in = reinterpret_cast< const float4* >(w.sums) + ((int64_t)blockIdx.x * w.parts * OUTPUTS + which) * SIZE + (c / 4) * kTileRows + threadIdx.x;
+   float x[16] = {};
+   for(int p = 0; p < w.parts; ++p, in += OUTPUTS * SIZE)
+#pragma unroll
+      for(int i = 0; i < 4; ++i) {
+         const float4 v = in[i * kTileRows];
+         x[4 * i] += v.x, x[4 * i + 1] += v.y, x[4 * i + 2] += v.z, x[4 * i + 3] += v.w;
+      }
+   const float mul = KV && which == 0 ? kDown : a.scale;
+   uint32_t o[8];
+#pragma unroll
+   for(int i = 0; i < 8; ++i) o[i] = pack2< T >(x[2 * i] * mul, x[2 * i + 1] * mul);
+   T* out = static_cast< T* >(!KV ? a.dq : which ? a.dk : a.dv) + ((s.first + row) * heads + head) * a.dim + c;
+   *reinterpret_cast< uint4* >(out) = make_uint4(o[0], o[1], o[2], o[3]);
+   if(c + 8 < a.dim) *reinterpret_cast< uint4* >(out + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
 // ---- dK, dV: one key tile, all query tiles of the group ------------------------------
 
 template < int DP, int QN >
@@ -120,7 +208,7 @@ struct Kv {
 
 template < typename T, int DP, int QN >
 __global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
-   k_attn_tc_backward_kv(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+   k_attn_tc_backward_kv(Args a, Share w, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
                          const __grid_constant__ CUtensorMap vm, const __grid_constant__ CUtensorMap gm)
 {
    using L = Kv< DP, QN >;
@@ -133,11 +221,15 @@ __global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads;
-   const Item it = item(a.kv_tiles, a.max_kv, kTileRows, blockIdx.x);
+   const Job job = job_of(w);
+   const int kv_head = job.head, group = a.heads / a.kv_heads;
+   const Item it = item(a.kv_tiles, a.max_kv, kTileRows, job.tile);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const int key0 = it.tile * kTileRows;
-   const int q_tiles = (qs.len + QN - 1) / QN, n = q_tiles * group;
+   const int q_tiles = (qs.len + QN - 1) / QN; // iteration i0 + i: a query tile of a head of the group
+   int i0, n;
+   part_of(w, job.part, q_tiles * group, i0, n);
+   n -= i0;
 
    if(threadIdx.x == 0) {
       mbar_init(&kv_full, 1);
@@ -171,7 +263,7 @@ __global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
          for(int i = 0; i < n; ++i) {
             const int s = i % L::ST, round = i / L::ST;
             if(round && !mbar_wait(&q_empty[s], (round - 1) & 1)) break;
-            const int head = kv_head * group + i / q_tiles, row = qr + (i % q_tiles) * QN;
+            const int head = kv_head * group + (i0 + i) / q_tiles, row = qr + (i0 + i) % q_tiles * QN;
             mbar_expect(&q_full[s], 2 * L::QT);
             for(int p = 0; p < DP / 64; ++p) {
                tma_load(base + L::Q + s * L::QT + p * QN * 128, &qm, &q_full[s], p * 64, row, head, b);
@@ -189,7 +281,7 @@ __global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
       if(elect_one() && n > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t out_id = instruction(BF, 128, steps * 16, true);
-         auto cols = [&](int i) { return min(QN, (qs.len - (i % q_tiles) * QN + 15) / 16 * 16); };
+         auto cols = [&](int i) { return min(QN, (qs.len - (i0 + i) % q_tiles * QN + 15) / 16 * 16); };
          // S^T = K Q^T or dP^T = V dO^T
          auto first = [&](uint32_t d, uint32_t left, uint32_t right, int i, uint64_t* bar) {
             product_columns< DP, kTileRows, QN >(tmem + d, base + left, base + right + (i % L::ST) * L::QT,
@@ -231,24 +323,27 @@ __global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
       const uint32_t st = lanes + L::S + half * HALF, pt = lanes + L::P + half * HALF;
       const bool in = key < ks.len && (!a.mask || a.mask[ks.first + key]);
       const float sc = a.scale * kLog2e;
-      // What this thread puts into shared memory for iteration i: an lse (log2) or a delta.
+      int tile = n > 0 ? i0 % q_tiles : 0; // of the next fetch, and the line of its head
+      int64_t line = (int64_t)(kv_head * group + (n > 0 ? i0 / q_tiles : 0)) * a.q_rows + qs.first;
+      // What this thread puts into shared memory for an iteration: an lse (log2) or a delta.
       const int col = threadIdx.x % QN;
       const bool puts_lse = threadIdx.x < QN, puts = threadIdx.x < 2 * QN;
-      auto fetch = [&](int i) {
-         const int q = (i % q_tiles) * QN + col;
-         if(!puts || i >= n || q >= qs.len) return puts_lse ? CUDART_INF_F : 0.f;
-         const int64_t at = (int64_t)(kv_head * group + i / q_tiles) * a.q_rows + qs.first + q;
+      auto fetch = [&] {
+         const int q = tile * QN + col;
+         if(!puts || q >= qs.len) return puts_lse ? CUDART_INF_F : 0.f;
+         const int64_t at = line + q;
          if(!puts_lse) return a.delta[at] * kDown;
          const float v = a.lse_in[at];
          return v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e - kUp; // a row without keys: weights 0
       };
-      float next = n > 0 ? fetch(0) : 0.f;
+      float next = n > 0 ? fetch() : 0.f;
       bool ok = true;
       for(int i = 0; i < n; ++i) {
-         const int valid = min(QN, qs.len - (i % q_tiles) * QN);
+         const int valid = min(QN, qs.len - tile * QN);
          if(puts) reinterpret_cast< float* >(puts_lse ? s_lse[i & 1] : s_delta[i & 1])[col] = next;
          soft_sync< L::SOFT >();
-         next = fetch(i + 1);
+         if(++tile == q_tiles) tile = 0, line += a.q_rows;
+         if(i + 1 < n) next = fetch();
          ok = ok && __all_sync(~0u, mbar_wait(&s_full, i & 1));
          fence_after();
          uint32_t s[HALF];
@@ -320,7 +415,11 @@ __global__ void __launch_bounds__(Kv< DP, QN >::THREADS, Kv< DP, QN >::RESIDENT)
       // One group writes dV, one dK, through the K and V tiles (their products are done).
       const int k0 = key0 + (warp & 3) * 32;
       T* out = static_cast< T* >(half ? a.dk : a.dv) + ((ks.first + k0) * a.kv_heads + kv_head) * a.dim;
-      if(half < 2) store_rows< T, DP >(lanes + (half ? L::DK : L::DV), n > 0, ok, half ? a.scale : kDown,
+      const int part = part_block(w);
+      if(half < 2 && part >= 0)
+         store_sums< DP >(lanes + (half ? L::DK : L::DV), n > 0, ok, w.sums + ((int64_t)part * 2 + half) * kTileRows * DP, row, a.dim);
+      else if(half < 2)
+         store_rows< T, DP >(lanes + (half ? L::DK : L::DV), n > 0, ok, half ? a.scale : kDown,
                           sm + (half ? L::V : L::K) + (warp & 3) * 32 * (DP * 2), out, (int64_t)a.kv_heads * a.dim, ks.len - k0, a.dim);
    }
    fence_before();
@@ -344,7 +443,7 @@ struct Dq {
 
 template < typename T, int DP, int KN >
 __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
-   k_attn_tc_backward_q(Args a, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+   k_attn_tc_backward_q(Args a, Share w, const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
                         const __grid_constant__ CUtensorMap vm, const __grid_constant__ CUtensorMap gm)
 {
    using L = Dq< DP, KN >;
@@ -356,10 +455,15 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x);
+   const Job job = job_of(w);
+   const int head = job.head, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, job.tile);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
-   const int row0 = it.tile * kTileRows, n = (ks.len + KN - 1) / KN;
+   const int row0 = it.tile * kTileRows;
+   int n, key0; // key tiles, and the first key of this part
+   part_of(w, job.part, (ks.len + KN - 1) / KN, key0, n);
+   n -= key0, key0 *= KN;
+   const int keys = ks.len - key0;
 
    if(threadIdx.x == 0) {
       mbar_init(&q_full, 1);
@@ -384,7 +488,7 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
 
    if(warp == L::MMA_WARP + 1) { // copies
       if(lane == 0 && n > 0) {
-         const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0), b = a.q_off ? 0 : it.seq;
+         const int qr = (int)(a.q_off ? qs.first : 0) + row0, kr = (int)(a.kv_off ? ks.first : 0) + key0, b = a.q_off ? 0 : it.seq;
          mbar_expect(&q_full, 2 * L::QT);
          for(int p = 0; p < DP / 64; ++p) {
             tma_load(base + L::Q + p * kTileRows * 128, &qm, &q_full, p * 64, qr, head, b);
@@ -413,7 +517,7 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
       if(elect_one() && n > 0) {
          const int steps = (a.dim + 15) / 16;
          const uint32_t out_id = instruction(BF, 128, steps * 16, true);
-         auto cols = [&](int j) { return min(KN, (ks.len - j * KN + 15) / 16 * 16); };
+         auto cols = [&](int j) { return min(KN, (keys - j * KN + 15) / 16 * 16); };
          // S = Q K^T or dP = dO V^T
          auto first = [&](uint32_t d, uint32_t left, uint32_t right, int j, uint64_t* bar) {
             product_columns< DP, kTileRows, KN >(tmem + d, base + left, base + right + (j % L::ST) * L::KT,
@@ -452,7 +556,7 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
       const int half = warp >> 2, row = row0 + (warp & 3) * 32 + lane;
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) * 32 << 16);
       const uint32_t pt = lanes + L::P + half * HALF;
-      const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
+      const unsigned char* keep = a.mask ? a.mask + ks.first + key0 : nullptr;
       const float sc = a.scale * kLog2e;
       float lse = CUDART_INF_F, delta = 0.f; // rows past the sequence or without keys: weights 0
       if(row < qs.len) {
@@ -464,7 +568,7 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
       const uint64_t sc2 = pair(sc, sc), lse2 = pair(-lse, -lse), delta2 = pair(-delta, -delta);
       bool ok = true;
       for(int j = 0; j < n; ++j) {
-         const int left = ks.len - j * KN;
+         const int left = keys - j * KN;
          bool all = left >= KN && !keep;
          unsigned bits[HALF / 32];
 #pragma unroll
@@ -516,7 +620,10 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
       if(!ok) gave_up = 1;
       // Through the Q tile's shared memory; the first group writes.
       const int r0 = row0 + (warp & 3) * 32;
-      if(half == 0) {
+      const int part = part_block(w);
+      if(half == 0 && part >= 0) {
+         store_sums< DP >(lanes + L::DQ, n > 0, ok, w.sums + (int64_t)part * kTileRows * DP, (warp & 3) * 32 + lane, a.dim);
+      } else if(half == 0) {
          T* out = static_cast< T* >(a.dq) + ((qs.first + r0) * a.heads + head) * a.dim;
          store_rows< T, DP >(lanes + L::DQ, n > 0, ok, a.scale, sm + L::Q + (warp & 3) * 32 * (DP * 2), out, (int64_t)a.heads * a.dim,
                              qs.len - r0, a.dim);
@@ -529,19 +636,58 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
    if(threadIdx.x == 0 && gave_up) atomicExch(a.gave_up, 1);
 }
 
-template < typename F >
-int launch(SmemLimit& limit, F fn, int threads, int bytes, dim3 grid, const Args& a, const TcMaps& m, cudaStream_t st, const char* what)
+// The jobs of a partial wave in parts where that saves more than it costs: in iterations of the longest job, with
+// eight for the join and its launch, at least four a part and at most two waves of parts. Backward of 4 x 2048 x 4096,
+// 16 heads over 4 of 128 (512 jobs on 148 SMs) 856 us against 906 whole; one sequence of 1000 x 1000, 8 over 2, 52
+// against 99; 3000 x 300, 16 over 4 of 64, 68 against 294; 200 x 20000, 8 heads, 171 against 384.
+Share share(int64_t tiles, int64_t heads, int64_t n, int resident, float* sums)
 {
-   if(grid.x == 0) return RELM_MP_OK;
+   const int64_t jobs = tiles * heads, slots = 148 * resident, rest = jobs % slots;
+   Share w{(int)std::min< int64_t >(tiles, INT_MAX), 0, (int)rest, 1, sums};
+   if(rest == 0 || jobs > 64 * slots) return w; // nothing to cut, or a small part of the whole
+   int64_t best = n;
+   for(int64_t s = 2; s * 4 <= n && rest * s <= 2 * slots; ++s) {
+      const int64_t cost = ceil_div(rest * s, slots) * ceil_div(n, s) + 8;
+      if(cost < best) best = cost, w.parts = (int)s;
+   }
+   w.full = (int)(jobs - rest);
+   return w;
+}
+template < int DP, int N >
+Share share_kv(const Args& a, int64_t tiles, float* sums)
+{
+   return share(tiles, a.kv_heads, ceil_div(a.max_q, N) * (a.heads / a.kv_heads), Kv< DP, N >::RESIDENT, sums);
+}
+template < int DP, int N >
+Share share_q(const Args& a, int64_t tiles, float* sums)
+{
+   return share(tiles, a.heads, ceil_div(a.max_kv, N), Dq< DP, N >::RESIDENT, sums);
+}
+template < int DP, int N >
+size_t sums_bytes(const Args& a, int64_t q_tiles, int64_t kv_tiles)
+{
+   const Share q = share_q< DP, N >(a, q_tiles, nullptr), kv = share_kv< DP, N >(a, kv_tiles, nullptr);
+   const size_t rows = std::max(q.parts > 1 ? (size_t)q.rest * q.parts : 0, kv.parts > 1 ? (size_t)kv.rest * kv.parts * 2 : 0) * kTileRows;
+   return rows * DP * sizeof(float);
+}
+
+template < typename F, typename J >
+int launch(SmemLimit& limit, F fn, J join, int threads, int bytes, int heads, int outputs, int columns, const Args& a, const Share& w,
+           const TcMaps& m, cudaStream_t st, const char* what)
+{
+   if(w.tiles == 0) return RELM_MP_OK;
    int rc = limit((const void*)fn, bytes, what);
    if(rc) return rc;
-   fn<<< grid, threads, bytes, st >>>(a, m.q, m.k, m.v, m.go);
-   return check_launch(what);
+   const dim3 grid = w.parts > 1 ? dim3(w.full + w.rest * w.parts) : dim3(w.tiles, heads);
+   fn<<< grid, threads, bytes, st >>>(a, w, m.q, m.k, m.v, m.go);
+   if((rc = check_launch(what)) || w.parts == 1) return rc;
+   join<<< dim3(w.rest, columns, outputs), kTileRows, 0, st >>>(a, w);
+   return check_launch("k_attn_tc_backward_join");
 }
 
 // N: rows of the streamed tile of both kernels.
 template < typename T, int DP, int N >
-int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st)
+int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, float* sums, cudaStream_t st)
 {
    const bool packed = a.q_off != nullptr;
    const int64_t qrows = packed ? a.q_rows : a.max_q, krows = packed ? a.kv_rows : a.max_kv, seqs = packed ? 1 : a.seqs;
@@ -557,23 +703,30 @@ int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_til
    int rc;
    if((rc = maps(&m, N, kTileRows))) return rc;
    static SmemLimit kv_limit, q_limit;
-   if((rc = launch(kv_limit, k_attn_tc_backward_kv< T, DP, N >, Kv< DP, N >::THREADS, (int)Kv< DP, N >::BYTES + 1024, dim3((unsigned)kv_tiles, a.kv_heads), a, m, st,
-                   "k_attn_tc_backward_kv")))
+   const int columns = (a.dim + 15) / 16;
+   if((rc = launch(kv_limit, k_attn_tc_backward_kv< T, DP, N >, k_attn_tc_backward_join< T, DP, true >, Kv< DP, N >::THREADS,
+                   (int)Kv< DP, N >::BYTES + 1024, a.kv_heads, 2, columns, a, share_kv< DP, N >(a, kv_tiles, sums), m, st, "k_attn_tc_backward_kv")))
       return rc;
    if(N != kTileRows && (rc = maps(&m, kTileRows, N))) return rc;
-   return launch(q_limit, k_attn_tc_backward_q< T, DP, N >, Dq< DP, N >::THREADS, (int)Dq< DP, N >::BYTES + 1024, dim3((unsigned)q_tiles, a.heads), a, m, st,
-                 "k_attn_tc_backward_q");
+   return launch(q_limit, k_attn_tc_backward_q< T, DP, N >, k_attn_tc_backward_join< T, DP, false >, Dq< DP, N >::THREADS,
+                 (int)Dq< DP, N >::BYTES + 1024, a.heads, 1, columns, a, share_q< DP, N >(a, q_tiles, sums), m, st, "k_attn_tc_backward_q");
 }
 
 }  // namespace
 
-int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, cudaStream_t st)
+size_t tc_backward_bytes(const Args& a, int64_t q_tiles, int64_t kv_tiles)
 {
+   return a.dim <= 64 ? sums_bytes< 64, 64 >(a, q_tiles, kv_tiles) : sums_bytes< 128, 128 >(a, q_tiles, kv_tiles);
+}
+
+int tc_backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_tiles, void* workspace, cudaStream_t st)
+{
+   float* sums = static_cast< float* >(workspace);
    if(dtype == RELM_MP_BFLOAT16)
-      return a.dim <= 64 ? backward< __nv_bfloat16, 64, 64 >(dtype, a, q_tiles, kv_tiles, st)
-                         : backward< __nv_bfloat16, 128, 128 >(dtype, a, q_tiles, kv_tiles, st);
-   return a.dim <= 64 ? backward< __half, 64, 64 >(dtype, a, q_tiles, kv_tiles, st)
-                      : backward< __half, 128, 128 >(dtype, a, q_tiles, kv_tiles, st);
+      return a.dim <= 64 ? backward< __nv_bfloat16, 64, 64 >(dtype, a, q_tiles, kv_tiles, sums, st)
+                         : backward< __nv_bfloat16, 128, 128 >(dtype, a, q_tiles, kv_tiles, sums, st);
+   return a.dim <= 64 ? backward< __half, 64, 64 >(dtype, a, q_tiles, kv_tiles, sums, st)
+                      : backward< __half, 128, 128 >(dtype, a, q_tiles, kv_tiles, sums, st);
 }
 
 }  // namespace attn

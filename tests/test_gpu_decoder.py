@@ -335,6 +335,30 @@ def test_attention_many_tiles_neighbours_and_growing_scores(dim):
     assert torch.equal(o[600:], same[600:])
 
 
+# Few tiles with a long other side: the backward cuts them into parts, some of them empty for the short sequences.
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (4, 4, 64), (6, 2, 40), (6, 3, 104)])
+@pytest.mark.parametrize("ql,kl", [([2100, 1, 130], [300, 500, 64]), ([200, 130, 40], [4000, 70, 1]), ([1300], [1300]), ([1500, 0], [1200, 9])])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_backward_in_parts(dtype, heads, kv_heads, dim, ql, kl, masked):
+    q, k, v, do = make(dtype, ql, kl, heads, kv_heads, dim)
+    mask = None
+    if masked:
+        mask = torch.rand(sum(kl), generator=torch.Generator().manual_seed(6)).cuda() < 0.7
+        mask[100:300] = False
+        k[~mask], v[~mask] = math.nan, math.inf
+    check(q, k, v, do, ql, kl, mask)
+
+
+def test_attention_backward_in_parts_same_bits():
+    ql, kl = [1900, 130], [700, 900]
+    q, k, v, do = (t.requires_grad_() for t in make(BF16, ql, kl, 8, 2, 128))
+    plan = decoder.attention_plan(ql, kl)
+    runs = [torch.autograd.grad(decoder.cross_attention(q, k, v, plan), (q, k, v), do.detach()) for _ in range(3)]
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
 def test_operators_in_a_cuda_graph():
     ql, kl = [200, 31, 300], [333, 64, 500]
     runs = []
