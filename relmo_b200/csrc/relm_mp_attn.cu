@@ -6,6 +6,7 @@
 // with the longest loop start first (query tiles by the length of their keys
 // and the other way round).
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <cstring>
 #include <numeric>
@@ -380,9 +381,9 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
    const bool aligned = ((reinterpret_cast< uintptr_t >(grad_o) | reinterpret_cast< uintptr_t >(dq) |
                           reinterpret_cast< uintptr_t >(dk) | reinterpret_cast< uintptr_t >(dv)) & 15) == 0;
    // One block per sequence and key head walks all its query rows: not for long queries of few sequences.
-   const bool many = attn->seqs * a.kv_heads >= 296 || attn->max_q * (a.heads / a.kv_heads) <= 256;
+   const bool many = attn->seqs * a.kv_heads <= INT_MAX && (attn->seqs * a.kv_heads >= 296 || attn->max_q * (a.heads / a.kv_heads) <= 256);
    if(short_keys(*attn) && aligned && many && (((reinterpret_cast< uintptr_t >(o) | reinterpret_cast< uintptr_t >(o_rest)) & 15) == 0))
-      return short_backward(attn->dtype, a, st);
+      return short_backward(attn->dtype, a, c.kv_tiles, st);
    if(attn->q_rows) {
       switch(attn->dtype) {
          case RELM_MP_FLOAT32: rc = launch_delta< float >(grad_o, o, o_rest, attn->q_rows, a.heads, a.dim, delta, st); break;

@@ -117,7 +117,7 @@ int split_forward(relm_mp_dtype dtype, const Args& a, int64_t blocks, bool align
 
 // Up to 128 keys a sequence, dim up to 64, 2-byte types, aligned rows (relm_mp_attn_short.cu).
 int short_forward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, cudaStream_t st);
-int short_backward(relm_mp_dtype dtype, const Args& a, cudaStream_t st);
+int short_backward(relm_mp_dtype dtype, const Args& a, int64_t kv_tiles, cudaStream_t st);
 
 // Tensor cores: 2-byte types, dim a multiple of 8 up to 128, rows on 16-byte
 // boundaries (relm_mp_attn_tc.cu).

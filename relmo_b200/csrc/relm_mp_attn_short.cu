@@ -16,8 +16,10 @@
 // never read) and get weight 0.
 //
 // Measured: 512 states of 8 to 160 query rows over 100 keys, 4 heads of 32, bf16:
-// forward 43 us, backward 67 us (197 us for both on the tcgen05 kernels); bound by
-// instruction issue.
+// forward 35 us, backward 63 us (197 us for both on the tcgen05 kernels). The
+// schedulers issue in 58% and 41% of the cycles; the rest are the latencies of
+// products and copies with five and four blocks on an SM (four and three: 40 and
+// 65 us), which registers limit.
 #include <math_constants.h>
 
 #include "relm_mp_attn_mma.cuh"
@@ -33,11 +35,16 @@ template < typename T, int DP >
 __device__ __forceinline__ void copy_rows(uint32_t dst, const T* src, int64_t stride, int rows, int row0, int len, int dim,
                                           const unsigned char* keep)
 {
-   constexpr int CH = DP / 8;
-   for(int i = threadIdx.x; i < rows * CH; i += kShortThreads) {
-      const int r = i / CH, c = i % CH;
-      const bool in = row0 + r < len && c * 8 < dim && (!keep || keep[row0 + r]);
-      copy16(dst + swizzled< DP >(r, c), in ? src + (int64_t)(row0 + r) * stride + c * 8 : src, in);
+   constexpr int CH = DP / 8, STEP = kShortThreads / CH; // (a multiple of the pattern's 8 rows)
+   int r = threadIdx.x / CH;
+   const int c = threadIdx.x % CH;
+   const T* from = src + (int64_t)(row0 + r) * stride + c * 8;
+   const int64_t ahead = STEP * stride;
+   dst += swizzled< DP >(r, c);
+   len = c * 8 < dim ? len - row0 : 0;
+   for(; r < rows; r += STEP, from += ahead, dst += STEP * DP * 2) {
+      const bool in = r < len && (!keep || keep[row0 + r]);
+      copy16(dst, in ? from : src, in);
    }
 }
 __device__ __forceinline__ void copies_done()
@@ -85,7 +92,7 @@ __device__ __forceinline__ void store2(T* p, float x, float y)
 }
 
 template < typename T, int DP >
-__global__ void __launch_bounds__(kShortThreads) k_attn_short_forward(Args a)
+__global__ void __launch_bounds__(kShortThreads, DP == 32 ? 5 : 4) k_attn_short_forward(Args a)
 {
    constexpr int KS = DP / 16;
    extern __shared__ __align__(128) unsigned char smem[];
@@ -117,6 +124,7 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_forward(Args a)
    unsigned bits[4];
    key_bits(bits, ks.len, keep);
    copies_done();
+   if(row0 + warp * 16 >= qs.len) return;
    const float sc = a.scale * kLog2e;
    float s[kKeys / 8][4];
    float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
@@ -132,21 +140,27 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_forward(Args a)
          Mma< T >::run(s[2 * n], qf[kk], b[0], b[1]);
          Mma< T >::run(s[2 * n + 1], qf[kk], b[2], b[3]);
       }
-      const unsigned w = bits[n / 2] >> (n % 2 * 16) >> (2 * t4);
+      const unsigned step = bits[n / 2] >> (n % 2 * 16) & 0xffffu;
+      if(step != 0xffffu) {
 #pragma unroll
-      for(int e = 0; e < 2; ++e)
+         for(int e = 0; e < 2; ++e)
 #pragma unroll
-         for(int i = 0; i < 4; ++i) {
-            s[2 * n + e][i] = w >> (e * 8 + (i & 1)) & 1 ? s[2 * n + e][i] * sc : -CUDART_INF_F;
-            top[i >> 1] = fmaxf(top[i >> 1], s[2 * n + e][i]);
-         }
+            for(int i = 0; i < 4; ++i)
+               if(!(step >> (2 * t4 + e * 8 + (i & 1)) & 1)) s[2 * n + e][i] = -CUDART_INF_F;
+      }
+#pragma unroll
+      for(int h = 0; h < 2; ++h)
+         top[h] = fmaxf(fmaxf(fmaxf(top[h], s[2 * n][2 * h]), fmaxf(s[2 * n][2 * h + 1], s[2 * n + 1][2 * h])), s[2 * n + 1][2 * h + 1]);
    }
-   float l[2] = {0.f, 0.f}, ref[2];
+   float l[2];
+   float2 sum[2] = {}, ref[2]; // (-ref, -ref)
+   const float2 sc2 = make_float2(sc, sc);
 #pragma unroll
    for(int h = 0; h < 2; ++h) {
       top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 1));
       top[h] = fmaxf(top[h], __shfl_xor_sync(~0u, top[h], 2));
-      ref[h] = top[h] == -CUDART_INF_F ? 0.f : top[h];
+      top[h] *= sc;
+      ref[h].x = ref[h].y = top[h] == -CUDART_INF_F ? 0.f : -top[h];
    }
    float o[DP / 8][4];
 #pragma unroll
@@ -157,9 +171,11 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_forward(Args a)
 #pragma unroll
       for(int e = 0; e < 2; ++e)
 #pragma unroll
-         for(int i = 0; i < 4; ++i) {
-            s[2 * n + e][i] = exp2_fast(s[2 * n + e][i] - ref[i >> 1]);
-            l[i >> 1] += s[2 * n + e][i];
+         for(int h = 0; h < 2; ++h) {
+            float* x = s[2 * n + e] + 2 * h;
+            const float2 y = __ffma2_rn(make_float2(x[0], x[1]), sc2, ref[h]);
+            x[0] = exp2_fast(y.x), x[1] = exp2_fast(y.y);
+            sum[h] = __fadd2_rn(sum[h], make_float2(x[0], x[1]));
          }
       // The weights enter the second product in the inputs' type, their sum l stays float32.
       const uint32_t p[4] = {Mma< T >::pack(s[2 * n][0], s[2 * n][1]), Mma< T >::pack(s[2 * n][2], s[2 * n][3]),
@@ -174,6 +190,7 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_forward(Args a)
    }
 #pragma unroll
    for(int h = 0; h < 2; ++h) {
+      l[h] = sum[h].x + sum[h].y;
       l[h] += __shfl_xor_sync(~0u, l[h], 1);
       l[h] += __shfl_xor_sync(~0u, l[h], 2);
       const int row = row0 + warp * 16 + g + 8 * h;
@@ -207,14 +224,14 @@ struct Bwd {
 };
 
 template < typename T, int DP >
-__global__ void __launch_bounds__(kShortThreads) k_attn_short_backward(Args a)
+__global__ void __launch_bounds__(kShortThreads, DP == 32 ? 4 : 2) k_attn_short_backward(Args a)
 {
    using L = Bwd< DP >;
    extern __shared__ __align__(128) unsigned char smem[];
-   __shared__ float s_lse[kTile], s_delta[kTile];
    const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem);
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, seq = blockIdx.x;
+   const int kv_head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads, job = blockIdx.x / a.kv_heads;
+   const int seq = a.kv_tiles ? a.kv_tiles[job].seq : job;
    const Seq qs = locate(a.q_off, a.max_q, a.qs, seq), ks = locate(a.kv_off, a.max_kv, a.ks, seq);
    const Seq vs = locate(a.kv_off, a.max_kv, a.vs, seq);
    const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
@@ -239,7 +256,8 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_backward(Args a)
          const int m16 = (min(kTile, qs.len - q0) + 15) / 16; // 16-row steps
          copy_rows< T, DP >(base + L::Q, static_cast< const T* >(a.q) + qs.base + head * a.qs[2], a.qs[1], m16 * 16, q0, qs.len, a.dim, nullptr);
          copy_rows< T, DP >(base + L::G, go, go_row, m16 * 16, q0, qs.len, a.dim, nullptr);
-         { // delta = do . (o + o_rest): two threads a row
+         float line_lse, line_delta; // of the row of this pair of threads: each warp has the 16 rows that it works on
+         { // delta = do . (o + o_rest)
             const int r = threadIdx.x >> 1, row = q0 + r;
             float s = 0.f;
             if(row < qs.len) {
@@ -261,19 +279,21 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_backward(Args a)
                   }
                }
             }
-            s += __shfl_xor_sync(~0u, s, 1);
-            if((threadIdx.x & 1) == 0) {
-               const float v = row < qs.len ? a.lse_in[(int64_t)head * a.q_rows + qs.first + row] : -CUDART_INF_F;
-               s_lse[r] = v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e; // no such row, or a row without keys: weights 0
-               s_delta[r] = s;
-            }
+            line_delta = s + __shfl_xor_sync(~0u, s, 1);
+            const float v = row < qs.len ? a.lse_in[(int64_t)head * a.q_rows + qs.first + row] : -CUDART_INF_F;
+            line_lse = v == -CUDART_INF_F ? CUDART_INF_F : v * kLog2e; // no such row, or a row without keys: weights 0
          }
          copies_done();
 
          // Query rows: warp has 16. Weights and score gradients of 32 keys at a time.
          if(warp < m16) {
             const int r0 = warp * 16;
-            const float lse[2] = {s_lse[r0 + g], s_lse[r0 + g + 8]}, delta[2] = {s_delta[r0 + g], s_delta[r0 + g + 8]};
+            float2 lse[2], delta[2]; // negative, twice
+#pragma unroll
+            for(int h = 0; h < 2; ++h) {
+               lse[h].x = lse[h].y = -__shfl_sync(~0u, line_lse, 2 * g + 16 * h);
+               delta[h].x = delta[h].y = -__shfl_sync(~0u, line_delta, 2 * g + 16 * h);
+            }
             float dq[DP / 8][4];
 #pragma unroll
             for(int d = 0; d < DP / 8; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.f;
@@ -296,23 +316,32 @@ __global__ void __launch_bounds__(kShortThreads) k_attn_short_backward(Args a)
                   Mma< T >::run(dp[1], f, b[2], b[3]);
                }
                const unsigned word = n < 2 ? bits[0] : n < 4 ? bits[1] : n < 6 ? bits[2] : bits[3];
-               const unsigned w = word >> (n % 2 * 16) >> (2 * t4);
-               uint32_t df[4];
+               const unsigned step = word >> (n % 2 * 16) & 0xffffu;
+               uint32_t pw[4], df[4];
 #pragma unroll
                for(int e = 0; e < 2; ++e)
 #pragma unroll
                   for(int h = 0; h < 2; ++h) {
-                     float p[2], x[2];
-#pragma unroll
-                     for(int i = 0; i < 2; ++i) {
-                        p[i] = w >> (e * 8 + i) & 1 ? exp2_fast(fmaf(s[e][2 * h + i], sc, -lse[h])) : 0.f;
-                        x[i] = p[i] * (dp[e][2 * h + i] - delta[h]);
-                     }
+                     const float2 y = __ffma2_rn(make_float2(s[e][2 * h], s[e][2 * h + 1]), make_float2(sc, sc), lse[h]);
+                     const float2 p = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                     const float2 x = __fmul2_rn(p, __fadd2_rn(make_float2(dp[e][2 * h], dp[e][2 * h + 1]), delta[h]));
                      // Rounded to the inputs' type for the products that follow.
-                     const uint32_t pw = Mma< T >::pack(p[0], p[1]);
-                     df[e * 2 + h] = Mma< T >::pack(x[0], x[1]);
+                     pw[e * 2 + h] = Mma< T >::pack(p.x, p.y);
+                     df[e * 2 + h] = Mma< T >::pack(x.x, x.y);
+                  }
+               if(step != 0xffffu) // what came of keys that take no part may be anything
+#pragma unroll
+                  for(int e = 0; e < 2; ++e) {
+                     const unsigned w = step >> (2 * t4 + e * 8), in = (w & 1 ? 0xffffu : 0u) | (w & 2 ? 0xffff0000u : 0u);
+#pragma unroll
+                     for(int h = 0; h < 2; ++h) pw[e * 2 + h] &= in, df[e * 2 + h] &= in;
+                  }
+#pragma unroll
+               for(int e = 0; e < 2; ++e)
+#pragma unroll
+                  for(int h = 0; h < 2; ++h) {
                      const uint32_t at = weight_at(r0 + g + 8 * h, n * 2 + e) + t4 * 4;
-                     *reinterpret_cast< uint32_t* >(smem + L::P + at) = pw;
+                     *reinterpret_cast< uint32_t* >(smem + L::P + at) = pw[e * 2 + h];
                      *reinterpret_cast< uint32_t* >(smem + L::DS + at) = df[e * 2 + h];
                   }
 #pragma unroll
@@ -388,12 +417,14 @@ int forward(const Args& a, int64_t q_tiles, cudaStream_t st)
 }
 
 template < typename T, int DP >
-int backward(const Args& a, cudaStream_t st)
+int backward(Args a, int64_t kv_tiles, cudaStream_t st)
 {
+   // The key tiles are the sequences, most queries first, so that the last blocks are short; not where some have no keys.
+   if(kv_tiles != a.seqs) a.kv_tiles = nullptr;
    static SmemLimit limit;
    const int rc = limit((const void*)k_attn_short_backward< T, DP >, Bwd< DP >::BYTES, "k_attn_short_backward");
    if(rc) return rc;
-   k_attn_short_backward< T, DP ><<< dim3((unsigned)a.seqs, a.kv_heads), kShortThreads, Bwd< DP >::BYTES, st >>>(a);
+   k_attn_short_backward< T, DP ><<< (unsigned)(a.seqs * a.kv_heads), kShortThreads, Bwd< DP >::BYTES, st >>>(a);
    return check_launch("k_attn_short_backward");
 }
 
@@ -405,10 +436,10 @@ int short_forward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, cudaStrea
    return a.dim <= 32 ? forward< __half, 32 >(a, q_tiles, st) : forward< __half, 64 >(a, q_tiles, st);
 }
 
-int short_backward(relm_mp_dtype dtype, const Args& a, cudaStream_t st)
+int short_backward(relm_mp_dtype dtype, const Args& a, int64_t kv_tiles, cudaStream_t st)
 {
-   if(dtype == RELM_MP_BFLOAT16) return a.dim <= 32 ? backward< __nv_bfloat16, 32 >(a, st) : backward< __nv_bfloat16, 64 >(a, st);
-   return a.dim <= 32 ? backward< __half, 32 >(a, st) : backward< __half, 64 >(a, st);
+   if(dtype == RELM_MP_BFLOAT16) return a.dim <= 32 ? backward< __nv_bfloat16, 32 >(a, kv_tiles, st) : backward< __nv_bfloat16, 64 >(a, kv_tiles, st);
+   return a.dim <= 32 ? backward< __half, 32 >(a, kv_tiles, st) : backward< __half, 64 >(a, kv_tiles, st);
 }
 
 }  // namespace attn
