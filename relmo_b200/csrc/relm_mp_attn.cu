@@ -125,10 +125,11 @@ bool aligned_any(const relm_mp_attn& in)
 }
 bool aligned_rows(const relm_mp_attn& in) { return in.dtype != RELM_MP_FLOAT32 && aligned_any(in); }
 
-// Tensor maps hold these strides and coordinates.
+// Tensor maps hold these strides and coordinates, and a grid a block per tile and head.
 bool use_tc(const relm_mp_attn& in)
 {
    if(!aligned_rows(in) || in.dim > 128) return false;
+   if((std::max(in.q_rows, in.kv_rows) / kTileRows + in.seqs) * in.heads > INT_MAX) return false;
    auto ok = [&](const int64_t* s, int64_t rows, int64_t max_rows, int heads) {
       auto fits = [](int64_t v, int64_t extent) { return extent <= 1 || (v > 0 && v < (1ll << 38)); };
       return rows < (1ll << 31) - 512 && fits(s[1], max_rows) && fits(s[2], heads) && (in.plan || fits(s[0], in.seqs));

@@ -24,7 +24,7 @@
 // Measured: 4 sequences of 2 048 queries over 4 001 to 4 096 keys, 16 heads of 128
 // over 4, bf16: 300 us (0.91 PFLOP/s), bound by the latency of a tile's chain; 16
 // sequences of 100 to 3 001 queries over 301 to 6 000 masked keys, 16 heads of 64,
-// f16: 0.83 ms (0.42 PFLOP/s, half as many products per score).
+// f16: 0.78 ms (0.45 PFLOP/s, half as many products per score).
 #include <math_constants.h>
 
 #include <type_traits>
@@ -157,8 +157,10 @@ __global__ void __launch_bounds__(Fwd< DP, QT >::THREADS, QT == 1 ? 2 : 1)
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-   const Item it = item(QT == 2 ? a.q_pairs : a.q_tiles, a.max_q, QT * kTileRows, blockIdx.x);
+   // Heads run first, so that the longest tiles of all heads start first (16 ragged masked sequences of 16 heads: 781 us
+   // against 832 with the heads one after another).
+   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(QT == 2 ? a.q_pairs : a.q_tiles, a.max_q, QT * kTileRows, blockIdx.x / a.heads);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const int row0 = it.tile * QT * kTileRows;
    const int active = QT == 1 || row0 + kTileRows >= qs.len ? 1 : QT;
@@ -565,7 +567,7 @@ __global__ void __launch_bounds__(Quad::THREADS, 1)
    __shared__ uint32_t tmem_base;
    __shared__ int gave_up;
    // The pairs' list serves: the n tiles of a sequence go evenly to the first ceil(n / 4) of its ceil(n / 2) items.
-   const Item it = item(a.q_pairs, a.max_q, 2 * kTileRows, blockIdx.x);
+   const Item it = item(a.q_pairs, a.max_q, 2 * kTileRows, blockIdx.x / a.heads);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const int q_tiles = (qs.len + kTileRows - 1) / kTileRows, blocks = (q_tiles + L::QT - 1) / L::QT;
    if(it.tile >= blocks) return;
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(Quad::THREADS, 1)
    const int row0 = tile0 * kTileRows;
    unsigned char* sm = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
+   const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
    const int tiles = (ks.len + KN - 1) / KN;
    const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
 
@@ -840,7 +842,7 @@ int launch_quad(const Args& a, const TcMaps& m, int64_t pairs, cudaStream_t st)
    static SmemLimit limit;
    const int rc = limit((const void*)k_attn_tc_forward_quad< T >, bytes, "k_attn_tc_forward_quad");
    if(rc) return rc;
-   k_attn_tc_forward_quad< T ><<< dim3((unsigned)pairs, a.heads), Quad::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
+   k_attn_tc_forward_quad< T ><<< (unsigned)(pairs * a.heads), Quad::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
    return check_launch("k_attn_tc_forward_quad");
 }
 
@@ -852,7 +854,7 @@ int launch(const Args& a, const TcMaps& m, int64_t items, int parts, cudaStream_
    static SmemLimit limit;
    int rc = limit((const void*)k_attn_tc_forward< T, DP, QT >, bytes, "k_attn_tc_forward");
    if(rc) return rc;
-   k_attn_tc_forward< T, DP, QT ><<< dim3((unsigned)items, a.heads, parts), L::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
+   k_attn_tc_forward< T, DP, QT ><<< dim3((unsigned)(items * a.heads), 1, parts), L::THREADS, bytes, st >>>(a, m.q, m.k, m.v);
    return check_launch("k_attn_tc_forward");
 }
 

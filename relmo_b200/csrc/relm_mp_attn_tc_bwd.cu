@@ -21,14 +21,13 @@
 // warp overwrites what another has still to read).
 //
 // Measured: 4 sequences of 2 048 queries over 4 001 to 4 096 keys, 16 heads of 128
-// over 4, bf16: dK/dV 502 us (3 040 cycles per iteration of four 128 x 128 x 128
-// products), dQ 362 us (2 505 for three). The
+// over 4, bf16: dK/dV 460 us (3 040 cycles per iteration of four 128 x 128 x 128
+// products), dQ 359 us (2 505 for three). The
 // tensor pipe is busy for about nine tenths of that: with an operand or two in
 // shared memory such a product takes some 720 cycles, 512 by its arithmetic.
 #include <math_constants.h>
 
 #include <algorithm>
-#include <climits>
 #include <type_traits>
 
 #include "relm_mp_attn_tc.cuh"
@@ -116,11 +115,11 @@ __device__ __forceinline__ void store_rows(uint32_t acc, bool any, bool ok, floa
 
 // ---- work in parts ---------------------------------------------------------------------
 
-// A job is a tile of one head. The jobs of the last, partial wave of blocks are cut
-// into `parts` along the other side; their sums go to the workspace in float32 and
-// k_attn_tc_backward_join adds them in order. parts == 1: the grid is (tiles, heads).
+// A job is a tile of one head. Heads run first: a plan's list has the longest tiles in front, and so has the whole
+// grid (heads one after another: four ragged sequences 257 us against 237). The jobs of the last, partial wave of blocks are cut into `parts` along the other
+// side; their sums go to the workspace in float32 and k_attn_tc_backward_join adds them in order.
 struct Share {
-   int tiles, full, rest, parts; // `full` jobs whole, then `rest` in parts
+   int heads, full, rest, parts; // `full` jobs whole, then `rest` in parts
    float* sums;                  // [rest * parts][outputs][DP / 4][kTileRows][4]
 };
 
@@ -130,10 +129,9 @@ struct Job {
 
 __device__ __forceinline__ Job job_of(const Share& w)
 {
-   if(w.parts == 1) return Job{(int)blockIdx.x, (int)blockIdx.y, -1};
    const int past = (int)blockIdx.x - w.full;
    const int job = past < 0 ? (int)blockIdx.x : w.full + past / w.parts;
-   return Job{job % w.tiles, job / w.tiles, past < 0 ? -1 : past % w.parts};
+   return Job{job / w.heads, job % w.heads, past < 0 ? -1 : past % w.parts};
 }
 
 // Iterations [begin, end) of `n`.
@@ -143,8 +141,8 @@ __device__ __forceinline__ void part_of(const Share& w, int part, int n, int& be
    end = part < 0 ? n : (int)((int64_t)n * (part + 1) / w.parts);
 }
 
-// The number of this block's part, -1 for a whole job (worked out again at a kernel's end, not held through it).
-__device__ __forceinline__ int part_block(const Share& w) { return w.parts == 1 ? -1 : (int)blockIdx.x - w.full; }
+// The number of this block's part, negative for a whole job (worked out again at a kernel's end, not held through it).
+__device__ __forceinline__ int part_block(const Share& w) { return (int)blockIdx.x - w.full; }
 
 // This thread's accumulator row to `out` ([DP / 4][kTileRows][4], row `row`).
 template < int DP >
@@ -171,7 +169,7 @@ __device__ __forceinline__ void store_sums(uint32_t acc, bool any, bool ok, floa
 template < typename T, int DP, bool KV >
 __global__ void __launch_bounds__(kTileRows) k_attn_tc_backward_join(Args a, Share w)
 {
-   const int job = w.full + blockIdx.x, tile = job % w.tiles, head = job / w.tiles, c = blockIdx.y * 16, which = blockIdx.z;
+   const int job = w.full + blockIdx.x, tile = job / w.heads, head = job % w.heads, c = blockIdx.y * 16, which = blockIdx.z;
    const Item it = KV ? item(a.kv_tiles, a.max_kv, kTileRows, tile) : item(a.q_tiles, a.max_q, kTileRows, tile);
    const Seq s = KV ? locate(a.kv_off, a.max_kv, a.ks, it.seq) : locate(a.q_off, a.max_q, a.qs, it.seq);
    const int row = it.tile * kTileRows + threadIdx.x, heads = KV ? a.kv_heads : a.heads;
@@ -638,19 +636,19 @@ __global__ void __launch_bounds__(Dq< DP, KN >::THREADS, Dq< DP, KN >::RESIDENT)
 
 // The jobs of a partial wave in parts where that saves more than it costs: in iterations of the longest job, with
 // eight for the join and its launch, at least four a part and at most two waves of parts. Backward of 4 x 2048 x 4096,
-// 16 heads over 4 of 128 (512 jobs on 148 SMs) 856 us against 906 whole; one sequence of 1000 x 1000, 8 over 2, 52
-// against 99; 3000 x 300, 16 over 4 of 64, 68 against 294; 200 x 20000, 8 heads, 171 against 384.
+// 16 heads over 4 of 128 (512 jobs on 148 SMs) 849 us against 906 whole; one sequence of 1000 x 1000, 8 over 2, 52
+// against 99; 3000 x 300, 16 over 4 of 64, 65 against 294; 200 x 20000, 8 heads, 169 against 384.
 Share share(int64_t tiles, int64_t heads, int64_t n, int resident, float* sums)
 {
    const int64_t jobs = tiles * heads, slots = 148 * resident, rest = jobs % slots;
-   Share w{(int)std::min< int64_t >(tiles, INT_MAX), 0, (int)rest, 1, sums};
-   if(rest == 0 || jobs > 64 * slots) return w; // nothing to cut, or a small part of the whole
+   Share w{(int)heads, (int)jobs, 0, 1, sums};
+   if(jobs > 64 * slots) return w; // the last wave is a small part of the whole
    int64_t best = n;
-   for(int64_t s = 2; s * 4 <= n && rest * s <= 2 * slots; ++s) {
+   for(int64_t s = 2; rest > 0 && s * 4 <= n && rest * s <= 2 * slots; ++s) {
       const int64_t cost = ceil_div(rest * s, slots) * ceil_div(n, s) + 8;
       if(cost < best) best = cost, w.parts = (int)s;
    }
-   w.full = (int)(jobs - rest);
+   if(w.parts > 1) w.full = (int)(jobs - rest), w.rest = (int)rest;
    return w;
 }
 template < int DP, int N >
@@ -672,14 +670,13 @@ size_t sums_bytes(const Args& a, int64_t q_tiles, int64_t kv_tiles)
 }
 
 template < typename F, typename J >
-int launch(SmemLimit& limit, F fn, J join, int threads, int bytes, int heads, int outputs, int columns, const Args& a, const Share& w,
+int launch(SmemLimit& limit, F fn, J join, int threads, int bytes, int outputs, int columns, const Args& a, const Share& w,
            const TcMaps& m, cudaStream_t st, const char* what)
 {
-   if(w.tiles == 0) return RELM_MP_OK;
+   if(w.full + w.rest == 0) return RELM_MP_OK;
    int rc = limit((const void*)fn, bytes, what);
    if(rc) return rc;
-   const dim3 grid = w.parts > 1 ? dim3(w.full + w.rest * w.parts) : dim3(w.tiles, heads);
-   fn<<< grid, threads, bytes, st >>>(a, w, m.q, m.k, m.v, m.go);
+   fn<<< w.full + w.rest * w.parts, threads, bytes, st >>>(a, w, m.q, m.k, m.v, m.go);
    if((rc = check_launch(what)) || w.parts == 1) return rc;
    join<<< dim3(w.rest, columns, outputs), kTileRows, 0, st >>>(a, w);
    return check_launch("k_attn_tc_backward_join");
@@ -705,11 +702,11 @@ int backward(relm_mp_dtype dtype, const Args& a, int64_t q_tiles, int64_t kv_til
    static SmemLimit kv_limit, q_limit;
    const int columns = (a.dim + 15) / 16;
    if((rc = launch(kv_limit, k_attn_tc_backward_kv< T, DP, N >, k_attn_tc_backward_join< T, DP, true >, Kv< DP, N >::THREADS,
-                   (int)Kv< DP, N >::BYTES + 1024, a.kv_heads, 2, columns, a, share_kv< DP, N >(a, kv_tiles, sums), m, st, "k_attn_tc_backward_kv")))
+                   (int)Kv< DP, N >::BYTES + 1024, 2, columns, a, share_kv< DP, N >(a, kv_tiles, sums), m, st, "k_attn_tc_backward_kv")))
       return rc;
    if(N != kTileRows && (rc = maps(&m, kTileRows, N))) return rc;
    return launch(q_limit, k_attn_tc_backward_q< T, DP, N >, k_attn_tc_backward_join< T, DP, false >, Dq< DP, N >::THREADS,
-                 (int)Dq< DP, N >::BYTES + 1024, a.heads, 1, columns, a, share_q< DP, N >(a, q_tiles, sums), m, st, "k_attn_tc_backward_q");
+                 (int)Dq< DP, N >::BYTES + 1024, 1, columns, a, share_q< DP, N >(a, q_tiles, sums), m, st, "k_attn_tc_backward_q");
 }
 
 }  // namespace
