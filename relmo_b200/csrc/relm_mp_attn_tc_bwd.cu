@@ -115,9 +115,11 @@ __device__ __forceinline__ void store_rows(uint32_t acc, bool any, bool ok, floa
 
 // ---- work in parts ---------------------------------------------------------------------
 
-// A job is a tile of one head. Heads run first: a plan's list has the longest tiles in front, and so has the whole
-// grid (heads one after another: four ragged sequences 257 us against 237). The jobs of the last, partial wave of blocks are cut into `parts` along the other
-// side; their sums go to the workspace in float32 and k_attn_tc_backward_join adds them in order.
+// A job is a tile of one head. Heads run first: a plan's list has the longest tiles
+// in front, and so has the whole grid (heads one after another: four ragged sequences
+// 257 us against 237). The jobs of the last, partial wave of blocks are cut into
+// `parts` along the other side; their sums go to the workspace in float32 and
+// k_attn_tc_backward_join adds them in order.
 struct Share {
    int heads, full, rest, parts; // `full` jobs whole, then `rest` in parts
    float* sums;                  // [rest * parts][outputs][DP / 4][kTileRows][4]

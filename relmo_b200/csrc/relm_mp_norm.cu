@@ -13,7 +13,7 @@
 // h the weight's gradient, a sum of terms of either sign, was 1.6 times as far
 // from its 64-bit value.
 //
-// Measured: 16384 x 8192 bf16 forward with residual 185 us (5.8 TB/s, 88% of the
+// Measured: 16384 x 8192 bf16 forward with residual 177 us (6.08 TB/s, 93% of the
 // copy rate); 51200 x 128 bf16 forward and backward 26 us of kernels, float32 rows
 // of an odd length (no 16-byte chunks) 63 us for 43 at the copy rate.
 #include <cuda_fp8.h>
@@ -417,7 +417,14 @@ int64_t grid_cap(int threads) { return (int64_t)kSms * (2048 / threads) * 4; }
 
 // Threads and chunks of a row from its number of chunks. Call as
 // f(integral_constant TPR, integral_constant NV); false if no group is wide enough.
-template < int VEC, typename F >
+// The forward with 16-byte chunks takes one or two a thread and as few idle threads
+// as it can: more rows are in flight on an SM, as each thread holds fewer registers
+// (bf16, TB/s: 8192 wide 5.75 with 256 threads of 4 chunks, 6.08 with 512 of 2; 6000
+// wide 5.40 and 6.08 with 384; 1024 wide 5.95 with a warp, 6.28 with 128 threads;
+// 12000 wide 5.02 and 5.67 with 768). Smaller chunks need more of them in flight per
+// thread (2900 wide in 4-byte chunks: 3.84 with 768 threads, 5.39 with 512), and the
+// backward's sums per column favour few threads.
+template < int VEC, bool FORWARD, typename F >
 bool with_shape(int64_t chunks, F&& f)
 {
    using std::integral_constant;
@@ -429,11 +436,24 @@ bool with_shape(int64_t chunks, F&& f)
    RELM_SHAPE(8, 1)
    RELM_SHAPE(16, 1)
    RELM_SHAPE(32, 1)
-   RELM_SHAPE(32, 2)
-   RELM_SHAPE(32, 4)
-   RELM_SHAPE(128, 2)
-   RELM_SHAPE(256, 2)
-   RELM_SHAPE(256, 4)
+   if constexpr(FORWARD && VEC >= 4) {
+      RELM_SHAPE(64, 1)
+      RELM_SHAPE(128, 1)
+      RELM_SHAPE(128, 2)
+      RELM_SHAPE(384, 1)
+      RELM_SHAPE(512, 1)
+      RELM_SHAPE(320, 2)
+      RELM_SHAPE(384, 2)
+      RELM_SHAPE(512, 2)
+      RELM_SHAPE(640, 2)
+      RELM_SHAPE(768, 2)
+   } else {
+      RELM_SHAPE(32, 2)
+      RELM_SHAPE(32, 4)
+      RELM_SHAPE(128, 2)
+      RELM_SHAPE(256, 2)
+      RELM_SHAPE(256, 4)
+   }
    RELM_SHAPE(512, 4)
    if constexpr(VEC <= 4) RELM_SHAPE(1024, 4)
    if constexpr(VEC <= 2) RELM_SHAPE(1024, 8)
@@ -445,10 +465,11 @@ template < typename T, int VEC, bool E4M3 >
 int launch_forward(const FwdArgs& a, cudaStream_t st)
 {
    const int64_t chunks = (a.width + VEC - 1) / VEC;
-   const bool done = with_shape< VEC >(chunks, [&](auto tpr, auto nv) {
+   const bool done = with_shape< VEC, true >(chunks, [&](auto tpr, auto nv) {
       constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
       const int64_t blocks = (a.rows + kBlockRows< TPR > - 1) / kBlockRows< TPR >;
-      const int64_t cap = grid_cap(kBlock< TPR >);
+      // Narrow rows: a block per 8 to 32 rows (400000 x 256 bf16: 124 us against 133 with the capped grid).
+      const int64_t cap = TPR <= 32 ? INT32_MAX : grid_cap(kBlock< TPR >);
       k_add_rms_norm< T, VEC, TPR, NV, E4M3 >
          <<< (unsigned)(blocks < cap ? blocks : cap), kBlock< TPR >, 0, st >>>(a);
    });
@@ -510,7 +531,7 @@ int64_t launch_backward(const BwdArgs& a, cudaStream_t st)
 {
    const int64_t chunks = (a.width + VEC - 1) / VEC;
    int64_t grid = 0;
-   const bool done = with_shape< VEC >(chunks, [&](auto tpr, auto nv) {
+   const bool done = with_shape< VEC, false >(chunks, [&](auto tpr, auto nv) {
       constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
       grid = backward_blocks< TPR >(a.rows);
       k_add_rms_norm_bwd< T, VEC, TPR, NV ><<< (unsigned)grid, kBlock< TPR >, 0, st >>>(a);

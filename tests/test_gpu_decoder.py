@@ -65,6 +65,33 @@ def test_norm_e4m3(dtype, rows, width):
     assert bool((err <= step * (1 + 1e-4) + 1e-12).all())
 
 
+# 16-byte chunks: a row just at and just past every number of threads and chunks, and rows past the resident blocks.
+@pytest.mark.parametrize("chunks", [c + d for c in (8, 16, 32, 64, 128, 256, 384, 512, 640, 768, 1024, 1280, 1536, 2048) for d in (0, 1)])
+@pytest.mark.parametrize("dtype,vec", [(F32, 4), (BF16, 8)])
+def test_norm_forward_of_every_width_class(dtype, vec, chunks):
+    width, rows = chunks * vec, 5
+    x, w, r = rnd((rows, width), dtype, 1), (1 + rnd((width,), F32, 2, 0.2)).to(dtype), rnd((rows, width), dtype, 3)
+    ye, he = ref.norm(x.double(), w.double(), r.double(), 1e-5)
+    y, h = decoder.add_rms_norm(x, w, r, eps=1e-5)
+    ref.close(y, ye, what="y")
+    ref.close(h, he, what="h")
+    q, scale, h = decoder.add_rms_norm_e4m3(x, w, r, eps=1e-5)
+    ref.close(h, he, what="h")
+    ref.close(scale, ye.abs().amax(1) / 448, what="scale")
+    err = (q.double() * scale.double()[:, None] - ye).abs()
+    step = torch.maximum(ye.abs() * 2.0**-4, scale.double()[:, None] * 2.0**-10)
+    assert bool((err <= step * (1 + 1e-4) + 1e-12).all())
+
+
+@pytest.mark.parametrize("rows,width", [(20011, 40), (20011, 512), (9001, 2600)])
+def test_norm_forward_of_many_rows(rows, width):
+    x, w, r = rnd((rows, width), BF16, 1), (1 + rnd((width,), F32, 2, 0.2)).to(BF16), rnd((rows, width), BF16, 3)
+    y, h = decoder.add_rms_norm(x, w, r)
+    ye, he = ref.norm(x.double(), w.double(), r.double(), 1e-6)
+    ref.close(y, ye, what="y")
+    ref.close(h, he, what="h")
+
+
 def test_norm_rows_of_zeros_infinity_and_nan():
     x = torch.zeros(4, 64, device="cuda")
     x[1, 3], x[2, 5] = math.inf, math.nan
