@@ -369,6 +369,7 @@ int relm_mp_cross_attention_backward(const relm_mp_attn* attn, const void* grad_
 {
    int rc;
    if((rc = check_attn(attn, "cross_attention_backward"))) return rc;
+   if(!attn->q_rows && !attn->kv_rows) return RELM_MP_OK;
    if((attn->q_rows && (!grad_o || !o || !lse || !dq)) || (attn->kv_rows && (!dk || !dv)))
       return fail(RELM_MP_ERR_INVALID_ARGUMENT, "cross_attention_backward: pointers must not be NULL.");
    if(attn->q_rows && (!workspace || workspace_bytes < relm_mp_cross_attention_backward_workspace_bytes(attn)))

@@ -88,6 +88,18 @@ def test_plan_on_the_host():
     assert lib.relm_mp_attn_plan_init(arr(-1), arr(1), 1, ctypes.byref(plan)) == 1
 
 
+def test_c_abi_without_rows_launches_nothing():
+    lib = capi.lib()
+    host = ctypes.create_string_buffer(512)
+    at = (ctypes.addressof(host) + 255) // 256 * 256  # aligned, and never read
+    for dtype in (capi.FLOAT32, capi.BFLOAT16):
+        a = capi.Attn(dtype=dtype, heads=4, kv_heads=2, dim=16, scale=0.25, q=at, k=at, v=at)
+        a.q_stride[1] = a.k_stride[1] = a.v_stride[1] = 64
+        a.q_stride[2] = a.k_stride[2] = a.v_stride[2] = 16
+        assert lib.relm_mp_cross_attention(ctypes.byref(a), at, None, None, None, 0, None) == 0
+        assert lib.relm_mp_cross_attention_backward(ctypes.byref(a), at, at, None, at, at, at, at, at, 256, None) == 0
+
+
 def test_c_abi_refusals():
     lib = capi.lib()
     attn = capi.Attn(dtype=capi.FLOAT32, heads=4, kv_heads=3, dim=16, scale=0.25)
