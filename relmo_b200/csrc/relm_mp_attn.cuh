@@ -70,6 +70,22 @@ __device__ __forceinline__ Item item(const Item* list, int64_t uniform, int tile
 constexpr int kTileRows = 128; // query rows or keys of a plan's tile
 constexpr int kBlockKeys = 64; // keys of a block of the split form
 
+// The block of a grid (items, heads) in the order of its blocks, but heads first: the
+// longest items are in front of a plan's lists, and so they start first for all heads
+// (64 ragged states of 100 to 400 rows, forward and backward: 171 us against 187).
+// `loop`: the longest other side. Loops of one tile have no long ones, and their small
+// blocks lose by it (dK, dV of 256 states of 50 keys: 27 us against 25).
+struct Place {
+   uint32_t item;
+   int head;
+};
+__device__ __forceinline__ Place heads_first(int64_t loop)
+{
+   if(loop <= kTileRows || (uint64_t)gridDim.x * gridDim.y >> 32) return Place{blockIdx.x, (int)blockIdx.y};
+   const uint32_t i = blockIdx.y * gridDim.x + blockIdx.x;
+   return Place{i / gridDim.y, (int)(i % gridDim.y)};
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 template < typename T >

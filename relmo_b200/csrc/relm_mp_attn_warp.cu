@@ -20,7 +20,7 @@
 //
 // Measured: float32 forward, 4 sequences of 1 000 queries over 2 000 keys, 8 heads of
 // 128, 0.97 ms (3.32 ms on the CUDA cores); 256 states of 4 to 40 queries over 50
-// keys with 2 heads of 16, forward and backward 72 us.
+// keys with 2 heads of 16, forward and backward 73 us.
 //
 // Rows that are masked or outside the sequence are zeros in shared memory (never
 // read) and get weight 0.
@@ -207,11 +207,12 @@ __global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_forwar
    extern __shared__ __align__(128) unsigned char smem[];
    T *sq = reinterpret_cast< T* >(smem), *sk = reinterpret_cast< T* >(smem + S::own), *sv = reinterpret_cast< T* >(smem + S::own + S::stream);
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x / PER);
+   const Place at = heads_first(a.max_kv);
+   const int head = at.head, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, at.item / PER);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
-   const int row0 = it.tile * kTileRows + (blockIdx.x % PER) * S::OWN;
+   const int row0 = it.tile * kTileRows + (int)(at.item % PER) * S::OWN;
    if(row0 >= qs.len) return;
    const T* k = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
    const T* v = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
@@ -309,8 +310,9 @@ __device__ __forceinline__ void weigh(float (&s)[NT][4], float (&dp)[NT][4], flo
 }
 
 // dK and dV of OWN keys and, for wide heads, of 128 columns (blockIdx.z). QN query rows at a time.
+// Two blocks an SM where the registers allow it (256 states of 50 keys: 22 us against 25).
 template < typename T, int DP, int QN, bool FINE >
-__global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_backward_kv(Args a, bool aligned)
+__global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32, DP * sizeof(T) <= 128 ? 2 : 1) k_attn_warp_backward_kv(Args a, bool aligned)
 {
    using S = Shape< T, DP >;
    constexpr int NT = QN / 8, DC = DP > 128 ? 128 : DP, ND = DC / 8, PER = kTileRows / S::OWN;
@@ -320,11 +322,12 @@ __global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_backwa
    T *sk = reinterpret_cast< T* >(smem), *sv = reinterpret_cast< T* >(smem + S::own), *sq = reinterpret_cast< T* >(smem + 2 * S::own),
      *sg = reinterpret_cast< T* >(smem + 2 * S::own + STREAM);
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-   const int kv_head = blockIdx.y, group = a.heads / a.kv_heads, col = blockIdx.z * DC;
-   const Item it = item(a.kv_tiles, a.max_kv, kTileRows, blockIdx.x / PER);
+   const Place at = heads_first(a.max_q);
+   const int kv_head = at.head, group = a.heads / a.kv_heads, col = blockIdx.z * DC;
+   const Item it = item(a.kv_tiles, a.max_kv, kTileRows, at.item / PER);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
-   const int key0 = it.tile * kTileRows + (blockIdx.x % PER) * S::OWN;
+   const int key0 = it.tile * kTileRows + (int)(at.item % PER) * S::OWN;
    if(key0 >= ks.len) return;
    const unsigned char* keep = a.mask ? a.mask + ks.first : nullptr;
    fill_tile< T, DP >(sk, static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2], a.ks[1], S::OWN, key0, ks.len, a.dim, keep, aligned);
@@ -391,11 +394,12 @@ __global__ void __launch_bounds__(Shape< T, DP >::WARPS * 32) k_attn_warp_backwa
    T *sq = reinterpret_cast< T* >(smem), *sg = reinterpret_cast< T* >(smem + S::own), *sk = reinterpret_cast< T* >(smem + 2 * S::own),
      *sv = reinterpret_cast< T* >(smem + 2 * S::own + S::stream);
    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-   const int head = blockIdx.y, kv_head = head / (a.heads / a.kv_heads);
-   const Item it = item(a.q_tiles, a.max_q, kTileRows, blockIdx.x / PER);
+   const Place at = heads_first(a.max_kv);
+   const int head = at.head, kv_head = head / (a.heads / a.kv_heads);
+   const Item it = item(a.q_tiles, a.max_q, kTileRows, at.item / PER);
    const Seq qs = locate(a.q_off, a.max_q, a.qs, it.seq), ks = locate(a.kv_off, a.max_kv, a.ks, it.seq);
    const Seq vs = locate(a.kv_off, a.max_kv, a.vs, it.seq);
-   const int row0 = it.tile * kTileRows + (blockIdx.x % PER) * S::OWN;
+   const int row0 = it.tile * kTileRows + (int)(at.item % PER) * S::OWN;
    if(row0 >= qs.len) return;
    const T* k = static_cast< const T* >(a.k) + ks.base + kv_head * a.ks[2];
    const T* v = static_cast< const T* >(a.v) + vs.base + kv_head * a.vs[2];
